@@ -290,6 +290,99 @@ int vmps_batch_gemm(void* out, int64_t out_row_stride, const void* x, int64_t x_
                     int dtype, void* stream);
 
 /*
+ * Attention of drafted tokens (a tree, or any set of drafts) over the paged
+ * cache: the check of speculative decoding.  No counterpart in the reference,
+ * which decodes one token per pass.
+ *
+ * Sequence i holds seq_lens[i] slots: ctx_lens[i] cached tokens, then its
+ * drafted tokens (draft j at slot ctx_lens[i] + j, K/V already written, e.g.
+ * by vmps_rope_reshape_and_cache).  Its query rows are cu_q[i] + r, r <
+ * q_lens[i]; a row sees every slot t < ctx_lens[i] and the draft j whose bit
+ * (j & 31) of tree_mask[row][j >> 5] is set:
+ *   out[row][h] = softmax_t(scale * q[row][h] . K[t][h / G]) . V[t][h / G].
+ * A row that sees no slot is zero.  Slots no row sees and drafts outside a
+ * row's mask take no part, whatever they hold (NaN and infinities included).
+ * Mask bits of drafts past seq_lens[i] are ignored; drafts past
+ * 32 * mask_words are seen by no row.  ctx_lens[i] above seq_lens[i] counts
+ * as seq_lens[i].
+ *
+ * q:    [total_q][n_q][head_dim], rotated, row stride q_row_stride elements
+ *       (multiple of 8), 16-byte aligned.  One row per sequence is a decode
+ *       step; the last rows of a tree alone are one level of its drafting.
+ * out:  [total_q][n_q][head_dim] contiguous, 16-byte aligned; only the rows
+ *       of a sequence are written.
+ * tree_mask: int32 [total_q][mask_words], contiguous.
+ * ctx_lens, seq_lens, q_lens, cu_q: int32 [num_seqs] on the device.
+ * max_q_len bounds q_lens (rows past it are not computed and set error bit
+ *       64, as do rows outside [0, total_q)).
+ * workspace: vmps_paged_tree_attention_workspace_bytes bytes, 256-byte
+ *       aligned, no initialisation; calls that may overlap on the GPU need
+ *       different workspaces.  The size depends on the device and on the
+ *       arguments given, not on the lengths.
+ * Supported: head_dim 64 or 128, block_size 16, n_q / n_kv a whole number up
+ * to 16, n_kv <= 64, num_seqs <= 4096, max_q_len <= 65535.
+ */
+size_t vmps_paged_tree_attention_workspace_bytes(int num_seqs, int max_q_len, int n_q, int n_kv,
+                                                 int head_dim, int dtype);
+int vmps_paged_tree_attention(void* out, const void* q, int64_t q_row_stride, const void* pool,
+                              const int32_t* block_tables, int max_blocks_per_seq,
+                              const int32_t* ctx_lens, const int32_t* seq_lens,
+                              const int32_t* q_lens, const int32_t* cu_q,
+                              const int32_t* tree_mask, int mask_words, int num_seqs,
+                              int total_q, int max_q_len, int n_q, int n_kv, int head_dim,
+                              int block_size, int num_blocks, float scale, void* workspace,
+                              size_t workspace_bytes, int dtype, void* stream);
+
+/*
+ * Commit of the drafted branch that the model agrees with.  No counterpart
+ * in the reference.
+ *
+ * Sequence i's n = seq_lens[i] - ctx_lens[i] drafted nodes are rows
+ * cu_tree[i] .. of parents, tokens and target_ids.  Node 0 is the root (the
+ * last token already decided, accepted by definition); parents[node] is the
+ * index of an earlier node of the same tree (node 0's is not read).
+ * target_ids[node] is the model's own next token after that node.  From the
+ * root the walk goes to the lowest-numbered child whose token is
+ * target_ids[current] and stops where there is none:
+ *   path[i][k]    k-th accepted node, -1 from count[i] on   int32 [num_seqs][max_tree]
+ *   count[i]      accepted nodes (0 only if n is 0)         int32 [num_seqs]
+ *   next_token[i] target_ids of the last one, -1 if none    int64 [num_seqs]
+ * and in every layer of pool ([num_layers][num_blocks][2][16][n_kv][head_dim]
+ * contiguous) the K and V of slot ctx + path[k] move to slot ctx + k.  Blocks
+ * must not be shared between sequences from slot ctx on.  What the slots past
+ * ctx + count hold afterwards is not meaningful.
+ * A tree above max_tree (<= 1024) or outside [0, total_nodes) sets error bit
+ * 64 and counts as empty; a slot outside the block table or the pool sets bit
+ * 4 or 2 and is not moved.  n_kv * head_dim: a multiple of 8, at most 65536.
+ */
+int vmps_commit_tree(int32_t* path, int32_t* count, int64_t* next_token, void* pool,
+                     int num_layers, const int32_t* block_tables, int max_blocks_per_seq,
+                     const int32_t* ctx_lens, const int32_t* seq_lens, const int32_t* cu_tree,
+                     const int32_t* parents, const int32_t* tokens, const int64_t* target_ids,
+                     int num_seqs, int total_nodes, int max_tree, int n_kv, int head_dim,
+                     int block_size, int num_blocks, int dtype, void* stream);
+
+/*
+ * Products with 4-bit weights (a drafter's projections).  No counterpart in
+ * the reference, whose weights are 16-bit nn.Linear modules.
+ *   out[m][n] = sum_g scales[n][g] * sum_{k in group g} x[m][k] * (code[n][k] - zeros[n][g])
+ * codes:  uint8 [N][K / 2], row n's code k in byte k / 2, the even k in the
+ *         low four bits.  scales: [N][K / group_size] in x's type.
+ * zeros:  uint8 [N][K / group_size], or NULL for 8 everywhere.
+ * All contiguous and 16-byte aligned.  Sums and scaling in fp32, one rounding.
+ * With silu_mul != 0 the weight is the fused [gate; up] of 2N rows and
+ * out[m][n] = silu(gate) * up of the unrounded fp32 products.
+ * Shapes: M <= 32, any N, group_size 32, 64 or 128, K a multiple of it; x
+ * 16-byte aligned with rows a multiple of 8 elements apart, out rows at least
+ * N apart, 2-byte aligned.  vmps_w4_gemm_supported says whether a shape is
+ * built (1) or not (0).
+ */
+int vmps_w4_gemm_supported(int M, int N, int K, int group_size);
+int vmps_w4_gemm(void* out, int64_t out_row_stride, const void* x, int64_t x_row_stride,
+                 const void* codes, const void* scales, const void* zeros, int M, int N, int K,
+                 int group_size, int silu_mul, int dtype, void* stream);
+
+/*
  * Copies `bytes` from `src` to `dst` with the GPU's own loads and stores,
  * as a link of a chain of kernels launched with programmatic dependent
  * launch.  No counterpart in the reference (whose inputs never leave host
@@ -315,8 +408,8 @@ int vmps_stage_copy(void* dst, const void* src, size_t bytes, void* stream);
  * of index violations the kernels skipped since the last call).  Synchronises
  * `stream`.  Bits: 1 slot out of range, 2 block id out of range, 4 seq_len
  * beyond the block table, 8 an internal wait timed out, 16 negative position,
- * 32 a fused-step slot outside the sequence's last page, 64 prefill query
- * rows outside [0, total_q) or a q_len above max_q_len.
+ * 32 a fused-step slot outside the sequence's last page, 64 prefill or tree
+ * rows outside [0, total_q) or a q_len (tree) above max_q_len (max_tree).
  */
 int vmps_debug_error_word(void* stream, int* word_out);
 

@@ -16,6 +16,10 @@ Public functions
   already-rotated new K/V into the slot given by ``write_info`` and attend.
 * :func:`gather_kv` -- the reference's padded paged gather
   (kernels/__init__.py:279-312), kept for API compatibility.
+* :func:`paged_tree_attention`, :func:`commit_tree`, :func:`w4_gemm` --
+  speculative decoding: attention of a tree of drafted tokens over the cache,
+  the commit of the branch the model agrees with, and the 4-bit products of
+  a drafter (:class:`W4Weight`, :func:`quantize_w4`).
 """
 
 from __future__ import annotations
@@ -59,6 +63,11 @@ EXPORTED_SYMBOLS = (
     "vmps_batch_gemm_split",
     "vmps_batch_gemm_workspace_bytes",
     "vmps_batch_gemm",
+    "vmps_paged_tree_attention_workspace_bytes",
+    "vmps_paged_tree_attention",
+    "vmps_commit_tree",
+    "vmps_w4_gemm_supported",
+    "vmps_w4_gemm",
     "vmps_stage_copy",
     "vmps_debug_error_word",
 )
@@ -122,6 +131,20 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.vmps_batch_gemm.restype = i32
         lib.vmps_batch_gemm.argtypes = [vp, i64, vp, i64, vp, i32, i32, i32, vp, ctypes.c_size_t,
                                         i32, vp]
+        lib.vmps_paged_tree_attention_workspace_bytes.restype = sz
+        lib.vmps_paged_tree_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32]
+        lib.vmps_paged_tree_attention.restype = i32
+        lib.vmps_paged_tree_attention.argtypes = [
+            vp, vp, i64, vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32,
+            i32, f32, vp, sz, i32, vp]
+        lib.vmps_commit_tree.restype = i32
+        lib.vmps_commit_tree.argtypes = [
+            vp, vp, vp, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32,
+            i32, i32, vp]
+        lib.vmps_w4_gemm_supported.restype = i32
+        lib.vmps_w4_gemm_supported.argtypes = [i32, i32, i32, i32]
+        lib.vmps_w4_gemm.restype = i32
+        lib.vmps_w4_gemm.argtypes = [vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]
         lib.vmps_stage_copy.restype = i32
         lib.vmps_stage_copy.argtypes = [vp, vp, sz, vp]
         lib.vmps_debug_error_word.restype = i32
@@ -642,6 +665,238 @@ def batch_gemm(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None
         rc = lib.vmps_batch_gemm(_ptr(out), out.stride(0), _ptr(x), x.stride(0), _ptr(w), M, N, K,
                                  _ptr(workspace), ws_bytes, dtype_code(x.dtype), _stream(dev))
     _check(rc, "batch_gemm")
+    return out
+
+
+# ── speculative decoding: tree attention, commit, 4-bit products ─────────────
+
+
+def paged_tree_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Tensor,
+                         ctx_lens: torch.Tensor, seq_lens: torch.Tensor, q_lens: torch.Tensor,
+                         cu_q: torch.Tensor, tree_mask: torch.Tensor, max_q_len: int,
+                         scale: float | None = None, out: torch.Tensor | None = None,
+                         workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted tokens over their sequences' paged K/V.
+
+    Sequence i has ``ctx_lens[i]`` cached slots and then its drafted tokens up
+    to ``seq_lens[i]`` (K/V already in ``pool``: ``rope_reshape_and_cache``
+    writes them).  Query row ``cu_q[i] + r`` (``r < q_lens[i]``) sees every
+    cached slot and draft j where bit ``j % 32`` of ``tree_mask[row, j // 32]``
+    is set (``core.draft_tree.DraftTree`` builds the masks).  A row that sees
+    nothing is zero; slots a row does not see take no part, whatever they hold.
+
+    ``q``: (total_q, n_q, D) rotated queries, heads packed (rows may be
+    strided); ``tree_mask``: int32 (total_q, words); the length tensors int32
+    (B,) on the device; ``max_q_len`` >= every ``q_lens`` entry (host int).
+    One row per sequence is a decode step.  ``workspace``: a device tensor of
+    :func:`paged_tree_attention_workspace_bytes` bytes, else one from torch's
+    caching allocator for this call (stream-ordered, so calls on different
+    streams never share it).  Returns ``out`` (total_q, n_q, D).
+    """
+    num_blocks, block_size, n_kv, D = _check_pool(pool)
+    if q.dim() == 2:
+        q = q.view(q.shape[0], -1, D)
+    if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or q.stride(1) != D:
+        raise ValueError(f"q must be (total_q, n_q, {D}) with packed heads; got {tuple(q.shape)}")
+    total_q, n_q = q.shape[0], q.shape[1]
+    B = q_lens.numel()
+    if block_tables.dim() != 2 or block_tables.shape[0] != B:
+        raise ValueError("block_tables must be (B, max_blocks)")
+    if ctx_lens.numel() != B or seq_lens.numel() != B or cu_q.numel() != B:
+        raise ValueError("ctx_lens, seq_lens, q_lens and cu_q must have one entry per sequence")
+    if tree_mask.dim() != 2 or tree_mask.shape[0] != total_q or tree_mask.shape[1] < 1:
+        raise ValueError(f"tree_mask must be (total_q, words) with total_q={total_q}")
+    if q.dtype != pool.dtype:
+        raise TypeError(f"q dtype {q.dtype} != pool dtype {pool.dtype}")
+    for t, name in ((block_tables, "block_tables"), (ctx_lens, "ctx_lens"), (seq_lens, "seq_lens"),
+                    (q_lens, "q_lens"), (cu_q, "cu_q"), (tree_mask, "tree_mask")):
+        _int32(t, name)
+    if out is None:
+        out = torch.empty((total_q, n_q, D), dtype=q.dtype, device=q.device)
+    elif out.shape != (total_q, n_q, D) or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be a contiguous (total_q, n_q, D) tensor of q's dtype")
+    dev = _require_cuda(q, pool, block_tables, ctx_lens, seq_lens, q_lens, cu_q, tree_mask, out,
+                        workspace)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    lib = load_library()
+    code = dtype_code(pool.dtype)
+    with torch.cuda.device(dev):
+        if workspace is None:
+            need = lib.vmps_paged_tree_attention_workspace_bytes(B, int(max_q_len), n_q, n_kv, D,
+                                                                 code)
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        # torch gives a single row any stride; the kernel never steps by it.
+        rc = lib.vmps_paged_tree_attention(
+            _ptr(out), _ptr(q), q.stride(0) if total_q > 1 else n_q * D, _ptr(pool), _ptr(block_tables), block_tables.shape[1],
+            _ptr(ctx_lens), _ptr(seq_lens), _ptr(q_lens), _ptr(cu_q), _ptr(tree_mask),
+            tree_mask.shape[1], B, total_q, int(max_q_len), n_q, n_kv, D, block_size, num_blocks,
+            float(scale), _ptr(workspace), workspace.numel() * workspace.element_size(), code,
+            _stream(dev))
+    _check(rc, "paged_tree_attention")
+    return out
+
+
+def paged_tree_attention_workspace_bytes(num_seqs: int, max_q_len: int, n_q: int, n_kv: int,
+                                         d: int, dtype: torch.dtype) -> int:
+    """Bytes of workspace ``paged_tree_attention`` needs (0: shape not built).  Needs a CUDA device."""
+    return int(load_library().vmps_paged_tree_attention_workspace_bytes(
+        int(num_seqs), int(max_q_len), int(n_q), int(n_kv), int(d), dtype_code(dtype)))
+
+
+def commit_tree(pool: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
+                seq_lens: torch.Tensor, cu_tree: torch.Tensor, parents: torch.Tensor,
+                tokens: torch.Tensor, target_ids: torch.Tensor, max_tree: int,
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Accept the drafted branch the model agrees with and keep its K/V.
+
+    Sequence i's drafted nodes (slots ``ctx_lens[i] ..  seq_lens[i] - 1``) are
+    rows ``cu_tree[i] ..`` of ``parents``/``tokens`` (int32) and ``target_ids``
+    (int64: the model's own next token after each node, e.g. the argmax of its
+    logits).  Node 0 is the root and always accepted; from there the walk goes
+    to the lowest-numbered child whose token is the current node's target.
+    The accepted nodes' K/V move, in place and in every layer, to the slots
+    right after the context.  ``pool``: one layer's (num_blocks, 2, 16, n_kv,
+    D) or all layers' (L, num_blocks, 2, 16, n_kv, D); ``max_tree`` >= every
+    tree (host int, <= 1024).
+
+    Returns ``(path, count, next_token)``: int32 (B, max_tree) accepted nodes,
+    -1 after the last; int32 (B,) how many; int64 (B,) the model's token after
+    the last of them.
+    """
+    layers = 1
+    one = pool
+    if pool.dim() == 6:
+        layers = pool.shape[0]
+        if layers == 0 or not pool.is_contiguous():
+            raise ValueError("pool must be contiguous with at least one layer")
+        one = pool[0]
+    num_blocks, block_size, n_kv, D = _check_pool(one)
+    B = ctx_lens.numel()
+    if block_tables.dim() != 2 or block_tables.shape[0] != B:
+        raise ValueError("block_tables must be (B, max_blocks)")
+    if seq_lens.numel() != B or cu_tree.numel() != B:
+        raise ValueError("ctx_lens, seq_lens and cu_tree must have one entry per sequence")
+    n = tokens.numel()
+    if parents.numel() != n or target_ids.numel() != n:
+        raise ValueError("parents, tokens and target_ids must have one entry per drafted node")
+    for t, name in ((block_tables, "block_tables"), (ctx_lens, "ctx_lens"), (seq_lens, "seq_lens"),
+                    (cu_tree, "cu_tree"), (parents, "parents"), (tokens, "tokens")):
+        _int32(t, name)
+    if target_ids.dtype != torch.int64 or not target_ids.is_contiguous():
+        raise TypeError("target_ids must be contiguous int64")
+    dev = _require_cuda(pool, block_tables, ctx_lens, seq_lens, cu_tree, parents, tokens, target_ids)
+    path = torch.empty((B, int(max_tree)), dtype=torch.int32, device=dev)
+    count = torch.empty(B, dtype=torch.int32, device=dev)
+    nxt = torch.empty(B, dtype=torch.int64, device=dev)
+    lib = load_library()
+    with torch.cuda.device(dev):
+        rc = lib.vmps_commit_tree(
+            _ptr(path), _ptr(count), _ptr(nxt), _ptr(pool), layers, _ptr(block_tables),
+            block_tables.shape[1], _ptr(ctx_lens), _ptr(seq_lens), _ptr(cu_tree), _ptr(parents),
+            _ptr(tokens), _ptr(target_ids), B, n, int(max_tree), n_kv, D, block_size, num_blocks,
+            dtype_code(pool.dtype), _stream(dev))
+    _check(rc, "commit_tree")
+    return path, count, nxt
+
+
+class W4Weight:
+    """A weight matrix of 4-bit codes with a scale (and a zero point) per group.
+
+    ``codes``: uint8 (N, K/2), code k of a row in byte k // 2, even k in the
+    low four bits; ``scales``: (N, K/group) in the activations' dtype;
+    ``zeros``: uint8 (N, K/group) or None (8 everywhere).  The weight it
+    stands for is ``scales * (code - zeros)``.  All contiguous.
+    """
+
+    __slots__ = ("codes", "scales", "zeros", "N", "K", "group_size")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor,
+                 zeros: torch.Tensor | None = None) -> None:
+        if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous():
+            raise ValueError("codes must be a contiguous uint8 (N, K/2) matrix")
+        self.N, self.K = codes.shape[0], 2 * codes.shape[1]
+        if scales.dim() != 2 or scales.shape[0] != self.N or not scales.is_contiguous() \
+                or scales.shape[1] < 1 or self.K % scales.shape[1]:
+            raise ValueError(f"scales must be contiguous ({self.N}, groups) with groups dividing {self.K}")
+        if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape
+                                  or not zeros.is_contiguous()):
+            raise ValueError("zeros must be contiguous uint8 of scales' shape")
+        self.codes, self.scales, self.zeros = codes, scales, zeros
+        self.group_size = self.K // scales.shape[1]
+
+    def dequantize(self) -> torch.Tensor:
+        """The (N, K) fp32 matrix this weight stands for."""
+        q = torch.stack([self.codes & 15, self.codes >> 4], 2).view(self.N, -1, self.group_size)
+        z = 8.0 if self.zeros is None else self.zeros.float().unsqueeze(2)
+        return ((q.float() - z) * self.scales.float().unsqueeze(2)).view(self.N, self.K)
+
+
+def quantize_w4(w: torch.Tensor, group_size: int = 128, zero_points: bool = True) -> W4Weight:
+    """Round a (N, K) 16-bit weight to 4-bit codes per group of ``group_size`` columns.
+
+    With ``zero_points`` a group's codes span its range (extended to hold
+    zero); without, they are symmetric around code 8.  The scale is rounded
+    to ``w``'s dtype first and the codes are the nearest to that scale.
+    """
+    if w.dim() != 2 or w.shape[1] % group_size or group_size not in (32, 64, 128):
+        raise ValueError("w must be (N, K) with K a multiple of group_size (32, 64 or 128)")
+    N, K = w.shape
+    g = w.detach().float().view(N, K // group_size, group_size)
+    if zero_points:
+        lo, hi = g.amin(2).clamp(max=0.0), g.amax(2).clamp(min=0.0)
+        scale = (hi - lo) / 15.0
+    else:
+        scale = g.abs().amax(2) / 7.0
+    scale = torch.where(scale > 0, scale, torch.ones_like(scale)).to(w.dtype)
+    # A scale that underflows the dtype would divide by zero: the smallest normal stands in.
+    scale = scale.clamp(min=torch.finfo(w.dtype).tiny)
+    s = scale.float()
+    zeros = torch.round(-lo / s).clamp(0, 15) if zero_points else torch.full_like(s, 8.0)
+    q = (torch.round(g / s.unsqueeze(2)) + zeros.unsqueeze(2)).clamp(0, 15).to(torch.uint8).view(N, K)
+    codes = (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous()
+    return W4Weight(codes, scale.contiguous(), zeros.to(torch.uint8) if zero_points else None)
+
+
+def w4_gemm_supported(m: int, n: int, k: int, group_size: int) -> bool:
+    """Whether ``w4_gemm`` is built for this shape (M <= 32, group 32, 64 or 128 dividing K)."""
+    return bool(load_library().vmps_w4_gemm_supported(int(m), int(n), int(k), int(group_size)))
+
+
+def w4_gemm(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None,
+            silu_mul: bool = False) -> torch.Tensor:
+    """``x @ w.T`` with a 4-bit weight, for up to 32 rows (a drafter's projections).
+
+    ``x``: (M, K) fp16 or bf16 with unit inner stride, rows a multiple of 8
+    elements apart.  Sums and scales in fp32, one rounding.  With
+    ``silu_mul`` the weight is the fused [gate; up] matrix of 2I rows and the
+    result is ``silu(x @ Wg.T) * (x @ Wu.T)`` (M, I), rounded once at the end.
+    Returns ``out`` (M, N).
+    """
+    if x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError("x must be 2-D (M, K) with unit inner stride")
+    M, K = x.shape
+    if w.K != K:
+        raise ValueError(f"x has K={K}, w has K={w.K}")
+    if w.scales.dtype != x.dtype:
+        raise TypeError(f"scales dtype {w.scales.dtype} != x dtype {x.dtype}")
+    if silu_mul and w.N % 2:
+        raise ValueError("silu_mul needs a [gate; up] weight with an even row count")
+    N = w.N // 2 if silu_mul else w.N
+    if out is None:
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    elif out.shape != (M, N) or out.dtype != x.dtype or out.stride(1) != 1:
+        raise ValueError(f"out must be ({M}, {N}) of x's dtype with unit inner stride")
+    dev = _require_cuda(x, w.codes, w.scales, w.zeros, out)
+    lib = load_library()
+    # torch gives a single row any stride; the kernel never steps by it.
+    xs = x.stride(0) if M > 1 else K
+    os_ = out.stride(0) if M > 1 else N
+    with torch.cuda.device(dev):
+        rc = lib.vmps_w4_gemm(_ptr(out), os_, _ptr(x), xs, _ptr(w.codes), _ptr(w.scales),
+                              _ptr(w.zeros), M, N, K, w.group_size, int(bool(silu_mul)),
+                              dtype_code(x.dtype), _stream(dev))
+    _check(rc, "w4_gemm")
     return out
 
 
