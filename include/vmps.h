@@ -320,7 +320,7 @@ int vmps_batch_gemm(void* out, int64_t out_row_stride, const void* x, int64_t x_
  *       different workspaces.  The size depends on the device and on the
  *       arguments given, not on the lengths.
  * Supported: head_dim 64 or 128, block_size 16, n_q / n_kv a whole number up
- * to 16, n_kv <= 64, num_seqs <= 4096, max_q_len <= 65535.
+ * to 16, n_kv <= 64, num_seqs <= 4096, max_q_len <= 1024.
  */
 size_t vmps_paged_tree_attention_workspace_bytes(int num_seqs, int max_q_len, int n_q, int n_kv,
                                                  int head_dim, int dtype);

@@ -36,16 +36,15 @@
 // kDevErrTimeout and a CTA-wide abort flag, all roles leave their loops,
 // the MMA lane waits (bounded) for its own MMAs, the producer for its own
 // loads, and the TMEM columns are always freed before the CTA exits.
-#include <type_traits>
 #include <mutex>
 
 #include "vmps_abi_internal.h"
 #include "vmps_common.cuh"
+#include "vmps_tcgen05.cuh"
 
 namespace vmps {
 namespace {
 
-constexpr int kPfRows = 128;       // MMA M: rows per tile
 constexpr int kPfKeys = 64;        // keys per key tile (4 pages)
 constexpr int kPfPages = kPfKeys / 16;
 constexpr int kPfStages = 2;       // K ring and V ring depth
@@ -81,128 +80,6 @@ struct PrefillParams {
   float scale_log2;
   int* err;
 };
-
-// ── tcgen05 wrappers (PTX ISA 8.7, sm_100a) ──────────────────────────────────
-
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                       uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n"
-      ".reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-      "}\n" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// Same with A read from TMEM (K-major: row = lane, 16-bit pairs along K per
-// 32-bit column, 8 columns per K-step of 16).
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                          uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n"
-      ".reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-      "}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// 16 consecutive 32-bit TMEM columns of this thread's lane.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-      "r"(r[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-// Ties registers written by tcgen05.ld to the wait that follows it: the
-// compiler sees each value pass through an asm placed after the wait, so no
-// use can be scheduled before the load has landed.
-__device__ __forceinline__ void tmem_ld_fence_regs(uint32_t (&r)[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[i]));
-}
-
-// Shared-memory matrix descriptor for a 128-byte-swizzled operand
-// (sm_100 format: start, leading and stride byte offsets in 16-byte units,
-// descriptor version 1 at bit 46, layout type 2 = SWIZZLE_128B at bit 61).
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo_bytes,
-                                               uint32_t sbo_bytes) {
-  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) |
-         (static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFFu) << 16) |
-         (static_cast<uint64_t>((sbo_bytes >> 4) & 0x3FFFu) << 32) | (1ull << 46) |
-         (2ull << 61);
-}
-
-// Instruction descriptor of kind::f16 with fp32 accumulation: A and B both
-// fp16 or both bf16, A K-major, B K-major or MN-major, M = 128.
-template <typename T>
-__device__ __forceinline__ uint32_t f16_idesc(int n, bool b_mn_major) {
-  const uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
-  return (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(b_mn_major) << 16) |
-         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kPfRows >> 4) << 24);
-}
-
-__device__ __forceinline__ bool aborted(volatile int* flag) { return *flag != 0; }
-
-// ── packed fp32 pairs (f32x2 arithmetic of sm_100) for the softmax ───────────
-// Each op computes two independent fp32 results, rounded exactly as the
-// scalar op would, in one instruction.
-
-__device__ __forceinline__ uint64_t f2_make(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void f2_split(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPfThreads, 2)

@@ -1,28 +1,95 @@
-// Paged attention of drafted tree tokens over a sequence's cache.
+// Paged attention of drafted tree tokens over a sequence's cache, on the
+// sm_100a tensor cores (tcgen05 MMA with TMEM accumulators).
 //
 // Row r of sequence i (one drafted token, one query head) sees every cached
 // slot t < ctx_lens[i] and the drafted slots ctx_lens[i] + j whose bit j is
 // set in its mask row:
 //     s_t = scale * q . K_t,   out = sum_t e^(s_t - m) V_t / sum_t e^(s_t - m).
-// A row that sees no slot is zero.  Slots that no row may see (past the
-// sequence's end) and drafted slots outside a row's mask take no part,
-// whatever their bits (a product with their stale values is never formed).
+// A row that sees no slot is zero.
 //
-// One warp per (row, query head): 32 keys a step, one per lane for the
-// scores, then the lanes split head_dim for P . V.
+// What bounds it.  Every K and V element is read once for all rows of its kv
+// head: 128 rows do 128 flops per byte, so up to about 200 rows per kv head
+// the cache stream from HBM is the bound, above that the arithmetic (first
+// the softmax, which the MMAs of the other CTA on the SM overlap).
+//
+// Work split.  A row tile is 128 MMA rows: 128 / G drafted tokens x the G
+// query heads of a kv head, so K and V are read once per kv head and GQA is
+// never materialised.  Within one row tile index the key tiles (64 keys, 4
+// pages) of all sequences and kv heads are laid end to end, each sequence
+// start weighing kSegWeight / kTileWeight tiles, and every CTA of a
+// persistent grid (2 per SM) takes one contiguous, equal share: ragged
+// batches and a few long contexts both fill the machine.  Row tile indices
+// get CTAs in proportion to their work, each starting on a CTA of its own, so
+// that the row tiles of one context stream the same pages at the same time
+// (the second reader finds them in L2).  Every CTA works the plan out from the
+// lengths on the device; the host needs none of them.
+//
+// A sequence cut between CTAs: each piece stores its running maximum, sum and
+// unnormalised output in fp32, and a second small kernel (programmatic
+// dependent launch) joins the pieces in a fixed order.  Calls whose block
+// tables are at most kWholeTiles key tiles wide are never cut and skip it.
+//
+// Data movement, MMA order and softmax are those of the prefill kernel (warp 4
+// loads Q and K pages, warp 5 V pages, warp 6 issues the MMAs, warps 0-3 own a
+// row per thread; S is double-buffered in TMEM, P overwrites S and is PV's A
+// operand), run as one pipeline over all tiles of all segments of the CTA's
+// share: the next segment's first tiles load and multiply while the current
+// one finishes.
+//
+// Masks.  Tiles inside the cached context need none.  In a tile that reaches
+// past it a row's 64 visibility bits are cut out of its mask words; masked
+// scores become -inf before the maximum.  There V is also cleaned in shared
+// memory: rows past the sequence's end are zeroed and non-finite values of
+// drafted tokens are replaced by 0 (0 * inf would reach rows that do not see
+// them); a row that does see such a value adds it in its epilogue.
+//
+// Rounding: P is rounded to the 16-bit type as PV's operand (its sum is not),
+// the output once; scores, maxima, sums and accumulators are fp32.
+//
+// Safety.  Every mbarrier wait is bounded; a wait that gives up sets
+// kDevErrTimeout and a CTA-wide abort flag, all roles leave their loops, loads
+// and MMAs in flight are waited for (bounded) and the TMEM is always freed.
+#include <mutex>
+
 #include "vmps_abi_internal.h"
 #include "vmps_common.cuh"
+#include "vmps_tcgen05.cuh"
 
 namespace vmps {
 namespace {
 
-constexpr int kTreeWarps = 4;
 constexpr int kPage = 16;
+constexpr int kTtRows = 128;                  // MMA M
+constexpr int kTtKeys = 64;                   // keys per tile
+constexpr int kTtPages = kTtKeys / kPage;
+constexpr int kTtStages = 2;                  // K ring and V ring depth
+constexpr int kTtThreads = 224;
+constexpr int kTtKWarp = 4, kTtVWarp = 5, kTtMmaWarp = 6;
+constexpr int kTtQChunk = kTtRows * 128;      // 128 rows x 64 16-bit columns
+constexpr int kTtKChunk = kTtKeys * 128;
+constexpr int kTtCtasPerSm = 2;
+constexpr int kTtMaxSeqs = 4096;
+constexpr int kTtMaxQLen = 1024;
+constexpr int kTtMaxRowTiles = 128;           // 1024 tokens x 16 heads / 128
+constexpr int kTileWeight = 4;
+constexpr int kSegWeight = 8;
+constexpr int kMinTiles = 4;                  // a share holds at least this many tiles
+constexpr int kWholeTiles = 8;                // contexts up to this many tiles are not cut
+constexpr int kMergeThreads = 256;
+constexpr int kMergeCols = 16;                // output columns per merge unit
+
+template <int D>
+struct TreeShape {
+  static constexpr int kChunks = D / 64;
+  static constexpr int kQBytes = kChunks * kTtQChunk;
+  static constexpr int kTileBytes = kChunks * kTtKChunk;  // K (or V) of one key tile
+  static constexpr int kBarBytes = 512 + kTtMaxRowTiles * 4;
+  static constexpr int kFixedBytes = kQBytes + 2 * kTtStages * kTileBytes + kBarBytes;
+  static constexpr uint32_t kTmemCols = 256;  // S 2 x 64 columns, O up to 128
+};
 
 struct TreeParams {
   void* out;
-  const void* q;
-  int64_t q_stride;
   const void* pool;
   const int32_t* block_tables;
   const int32_t* ctx_lens;
@@ -30,84 +97,928 @@ struct TreeParams {
   const int32_t* q_lens;
   const int32_t* cu_q;
   const uint32_t* mask;
-  int mask_words, max_blocks, total_q, max_q_len, n_q, n_kv, G, num_blocks;
+  int mask_words, max_blocks, num_seqs, total_q, max_q_len, n_q, n_kv, G, num_blocks;
+  int tokens_per_tile, row_tiles, n_cta, whole, box_tokens;
+  int part_rows;     // rows of a partial record (a multiple of 32)
   float scale_log2;
+  int* records;      // [n_cta][8]: a cut sequence whose second piece CTA b holds
+  float2* part_ml;   // [n_cta * 2][part_rows]
+  float4* part_o;    // [n_cta * 2][D / 4][part_rows]
   int* err;
 };
 
+struct TreeSeq {
+  int ctx, n, q_len, row0;
+};
+
+// Lengths of a sequence, clamped to what the buffers hold.
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int s, bool report) {
+  TreeSeq r;
+  r.n = p.seq_lens[s];
+  r.ctx = p.ctx_lens[s];
+  r.q_len = p.q_lens[s];
+  r.row0 = p.cu_q[s];
+  if (r.q_len <= 0) {
+    r.q_len = 0;
+  } else if (r.row0 < 0 || static_cast<long long>(r.row0) + r.q_len > p.total_q) {
+    if (report) set_error(p.err, kDevErrQueryRange);
+    r.q_len = 0;
+  } else if (r.q_len > p.max_q_len) {
+    if (report) set_error(p.err, kDevErrQueryRange);
+    r.q_len = p.max_q_len;
+  }
+  if (r.n > p.max_blocks * kPage) {
+    if (report) set_error(p.err, kDevErrSeqLen);
+    r.n = p.max_blocks * kPage;
+  }
+  if (r.n < 0) r.n = 0;
+  r.ctx = min(max(r.ctx, 0), r.n);
+  return r;
+}
+
+// A sequence with query rows has at least one tile (its rows are written even
+// if it holds no slot).
+__device__ __forceinline__ int tree_tiles(int n) { return n > 0 ? (n + kTtKeys - 1) / kTtKeys : 1; }
+
+__device__ __forceinline__ int tree_weight(const TreeSeq& q, int first_token) {
+  return q.q_len > first_token ? tree_tiles(q.n) * kTileWeight + kSegWeight : 0;
+}
+
+// Largest s in [0, n) with pref[s] <= f (pref non-decreasing, pref[0] = 0).
+__device__ __forceinline__ int tree_find(const int* pref, int n, int f) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pref[mid] <= f) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+struct TreePos {  // a tile of a row tile's linear order
+  int kvh, s, j;
+};
+
+// What a CTA does: row tile index, its place among that index's CTAs, its share.
+struct TreeShare {
+  int rt;
+  int first_cta;      // first CTA of this row tile index
+  int chunk;          // weight of a share (fits 31 bits: see the host's check)
+  TreePos begin, end; // tiles [begin, end)
+};
+
+// The share of tiles before weighted position w.
+__device__ __forceinline__ TreePos tree_pos(const int* wpref, int num_seqs, int n_kv, int whole,
+                                            long long w) {
+  TreePos r;
+  const int wt = wpref[num_seqs];
+  if (w >= static_cast<long long>(n_kv) * wt) {
+    r.kvh = n_kv;
+    r.s = 0;
+    r.j = 0;
+    return r;
+  }
+  r.kvh = static_cast<int>(w / wt);
+  const int f = static_cast<int>(w - static_cast<long long>(r.kvh) * wt);
+  r.s = tree_find(wpref, num_seqs, f);
+  const int off = f - wpref[r.s];
+  const int tiles = (wpref[r.s + 1] - wpref[r.s] - kSegWeight) / kTileWeight;
+  r.j = off <= kSegWeight ? 0 : (off - kSegWeight + kTileWeight - 1) / kTileWeight;
+  if (whole && off > 0) r.j = tiles;
+  return r;
+}
+
+// Walks the segments (runs of tiles of one sequence and kv head) of a share.
+struct TreeWalk {
+  TreePos at;
+  int j1;  // tiles [at.j, j1) of the segment
+  int tiles;
+  bool valid;
+
+  __device__ __forceinline__ void settle(const int* wpref, int num_seqs, const TreePos& end) {
+    for (;;) {
+      if (at.kvh > end.kvh || (at.kvh == end.kvh && at.s > end.s)) break;
+      const bool last = at.kvh == end.kvh && at.s == end.s;
+      if (last && end.j <= at.j) break;
+      const int w = wpref[at.s + 1] - wpref[at.s];
+      if (w > 0) {
+        tiles = (w - kSegWeight) / kTileWeight;
+        j1 = last ? min(end.j, tiles) : tiles;
+        if (j1 > at.j) {
+          valid = true;
+          return;
+        }
+      }
+      if (++at.s == num_seqs) {
+        at.s = 0;
+        ++at.kvh;
+      }
+      at.j = 0;
+    }
+    valid = false;
+  }
+  __device__ __forceinline__ void start(const int* wpref, int num_seqs, const TreeShare& sh) {
+    at = sh.begin;
+    settle(wpref, num_seqs, sh.end);
+  }
+  __device__ __forceinline__ void next(const int* wpref, int num_seqs, const TreeShare& sh) {
+    if (++at.s == num_seqs) {
+      at.s = 0;
+      ++at.kvh;
+    }
+    at.j = 0;
+    settle(wpref, num_seqs, sh.end);
+  }
+};
+
+// The CTA (within its row tile index) that owns tile j of the segment.
+__device__ __forceinline__ int tree_owner(const int* wpref, int num_seqs, const TreeShare& sh,
+                                          int kvh, int s, int j) {
+  const long long w = static_cast<long long>(kvh) * wpref[num_seqs] + wpref[s] + kSegWeight +
+                      static_cast<long long>(j) * kTileWeight;
+  return static_cast<int>(w / sh.chunk);
+}
+
+// 64 visibility bits of a row for keys [t0, t0 + 64).
+__device__ __forceinline__ uint64_t tree_visible(const uint32_t* mrow, int words, int t0, int ctx,
+                                                 int n) {
+  const int lead = ctx - t0;  // keys below this are cached context
+  uint64_t vis = lead >= 64 ? ~0ull : (lead > 0 ? (1ull << lead) - 1 : 0ull);
+  if (lead < 64) {
+    const int sh = lead > 0 ? lead : 0;
+    const int bit = lead > 0 ? 0 : -lead;  // first draft of the tile
+    const int w = bit >> 5;
+    const uint32_t w0 = w < words ? mrow[w] : 0u;
+    const uint32_t w1 = w + 1 < words ? mrow[w + 1] : 0u;
+    const uint32_t w2 = w + 2 < words ? mrow[w + 2] : 0u;
+    const uint32_t lo = __funnelshift_r(w0, w1, bit & 31);
+    const uint32_t hi = __funnelshift_r(w1, w2, bit & 31);
+    vis |= ((static_cast<uint64_t>(hi) << 32) | lo) << sh;
+  }
+  const int left = n - t0;
+  if (left < 64) vis &= left > 0 ? (1ull << left) - 1 : 0ull;
+  return vis;
+}
+
+// Whether either 16-bit half is an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ bool nonfinite16(uint32_t half) {
+  const uint32_t e = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  return (half & e) == e;
+}
+
+// Sum of the non-finite values that the drafts t_begin .. t_end - 1 which a row
+// sees hold in column d: they were kept out of the MMA.  Only ever runs after
+// such a value was found.
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kTreeWarps) tree_kernel(const TreeParams p) {
-  __shared__ float s_q[kTreeWarps][D];
-  const int seq = blockIdx.z, r = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int head = blockIdx.x * kTreeWarps + warp;
-  const int q_len = p.q_lens[seq], row0 = p.cu_q[seq];
-  if (r >= q_len || head >= p.n_q) return;
-  if (row0 < 0 || static_cast<long long>(row0) + q_len > p.total_q || q_len > p.max_q_len) {
-    if (lane == 0) set_error(p.err, kDevErrQueryRange);
-    if (row0 < 0 || static_cast<long long>(row0) + q_len > p.total_q) return;
+__device__ __noinline__ float tree_nonfinite(const TreeParams& p, const uint32_t* mrow, int s,
+                                             int kvh, int ctx, int t_begin, int t_end, int d) {
+  float sum = 0.f;
+  for (int t = max(t_begin, ctx); t < t_end; ++t) {
+    const int j = t - ctx;
+    if ((j >> 5) >= p.mask_words || !((mrow[j >> 5] >> (j & 31)) & 1u)) continue;
+    const int b = p.block_tables[static_cast<size_t>(s) * p.max_blocks + t / kPage];
+    if (b < 0 || b >= p.num_blocks) continue;
+    const float x = Elt<T>::to_f(static_cast<const T*>(
+        p.pool)[(((static_cast<int64_t>(b) * 2 + 1) * kPage + t % kPage) * p.n_kv + kvh) * D + d]);
+    if (!(fabsf(x) <= 3.4e38f)) sum += x;
   }
-  const int row = row0 + r;
-  int n = p.seq_lens[seq];
-  if (n > p.max_blocks * kPage) {
-    if (lane == 0) set_error(p.err, kDevErrSeqLen);
-    n = p.max_blocks * kPage;
+  return sum;
+}
+
+__device__ __forceinline__ void tt_pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void tt_pdl_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+// Orders this thread's shared-memory writes before later reads by the async
+// proxy (MMA operands).
+__device__ __forceinline__ void tt_fence_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
+    paged_tree_kernel(const __grid_constant__ CUtensorMap kv_map,
+                      const __grid_constant__ CUtensorMap q_map,
+                      const __grid_constant__ TreeParams p) {
+  using Shape = TreeShape<D>;
+  constexpr int KEYS = kTtKeys;
+  // The swizzled tiles need 1024-byte alignment; the dynamic window is
+  // declared so, and a launch that did not get it reports it and does nothing.
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  if (smem_u32(smem_raw) & 1023u) {
+    if (threadIdx.x == 0) set_error(p.err, kDevErrTimeout);
+    return;
   }
-  const int ctx = min(max(p.ctx_lens[seq], 0), max(n, 0));
-  const T* q = static_cast<const T*>(p.q) + row * p.q_stride + static_cast<int64_t>(head) * D;
-  for (int d = lane; d < D; d += 32) s_q[warp][d] = Elt<T>::to_f(q[d]);
-  __syncwarp();
-  const T* pool = static_cast<const T*>(p.pool);
-  const int64_t tok = static_cast<int64_t>(p.n_kv) * D;
-  const int kvh = head / p.G;
-  float m = -INFINITY, l = 0.f, o[D / 32] = {};
-  for (int t0 = 0; t0 < n; t0 += 32) {
-    const int t = t0 + lane;
-    bool see = t < n;
-    if (see && t >= ctx) {
-      const int j = t - ctx;
-      see = (j >> 5) < p.mask_words &&
-            ((p.mask[static_cast<int64_t>(row) * p.mask_words + (j >> 5)] >> (j & 31)) & 1u);
+  uint8_t* sQ = smem_raw;
+  uint8_t* sK = sQ + Shape::kQBytes;
+  uint8_t* sV = sK + kTtStages * Shape::kTileBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kTtStages * Shape::kTileBytes);
+  uint64_t* q_full = bars + 0;
+  uint64_t* q_empty = bars + 1;  // the segment's last QK is done with Q
+  // [2]: MMA -> softmax, PV of a tile complete, by tile parity.  S of tile i in
+  // TMEM says that PV(i - 2) has completed but not PV(i - 1): with one barrier
+  // the parity of PV(i) could be taken for PV(i - 2)'s.
+  uint64_t* o_ready = bars + 2;
+  uint64_t* s_full = bars + 4;   // [2]: S in TMEM buffer (tile & 1)
+  uint64_t* p_full = bars + 6;   // [2]: softmax -> MMA, P in that buffer and O rescaled
+  uint64_t* mma_done = bars + 8; // everything issued has completed
+  uint64_t* k_full = bars + 9;
+  uint64_t* k_empty = k_full + kTtStages;
+  uint64_t* v_full = k_empty + kTtStages;
+  uint64_t* v_empty = v_full + kTtStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + kTtStages);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  // Segment number (+1) whose V held a non-finite draft, by segment parity.
+  volatile int* odd_seg = abort_flag + 1;  // [2]
+  TreeShare* share = reinterpret_cast<TreeShare*>(smem_raw + (reinterpret_cast<uint8_t*>(bars) - smem_raw) + 256);
+  int* rt_weight = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 512);
+  int* wpref = rt_weight + kTtMaxRowTiles;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int num_seqs = p.num_seqs;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(mma_done, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(o_ready + b, 1);
+      mbar_init(s_full + b, 1);
+      mbar_init(p_full + b, 4);
     }
-    int blk = -1;
-    if (see) {
-      blk = p.block_tables[static_cast<int64_t>(seq) * p.max_blocks + t / kPage];
-      if (blk < 0 || blk >= p.num_blocks) {
+    for (int st = 0; st < kTtStages; ++st) {
+      mbar_init(k_full + st, 1);
+      mbar_init(k_empty + st, 1);
+      mbar_init(v_full + st, 1);
+      mbar_init(v_empty + st, 1);
+    }
+    *abort_flag = 0;
+    odd_seg[0] = odd_seg[1] = 0;
+    fence_mbar_init();
+  }
+  if (warp == kTtMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(Shape::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (p.box_tokens * p.G < kTtRows) {
+    // Rows the Q loads never write: zeros, so their scores raise no maximum.
+    for (int i = threadIdx.x; i < Shape::kQBytes / 16; i += kTtThreads) {
+      reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    tt_fence_async();
+  }
+  if (lane == 0 && warp == kTtKWarp) prefetch_tmap(&q_map);
+  if (lane == 0 && warp == kTtVWarp) prefetch_tmap(&kv_map);
+  tt_pdl_wait();  // the lengths, q and the pool may come from the kernel before
+  tt_pdl_trigger();
+
+  // ── plan ───────────────────────────────────────────────────────────────────
+  for (int rt = warp; rt < p.row_tiles; rt += kTtThreads / 32) {
+    int sum = 0;
+    for (int s = lane; s < num_seqs; s += 32) {
+      const bool report = blockIdx.x == 0 && rt == 0;
+      sum += tree_weight(tree_seq(p, s, report), rt * p.tokens_per_tile);
+    }
+    for (int sh = 16; sh; sh >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
+    if (lane == 0) rt_weight[rt] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    long long total = 0;
+    int used = 0;  // row tile indices with work: the first ones
+    for (int rt = 0; rt < p.row_tiles && rt_weight[rt] > 0; ++rt, ++used) {
+      total += static_cast<long long>(rt_weight[rt]) * p.n_kv;
+    }
+    // Row tile indices start on a CTA of their own, which can leave up to
+    // used - 1 shares partly empty.
+    const int div = p.n_cta - (used > 0 ? used - 1 : 0);
+    long long chunk = (total + div - 1) / div;
+    const long long least = kMinTiles * kTileWeight + kSegWeight;
+    if (chunk < least) chunk = least;
+    int first = 0, rt = 0;
+    for (; rt < used; ++rt) {
+      const long long w = static_cast<long long>(rt_weight[rt]) * p.n_kv;
+      const int n = static_cast<int>((w + chunk - 1) / chunk);
+      if (static_cast<int>(blockIdx.x) < first + n) break;
+      first += n;
+    }
+    share->rt = rt < used ? rt : -1;
+    share->first_cta = first;
+    share->chunk = static_cast<int>(chunk);
+  }
+  __syncthreads();
+  const int rt = share->rt;
+  const int tok0 = rt * p.tokens_per_tile;
+  if (warp == 0) {
+    int carry = 0;
+    if (lane == 0) wpref[0] = 0;
+    for (int base = 0; base < num_seqs; base += 32) {
+      const int s = base + lane;
+      int v = rt >= 0 && s < num_seqs ? tree_weight(tree_seq(p, s, false), tok0) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += y;
+      }
+      if (s < num_seqs) wpref[s + 1] = v + carry;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+    __syncwarp();
+    if (lane == 0) {
+      TreePos b, e;
+      if (rt >= 0) {
+        const long long w0 = static_cast<long long>(blockIdx.x - share->first_cta) * share->chunk;
+        b = tree_pos(wpref, num_seqs, p.n_kv, p.whole, w0);
+        e = tree_pos(wpref, num_seqs, p.n_kv, p.whole, w0 + share->chunk);
+      } else {
+        b.kvh = e.kvh = 0;
+        b.s = e.s = 0;
+        b.j = e.j = 0;
+      }
+      share->begin = b;
+      share->end = e;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const TreeShare sh = *share;
+
+  if (warp == kTtKWarp || warp == kTtVWarp) {
+    // ── loads: one warp streams K tiles (and Q), another V tiles ──────────────
+    const bool is_v = warp == kTtVWarp;
+    const int oob = 2 * p.num_blocks;  // past the pool: the TMA fills zeros
+    uint64_t* full = is_v ? v_full : k_full;
+    uint64_t* empty = is_v ? v_empty : k_empty;
+    uint8_t* ring = is_v ? sV : sK;
+    auto fetch = [&](int s, int n_pages, int page) -> int {  // block id of `page`, or -1
+      if (page >= n_pages) return -1;
+      const int b = p.block_tables[static_cast<size_t>(s) * p.max_blocks + page];
+      if (b < 0 || b >= p.num_blocks) {
         set_error(p.err, kDevErrBlockRange);
-        blk = -1;
+        return -1;
+      }
+      return b;
+    };
+    TreeWalk w;
+    w.start(wpref, num_seqs, sh);
+    int it = 0, seg = 0;
+    bool go = true;
+    int first_ids = -1;  // this lane's page of the segment's first 32
+    TreeSeq q = {};
+    if (w.valid) {
+      q = tree_seq(p, w.at.s, false);
+      first_ids = fetch(w.at.s, (q.n + kPage - 1) / kPage, w.at.j * kTtPages + lane);
+    }
+    while (w.valid && go) {
+      const int s = w.at.s, kvh = w.at.kvh, j0 = w.at.j, j1 = w.j1;
+      const int n_pages = (q.n + kPage - 1) / kPage;
+      const int page_begin = j0 * kTtPages;
+      int ids = first_ids;
+      int nxt = fetch(s, n_pages, page_begin + 32 + lane);
+      if (!is_v && lane == 0) {
+        if (seg > 0 && (!mbar_wait(q_empty, (seg - 1) & 1, p.err) || aborted(abort_flag))) {
+          *abort_flag = 1;
+          go = false;
+        } else {
+          mbar_arrive_expect_tx(q_full, Shape::kChunks * p.box_tokens * p.G * 128);
+#pragma unroll
+          for (int c = 0; c < Shape::kChunks; ++c) {
+            tma_load_3d(sQ + c * kTtQChunk, &q_map, q_full, c * 64, kvh * p.G, q.row0 + tok0);
+          }
+        }
+      }
+      go = __shfl_sync(0xffffffffu, go ? 1 : 0, 0);
+      if (!go) break;
+      ++seg;
+      // The next segment's lengths and first block ids, long before they are needed.
+      w.next(wpref, num_seqs, sh);
+      if (w.valid) {
+        q = tree_seq(p, w.at.s, false);
+        first_ids = fetch(w.at.s, (q.n + kPage - 1) / kPage, w.at.j * kTtPages + lane);
+      }
+      for (int j = j0; j < j1; ++j, ++it) {
+        const int page0 = (j - j0) * kTtPages;  // within the segment
+        if (page0 > 0 && (page0 & 31) == 0) {
+          ids = nxt;
+          nxt = fetch(s, n_pages, page_begin + page0 + 32 + lane);
+        }
+        int blk[kTtPages];
+#pragma unroll
+        for (int pg = 0; pg < kTtPages; ++pg) {
+          blk[pg] = __shfl_sync(0xffffffffu, ids, (page0 + pg) & 31);
+        }
+        if (lane == 0) {
+          const int st = it % kTtStages;
+          if (it >= kTtStages &&
+              (!mbar_wait(empty + st, ((it / kTtStages) - 1) & 1, p.err) || aborted(abort_flag))) {
+            *abort_flag = 1;
+            go = false;
+          } else {
+            mbar_arrive_expect_tx(full + st, Shape::kTileBytes);
+#pragma unroll
+            for (int pg = 0; pg < kTtPages; ++pg) {
+              const int coord = blk[pg] < 0 ? oob : 2 * blk[pg] + (is_v ? 1 : 0);
+#pragma unroll
+              for (int c = 0; c < Shape::kChunks; ++c) {
+                tma_load_4d(ring + st * Shape::kTileBytes + c * kTtKChunk + pg * 2048, &kv_map,
+                            full + st, c * 64, 0, kvh, coord);
+              }
+            }
+          }
+        }
+        go = __shfl_sync(0xffffffffu, go ? 1 : 0, 0);
+        if (!go) break;
       }
     }
-    float s = -INFINITY;
-    const int64_t at = ((static_cast<int64_t>(blk) * 2) * kPage + t % kPage) * tok + kvh * D;
-    if (see) {
-      s = 0.f;
-      if (blk >= 0) {
-        for (int d = 0; d < D; ++d) s += s_q[warp][d] * Elt<T>::to_f(pool[at + d]);
+    // Whatever happened, this warp's own loads land before the shared memory
+    // is released.
+    if (lane == 0) {
+      if (!is_v && seg > 0) mbar_wait(q_full, (seg - 1) & 1, p.err);
+      for (int i = max(0, it - kTtStages); i < it; ++i) {
+        mbar_wait(full + (i % kTtStages), (i / kTtStages) & 1, p.err);
       }
-      s *= p.scale_log2;
     }
-    float mx = s;
-    for (int sh = 16; sh; sh >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
-    const float mn = fmaxf(m, mx);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float al = exp2f(m - base);
-    const float e = see ? exp2f(s - base) : 0.f;
-    m = mn;
-    l = l * al + e;
-    for (int i = 0; i < D / 32; ++i) o[i] *= al;
-    unsigned todo = __ballot_sync(0xffffffffu, see && blk >= 0);
-    while (todo) {
-      const int j = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const float pj = __shfl_sync(0xffffffffu, e, j);
-      const int64_t vat = __shfl_sync(0xffffffffu, at, j) + kPage * tok;
-      for (int i = 0; i < D / 32; ++i) o[i] += pj * Elt<T>::to_f(pool[vat + i * 32 + lane]);
+  } else if (warp == kTtMmaWarp) {
+    // ── MMA issue: QK(0), QK(1), then per tile i: PV(i) after its softmax,
+    // QK(i + 2) into the S buffer PV(i) just read P from (the MMAs of one
+    // thread execute in issue order).  Tiles are numbered through all segments.
+    if (lane == 0) {
+      const uint32_t t_o = tmem_base + 2 * KEYS;
+      const uint32_t idesc_qk = f16_idesc<T>(KEYS, false);
+      const uint32_t idesc_pv = f16_idesc<T>(D, true);
+      const uint32_t q_addr = smem_u32(sQ);
+      TreeWalk wq, wp;  // the next QK's segment, the next PV's segment
+      wq.start(wpref, num_seqs, sh);
+      wp = wq;
+      int jq = wq.at.j, jp = wp.at.j, seg_q = 0, iq = 0, ip = 0;
+      bool ok = true;
+      auto issue_qk = [&]() -> bool {  // one tile, if any is left
+        if (!wq.valid) return true;
+        const int st = iq % kTtStages;
+        if (jq == wq.at.j && !mbar_wait(q_full, seg_q & 1, p.err)) return false;
+        if (!mbar_wait(k_full + st, (iq / kTtStages) & 1, p.err) || aborted(abort_flag)) return false;
+        tc_fence_after();
+        const uint32_t k_addr = smem_u32(sK + st * Shape::kTileBytes);
+        const uint32_t t_s = tmem_base + (iq & 1) * KEYS;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t a = sw128_desc(q_addr + (k >> 2) * kTtQChunk + (k & 3) * 32, 16, 1024);
+          const uint64_t b = sw128_desc(k_addr + (k >> 2) * kTtKChunk + (k & 3) * 32, 16, 1024);
+          tc_mma(t_s, a, b, idesc_qk, k > 0 ? 1u : 0u);
+        }
+        tc_commit(k_empty + st);
+        tc_commit(s_full + (iq & 1));
+        ++iq;
+        if (++jq == wq.j1) {
+          tc_commit(q_empty);
+          wq.next(wpref, num_seqs, sh);
+          jq = wq.at.j;
+          ++seg_q;
+        }
+        return true;
+      };
+      ok = issue_qk() && issue_qk();
+      while (ok && wp.valid) {
+        const int st = ip % kTtStages;
+        if (!mbar_wait(p_full + (ip & 1), (ip >> 1) & 1, p.err) || aborted(abort_flag) ||
+            !mbar_wait(v_full + st, (ip / kTtStages) & 1, p.err) || aborted(abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t v_addr = smem_u32(sV + st * Shape::kTileBytes);
+        const uint32_t t_p = tmem_base + (ip & 1) * KEYS;
+        const bool first = jp == wp.at.j;  // a segment's first PV overwrites O
+#pragma unroll
+        for (int k = 0; k < KEYS / 16; ++k) {
+          const uint64_t b = sw128_desc(v_addr + k * 2048, kTtKChunk, 1024);
+          tc_mma_ts(t_o, t_p + k * 8, b, idesc_pv, (!first || k > 0) ? 1u : 0u);
+        }
+        tc_commit(v_empty + st);
+        tc_commit(o_ready + (ip & 1));
+        ++ip;
+        if (++jp == wp.j1) {
+          wp.next(wpref, num_seqs, sh);
+          jp = wp.at.j;
+        }
+        ok = issue_qk();
+      }
+      if (!ok) *abort_flag = 1;
+      // Every MMA this lane issued completes before the TMEM is freed.
+      tc_commit(mma_done);
+      mbar_wait(mma_done, 0, p.err);
+    }
+  } else {
+    // ── softmax and epilogue: one row per thread ─────────────────────────────
+    const int m = threadIdx.x;  // row = TMEM lane
+    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t t_o = tmem_base + lane_base + 2 * KEYS;
+    const int t_row = m / p.G;  // drafted token of the row tile
+    const int head_in_group = m - t_row * p.G;
+    const float scale = p.scale_log2;
+    bool ok = true;
+    int it = 0, seg = 0;
+    TreeWalk w;
+    w.start(wpref, num_seqs, sh);
+    // A sequence that began in the CTA before this one and continues here:
+    // this CTA describes the join of its pieces (it is the second of them).
+    int rec[6] = {-1, 0, 0, 0, 0, 0};
+    while (w.valid && ok) {
+      const int s = w.at.s, kvh = w.at.kvh, j0 = w.at.j, j1 = w.j1, tiles = w.tiles;
+      const TreeSeq q = tree_seq(p, s, false);
+      const int rows = min(p.tokens_per_tile, q.q_len - tok0) * p.G;
+      const bool active = warp * 32 < rows;  // warp-uniform
+      const bool valid = m < rows;
+      const int row = q.row0 + tok0 + (valid ? t_row : 0);
+      const uint32_t* mrow = p.mask + static_cast<size_t>(row) * p.mask_words;
+      float m_run = -INFINITY;
+      float l_run = 0.f;
+      for (int j = j0; j < j1; ++j, ++it) {
+        ok = mbar_wait(s_full + (it & 1), (it >> 1) & 1, p.err);
+        ok = __all_sync(0xffffffffu, ok) && !aborted(abort_flag);
+        if (!ok) break;
+        const int key0 = j * KEYS;
+        const bool tail = key0 + KEYS > q.ctx;  // reaches drafts or the end
+        if (tail) {
+          // Clean V: every warp takes its share of the tile's 128-byte lines.
+          const int st = it % kTtStages;
+          ok = mbar_wait(v_full + st, (it / kTtStages) & 1, p.err);
+          ok = __all_sync(0xffffffffu, ok) && !aborted(abort_flag);
+          if (!ok) break;
+          if (m < Shape::kChunks * KEYS) {
+            const int t = key0 + (m & (KEYS - 1));
+            uint4* line = reinterpret_cast<uint4*>(sV + st * Shape::kTileBytes + m * 128);
+            if (t >= q.n) {
+#pragma unroll
+              for (int u = 0; u < 8; ++u) line[u ^ (lane & 7)] = make_uint4(0u, 0u, 0u, 0u);
+            } else if (t >= q.ctx) {
+              bool found = false;
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                uint4 x = line[u ^ (lane & 7)];
+                uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  if (nonfinite16<T>(xs[i] & 0xffffu)) { xs[i] &= 0xffff0000u; odd = true; }
+                  if (nonfinite16<T>(xs[i] >> 16)) { xs[i] &= 0x0000ffffu; odd = true; }
+                }
+                if (odd) {
+                  line[u ^ (lane & 7)] = x;
+                  found = true;
+                }
+              }
+              if (found) odd_seg[seg & 1] = seg + 1;
+            }
+          }
+          tt_fence_async();
+        }
+        if (active) {
+          tc_fence_after();
+          const uint32_t t_s = tmem_base + lane_base + (it & 1) * KEYS;
+          uint32_t sc[KEYS / 16][16];
+#pragma unroll
+          for (int c = 0; c < KEYS / 16; ++c) tmem_ld16(t_s + c * 16, sc[c]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < KEYS / 16; ++c) tmem_ld_fence_regs(sc[c]);
+          if (tail) {
+            const uint64_t vis = valid ? tree_visible(mrow, p.mask_words, key0, q.ctx, q.n) : 0ull;
+            const uint32_t v0 = static_cast<uint32_t>(vis), v1 = static_cast<uint32_t>(vis >> 32);
+#pragma unroll
+            for (int c = 0; c < KEYS / 16; ++c) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int bit = (c & 1) * 16 + i;
+                if (!(((c < 2 ? v0 : v1) >> bit) & 1u)) sc[c][i] = __float_as_uint(-INFINITY);
+              }
+            }
+          }
+          // The maximum is taken on raw scores (the scale is positive) in four
+          // independent chains; the scale is folded into the exponent.
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < KEYS / 16; ++c) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              mx4[i & 3] = fmax3(mx4[i & 3], __uint_as_float(sc[c][2 * i]),
+                                 __uint_as_float(sc[c][2 * i + 1]));
+            }
+          }
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
+          const float m_new = fmaxf(m_run, mx);
+          if (j == j0) {
+            m_run = m_new;
+          } else if (__any_sync(0xffffffffu, m_new > m_run + 8.f)) {
+            // The running maximum only has to bound the scores to within 2^8:
+            // O is rescaled (once the PV before has landed) when it grew by more.
+            ok = mbar_wait(o_ready + ((it - 1) & 1), ((it - 1) >> 1) & 1, p.err);
+            ok = __all_sync(0xffffffffu, ok) && !aborted(abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            // -inf - -inf: a row that has seen nothing yet keeps its zeros.
+            const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(t_o + c * 16, o);
+              tmem_ld_wait();
+              tmem_ld_fence_regs(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st16(t_o + c * 16, o);
+            }
+            l_run *= alpha;
+            m_run = m_new;
+          }
+          uint32_t pk[KEYS / 32][16];
+          uint64_t acc2[2] = {0ull, 0ull};
+          const float base = m_run == -INFINITY ? 0.f : m_run;
+          const uint64_t scale2 = f2_make(scale, scale);
+          const uint64_t neg_m2 = f2_make(-base, -base);
+#pragma unroll
+          for (int c = 0; c < KEYS / 16; ++c) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float a, b;
+              f2_split(f2_fma(f2_make(__uint_as_float(sc[c][2 * i]),
+                                      __uint_as_float(sc[c][2 * i + 1])),
+                              scale2, neg_m2),
+                       a, b);
+              a = fast_exp2(a);
+              b = fast_exp2(b);
+              acc2[i & 1] = f2_add(acc2[i & 1], f2_make(a, b));
+              pk[c >> 1][(c & 1) * 8 + i] = Elt<T>::pack(a, b);
+            }
+          }
+          float s0, s1, s2, s3;
+          f2_split(acc2[0], s0, s1);
+          f2_split(acc2[1], s2, s3);
+#pragma unroll
+          for (int c = 0; c < KEYS / 32; ++c) tmem_st16(t_s + c * 16, pk[c]);
+          tmem_st_wait();
+          l_run += (s0 + s1) + (s2 + s3);
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + (it & 1));
+      }
+      if (!ok) break;
+      // ── the segment's result ──────────────────────────────────────────────
+      const bool complete = j0 == 0 && j1 == tiles;
+      int slot = 0;
+      if (!complete) {
+        const int c0 = tree_owner(wpref, num_seqs, sh, kvh, s, 0) + sh.first_cta;
+        slot = c0 == static_cast<int>(blockIdx.x) ? 1 : 0;
+        if (c0 + 1 == static_cast<int>(blockIdx.x)) {
+          rec[0] = s;
+          rec[1] = kvh;
+          rec[2] = tok0;
+          rec[3] = c0;
+          rec[4] = tree_owner(wpref, num_seqs, sh, kvh, s, tiles - 1) + sh.first_cta;
+          rec[5] = rows;
+        }
+      }
+      if (active) {
+        ok = mbar_wait(o_ready + ((it - 1) & 1), ((it - 1) >> 1) & 1, p.err);
+        ok = __all_sync(0xffffffffu, ok) && !aborted(abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const bool odd = odd_seg[seg & 1] == seg + 1;
+        // A row that saw nothing has l = 0 and O = 0.
+        const float inv_l = l_run == 0.f ? 0.f : 1.f / l_run;
+        const size_t piece = static_cast<size_t>(blockIdx.x) * 2 + slot;
+        T* orow = static_cast<T*>(p.out) +
+                  (static_cast<size_t>(row) * p.n_q + kvh * p.G + head_in_group) * D;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld16(t_o + c * 16, o);
+          tmem_ld_wait();
+          tmem_ld_fence_regs(o);
+          float f[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]);
+          if (odd && valid) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              f[i] += tree_nonfinite<T, D>(p, mrow, s, kvh, q.ctx, j0 * KEYS, min(j1 * KEYS, q.n),
+                                           c * 16 + i);
+            }
+          }
+          if (complete) {
+            uint32_t packed[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) packed[i] = Elt<T>::pack(f[2 * i] * inv_l, f[2 * i + 1] * inv_l);
+            if (valid) {
+              uint4* dst = reinterpret_cast<uint4*>(orow + c * 16);
+              dst[0] = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+              dst[1] = make_uint4(packed[4], packed[5], packed[6], packed[7]);
+            }
+          } else {
+            // Column-quad major, so that a warp's 32 rows are adjacent.
+            float4* dst = p.part_o + (piece * (D / 4) + c * 4) * p.part_rows + m;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              dst[static_cast<size_t>(i) * p.part_rows] =
+                  make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+            }
+          }
+        }
+        if (!complete) p.part_ml[piece * p.part_rows + m] = make_float2(m_run, l_run);
+        tc_fence_before();
+      }
+      ++seg;
+      w.next(wpref, num_seqs, sh);
+    }
+    if (!ok) *abort_flag = 1;
+    if (threadIdx.x == 0 && !p.whole) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) p.records[blockIdx.x * 8 + i] = rec[i];
     }
   }
-  for (int sh = 16; sh; sh >>= 1) l += __shfl_xor_sync(0xffffffffu, l, sh);
-  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-  T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(row) * p.n_q + head) * D;
-  for (int i = 0; i < D / 32; ++i) out[i * 32 + lane] = Elt<T>::from_f(o[i] * inv);
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kTtMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                 "r"(Shape::kTmemCols)
+                 : "memory");
+  }
+}
+
+// Joins the pieces of cut sequences.  A unit is 32 rows x 16 columns of one of
+// them; the block's warps take its pieces in turn and their partial results
+// are joined through shared memory, all in a fixed order.
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeThreads) paged_tree_merge_kernel(const __grid_constant__ TreeParams p) {
+  constexpr int kWarps = kMergeThreads / 32;
+  constexpr int kQuads = kMergeCols / 4;
+  constexpr int kColUnits = D / kMergeCols;
+  __shared__ int s_item[1024];  // CTAs whose record is a join, in order
+  __shared__ int s_base[kWarps + 1];
+  __shared__ float s_ml[kWarps][32][2];
+  __shared__ float4 s_o[kWarps][kQuads][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  tt_pdl_wait();
+  int n_items = 0;
+  for (int base = 0; base < p.n_cta; base += kMergeThreads) {
+    const int b = base + threadIdx.x;
+    const bool on = b < p.n_cta && p.records[b * 8] >= 0;
+    const unsigned mask = __ballot_sync(0xffffffffu, on);
+    if (lane == 0) s_base[warp + 1] = __popc(mask);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      s_base[0] = n_items;
+      for (int i = 0; i < kWarps; ++i) s_base[i + 1] += s_base[i];
+    }
+    __syncthreads();
+    if (on) s_item[s_base[warp] + __popc(mask & ((1u << lane) - 1))] = b;
+    n_items = s_base[kWarps];
+    __syncthreads();
+  }
+  const int row_units = p.part_rows / 32;
+  const int units = n_items * row_units * kColUnits;
+  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int item = unit / (row_units * kColUnits);
+    const int rest = unit - item * (row_units * kColUnits);
+    const int ru = rest / kColUnits, cu = rest - ru * kColUnits;
+    const int* rec = p.records + s_item[item] * 8;
+    const int s = rec[0], kvh = rec[1], tok0 = rec[2], c0 = rec[3], c1 = rec[4], rows = rec[5];
+    if (ru * 32 >= rows) continue;
+    const int row = ru * 32 + lane;
+    float m_run = -INFINITY, l_run = 0.f;
+    float4 o[kQuads];
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto fold = [&](float m2, float l2, const float4* v) {
+      const float mn = fmaxf(m_run, m2);
+      const float base = mn == -INFINITY ? 0.f : mn;
+      const float a = fast_exp2(m_run - base), b = fast_exp2(m2 - base);
+      l_run = l_run * a + l2 * b;
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i) {
+        o[i].x = o[i].x * a + v[i].x * b;
+        o[i].y = o[i].y * a + v[i].y * b;
+        o[i].z = o[i].z * a + v[i].z * b;
+        o[i].w = o[i].w * a + v[i].w * b;
+      }
+      m_run = mn;
+    };
+#pragma unroll 2
+    for (int c = c0 + warp; c <= c1; c += kWarps) {
+      const size_t piece = static_cast<size_t>(c) * 2 + (c == c0 ? 1 : 0);
+      const float2 ml = __ldcg(p.part_ml + piece * p.part_rows + row);
+      const float4* src = p.part_o + (piece * (D / 4) + cu * kQuads) * p.part_rows + row;
+      float4 v[kQuads];
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i) v[i] = __ldcg(src + static_cast<size_t>(i) * p.part_rows);
+      fold(ml.x, ml.y, v);
+    }
+    s_ml[warp][lane][0] = m_run;
+    s_ml[warp][lane][1] = l_run;
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) s_o[warp][i][lane] = o[i];
+    __syncthreads();
+    if (warp == 0) {
+      for (int x = 1; x < kWarps; ++x) {
+        float4 v[kQuads];
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) v[i] = s_o[x][i][lane];
+        fold(s_ml[x][lane][0], s_ml[x][lane][1], v);
+      }
+      if (row < rows) {
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        const int token = row / p.G;
+        T* dst = static_cast<T*>(p.out) +
+                 (static_cast<size_t>(p.cu_q[s] + tok0 + token) * p.n_q + kvh * p.G + row - token * p.G) * D +
+                 cu * kMergeCols;
+        uint32_t packed[2 * kQuads];
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+          packed[2 * i] = Elt<T>::pack(o[i].x * inv, o[i].y * inv);
+          packed[2 * i + 1] = Elt<T>::pack(o[i].z * inv, o[i].w * inv);
+        }
+        uint4* d4 = reinterpret_cast<uint4*>(dst);
+        d4[0] = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+        d4[1] = make_uint4(packed[4], packed[5], packed[6], packed[7]);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ── host side ────────────────────────────────────────────────────────────────
+
+bool tree_shape_ok(int n_q, int n_kv, int D) {
+  return (D == 64 || D == 128) && n_kv > 0 && n_kv <= 64 && n_q > 0 && n_q % n_kv == 0 &&
+         n_q / n_kv <= 16;
+}
+
+struct TreeLayout {
+  int part_rows;
+  size_t records, ml, o, total;
+};
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+TreeLayout tree_layout(int max_q_len, int n_q, int n_kv, int D, int n_cta) {
+  const int G = n_q / n_kv;
+  const int tpt = kTtRows / G;
+  const int tokens = max_q_len < tpt ? (max_q_len > 0 ? max_q_len : 1) : tpt;
+  TreeLayout l;
+  l.part_rows = (tokens * G + 31) / 32 * 32;
+  l.records = 0;
+  l.ml = align256(static_cast<size_t>(n_cta) * 8 * sizeof(int));
+  l.o = l.ml + align256(static_cast<size_t>(n_cta) * 2 * l.part_rows * sizeof(float2));
+  l.total = l.o + align256(static_cast<size_t>(n_cta) * 2 * l.part_rows * D * sizeof(float));
+  return l;
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t tree_launch(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t s,
+                        Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+template <typename T, int D>
+int launch_tree(const CUtensorMap& kv_map, const CUtensorMap& q_map, const TreeParams& p, int sms,
+                cudaStream_t s) {
+  using Shape = TreeShape<D>;
+  static std::once_flag flags[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return fail(VMPS_ERR_CUDA, "device index %d", dev);
+  std::call_once(flags[dev], [] {
+    cudaFuncSetAttribute(paged_tree_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         Shape::kFixedBytes + (kTtMaxSeqs + 1) * static_cast<int>(sizeof(int)));
+  });
+  const size_t smem = Shape::kFixedBytes + static_cast<size_t>(p.num_seqs + 1) * sizeof(int);
+  cudaError_t e = tree_launch(paged_tree_kernel<T, D>, p.n_cta, kTtThreads, smem, s, kv_map, q_map, p);
+  if (e == cudaSuccess && !p.whole) {
+    e = tree_launch(paged_tree_merge_kernel<T, D>, 2 * sms, kMergeThreads, 0, s, p);
+  }
+  if (e != cudaSuccess) {
+    return fail(VMPS_ERR_CUDA, "paged_tree_attention: launch failed: %s", cudaGetErrorString(e));
+  }
+  return VMPS_OK;
 }
 
 }  // namespace
@@ -117,8 +1028,14 @@ using namespace vmps;
 
 extern "C" size_t vmps_paged_tree_attention_workspace_bytes(int num_seqs, int max_q_len, int n_q,
                                                             int n_kv, int head_dim, int dtype) {
-  (void)num_seqs, (void)max_q_len, (void)n_q, (void)n_kv, (void)head_dim, (void)dtype;
-  return 256;
+  if (num_seqs < 0 || max_q_len < 0 || max_q_len > kTtMaxQLen ||
+      (dtype != VMPS_DTYPE_F16 && dtype != VMPS_DTYPE_BF16) ||
+      !tree_shape_ok(n_q, n_kv, head_dim)) {
+    return 0;
+  }
+  int sms = 0;
+  if (device_sm_count(&sms)) return 0;
+  return tree_layout(max_q_len, n_q, n_kv, head_dim, sms * kTtCtasPerSm).total;
 }
 
 extern "C" int vmps_paged_tree_attention(
@@ -143,16 +1060,20 @@ extern "C" int vmps_paged_tree_attention(
   if (block_size != kPage) {
     return fail(VMPS_ERR_UNSUPPORTED, "%s: block_size %d (only 16 is built)", what, block_size);
   }
-  if ((head_dim != 64 && head_dim != 128) || n_kv <= 0 || n_kv > 64 || n_q <= 0 || n_q % n_kv ||
-      n_q / n_kv > 16) {
+  if (!tree_shape_ok(n_q, n_kv, head_dim)) {
     return fail(VMPS_ERR_UNSUPPORTED,
                 "%s: n_q=%d n_kv=%d head_dim=%d not supported (head_dim 64/128, n_kv <= 64, "
                 "n_q/n_kv a whole number up to 16)",
                 what, n_q, n_kv, head_dim);
   }
-  if (num_seqs > 4096 || max_q_len > 65535 || max_blocks_per_seq > (1 << 26)) {
-    return fail(VMPS_ERR_UNSUPPORTED, "%s: num_seqs %d > 4096, max_q_len %d > 65535 or max_blocks %d",
-                what, num_seqs, max_q_len, max_blocks_per_seq);
+  // The plan sums a row tile's tiles over all sequences in 31 bits.
+  const long long max_tiles = (static_cast<long long>(max_blocks_per_seq) + kTtPages - 1) / kTtPages;
+  if (num_seqs > kTtMaxSeqs || max_q_len > kTtMaxQLen || max_blocks_per_seq > (1 << 26) ||
+      num_seqs * (max_tiles * kTileWeight + kSegWeight) > 0x7fffffffLL) {
+    return fail(VMPS_ERR_UNSUPPORTED,
+                "%s: num_seqs=%d max_q_len=%d max_blocks=%d (num_seqs <= %d, max_q_len <= %d, "
+                "num_seqs * max_blocks < 2^31)",
+                what, num_seqs, max_q_len, max_blocks_per_seq, kTtMaxSeqs, kTtMaxQLen);
   }
   if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return VMPS_OK;
   if (!out || !q || !pool || !block_tables || !ctx_lens || !seq_lens || !q_lens || !cu_q ||
@@ -171,15 +1092,54 @@ extern "C" int vmps_paged_tree_attention(
   if (!(scale > 0.f) || !(scale < 1e30f)) {
     return fail(VMPS_ERR_INVALID_ARG, "%s: scale %g", what, (double)scale);
   }
-  if (!workspace || workspace_bytes < 256) {
-    return fail(VMPS_ERR_WORKSPACE, "%s: workspace %zu bytes < %d needed", what, workspace_bytes, 256);
+  int sms = 0;
+  if (int rc = device_sm_count(&sms)) return rc;
+  TreeParams p;
+  p.n_cta = sms * kTtCtasPerSm;
+  if (p.n_cta > 1024) return fail(VMPS_ERR_UNSUPPORTED, "%s: %d SMs", what, sms);
+  const TreeLayout wl = tree_layout(max_q_len, n_q, n_kv, head_dim, p.n_cta);
+  if (!workspace || workspace_bytes < wl.total) {
+    return fail(VMPS_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu needed", what, workspace_bytes,
+                wl.total);
+  }
+  if (reinterpret_cast<uintptr_t>(workspace) & 255) {
+    return fail(VMPS_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", what);
   }
   int* err = nullptr;
   if (int rc = device_error_word(&err)) return rc;
-  TreeParams p;
+
+  const CUtensorMapDataType tdt =
+      dtype == VMPS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t e = 2;
+  const int G = n_q / n_kv;
+  // Pool as {d, token, kv head, (block, K|V)}: a box [64][16][1][1] is one
+  // page of one head, 16 rows of 128 bytes.
+  CUtensorMap kv_map;
+  {
+    const uint64_t dims[4] = {(uint64_t)head_dim, kPage, (uint64_t)n_kv, (uint64_t)2 * num_blocks};
+    const uint64_t strides[3] = {(uint64_t)n_kv * head_dim * e, (uint64_t)head_dim * e,
+                                 (uint64_t)kPage * n_kv * head_dim * e};
+    const uint32_t box[4] = {64, kPage, 1, 1};
+    if (int rc = encode_tiled(&kv_map, tdt, 4, const_cast<void*>(pool), dims, strides, box,
+                              CU_TENSOR_MAP_SWIZZLE_128B)) {
+      return rc;
+    }
+  }
+  // Queries as {d, head, row}: a box [64][G][tokens] is the rows (token-major,
+  // head-minor) of one 64-column chunk of a row tile.
+  p.tokens_per_tile = kTtRows / G;
+  p.box_tokens = max_q_len < p.tokens_per_tile ? max_q_len : p.tokens_per_tile;
+  CUtensorMap q_map;
+  {
+    const uint64_t dims[3] = {(uint64_t)head_dim, (uint64_t)n_q, (uint64_t)total_q};
+    const uint64_t strides[2] = {(uint64_t)head_dim * e, (uint64_t)q_row_stride * e};
+    const uint32_t box[3] = {64, (uint32_t)G, (uint32_t)p.box_tokens};
+    if (int rc = encode_tiled(&q_map, tdt, 3, const_cast<void*>(q), dims, strides, box,
+                              CU_TENSOR_MAP_SWIZZLE_128B)) {
+      return rc;
+    }
+  }
   p.out = out;
-  p.q = q;
-  p.q_stride = q_row_stride;
   p.pool = pool;
   p.block_tables = block_tables;
   p.ctx_lens = ctx_lens;
@@ -189,23 +1149,27 @@ extern "C" int vmps_paged_tree_attention(
   p.mask = reinterpret_cast<const uint32_t*>(tree_mask);
   p.mask_words = mask_words;
   p.max_blocks = max_blocks_per_seq;
+  p.num_seqs = num_seqs;
   p.total_q = total_q;
   p.max_q_len = max_q_len;
   p.n_q = n_q;
   p.n_kv = n_kv;
-  p.G = n_q / n_kv;
+  p.G = G;
   p.num_blocks = num_blocks;
+  p.row_tiles = (max_q_len + p.tokens_per_tile - 1) / p.tokens_per_tile;
+  p.whole = max_tiles <= kWholeTiles ? 1 : 0;
+  p.part_rows = wl.part_rows;
   p.scale_log2 = scale * 1.4426950408889634f;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.records = reinterpret_cast<int*>(ws + wl.records);
+  p.part_ml = reinterpret_cast<float2*>(ws + wl.ml);
+  p.part_o = reinterpret_cast<float4*>(ws + wl.o);
   p.err = err;
-  const dim3 grid((n_q + kTreeWarps - 1) / kTreeWarps, max_q_len, num_seqs);
-  const dim3 block(32 * kTreeWarps);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == VMPS_DTYPE_F16) {
-    if (head_dim == 64) tree_kernel<__half, 64><<<grid, block, 0, s>>>(p);
-    else tree_kernel<__half, 128><<<grid, block, 0, s>>>(p);
-  } else {
-    if (head_dim == 64) tree_kernel<__nv_bfloat16, 64><<<grid, block, 0, s>>>(p);
-    else tree_kernel<__nv_bfloat16, 128><<<grid, block, 0, s>>>(p);
+    return head_dim == 64 ? launch_tree<__half, 64>(kv_map, q_map, p, sms, s)
+                          : launch_tree<__half, 128>(kv_map, q_map, p, sms, s);
   }
-  return check_launch(what);
+  return head_dim == 64 ? launch_tree<__nv_bfloat16, 64>(kv_map, q_map, p, sms, s)
+                        : launch_tree<__nv_bfloat16, 128>(kv_map, q_map, p, sms, s);
 }
