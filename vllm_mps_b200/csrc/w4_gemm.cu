@@ -29,7 +29,7 @@
 // memory would otherwise be the bound) over all of K belongs to one CTA;
 // contiguous equal shares of blocks go to one persistent CTA per SM.  A
 // producer warp streams the codes with the tiled TMA (boxes of kRows rows x
-// up to 16 chunks of 256 codes, 128-byte swizzle) into a ring; eight consumer
+// up to 16 chunks of 256 codes, 128-byte swizzle) into a ring; consumer
 // warps take the chunks in turn; an epilogue warp adds their partial sums of a
 // block in a fixed order, so no consumer waits for the adds and stores.
 // Scales and zero points go straight to the registers of the lane quad that
@@ -51,9 +51,10 @@ namespace vmps {
 namespace {
 
 constexpr int kW4MaxRows = 32;
-constexpr int kW4Consumers = 8;
-constexpr int kW4EpiWarp = 1 + kW4Consumers;
-constexpr int kW4Threads = 32 * (2 + kW4Consumers);  // producer, consumers, epilogue
+// Consumer warps: a chunk is a chain of dependent steps, so four warps per
+// scheduler where the registers allow it (one activation tile), else two.
+__host__ __device__ constexpr int w4_consumers(int nt) { return nt == 1 ? 16 : 8; }
+constexpr int w4_threads(int nt) { return 32 * (2 + w4_consumers(nt)); }  // + producer, epilogue
 constexpr int kW4Chunk = 256;                        // codes of a row in a 128-byte line
 constexpr int kW4MaxStages = 16;
 constexpr int kW4SmemLimit = 226 * 1024;
@@ -99,23 +100,46 @@ __device__ __forceinline__ void w4_tma_2d(void* dst, const CUtensorMap* map, uin
 template <typename T> struct Code;
 template <> struct Code<__nv_bfloat16> {
   static constexpr uint32_t kBits = 0x43004300u;  // 128, 128
-  static constexpr float kOffset = 128.f;
+  // 128 + z (z < 128) in fp32, by its mantissa bits.
+  static __device__ __forceinline__ float offset_plus(uint32_t z) {
+    return __uint_as_float(0x43000000u | (z << 16));
+  }
 };
 template <> struct Code<__half> {
   static constexpr uint32_t kBits = 0x64006400u;  // 1024, 1024
-  static constexpr float kOffset = 1024.f;
+  static __device__ __forceinline__ float offset_plus(uint32_t z) {
+    return __uint_as_float(0x44800000u | (z << 13));
+  }
 };
-// Codes (i, i + 4) of a word as OFF + code.
-template <typename T>
-__device__ __forceinline__ uint32_t code_pair(uint32_t word, int i) {
-  return ((word >> (4 * i)) & 0x000F000Fu) | Code<T>::kBits;
+// Codes (i, i + 4) of a word as OFF + code: one shift and one three-input
+// logic operation, whose two constants have to be registers for that.
+__device__ __forceinline__ uint32_t code_pair(uint32_t word, int i, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(word >> (4 * i)), "r"(mask), "r"(bits));
+  return r;
+}
+// A wait that gives up, or finds that another has, leaves the CTA's abort flag
+// set and returns: the roles then run to their ends on whatever is in shared
+// memory, every access in bounds, no further wait lasting.
+__device__ __forceinline__ void w4_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                        int* err) {
+  if (mbar_try_wait(bar, parity)) return;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) return;
+    if (clock64() - t0 > kWaitLimitCycles) {
+      set_error(err, kDevErrTimeout);
+      *abort_flag = 1;
+      return;
+    }
+  }
 }
 
 // The order of a CTA's work, the same for all roles: panels of blocks, phases
 // of a panel, blocks of the panel.  With silu a feature block is two blocks in
 // a row, gate then up.
 template <typename T, int GROUP, int NT, int MT>
-__global__ void __launch_bounds__(kW4Threads, 1)
+__global__ void __launch_bounds__(w4_threads(NT), 1)
     w4_kernel(const __grid_constant__ CUtensorMap map3, const __grid_constant__ CUtensorMap map2,
               const __grid_constant__ W4Params p) {
   constexpr int kRows = 16 * MT;
@@ -123,6 +147,7 @@ __global__ void __launch_bounds__(kW4Threads, 1)
   constexpr int UPG = GROUP / 32;          // 32-code units per group
   constexpr int NSZ = 2 * MT * GP / 4;     // (row, group) pairs a lane fetches per chunk
   constexpr int kFrag = MT * NT;
+  constexpr int kConsumers = w4_consumers(NT);
   constexpr int kRedSlots = w4_red_slots(NT);
   __shared__ uint64_t full_bar[kW4MaxStages];
   __shared__ uint64_t empty_bar[kW4MaxStages];
@@ -132,7 +157,7 @@ __global__ void __launch_bounds__(kW4Threads, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
 
   const int tid = threadIdx.x;
-  const int warp = tid >> 5, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // warp-uniform
   if (smem_u32(smem) & 1023u) {
     if (tid == 0) set_error(p.err, kDevErrTimeout);
     return;
@@ -148,10 +173,10 @@ __global__ void __launch_bounds__(kW4Threads, 1)
     s_abort = 0;
     for (int i = 0; i < S; ++i) {
       mbar_init(&full_bar[i], 1);
-      mbar_init(&empty_bar[i], kW4Consumers);
+      mbar_init(&empty_bar[i], kConsumers);
     }
     for (int i = 0; i < kRedSlots; ++i) {
-      mbar_init(&red_full[i], kW4Consumers);
+      mbar_init(&red_full[i], kConsumers);
       mbar_init(&red_empty[i], 1);
     }
     fence_mbar_init();
@@ -181,10 +206,8 @@ __global__ void __launch_bounds__(kW4Threads, 1)
           for (int v = pv; v < pe && !s_abort; ++v) {
             for (int ch = ph * p.slice; ch < c_end; ch += p.cps, ++it) {
               const int st = it % S;
-              if (!mbar_wait(&empty_bar[st], ((it / S) & 1) ^ 1, p.err)) {
-                s_abort = 1;
-                break;
-              }
+              w4_wait(&empty_bar[st], ((it / S) & 1) ^ 1, &s_abort, p.err);
+              if (s_abort) break;
               uint8_t* dst = ring + st * p.stage_bytes;
               const int row = row_of(v);
               if (ch + p.cps <= p.full_chunks || p.full_chunks == p.chunks) {
@@ -210,7 +233,7 @@ __global__ void __launch_bounds__(kW4Threads, 1)
     return;
   }
 
-  if (warp == kW4EpiWarp) {
+  if (warp == 1 + kConsumers) {
     // ── epilogue: adds the consumers' partial sums of each block ─────────────
     w4_pdl_wait();  // out may still be read by the previous kernel
     const int g = lane >> 2, c = lane & 3;
@@ -222,7 +245,7 @@ __global__ void __launch_bounds__(kW4Threads, 1)
       for (int ph = 0; ph < p.phases; ++ph) {
         for (int v = pv; v < pe; ++v, ++n) {
           const int slot = n % kRedSlots;
-          if (!s_abort && !mbar_wait(&red_full[slot], (n / kRedSlots) & 1, p.err)) s_abort = 1;
+          w4_wait(&red_full[slot], (n / kRedSlots) & 1, &s_abort, p.err);
           float4 sum[kFrag];
 #pragma unroll
           for (int f = 0; f < kFrag; ++f) sum[f] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -231,10 +254,10 @@ __global__ void __launch_bounds__(kW4Threads, 1)
             for (int f = 0; f < kFrag; ++f) sum[f] = acc[((v - pv) * kFrag + f) * 32 + lane];
           }
 #pragma unroll
-          for (int w = 0; w < kW4Consumers; ++w) {
+          for (int w = 0; w < kConsumers; ++w) {
 #pragma unroll
             for (int f = 0; f < kFrag; ++f) {
-              const float4 a = red[((slot * kW4Consumers + w) * kFrag + f) * 32 + lane];
+              const float4 a = red[((slot * kConsumers + w) * kFrag + f) * 32 + lane];
               sum[f].x += a.x;
               sum[f].y += a.y;
               sum[f].z += a.z;
@@ -280,19 +303,19 @@ __global__ void __launch_bounds__(kW4Threads, 1)
   const int g = lane >> 2, c = lane & 3;
   const T* scales = static_cast<const T*>(p.scales);
   // The (row, group) pairs e = 4 i + c this lane fetches for its quad: group
-  // e % GP of the chunk, row g + 8 * (e / GP) of the block.  A group past K
-  // has scale 0.  Nothing here uses a loaded value (that would wait for it).
+  // e % GP of the chunk, row g + 8 * (e / GP) of the block; scale 0 past the
+  // last group or row.  Nothing here uses a loaded value (that would wait).
   auto fetch = [&](int v, int ch, uint16_t (&sc)[NSZ], uint8_t (&zp)[NSZ]) {
     const int row0 = row_of(v) + g;
 #pragma unroll
     for (int i = 0; i < NSZ; ++i) {
       const int e = 4 * i + c;
       const int grp = ch * GP + e % GP;
-      const int row = min(row0 + 8 * (e / GP), wrows - 1);
-      const int64_t at = static_cast<int64_t>(row) * p.ng + grp;
+      const int row = row0 + 8 * (e / GP);
       sc[i] = 0;
       zp[i] = 8;
-      if (grp < p.ng) {
+      if (grp < p.ng && row < wrows) {
+        const uint32_t at = static_cast<uint32_t>(row) * p.ng + grp;  // < 2^31 (host check)
         sc[i] = reinterpret_cast<const uint16_t*>(scales)[at];
         if (p.zeros) zp[i] = p.zeros[at];
       }
@@ -309,6 +332,9 @@ __global__ void __launch_bounds__(kW4Threads, 1)
     // Rows past M read row M - 1: their columns of the result are not used.
     x_lane[nt] = smem_u32(xs) + min(nt * 8 + g, p.M - 1) * p.x_pitch + c * 16;
   }
+  uint32_t mask, bits;
+  asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(mask));
+  asm volatile("mov.b32 %0, %1;" : "=r"(bits) : "n"(Code<T>::kBits));
   bool waited = false;
   int it = 0, n = 0;
   for (int pv = v0; pv < v1; pv += panel) {
@@ -316,26 +342,31 @@ __global__ void __launch_bounds__(kW4Threads, 1)
     for (int ph = 0; ph < p.phases; ++ph) {
       const int c_begin = ph * p.slice, c_end = min(c_begin + p.slice, p.chunks);
       const int nch = c_end - c_begin;
-      // Chunks of the phase's blocks, dealt to the warps in turn.
-      int nv = pv, nc = w;  // next chunk of this warp
-      while (nc >= nch && nv < pe) {
-        nc -= nch;
-        ++nv;
-      }
+      // The chunks of the phase's blocks are dealt to the warps in turn: `off`
+      // is this warp's next one, counted from the current stage's first.
+      int off = w;
+      int nv = pv, nc = w;  // block and chunk of the next one to fetch scales for
       uint16_t sc_next[NSZ];
       uint8_t zp_next[NSZ];
-      if (nv < pe) fetch(nv, c_begin + nc, sc_next, zp_next);
+      auto advance = [&]() {
+        while (nc >= nch) {
+          nc -= nch;
+          ++nv;
+        }
+        if (nv < pe) fetch(nv, c_begin + nc, sc_next, zp_next);
+      };
+      advance();
       if (!waited) {
         w4_pdl_wait();  // X is the previous kernel's output
         waited = true;
       }
-      if (p.phases > 1) named_barrier_sync(1, 32 * kW4Consumers);  // X of the last phase is done with
+      if (p.phases > 1) named_barrier_sync(1, 32 * kConsumers);  // X of the last phase is done with
       {
         // Stage the slice of X: 8 values a thread, in the order (0 4 1 5 2 6 3
         // 7), and each group's sum.  A group is GROUP / 8 adjacent lanes.
         const int k0 = c_begin * kW4Chunk;
         const int units = nch * (kW4Chunk / 8);  // a multiple of 32
-        for (int e = ctid; e < p.M * units; e += 32 * kW4Consumers) {
+        for (int e = ctid; e < p.M * units; e += 32 * kConsumers) {
           const int m = e / units, u = e - m * units;
           const int k = k0 + u * 8;
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -357,7 +388,7 @@ __global__ void __launch_bounds__(kW4Threads, 1)
           if (u % (GROUP / 8) == 0) sx[(u / (GROUP / 8)) * (8 * NT) + m] = s;
         }
       }
-      named_barrier_sync(1, 32 * kW4Consumers);
+      named_barrier_sync(1, 32 * kConsumers);
       if (pv == v0 && ph == 0) w4_pdl_trigger();
 
       for (int v = pv; v < pe; ++v, ++n) {
@@ -372,19 +403,16 @@ __global__ void __launch_bounds__(kW4Threads, 1)
         }
         for (int s0 = 0; s0 < nch; s0 += p.cps, ++it) {
           const int st = it % S;
-          if (!s_abort && !mbar_wait(&full_bar[st], (it / S) & 1, p.err)) s_abort = 1;
-          while (nv == v && nc < s0 + p.cps && !s_abort) {
+          w4_wait(&full_bar[st], (it / S) & 1, &s_abort, p.err);
+          const int n_stage = min(p.cps, nch - s0);
+          for (; off < n_stage; off += kConsumers) {
             uint32_t sz[NSZ];
 #pragma unroll
             for (int i = 0; i < NSZ; ++i) sz[i] = sc_next[i] | (static_cast<uint32_t>(zp_next[i]) << 16);
-            const int ch = nc;  // chunk within the slice
-            nc += kW4Consumers;
-            while (nc >= nch && nv < pe) {
-              nc -= nch;
-              ++nv;
-            }
-            if (nv < pe) fetch(nv, c_begin + nc, sc_next, zp_next);
-            const uint32_t base = ring_u32 + st * p.stage_bytes + (ch - s0) * (kRows * 128) + a_row;
+            nc += kConsumers;
+            advance();
+            const int ch = s0 + off;  // chunk within the slice
+            const uint32_t base = ring_u32 + st * p.stage_bytes + off * (kRows * 128) + a_row;
             uint32_t a[MT][4][4];  // [unit pair][(row half) + 2 * (unit in pair)]
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -405,7 +433,7 @@ __global__ void __launch_bounds__(kW4Threads, 1)
                   const uint32_t q = __shfl_sync(0xffffffffu, sz[e >> 2], (lane & ~3) | (e & 3));
                   const uint16_t sb = static_cast<uint16_t>(q);
                   sc[mt][h] = Elt<T>::to_f(*reinterpret_cast<const T*>(&sb));
-                  const float zz = Code<T>::kOffset + static_cast<float>(q >> 16);
+                  const float zz = Code<T>::offset_plus(q >> 16);
 #pragma unroll
                   for (int nt = 0; nt < NT; ++nt) {
                     const float2 s2 = *reinterpret_cast<const float2*>(
@@ -428,10 +456,10 @@ __global__ void __launch_bounds__(kW4Threads, 1)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                   const uint32_t lo = a[mt][U >> 1][(U & 1) * 2], hi = a[mt][U >> 1][(U & 1) * 2 + 1];
-                  const uint32_t f0[4] = {code_pair<T>(lo, 0), code_pair<T>(hi, 0),
-                                          code_pair<T>(lo, 1), code_pair<T>(hi, 1)};
-                  const uint32_t f1[4] = {code_pair<T>(lo, 2), code_pair<T>(hi, 2),
-                                          code_pair<T>(lo, 3), code_pair<T>(hi, 3)};
+                  const uint32_t f0[4] = {code_pair(lo, 0, mask, bits), code_pair(hi, 0, mask, bits),
+                                          code_pair(lo, 1, mask, bits), code_pair(hi, 1, mask, bits)};
+                  const uint32_t f1[4] = {code_pair(lo, 2, mask, bits), code_pair(hi, 2, mask, bits),
+                                          code_pair(lo, 3, mask, bits), code_pair(hi, 3, mask, bits)};
 #pragma unroll
                   for (int nt = 0; nt < NT; ++nt) {
                     Mma<T>::run(part[mt][nt], f0, xv[nt].x, xv[nt].y);
@@ -451,16 +479,17 @@ __global__ void __launch_bounds__(kW4Threads, 1)
               }
             }
           }
+          off -= n_stage;
           __syncwarp();
           if (lane == 0) mbar_arrive(&empty_bar[st]);
         }
         const int slot = n % kRedSlots;
-        if (!s_abort && !mbar_wait(&red_empty[slot], ((n / kRedSlots) & 1) ^ 1, p.err)) s_abort = 1;
+        w4_wait(&red_empty[slot], ((n / kRedSlots) & 1) ^ 1, &s_abort, p.err);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            red[((slot * kW4Consumers + w) * kFrag + mt * NT + nt) * 32 + lane] =
+            red[((slot * kConsumers + w) * kFrag + mt * NT + nt) * 32 + lane] =
                 make_float4(total[mt][nt][0], total[mt][nt][1], total[mt][nt][2], total[mt][nt][3]);
           }
         }
@@ -483,7 +512,7 @@ bool w4_plan(W4Params* p, int group, int cta_blocks) {
   const int nt = w4_nt(p->M), mt = nt > 1 ? 2 : 1;
   const int rows = 16 * mt;
   const int line = rows * 128;  // bytes of one chunk of a block
-  p->red_bytes = w4_red_slots(nt) * kW4Consumers * mt * nt * 512;
+  p->red_bytes = w4_red_slots(nt) * w4_consumers(nt) * mt * nt * 512;
   for (int phases = 1; phases <= 64; ++phases) {
     for (int cps = 16; cps >= 1; cps >>= 1) {
       if (cps * line > 32 * 1024 && cps > 1) continue;
@@ -523,7 +552,7 @@ int w4_launch(const CUtensorMap& m3, const CUtensorMap& m2, const W4Params& p, i
   });
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kW4Threads);
+  cfg.blockDim = dim3(w4_threads(NT));
   cfg.dynamicSmemBytes = static_cast<size_t>(p.stages) * p.stage_bytes + p.x_bytes + p.sx_bytes +
                          p.red_bytes + p.acc_bytes;
   cfg.stream = s;
@@ -578,7 +607,8 @@ extern "C" int vmps_w4_gemm(void* out, int64_t out_row_stride, const void* x, in
   if (dtype != VMPS_DTYPE_F16 && dtype != VMPS_DTYPE_BF16) {
     return fail(VMPS_ERR_INVALID_ARG, "%s: dtype %d", what, dtype);
   }
-  if (!vmps_w4_gemm_supported(M, N, K, group_size)) {
+  if (!vmps_w4_gemm_supported(M, N, K, group_size) ||
+      2 * static_cast<int64_t>(N) * (K / group_size) > 0x7fffffff) {
     return fail(VMPS_ERR_UNSUPPORTED,
                 "%s: M=%d N=%d K=%d group=%d (M <= %d, group 32, 64 or 128, K a multiple of it)",
                 what, M, N, K, group_size, kW4MaxRows);
