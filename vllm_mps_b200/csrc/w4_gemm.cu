@@ -59,9 +59,7 @@ constexpr int kW4Chunk = 256;                        // codes of a row in a 128-
 constexpr int kW4MaxStages = 16;
 constexpr int kW4SmemLimit = 226 * 1024;
 constexpr int kW4Panel = 16;  // blocks a CTA carries through the phases at once
-// Partial-sum slots between consumers and epilogue: two let the consumers run
-// ahead; with four activation tiles a slot is 32 KB and the ring needs it more.
-__host__ __device__ constexpr int w4_red_slots(int nt) { return nt > 2 ? 1 : 2; }
+constexpr int kW4MaxRedSlots = 32;
 
 struct W4Params {
   void* out;
@@ -78,6 +76,8 @@ struct W4Params {
   int slice;             // chunks per phase (a multiple of cps unless there is one phase)
   int phases;
   int stages;
+  int team;              // consumer warps that share a block (a power of two)
+  int red_slots;         // blocks whose partial sums can wait for the epilogue
   int blocks;            // of kRows features (per half with silu)
   int x_pitch;           // bytes between activation rows in shared memory
   int x_bytes, sx_bytes, red_bytes, acc_bytes, stage_bytes;
@@ -138,6 +138,19 @@ __device__ __forceinline__ void w4_wait(uint64_t* bar, uint32_t parity, volatile
 // The order of a CTA's work, the same for all roles: panels of blocks, phases
 // of a panel, blocks of the panel.  With silu a feature block is two blocks in
 // a row, gate then up.
+// A place in a ring of S slots and the parity of its current round.
+struct RingPos {
+  int at;
+  uint32_t round;
+  __device__ __forceinline__ void step(int n, int S) {
+    at += n;
+    while (at >= S) {
+      at -= S;
+      round ^= 1u;
+    }
+  }
+};
+
 template <typename T, int GROUP, int NT, int MT>
 __global__ void __launch_bounds__(w4_threads(NT), 1)
     w4_kernel(const __grid_constant__ CUtensorMap map3, const __grid_constant__ CUtensorMap map2,
@@ -148,11 +161,10 @@ __global__ void __launch_bounds__(w4_threads(NT), 1)
   constexpr int NSZ = 2 * MT * GP / 4;     // (row, group) pairs a lane fetches per chunk
   constexpr int kFrag = MT * NT;
   constexpr int kConsumers = w4_consumers(NT);
-  constexpr int kRedSlots = w4_red_slots(NT);
   __shared__ uint64_t full_bar[kW4MaxStages];
   __shared__ uint64_t empty_bar[kW4MaxStages];
-  __shared__ uint64_t red_full[kRedSlots];
-  __shared__ uint64_t red_empty[kRedSlots];
+  __shared__ uint64_t red_full[kW4MaxRedSlots];
+  __shared__ uint64_t red_empty[kW4MaxRedSlots];
   __shared__ volatile int s_abort;
   extern __shared__ __align__(1024) uint8_t smem[];
 
@@ -173,10 +185,10 @@ __global__ void __launch_bounds__(w4_threads(NT), 1)
     s_abort = 0;
     for (int i = 0; i < S; ++i) {
       mbar_init(&full_bar[i], 1);
-      mbar_init(&empty_bar[i], kConsumers);
+      mbar_init(&empty_bar[i], p.team);
     }
-    for (int i = 0; i < kRedSlots; ++i) {
-      mbar_init(&red_full[i], kConsumers);
+    for (int i = 0; i < p.red_slots; ++i) {
+      mbar_init(&red_full[i], p.team);
       mbar_init(&red_empty[i], 1);
     }
     fence_mbar_init();
@@ -198,15 +210,16 @@ __global__ void __launch_bounds__(w4_threads(NT), 1)
     if (lane == 0) {
       prefetch_tmap(&map3);
       prefetch_tmap(&map2);
+      RingPos rp = {0, 0u};
       int it = 0;
       for (int pv = v0; pv < v1 && !s_abort; pv += panel) {
         const int pe = min(pv + panel, v1);
         for (int ph = 0; ph < p.phases && !s_abort; ++ph) {
           const int c_end = min((ph + 1) * p.slice, p.chunks);
           for (int v = pv; v < pe && !s_abort; ++v) {
-            for (int ch = ph * p.slice; ch < c_end; ch += p.cps, ++it) {
-              const int st = it % S;
-              w4_wait(&empty_bar[st], ((it / S) & 1) ^ 1, &s_abort, p.err);
+            for (int ch = ph * p.slice; ch < c_end; ch += p.cps, ++it, rp.step(1, S)) {
+              const int st = rp.at;
+              w4_wait(&empty_bar[st], rp.round ^ 1u, &s_abort, p.err);
               if (s_abort) break;
               uint8_t* dst = ring + st * p.stage_bytes;
               const int row = row_of(v);
@@ -239,13 +252,13 @@ __global__ void __launch_bounds__(w4_threads(NT), 1)
     const int g = lane >> 2, c = lane & 3;
     T* out = static_cast<T*>(p.out);
     float gate[kFrag][4];
-    int n = 0;
+    RingPos rr = {0, 0u};
     for (int pv = v0; pv < v1; pv += panel) {
       const int pe = min(pv + panel, v1);
       for (int ph = 0; ph < p.phases; ++ph) {
-        for (int v = pv; v < pe; ++v, ++n) {
-          const int slot = n % kRedSlots;
-          w4_wait(&red_full[slot], (n / kRedSlots) & 1, &s_abort, p.err);
+        for (int v = pv; v < pe; ++v, rr.step(1, p.red_slots)) {
+          const int slot = rr.at;
+          w4_wait(&red_full[slot], rr.round, &s_abort, p.err);
           float4 sum[kFrag];
 #pragma unroll
           for (int f = 0; f < kFrag; ++f) sum[f] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -253,11 +266,10 @@ __global__ void __launch_bounds__(w4_threads(NT), 1)
 #pragma unroll
             for (int f = 0; f < kFrag; ++f) sum[f] = acc[((v - pv) * kFrag + f) * 32 + lane];
           }
-#pragma unroll
-          for (int w = 0; w < kConsumers; ++w) {
+          for (int w = 0; w < p.team; ++w) {
 #pragma unroll
             for (int f = 0; f < kFrag; ++f) {
-              const float4 a = red[((slot * kConsumers + w) * kFrag + f) * 32 + lane];
+              const float4 a = red[((slot * p.team + w) * kFrag + f) * 32 + lane];
               sum[f].x += a.x;
               sum[f].y += a.y;
               sum[f].z += a.z;
@@ -298,7 +310,9 @@ __global__ void __launch_bounds__(w4_threads(NT), 1)
   }
 
   // ── consumers ──────────────────────────────────────────────────────────────
-  const int w = warp - 1;
+  const int w = (warp - 1) & (p.team - 1);       // place in the team
+  const int team = (warp - 1) / p.team;          // takes blocks pv + team, + teams, ...
+  const int teams = kConsumers / p.team;
   const int ctid = tid - 32;
   const int g = lane >> 2, c = lane & 3;
   const T* scales = static_cast<const T*>(p.scales);
@@ -324,7 +338,7 @@ __global__ void __launch_bounds__(w4_threads(NT), 1)
   // ldmatrix rows of this lane: tiles (rows 0-7, unit u), (rows 8-15, u),
   // (rows 0-7, u + 1), (rows 8-15, u + 1) of a 16-row tile.
   const int mi = lane >> 3, r8 = lane & 7;
-  const uint32_t a_row = static_cast<uint32_t>((r8 + (mi & 1) * 8) * 128);
+  const uint32_t a_lane = static_cast<uint32_t>((r8 + (mi & 1) * 8) * 128 + (((mi >> 1) ^ r8) << 4));
   const uint32_t ring_u32 = smem_u32(ring);
   uint32_t x_lane[NT];
 #pragma unroll
@@ -336,22 +350,23 @@ __global__ void __launch_bounds__(w4_threads(NT), 1)
   asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(mask));
   asm volatile("mov.b32 %0, %1;" : "=r"(bits) : "n"(Code<T>::kBits));
   bool waited = false;
-  int it = 0, n = 0;
+  RingPos rp = {0, 0u}, rr = {0, 0u};  // of the current panel and phase's first block
   for (int pv = v0; pv < v1; pv += panel) {
     const int pe = min(pv + panel, v1);
     for (int ph = 0; ph < p.phases; ++ph) {
       const int c_begin = ph * p.slice, c_end = min(c_begin + p.slice, p.chunks);
       const int nch = c_end - c_begin;
-      // The chunks of the phase's blocks are dealt to the warps in turn: `off`
-      // is this warp's next one, counted from the current stage's first.
+      // The chunks of the team's blocks are dealt to its warps in turn: `off` is
+      // this warp's next one, counted from the current stage's first.
+      const int spv = (nch + p.cps - 1) / p.cps;  // stages per block
       int off = w;
-      int nv = pv, nc = w;  // block and chunk of the next one to fetch scales for
+      int nv = pv + team, nc = w;  // block and chunk of the next one to fetch scales for
       uint16_t sc_next[NSZ];
       uint8_t zp_next[NSZ];
       auto advance = [&]() {
         while (nc >= nch) {
           nc -= nch;
-          ++nv;
+          nv += teams;
         }
         if (nv < pe) fetch(nv, c_begin + nc, sc_next, zp_next);
       };
@@ -391,7 +406,10 @@ __global__ void __launch_bounds__(w4_threads(NT), 1)
       named_barrier_sync(1, 32 * kConsumers);
       if (pv == v0 && ph == 0) w4_pdl_trigger();
 
-      for (int v = pv; v < pe; ++v, ++n) {
+      RingPos cur = rp, red_at = rr;
+      cur.step(team * spv, S);
+      red_at.step(team, p.red_slots);
+      for (int v = pv + team; v < pe; v += teams) {
         float total[MT][NT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -401,24 +419,24 @@ __global__ void __launch_bounds__(w4_threads(NT), 1)
             for (int e = 0; e < 4; ++e) total[mt][nt][e] = 0.f;
           }
         }
-        for (int s0 = 0; s0 < nch; s0 += p.cps, ++it) {
-          const int st = it % S;
-          w4_wait(&full_bar[st], (it / S) & 1, &s_abort, p.err);
+        for (int s0 = 0; s0 < nch; s0 += p.cps, cur.step(1, S)) {
+          const int st = cur.at;
+          w4_wait(&full_bar[st], cur.round, &s_abort, p.err);
           const int n_stage = min(p.cps, nch - s0);
-          for (; off < n_stage; off += kConsumers) {
+          for (; off < n_stage; off += p.team) {
             uint32_t sz[NSZ];
 #pragma unroll
             for (int i = 0; i < NSZ; ++i) sz[i] = sc_next[i] | (static_cast<uint32_t>(zp_next[i]) << 16);
-            nc += kConsumers;
+            nc += p.team;
             advance();
             const int ch = s0 + off;  // chunk within the slice
-            const uint32_t base = ring_u32 + st * p.stage_bytes + off * (kRows * 128) + a_row;
+            const uint32_t base = ring_u32 + st * p.stage_bytes + off * (kRows * 128) + a_lane;
             uint32_t a[MT][4][4];  // [unit pair][(row half) + 2 * (unit in pair)]
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
               for (int u = 0; u < 4; ++u) {
-                ldmatrix_x4(a[mt][u], base + mt * 2048 + (((2 * u + (mi >> 1)) ^ r8) << 4));
+                ldmatrix_x4(a[mt][u], (base ^ (u << 5)) + mt * 2048);  // 16-byte unit 2 u (+ 1), swizzled
               }
             }
 #pragma unroll
@@ -483,19 +501,23 @@ __global__ void __launch_bounds__(w4_threads(NT), 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&empty_bar[st]);
         }
-        const int slot = n % kRedSlots;
-        w4_wait(&red_empty[slot], ((n / kRedSlots) & 1) ^ 1, &s_abort, p.err);
+        const int slot = red_at.at;
+        w4_wait(&red_empty[slot], red_at.round ^ 1u, &s_abort, p.err);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            red[((slot * kConsumers + w) * kFrag + mt * NT + nt) * 32 + lane] =
+            red[((slot * p.team + w) * kFrag + mt * NT + nt) * 32 + lane] =
                 make_float4(total[mt][nt][0], total[mt][nt][1], total[mt][nt][2], total[mt][nt][3]);
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&red_full[slot]);
+        cur.step((teams - 1) * spv, S);
+        red_at.step(teams, p.red_slots);
       }
+      rp.step((pe - pv) * spv, S);
+      rr.step(pe - pv, p.red_slots);
     }
   }
 }
@@ -512,7 +534,15 @@ bool w4_plan(W4Params* p, int group, int cta_blocks) {
   const int nt = w4_nt(p->M), mt = nt > 1 ? 2 : 1;
   const int rows = 16 * mt;
   const int line = rows * 128;  // bytes of one chunk of a block
-  p->red_bytes = w4_red_slots(nt) * w4_consumers(nt) * mt * nt * 512;
+  // A warp should take about four chunks of a block (its share of the block's
+  // fixed costs), but all warps should have a block.
+  const int cons = w4_consumers(nt);
+  p->team = 1;
+  while (p->team < cons && (p->team * 4 < p->chunks || p->team * cta_blocks < cons)) p->team *= 2;
+  // Two blocks per team in flight to the epilogue (one with four activation
+  // tiles, where a slot of a full team is 32 KB that the ring needs more).
+  p->red_slots = cons / p->team * (nt > 2 ? 1 : 2);
+  p->red_bytes = p->red_slots * p->team * mt * nt * 512;
   for (int phases = 1; phases <= 64; ++phases) {
     for (int cps = 16; cps >= 1; cps >>= 1) {
       if (cps * line > 32 * 1024 && cps > 1) continue;
