@@ -38,10 +38,10 @@
 // do not fit the registers) over all of K belongs to one CTA;
 // contiguous equal shares of blocks go to one persistent CTA per SM.  The
 // warps form teams; a team takes every teams-th block, its warps the block's
-// chunks (2 KB of codes) in turn, and adds their partial sums of the block
+// chunks (4 KB of codes) in turn, and adds their partial sums of the block
 // through shared memory in a fixed order.  Every warp streams its own chunks
-// with 16-byte asynchronous copies into a private ring, so nothing but the
-// block's sum is waited for by more than one warp.  (Bulk copies were tried:
+// with 16-byte asynchronous copies into a private pair of slots, so nothing but
+// the block's sum is waited for by more than one warp; 64 KB are in flight.  (Bulk copies were tried:
 // with one per row or one tensor box per block the copy engine's per-line cost
 // capped the stream at 60 % of the rate of these.)  Scales and zero points go
 // straight to the registers of the lane quad that uses them, as many chunks
@@ -66,10 +66,15 @@ namespace {
 constexpr int kW4MaxRows = 32;
 constexpr int kW4Warps = 16;
 constexpr int kW4Threads = 32 * kW4Warps;
-constexpr int kW4ChunkBytes = 2048;  // codes of a chunk: kRows rows x 4096 / kRows codes
-constexpr int kW4Depth = 4;          // ring slots per warp: three chunks in flight
+constexpr int kW4ChunkBytes = 4096;  // codes of a chunk: kRows rows x 8192 / kRows codes
+constexpr int kW4Depth = 2;          // ring slots per warp: one chunk in flight, one in use
 constexpr int kW4SmemLimit = 227 * 1024;
 constexpr int kW4XBatch = 8;         // activation loads in flight per thread
+
+// Buffers of partial sums: with two a team meets once per block instead of
+// twice; with more than one activation tile the second would cost the
+// activations their room.
+__host__ __device__ constexpr int w4_red_bufs(int nt) { return nt == 1 ? 2 : 1; }
 
 struct W4Params {
   void* out;
@@ -141,18 +146,17 @@ template <> struct ScaleZero<__nv_bfloat16> {
 template <typename T, int GROUP, int NT, int MT>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant__ W4Params p) {
   constexpr int kRows = 16 * MT;
-  constexpr int kCodes = kW4ChunkBytes * 2 / kRows;  // codes of a row in a chunk: 256 or 128
+  constexpr int kCodes = kW4ChunkBytes * 2 / kRows;  // codes of a row in a chunk: 512 or 256
   constexpr int kRowBytes = kCodes / 2;
   constexpr int kUnits = kRowBytes / 16;             // 32-code units of a row
   constexpr int GP = kCodes / GROUP;                 // groups per chunk
   constexpr int UPG = GROUP / 32;
   constexpr int NSZ = (2 * MT * GP + 3) / 4;         // (row, group) pairs a lane fetches per chunk
-  constexpr int kAhead = kW4Depth - 1;
   constexpr int kFrag = MT * NT;
   constexpr int kPlanes = std::is_same<T, __half>::value ? 2 : 3;
   // Shared memory: rings | activations | group sums | partial sums | gate sums
   // (silu) | panel sums (several phases).
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
 
   const int tid = threadIdx.x;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // warp-uniform
@@ -164,16 +168,18 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
   // Per group and activation row: -sum x OFF, sum x and, for bf16, what the
   // group's sum is multiplied by, [group][plane][row].
   float* sx = reinterpret_cast<float*>(xs + p.x_bytes);
-  float* red = sx + p.sx_bytes / 4 + team * T_ * kFrag * 128;  // the team's
-  float* gate = sx + p.sx_bytes / 4 + (kW4Warps + team) * kFrag * 128;  // the team's, with silu
-  float* acc = sx + p.sx_bytes / 4 + (kW4Warps + (p.silu ? teams : 0)) * kFrag * 128;  // the panel's
+  float* red = sx + p.sx_bytes / 4 + team * T_ * kFrag * 128;  // the team's (first buffer)
+  constexpr int kRedFloats = kW4Warps * kFrag * 128;           // of a buffer, all teams
+  constexpr int kRedBufs = w4_red_bufs(NT);
+  float* gate = sx + p.sx_bytes / 4 + kRedBufs * kRedFloats + team * kFrag * 128;  // with silu
+  float* acc = sx + p.sx_bytes / 4 + kRedBufs * kRedFloats + (p.silu ? teams : 0) * kFrag * 128;
 
   const int halves = p.silu ? 2 : 1;
   const int G = gridDim.x;
   const int v0 = halves * static_cast<int>(static_cast<long long>(blockIdx.x) * p.blocks / G);
   const int v1 = halves * static_cast<int>(static_cast<long long>(blockIdx.x + 1) * p.blocks / G);
   const int wrows = halves * p.N;  // rows of the weight
-  const int64_t row_bytes = p.K / 2;
+  const uint32_t row_bytes = static_cast<uint32_t>(p.K) / 2;
   // First weight row of block v.  With silu a feature block is two blocks in a
   // row, gate then up, both of one team.
   auto row_of = [&](int v) -> int {
@@ -188,21 +194,16 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
   // ── the stream: this warp's chunks in the order it will take them ──────────
   // (panel, phase, block, chunk); dealing starts at w in every phase.
   const uint32_t ring = smem_u32(smem) + warp * kW4Depth * kW4ChunkBytes;
-  // A copy instruction covers 512 / kRowBytes rows; 16-byte units are swizzled
-  // so that ldmatrix's eight rows never share a bank.
-  constexpr int kRowsPerCopy = 512 / kRowBytes;
-  const int l_row = lane / kUnits, l_unit = lane % kUnits;
-  auto swz = [](int row, int unit) -> int {
-    return MT == 1 ? unit ^ (row & 7) : unit ^ ((row >> 1) & 3);
-  };
+  // A copy instruction takes 64 bytes of eight rows (whole sectors); the 16-byte
+  // units of a row are swizzled so that ldmatrix's eight rows never share a
+  // bank.  Copies of one row differ in the unit's bits 2 and up, untouched by
+  // the lane's own, so their targets differ by an exclusive or.
+  constexpr int kCols = kRowBytes / 64, kRowSets = kRows / 8;
+  auto swz = [](int row, int unit) -> int { return unit ^ (row & 7); };
   const int g = lane >> 2, c = lane & 3;
-  // Copy i goes to row l_row + i * kRowsPerCopy; the swizzle of odd copies
-  // differs from that of even ones in one bit (MT 1) or not at all.
-  const uint32_t l_dst0 = l_row * kRowBytes + swz(l_row, l_unit) * 16;
-  const uint32_t l_dst1 = l_row * kRowBytes + swz(l_row + kRowsPerCopy, l_unit) * 16;
+  const uint32_t l_dst = g * kRowBytes + swz(g, c) * 16;
   // (row, group) pairs e = 4 i + c of this lane's quad: group e % GP of the
   // chunk, row g + 8 * (e / GP) of the block.
-  const int64_t copy_step = kRowsPerCopy * row_bytes;
   const uint32_t end_of_ring = ring + kW4Depth * kW4ChunkBytes;
   int s_pv = v0, s_ph = 0, s_v = v0 + halves * team, s_c = w;
   int s_nch = min(p.slice, p.chunks);  // of the phase
@@ -232,52 +233,59 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
     }
     const int ch = s_ph * p.slice + s_c, row0 = row_of(s_v);
     s_rows_full = row0 + kRows <= wrows;
-    s_src = p.codes + (row0 + l_row) * row_bytes + ch * kRowBytes + l_unit * 16;
+    s_src = p.codes + static_cast<uint64_t>(static_cast<uint32_t>(row0 + g)) * row_bytes +
+            (ch * kRowBytes + c * 16);
     s_at = static_cast<uint32_t>(row0 + g + 8 * (c / GP)) * p.ng + ch * GP + c % GP;
   };
-  uint16_t sc_buf[kAhead][NSZ];
-  uint8_t zp_buf[kAhead][NSZ];
+  uint16_t sc_next[NSZ];
+  uint8_t zp_next[NSZ];
   // Starts the stream's next chunk: its codes into the next ring slot, this
   // lane's scales and zero points into registers.  Nothing here uses a loaded
   // value (that would wait for it).
-  auto start_next = [&](uint16_t (&sc)[NSZ], uint8_t (&zp)[NSZ]) {
+  auto start_next = [&]() {
     if (s_on) {
       const uint16_t* scales = static_cast<const uint16_t*>(p.scales);
       const int ch = s_ph * p.slice + s_c;
       if (s_rows_full && (ch + 1) * kCodes <= p.K) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w4_copy16(s_dst + ((i & 1) ? l_dst1 : l_dst0) + i * kRowsPerCopy * kRowBytes,
-                    s_src + i * copy_step);
+        for (int r = 0; r < kRowSets; ++r) {
+          const uint8_t* src = s_src + static_cast<uint64_t>(row_bytes) * (8 * r);
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) {
+            w4_copy16((s_dst + (l_dst ^ (i << 6))) + r * 8 * kRowBytes, src + i * 64);
+          }
         }
 #pragma unroll
         for (int i = 0; i < NSZ; ++i) {
           const uint32_t j = s_at + (4 * i) % GP + 8 * (4 * i / GP) * p.ng;
-          if (2 * MT * GP >= 4 || c < 2 * MT * GP) sc[i] = scales[j];
-          zp[i] = 8;
-          if (p.zeros && (2 * MT * GP >= 4 || c < 2 * MT * GP)) zp[i] = p.zeros[j];
+          if (2 * MT * GP >= 4 || c < 2 * MT * GP) sc_next[i] = scales[j];
+          zp_next[i] = 8;
+          if (p.zeros && (2 * MT * GP >= 4 || c < 2 * MT * GP)) zp_next[i] = p.zeros[j];
         }
       } else {
         // The weight's last rows or a row's last codes: only what exists, and
         // scale 0 for the rest (what the slot holds there is finite).
         const int row0 = row_of(s_v);
-        const bool in_k = static_cast<int64_t>(ch) * kRowBytes + l_unit * 16 < row_bytes;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (in_k && row0 + l_row + i * kRowsPerCopy < wrows) {
-            w4_copy16(s_dst + ((i & 1) ? l_dst1 : l_dst0) + i * kRowsPerCopy * kRowBytes,
-                      s_src + i * copy_step);
+        for (int r = 0; r < kRowSets; ++r) {
+          const uint8_t* src = s_src + static_cast<uint64_t>(row_bytes) * (8 * r);
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) {
+            if (static_cast<uint32_t>(ch) * kRowBytes + i * 64 + c * 16 < row_bytes &&
+                row0 + g + 8 * r < wrows) {
+              w4_copy16((s_dst + (l_dst ^ (i << 6))) + r * 8 * kRowBytes, src + i * 64);
+            }
           }
         }
 #pragma unroll
         for (int i = 0; i < NSZ; ++i) {
           const int e = 4 * i + c;
-          sc[i] = 0;
-          zp[i] = 8;
+          sc_next[i] = 0;
+          zp_next[i] = 8;
           if (ch * GP + e % GP < p.ng && row0 + g + 8 * (e / GP) < wrows && e < 2 * MT * GP) {
             const uint32_t j = s_at + (4 * i) % GP + 8 * (4 * i / GP) * p.ng;
-            sc[i] = scales[j];
-            if (p.zeros) zp[i] = p.zeros[j];
+            sc_next[i] = scales[j];
+            if (p.zeros) zp_next[i] = p.zeros[j];
           }
         }
       }
@@ -294,8 +302,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
     if (s_dst == end_of_ring) s_dst = ring;
   };
   settle();
-#pragma unroll
-  for (int k = 0; k < kAhead; ++k) start_next(sc_buf[k], zp_buf[k]);
+  start_next();
 
   w4_pdl_wait();  // X is the previous kernel's output, out may still be read by it
 
@@ -318,16 +325,15 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
   asm volatile("mov.b32 %0, 0x54005400;" : "=r"(bits_hi));  // 64, 64
   float total[MT][NT][4];
   uint32_t r_src = ring;  // the next chunk's ring slot
-  int k_buf = 0;
 
   // One chunk: chunk `ch` of the slice, from the next ring slot.
-  auto chunk = [&](int ch, uint16_t (&sc_in)[NSZ], uint8_t (&zp_in)[NSZ]) {
-    w4_wait_pending<kAhead - 1>();
+  auto chunk = [&](int ch) {
+    w4_wait_pending<0>();
     __syncwarp();  // every lane's copies have landed, and the last chunk is read
     uint32_t sz[NSZ];
 #pragma unroll
-    for (int i = 0; i < NSZ; ++i) sz[i] = ScaleZero<T>::pack(sc_in[i], zp_in[i]);
-    start_next(sc_in, zp_in);
+    for (int i = 0; i < NSZ; ++i) sz[i] = ScaleZero<T>::pack(sc_next[i], zp_next[i]);
+    start_next();
     const uint32_t base = r_src + a_lane;
     r_src += kW4ChunkBytes;
     if (r_src == end_of_ring) r_src = ring;
@@ -412,6 +418,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
   };
 
   T* out = static_cast<T*>(p.out);
+  int red_buf = 0;
   for (int pv = v0; pv < v1; pv += p.panel) {
     const int pe = min(pv + p.panel, v1);
     for (int ph = 0; ph < p.phases; ++ph) {
@@ -513,22 +520,12 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
             for (int e = 0; e < 4; ++e) total[mt][nt][e] = 0.f;
           }
         }
-        for (; off < nch; off += T_) {
-          static_assert(kAhead == 3, "one case per chunk in flight");
-          if (k_buf == 0) {
-            chunk(off, sc_buf[0], zp_buf[0]);
-            k_buf = 1;
-          } else if (k_buf == 1) {
-            chunk(off, sc_buf[1], zp_buf[1]);
-            k_buf = 2;
-          } else {
-            chunk(off, sc_buf[2], zp_buf[2]);
-            k_buf = 0;
-          }
-        }
+        for (; off < nch; off += T_) chunk(off);
         off -= nch;
         // The team's sum of the block, the warps in order.
-        float4* mine = reinterpret_cast<float4*>(red + w * kFrag * 128);
+        const float* sums = red + (kRedBufs == 2 ? red_buf * kRedFloats : 0);
+        red_buf ^= 1;
+        float4* mine = reinterpret_cast<float4*>(const_cast<float*>(sums) + w * kFrag * 128);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -541,7 +538,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
         const bool up = p.silu && (v & 1);
         for (int x = w * 32 + lane; x < kFrag * 128; x += 32 * T_) {
           float y = ph > 0 ? acc[(v - pv) * kFrag * 128 + x] : 0.f;
-          for (int j = 0; j < T_; ++j) y += red[j * kFrag * 128 + x];
+          for (int j = 0; j < T_; ++j) y += sums[j * kFrag * 128 + x];
           if (ph + 1 < p.phases) {
             acc[(v - pv) * kFrag * 128 + x] = y;
           } else if (p.silu && !up) {
@@ -555,7 +552,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
             if (m < p.M && feat < p.N) out[m * p.out_stride + feat] = Elt<T>::from_f(y);
           }
         }
-        team_sync();  // the sums are taken before the next block's are written
+        if (kRedBufs == 1) team_sync();  // the sums are taken before the next block's are written
       }
     }
   }
@@ -581,7 +578,7 @@ bool w4_plan(W4Params* p, int group, int planes, int cta_blocks) {
   }
   const int block = mt * nt * 512;  // bytes of a block's sums
   const int fixed = kW4Warps * kW4Depth * kW4ChunkBytes +
-                    (kW4Warps + (p->silu ? kW4Warps / p->team : 0)) * block;
+                    (w4_red_bufs(nt) * kW4Warps + (p->silu ? kW4Warps / p->team : 0)) * block;
   long long best = -1;
   for (int phases = 1; phases <= p->chunks; ++phases) {
     const int slice = (p->chunks + phases - 1) / phases;
@@ -616,7 +613,7 @@ bool w4_plan(W4Params* p, int group, int planes, int cta_blocks) {
 size_t w4_smem(const W4Params& p) {
   const int block = w4_mt(p.M) * w4_nt(p.M) * 512;
   return kW4Warps * kW4Depth * kW4ChunkBytes + p.x_bytes + p.sx_bytes +
-         static_cast<size_t>(kW4Warps + (p.silu ? kW4Warps / p.team : 0) +
+         static_cast<size_t>(w4_red_bufs(w4_nt(p.M)) * kW4Warps + (p.silu ? kW4Warps / p.team : 0) +
                              (p.phases > 1 ? p.panel : 0)) *
              block;
 }
