@@ -315,15 +315,16 @@ int vmps_batch_gemm(void* out, int64_t out_row_stride, const void* x, int64_t x_
  * ctx_lens, seq_lens, q_lens, cu_q: int32 [num_seqs] on the device.
  * max_q_len bounds q_lens (rows past it are not computed and set error bit
  *       64, as do rows outside [0, total_q)).
- * workspace: vmps_paged_tree_attention_workspace_bytes bytes, 256-byte
- *       aligned, no initialisation; calls that may overlap on the GPU need
- *       different workspaces.  The size depends on the device and on the
- *       arguments given, not on the lengths.
+ * workspace: vmps_paged_tree_attention_workspace_bytes bytes (0: none is
+ *       needed, workspace may be NULL), 256-byte aligned, no initialisation;
+ *       calls that may overlap on the GPU need different workspaces.  The size
+ *       depends on the device and on the arguments given, not on the lengths;
+ *       a workspace that is given has at least the size of the widest table's.
  * Supported: head_dim 64 or 128, block_size 16, n_q / n_kv a whole number up
  * to 16, n_kv <= 64, num_seqs <= 4096, max_q_len <= 1024.
  */
 size_t vmps_paged_tree_attention_workspace_bytes(int num_seqs, int max_q_len, int n_q, int n_kv,
-                                                 int head_dim, int dtype);
+                                                 int head_dim, int max_blocks_per_seq, int dtype);
 int vmps_paged_tree_attention(void* out, const void* q, int64_t q_row_stride, const void* pool,
                               const int32_t* block_tables, int max_blocks_per_seq,
                               const int32_t* ctx_lens, const int32_t* seq_lens,

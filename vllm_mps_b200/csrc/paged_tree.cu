@@ -967,6 +967,9 @@ struct TreeLayout {
   size_t records, ml, o, total;
 };
 
+// Contexts of at most kWholeTiles key tiles are not cut into pieces.
+bool tree_whole(int max_blocks) { return max_blocks <= kWholeTiles * kTtPages; }
+
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 TreeLayout tree_layout(int max_q_len, int n_q, int n_kv, int D, int n_cta) {
@@ -1027,10 +1030,11 @@ int launch_tree(const CUtensorMap& kv_map, const CUtensorMap& q_map, const TreeP
 using namespace vmps;
 
 extern "C" size_t vmps_paged_tree_attention_workspace_bytes(int num_seqs, int max_q_len, int n_q,
-                                                            int n_kv, int head_dim, int dtype) {
-  if (num_seqs < 0 || max_q_len < 0 || max_q_len > kTtMaxQLen ||
+                                                            int n_kv, int head_dim,
+                                                            int max_blocks_per_seq, int dtype) {
+  if (num_seqs <= 0 || max_q_len <= 0 || max_q_len > kTtMaxQLen ||
       (dtype != VMPS_DTYPE_F16 && dtype != VMPS_DTYPE_BF16) ||
-      !tree_shape_ok(n_q, n_kv, head_dim)) {
+      !tree_shape_ok(n_q, n_kv, head_dim) || tree_whole(max_blocks_per_seq)) {
     return 0;
   }
   int sms = 0;
@@ -1098,7 +1102,9 @@ extern "C" int vmps_paged_tree_attention(
   p.n_cta = sms * kTtCtasPerSm;
   if (p.n_cta > 1024) return fail(VMPS_ERR_UNSUPPORTED, "%s: %d SMs", what, sms);
   const TreeLayout wl = tree_layout(max_q_len, n_q, n_kv, head_dim, p.n_cta);
-  if (!workspace || workspace_bytes < wl.total) {
+  const bool whole = tree_whole(max_blocks_per_seq);
+  // One that is given has to do for any context, one that is not needed may be missing.
+  if (workspace ? workspace_bytes < wl.total : !whole) {
     return fail(VMPS_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu needed", what, workspace_bytes,
                 wl.total);
   }
@@ -1157,7 +1163,7 @@ extern "C" int vmps_paged_tree_attention(
   p.G = G;
   p.num_blocks = num_blocks;
   p.row_tiles = (max_q_len + p.tokens_per_tile - 1) / p.tokens_per_tile;
-  p.whole = max_tiles <= kWholeTiles ? 1 : 0;
+  p.whole = whole ? 1 : 0;
   p.part_rows = wl.part_rows;
   p.scale_log2 = scale * 1.4426950408889634f;
   uint8_t* ws = static_cast<uint8_t*>(workspace);

@@ -132,7 +132,7 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.vmps_batch_gemm.argtypes = [vp, i64, vp, i64, vp, i32, i32, i32, vp, ctypes.c_size_t,
                                         i32, vp]
         lib.vmps_paged_tree_attention_workspace_bytes.restype = sz
-        lib.vmps_paged_tree_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32]
+        lib.vmps_paged_tree_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32, i32]
         lib.vmps_paged_tree_attention.restype = i32
         lib.vmps_paged_tree_attention.argtypes = [
             vp, vp, i64, vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32,
@@ -669,6 +669,37 @@ def batch_gemm(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None
 
 
 # ── speculative decoding: tree attention, commit, 4-bit products ─────────────
+#
+# A drafting step calls these a few hundred times per token, on small work, so
+# their checks and launches are kept to a few microseconds of host time.
+
+
+def _device_index(first: torch.Tensor, *tensors: torch.Tensor | None) -> int:
+    """The index of the CUDA device all tensors are on (raises as _require_cuda)."""
+    dev = first.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            _require_cuda(first, *tensors)
+    if dev < 0:
+        _require_cuda(first)
+    return dev
+
+
+def _launch(fn, dev: int, *args) -> int:
+    """``fn(*args, current stream of dev)`` with dev as the current device."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if torch.cuda.current_device() == dev:
+        return fn(*args, stream)
+    with torch.cuda.device(dev):
+        return fn(*args, stream)
+
+
+def _lengths(B: int, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            _int32(t, name)
+        if t.numel() != B:
+            raise ValueError(f"{name} must have one entry per sequence ({B}, got {t.numel()})")
 
 
 def paged_tree_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torch.Tensor,
@@ -687,61 +718,78 @@ def paged_tree_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torc
 
     ``q``: (total_q, n_q, D) rotated queries, heads packed (rows may be
     strided); ``tree_mask``: int32 (total_q, words); the length tensors int32
-    (B,) on the device; ``max_q_len`` >= every ``q_lens`` entry (host int).
-    One row per sequence is a decode step.  ``workspace``: a device tensor of
-    :func:`paged_tree_attention_workspace_bytes` bytes, else one from torch's
-    caching allocator for this call (stream-ordered, so calls on different
-    streams never share it).  Returns ``out`` (total_q, n_q, D).
+    (B,) on the device; ``max_q_len`` >= every ``q_lens`` entry (host int, <=
+    1024).  One row per sequence is a decode step.  ``workspace``: a device
+    tensor of :func:`paged_tree_attention_workspace_bytes` bytes, else one from
+    torch's caching allocator for this call (stream-ordered, so calls on
+    different streams never share it).  Returns ``out`` (total_q, n_q, D).
     """
-    num_blocks, block_size, n_kv, D = _check_pool(pool)
+    shape = pool.shape
+    if len(shape) != 5 or shape[1] != 2 or not pool.is_contiguous():
+        _check_pool(pool)
+    num_blocks, _, block_size, n_kv, D = shape
     if q.dim() == 2:
         q = q.view(q.shape[0], -1, D)
     if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or q.stride(1) != D:
         raise ValueError(f"q must be (total_q, n_q, {D}) with packed heads; got {tuple(q.shape)}")
-    total_q, n_q = q.shape[0], q.shape[1]
+    total_q, n_q, _ = q.shape
     B = q_lens.numel()
     if block_tables.dim() != 2 or block_tables.shape[0] != B:
         raise ValueError("block_tables must be (B, max_blocks)")
-    if ctx_lens.numel() != B or seq_lens.numel() != B or cu_q.numel() != B:
-        raise ValueError("ctx_lens, seq_lens, q_lens and cu_q must have one entry per sequence")
     if tree_mask.dim() != 2 or tree_mask.shape[0] != total_q or tree_mask.shape[1] < 1:
         raise ValueError(f"tree_mask must be (total_q, words) with total_q={total_q}")
     if q.dtype != pool.dtype:
         raise TypeError(f"q dtype {q.dtype} != pool dtype {pool.dtype}")
-    for t, name in ((block_tables, "block_tables"), (ctx_lens, "ctx_lens"), (seq_lens, "seq_lens"),
-                    (q_lens, "q_lens"), (cu_q, "cu_q"), (tree_mask, "tree_mask")):
-        _int32(t, name)
+    _lengths(B, ctx_lens=ctx_lens, seq_lens=seq_lens, q_lens=q_lens, cu_q=cu_q)
+    _int32(block_tables, "block_tables")
+    _int32(tree_mask, "tree_mask")
     if out is None:
-        out = torch.empty((total_q, n_q, D), dtype=q.dtype, device=q.device)
-    elif out.shape != (total_q, n_q, D) or out.dtype != q.dtype or not out.is_contiguous():
+        out = q.new_empty((total_q, n_q, D))
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous (total_q, n_q, D) tensor of q's dtype")
-    dev = _require_cuda(q, pool, block_tables, ctx_lens, seq_lens, q_lens, cu_q, tree_mask, out,
+    dev = _device_index(q, pool, block_tables, ctx_lens, seq_lens, q_lens, cu_q, tree_mask, out,
                         workspace)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    lib = load_library()
+    lib = _lib or load_library()
     code = dtype_code(pool.dtype)
-    with torch.cuda.device(dev):
-        if workspace is None:
-            need = lib.vmps_paged_tree_attention_workspace_bytes(B, int(max_q_len), n_q, n_kv, D,
-                                                                 code)
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        # torch gives a single row any stride; the kernel never steps by it.
-        rc = lib.vmps_paged_tree_attention(
-            _ptr(out), _ptr(q), q.stride(0) if total_q > 1 else n_q * D, _ptr(pool), _ptr(block_tables), block_tables.shape[1],
-            _ptr(ctx_lens), _ptr(seq_lens), _ptr(q_lens), _ptr(cu_q), _ptr(tree_mask),
-            tree_mask.shape[1], B, total_q, int(max_q_len), n_q, n_kv, D, block_size, num_blocks,
-            float(scale), _ptr(workspace), workspace.numel() * workspace.element_size(), code,
-            _stream(dev))
-    _check(rc, "paged_tree_attention")
+    max_blocks = block_tables.shape[1]
+    if workspace is None:
+        need = paged_tree_attention_workspace_bytes(B, max_q_len, n_q, n_kv, D, pool.dtype,
+                                                    max_blocks, dev)
+        if need:
+            workspace = pool.new_empty(need, dtype=torch.uint8)
+    ws_ptr, ws_bytes = (None, 0) if workspace is None else (
+        workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    # torch gives a single row any stride; the kernel never steps by it.
+    rc = _launch(lib.vmps_paged_tree_attention, dev,
+                 out.data_ptr(), q.data_ptr(), q.stride(0) if total_q > 1 else n_q * D,
+                 pool.data_ptr(), block_tables.data_ptr(), max_blocks, ctx_lens.data_ptr(),
+                 seq_lens.data_ptr(), q_lens.data_ptr(), cu_q.data_ptr(), tree_mask.data_ptr(),
+                 tree_mask.shape[1], B, total_q, max_q_len, n_q, n_kv, D, block_size, num_blocks,
+                 scale, ws_ptr, ws_bytes, code)
+    if rc:
+        _check(rc, "paged_tree_attention")
     return out
 
 
 def paged_tree_attention_workspace_bytes(num_seqs: int, max_q_len: int, n_q: int, n_kv: int,
-                                         d: int, dtype: torch.dtype) -> int:
-    """Bytes of workspace ``paged_tree_attention`` needs (0: shape not built).  Needs a CUDA device."""
-    return int(load_library().vmps_paged_tree_attention_workspace_bytes(
-        int(num_seqs), int(max_q_len), int(n_q), int(n_kv), int(d), dtype_code(dtype)))
+                                         d: int, dtype: torch.dtype,
+                                         max_blocks: int | None = None,
+                                         device: int | None = None) -> int:
+    """Bytes of workspace ``paged_tree_attention`` needs (0: none).  Needs a CUDA device.
+
+    ``max_blocks``: the width of the block tables (None: any); sequences are
+    cut into pieces, which is what takes a workspace, only where it allows
+    contexts that are worth it.
+    """
+    lib = _lib or load_library()
+    args = (num_seqs, max_q_len, n_q, n_kv, d, (1 << 26) if max_blocks is None else max_blocks,
+            dtype_code(dtype))
+    if device is None or torch.cuda.current_device() == device:
+        return lib.vmps_paged_tree_attention_workspace_bytes(*args)
+    with torch.cuda.device(device):
+        return lib.vmps_paged_tree_attention_workspace_bytes(*args)
 
 
 def commit_tree(pool: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
@@ -764,39 +812,42 @@ def commit_tree(pool: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.
     -1 after the last; int32 (B,) how many; int64 (B,) the model's token after
     the last of them.
     """
+    shape = pool.shape
     layers = 1
-    one = pool
-    if pool.dim() == 6:
-        layers = pool.shape[0]
-        if layers == 0 or not pool.is_contiguous():
-            raise ValueError("pool must be contiguous with at least one layer")
-        one = pool[0]
-    num_blocks, block_size, n_kv, D = _check_pool(one)
+    if len(shape) == 6:
+        layers, shape = shape[0], shape[1:]
+    if len(shape) != 5 or shape[1] != 2 or layers < 1 or not pool.is_contiguous():
+        raise ValueError("pool must be a contiguous ([layers,] num_blocks, 2, block_size, n_kv, "
+                         f"head_dim); got {tuple(pool.shape)}")
+    num_blocks, _, block_size, n_kv, D = shape
     B = ctx_lens.numel()
     if block_tables.dim() != 2 or block_tables.shape[0] != B:
         raise ValueError("block_tables must be (B, max_blocks)")
-    if seq_lens.numel() != B or cu_tree.numel() != B:
-        raise ValueError("ctx_lens, seq_lens and cu_tree must have one entry per sequence")
     n = tokens.numel()
     if parents.numel() != n or target_ids.numel() != n:
         raise ValueError("parents, tokens and target_ids must have one entry per drafted node")
-    for t, name in ((block_tables, "block_tables"), (ctx_lens, "ctx_lens"), (seq_lens, "seq_lens"),
-                    (cu_tree, "cu_tree"), (parents, "parents"), (tokens, "tokens")):
-        _int32(t, name)
+    _lengths(B, ctx_lens=ctx_lens, seq_lens=seq_lens, cu_tree=cu_tree)
+    _int32(block_tables, "block_tables")
+    _int32(parents, "parents")
+    _int32(tokens, "tokens")
     if target_ids.dtype != torch.int64 or not target_ids.is_contiguous():
         raise TypeError("target_ids must be contiguous int64")
-    dev = _require_cuda(pool, block_tables, ctx_lens, seq_lens, cu_tree, parents, tokens, target_ids)
-    path = torch.empty((B, int(max_tree)), dtype=torch.int32, device=dev)
-    count = torch.empty(B, dtype=torch.int32, device=dev)
-    nxt = torch.empty(B, dtype=torch.int64, device=dev)
-    lib = load_library()
-    with torch.cuda.device(dev):
-        rc = lib.vmps_commit_tree(
-            _ptr(path), _ptr(count), _ptr(nxt), _ptr(pool), layers, _ptr(block_tables),
-            block_tables.shape[1], _ptr(ctx_lens), _ptr(seq_lens), _ptr(cu_tree), _ptr(parents),
-            _ptr(tokens), _ptr(target_ids), B, n, int(max_tree), n_kv, D, block_size, num_blocks,
-            dtype_code(pool.dtype), _stream(dev))
-    _check(rc, "commit_tree")
+    dev = _device_index(pool, block_tables, ctx_lens, seq_lens, cu_tree, parents, tokens,
+                        target_ids)
+    if max_tree < 1:
+        raise ValueError(f"max_tree must be at least 1 (got {max_tree})")
+    path = tokens.new_empty((B, max_tree))
+    count = tokens.new_empty(B)
+    nxt = target_ids.new_empty(B)
+    lib = _lib or load_library()
+    rc = _launch(lib.vmps_commit_tree, dev,
+                 path.data_ptr(), count.data_ptr(), nxt.data_ptr(), pool.data_ptr(), layers,
+                 block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(),
+                 seq_lens.data_ptr(), cu_tree.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                 target_ids.data_ptr(), B, n, max_tree, n_kv, D, block_size, num_blocks,
+                 dtype_code(pool.dtype))
+    if rc:
+        _check(rc, "commit_tree")
     return path, count, nxt
 
 
@@ -884,19 +935,20 @@ def w4_gemm(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None,
         raise ValueError("silu_mul needs a [gate; up] weight with an even row count")
     N = w.N // 2 if silu_mul else w.N
     if out is None:
-        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        out = x.new_empty((M, N))
     elif out.shape != (M, N) or out.dtype != x.dtype or out.stride(1) != 1:
         raise ValueError(f"out must be ({M}, {N}) of x's dtype with unit inner stride")
-    dev = _require_cuda(x, w.codes, w.scales, w.zeros, out)
-    lib = load_library()
+    zeros = w.zeros
+    dev = _device_index(x, w.codes, w.scales, zeros, out)
+    lib = _lib or load_library()
     # torch gives a single row any stride; the kernel never steps by it.
-    xs = x.stride(0) if M > 1 else K
-    os_ = out.stride(0) if M > 1 else N
-    with torch.cuda.device(dev):
-        rc = lib.vmps_w4_gemm(_ptr(out), os_, _ptr(x), xs, _ptr(w.codes), _ptr(w.scales),
-                              _ptr(w.zeros), M, N, K, w.group_size, int(bool(silu_mul)),
-                              dtype_code(x.dtype), _stream(dev))
-    _check(rc, "w4_gemm")
+    rc = _launch(lib.vmps_w4_gemm, dev,
+                 out.data_ptr(), out.stride(0) if M > 1 else N, x.data_ptr(),
+                 x.stride(0) if M > 1 else K, w.codes.data_ptr(), w.scales.data_ptr(),
+                 None if zeros is None else zeros.data_ptr(), M, N, K, w.group_size,
+                 1 if silu_mul else 0, dtype_code(x.dtype))
+    if rc:
+        _check(rc, "w4_gemm")
     return out
 
 
