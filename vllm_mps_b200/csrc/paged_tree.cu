@@ -101,7 +101,7 @@ struct TreeParams {
   int tokens_per_tile, row_tiles, n_cta, whole, box_tokens;
   int part_rows;     // rows of a partial record (a multiple of 32)
   float scale_log2;
-  int* records;      // [n_cta][8]: a cut sequence whose second piece CTA b holds
+  int* records;      // [6][n_cta]: the cut sequence whose second piece CTA b holds, -1 if none
   float2* part_ml;   // [n_cta * 2][part_rows]
   float4* part_o;    // [n_cta * 2][D / 4][part_rows]
   int* err;
@@ -140,8 +140,15 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int s, bool rep
 // if it holds no slot).
 __device__ __forceinline__ int tree_tiles(int n) { return n > 0 ? (n + kTtKeys - 1) / kTtKeys : 1; }
 
-__device__ __forceinline__ int tree_weight(const TreeSeq& q, int first_token) {
-  return q.q_len > first_token ? tree_tiles(q.n) * kTileWeight + kSegWeight : 0;
+// Weight in row tile index rt of a sequence packed as tiles << 8 | row tiles.
+__device__ __forceinline__ int tree_weight(int packed, int rt) {
+  return (packed & 255) > rt ? (packed >> 8) * kTileWeight + kSegWeight : 0;
+}
+
+// Quotient of non-negative numbers: 32-bit where both fit (four times faster).
+__device__ __forceinline__ long long tree_div(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
 }
 
 // Largest s in [0, n) with pref[s] <= f (pref non-decreasing, pref[0] = 0).
@@ -177,7 +184,7 @@ __device__ __forceinline__ TreePos tree_pos(const int* wpref, int num_seqs, int 
     r.j = 0;
     return r;
   }
-  r.kvh = static_cast<int>(w / wt);
+  r.kvh = static_cast<int>(tree_div(w, wt));
   const int f = static_cast<int>(w - static_cast<long long>(r.kvh) * wt);
   r.s = tree_find(wpref, num_seqs, f);
   const int off = f - wpref[r.s];
@@ -235,7 +242,7 @@ __device__ __forceinline__ int tree_owner(const int* wpref, int num_seqs, const 
                                           int kvh, int s, int j) {
   const long long w = static_cast<long long>(kvh) * wpref[num_seqs] + wpref[s] + kSegWeight +
                       static_cast<long long>(j) * kTileWeight;
-  return static_cast<int>(w / sh.chunk);
+  return static_cast<int>(tree_div(w, sh.chunk));
 }
 
 // 64 visibility bits of a row for keys [t0, t0 + 64).
@@ -377,17 +384,22 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
   tt_pdl_trigger();
 
   // ── plan ───────────────────────────────────────────────────────────────────
+  // wpref[s + 1] first holds sequence s's tiles (upper bits) and how many row
+  // tiles it has (lower 8), so that the lengths are read from memory once.
+  for (int s = threadIdx.x; s < num_seqs; s += kTtThreads) {
+    const TreeSeq q = tree_seq(p, s, blockIdx.x == 0);
+    wpref[s + 1] = (tree_tiles(q.n) << 8) | ((q.q_len + p.tokens_per_tile - 1) / p.tokens_per_tile);
+  }
+  __syncthreads();
   for (int rt = warp; rt < p.row_tiles; rt += kTtThreads / 32) {
     int sum = 0;
-    for (int s = lane; s < num_seqs; s += 32) {
-      const bool report = blockIdx.x == 0 && rt == 0;
-      sum += tree_weight(tree_seq(p, s, report), rt * p.tokens_per_tile);
-    }
+    for (int s = lane; s < num_seqs; s += 32) sum += tree_weight(wpref[s + 1], rt);
     for (int sh = 16; sh; sh >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
     if (lane == 0) rt_weight[rt] = sum;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (warp == 0) {
+    // Every lane does the same (the divisions are what takes the time).
     long long total = 0;
     int used = 0;  // row tile indices with work: the first ones
     for (int rt = 0; rt < p.row_tiles && rt_weight[rt] > 0; ++rt, ++used) {
@@ -396,29 +408,21 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
     // Row tile indices start on a CTA of their own, which can leave up to
     // used - 1 shares partly empty.
     const int div = p.n_cta - (used > 0 ? used - 1 : 0);
-    long long chunk = (total + div - 1) / div;
+    long long chunk = tree_div(total + div - 1, div);
     const long long least = kMinTiles * kTileWeight + kSegWeight;
     if (chunk < least) chunk = least;
     int first = 0, rt = 0;
     for (; rt < used; ++rt) {
       const long long w = static_cast<long long>(rt_weight[rt]) * p.n_kv;
-      const int n = static_cast<int>((w + chunk - 1) / chunk);
+      const int n = static_cast<int>(tree_div(w + chunk - 1, chunk));
       if (static_cast<int>(blockIdx.x) < first + n) break;
       first += n;
     }
-    share->rt = rt < used ? rt : -1;
-    share->first_cta = first;
-    share->chunk = static_cast<int>(chunk);
-  }
-  __syncthreads();
-  const int rt = share->rt;
-  const int tok0 = rt * p.tokens_per_tile;
-  if (warp == 0) {
+    if (rt == used) rt = -1;
     int carry = 0;
-    if (lane == 0) wpref[0] = 0;
     for (int base = 0; base < num_seqs; base += 32) {
       const int s = base + lane;
-      int v = rt >= 0 && s < num_seqs ? tree_weight(tree_seq(p, s, false), tok0) : 0;
+      int v = rt >= 0 && s < num_seqs ? tree_weight(wpref[s + 1], rt) : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, v, o);
@@ -427,20 +431,24 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
       if (s < num_seqs) wpref[s + 1] = v + carry;
       carry += __shfl_sync(0xffffffffu, v, 31);
     }
+    if (lane == 0) wpref[0] = 0;
     __syncwarp();
-    if (lane == 0) {
-      TreePos b, e;
+    // Lane 0 finds the share's begin, lane 1 its end.
+    if (lane < 2) {
+      TreePos b;
+      b.kvh = b.s = b.j = 0;
       if (rt >= 0) {
-        const long long w0 = static_cast<long long>(blockIdx.x - share->first_cta) * share->chunk;
+        const long long w0 = static_cast<long long>(blockIdx.x - first + lane) * chunk;
         b = tree_pos(wpref, num_seqs, p.n_kv, p.whole, w0);
-        e = tree_pos(wpref, num_seqs, p.n_kv, p.whole, w0 + share->chunk);
-      } else {
-        b.kvh = e.kvh = 0;
-        b.s = e.s = 0;
-        b.j = e.j = 0;
       }
-      share->begin = b;
-      share->end = e;
+      if (lane == 0) {
+        share->rt = rt;
+        share->first_cta = first;
+        share->chunk = static_cast<int>(chunk);
+        share->begin = b;
+      } else {
+        share->end = b;
+      }
     }
   }
   tc_fence_before();
@@ -448,6 +456,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const TreeShare sh = *share;
+  const int tok0 = sh.rt * p.tokens_per_tile;
 
   if (warp == kTtKWarp || warp == kTtVWarp) {
     // ── loads: one warp streams K tiles (and Q), another V tiles ──────────────
@@ -840,7 +849,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
     if (!ok) *abort_flag = 1;
     if (threadIdx.x == 0 && !p.whole) {
 #pragma unroll
-      for (int i = 0; i < 6; ++i) p.records[blockIdx.x * 8 + i] = rec[i];
+      for (int i = 0; i < 6; ++i) p.records[i * p.n_cta + blockIdx.x] = rec[i];
     }
   }
 
@@ -855,13 +864,20 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
 }
 
 // Joins the pieces of cut sequences.  A unit is 32 rows x 16 columns of one of
-// them; the block's warps take its pieces in turn and their partial results
-// are joined through shared memory, all in a fixed order.
+// them.  A unit's pieces go to 1, 2, 4 or 8 warps of a block (as many as the
+// number of units leaves idle otherwise: a batch has many sequences of two or
+// three pieces, a long context few of dozens), each taking every n-th piece,
+// and the warps' results are joined through shared memory, all in a fixed
+// order.  Bound: the partial results, read from L2; one warp per unit alone
+// took 19 us for 74 pieces of 4 kv heads, eight always 30 us for 256 items of
+// two pieces.
 template <typename T, int D>
-__global__ void __launch_bounds__(kMergeThreads) paged_tree_merge_kernel(const __grid_constant__ TreeParams p) {
+__global__ void __launch_bounds__(kMergeThreads)
+    paged_tree_merge_kernel(const __grid_constant__ TreeParams p) {
   constexpr int kWarps = kMergeThreads / 32;
   constexpr int kQuads = kMergeCols / 4;
   constexpr int kColUnits = D / kMergeCols;
+  constexpr int kBatch = 4;     // pieces in flight per warp
   __shared__ int s_item[1024];  // CTAs whose record is a join, in order
   __shared__ int s_base[kWarps + 1];
   __shared__ float s_ml[kWarps][32][2];
@@ -871,7 +887,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_tree_merge_kernel(const _
   int n_items = 0;
   for (int base = 0; base < p.n_cta; base += kMergeThreads) {
     const int b = base + threadIdx.x;
-    const bool on = b < p.n_cta && p.records[b * 8] >= 0;
+    const bool on = b < p.n_cta && p.records[b] >= 0;
     const unsigned mask = __ballot_sync(0xffffffffu, on);
     if (lane == 0) s_base[warp + 1] = __popc(mask);
     __syncthreads();
@@ -886,13 +902,26 @@ __global__ void __launch_bounds__(kMergeThreads) paged_tree_merge_kernel(const _
   }
   const int row_units = p.part_rows / 32;
   const int units = n_items * row_units * kColUnits;
-  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+  int per_unit = 1;  // warps
+  while (per_unit < kWarps && units * per_unit * 2 <= static_cast<int>(gridDim.x) * kWarps) per_unit *= 2;
+  const int groups = kWarps / per_unit;  // units a block works on at once
+  const int sub = warp & (per_unit - 1), group = warp / per_unit;
+  for (int first = blockIdx.x * groups; first < units; first += gridDim.x * groups) {
+    const int unit = first + group;
     const int item = unit / (row_units * kColUnits);
     const int rest = unit - item * (row_units * kColUnits);
     const int ru = rest / kColUnits, cu = rest - ru * kColUnits;
-    const int* rec = p.records + s_item[item] * 8;
-    const int s = rec[0], kvh = rec[1], tok0 = rec[2], c0 = rec[3], c1 = rec[4], rows = rec[5];
-    if (ru * 32 >= rows) continue;
+    int s = 0, kvh = 0, tok0 = 0, c0 = 0, c1 = -1, rows = 0;
+    if (unit < units) {
+      const int* rec = p.records + s_item[item];
+      s = rec[0];
+      kvh = rec[p.n_cta];
+      tok0 = rec[2 * p.n_cta];
+      c0 = rec[3 * p.n_cta];
+      c1 = rec[4 * p.n_cta];
+      rows = rec[5 * p.n_cta];
+    }
+    const bool on = ru * 32 < rows;
     const int row = ru * 32 + lane;
     float m_run = -INFINITY, l_run = 0.f;
     float4 o[kQuads];
@@ -912,46 +941,59 @@ __global__ void __launch_bounds__(kMergeThreads) paged_tree_merge_kernel(const _
       }
       m_run = mn;
     };
-#pragma unroll 2
-    for (int c = c0 + warp; c <= c1; c += kWarps) {
-      const size_t piece = static_cast<size_t>(c) * 2 + (c == c0 ? 1 : 0);
-      const float2 ml = __ldcg(p.part_ml + piece * p.part_rows + row);
-      const float4* src = p.part_o + (piece * (D / 4) + cu * kQuads) * p.part_rows + row;
-      float4 v[kQuads];
+    if (on) {
+      for (int c = c0 + sub; c <= c1; c += per_unit * kBatch) {
+        float2 ml[kBatch];
+        float4 v[kBatch][kQuads];
 #pragma unroll
-      for (int i = 0; i < kQuads; ++i) v[i] = __ldcg(src + static_cast<size_t>(i) * p.part_rows);
-      fold(ml.x, ml.y, v);
-    }
-    s_ml[warp][lane][0] = m_run;
-    s_ml[warp][lane][1] = l_run;
+        for (int k = 0; k < kBatch; ++k) {
+          const int cc = c + k * per_unit;
+          if (cc <= c1) {
+            const size_t piece = static_cast<size_t>(cc) * 2 + (cc == c0 ? 1 : 0);
+            ml[k] = __ldcg(p.part_ml + piece * p.part_rows + row);
+            const float4* src = p.part_o + (piece * (D / 4) + cu * kQuads) * p.part_rows + row;
 #pragma unroll
-    for (int i = 0; i < kQuads; ++i) s_o[warp][i][lane] = o[i];
-    __syncthreads();
-    if (warp == 0) {
-      for (int x = 1; x < kWarps; ++x) {
-        float4 v[kQuads];
-#pragma unroll
-        for (int i = 0; i < kQuads; ++i) v[i] = s_o[x][i][lane];
-        fold(s_ml[x][lane][0], s_ml[x][lane][1], v);
-      }
-      if (row < rows) {
-        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-        const int token = row / p.G;
-        T* dst = static_cast<T*>(p.out) +
-                 (static_cast<size_t>(p.cu_q[s] + tok0 + token) * p.n_q + kvh * p.G + row - token * p.G) * D +
-                 cu * kMergeCols;
-        uint32_t packed[2 * kQuads];
-#pragma unroll
-        for (int i = 0; i < kQuads; ++i) {
-          packed[2 * i] = Elt<T>::pack(o[i].x * inv, o[i].y * inv);
-          packed[2 * i + 1] = Elt<T>::pack(o[i].z * inv, o[i].w * inv);
+            for (int i = 0; i < kQuads; ++i) v[k][i] = __ldcg(src + static_cast<size_t>(i) * p.part_rows);
+          }
         }
-        uint4* d4 = reinterpret_cast<uint4*>(dst);
-        d4[0] = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-        d4[1] = make_uint4(packed[4], packed[5], packed[6], packed[7]);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          if (c + k * per_unit <= c1) fold(ml[k].x, ml[k].y, v[k]);
+        }
       }
     }
-    __syncthreads();
+    if (per_unit > 1) {
+      s_ml[warp][lane][0] = m_run;
+      s_ml[warp][lane][1] = l_run;
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i) s_o[warp][i][lane] = o[i];
+      __syncthreads();
+      if (sub == 0) {
+        for (int x = warp + 1; x < warp + per_unit; ++x) {
+          float4 v[kQuads];
+#pragma unroll
+          for (int i = 0; i < kQuads; ++i) v[i] = s_o[x][i][lane];
+          fold(s_ml[x][lane][0], s_ml[x][lane][1], v);
+        }
+      }
+    }
+    if (sub == 0 && row < rows) {
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+      const int token = row / p.G;
+      T* dst = static_cast<T*>(p.out) +
+               (static_cast<size_t>(p.cu_q[s] + tok0 + token) * p.n_q + kvh * p.G + row - token * p.G) * D +
+               cu * kMergeCols;
+      uint32_t packed[2 * kQuads];
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i) {
+        packed[2 * i] = Elt<T>::pack(o[i].x * inv, o[i].y * inv);
+        packed[2 * i + 1] = Elt<T>::pack(o[i].z * inv, o[i].w * inv);
+      }
+      uint4* d4 = reinterpret_cast<uint4*>(dst);
+      d4[0] = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+      d4[1] = make_uint4(packed[4], packed[5], packed[6], packed[7]);
+    }
+    if (per_unit > 1) __syncthreads();
   }
 }
 
@@ -1072,11 +1114,11 @@ extern "C" int vmps_paged_tree_attention(
   }
   // The plan sums a row tile's tiles over all sequences in 31 bits.
   const long long max_tiles = (static_cast<long long>(max_blocks_per_seq) + kTtPages - 1) / kTtPages;
-  if (num_seqs > kTtMaxSeqs || max_q_len > kTtMaxQLen || max_blocks_per_seq > (1 << 26) ||
+  if (num_seqs > kTtMaxSeqs || max_q_len > kTtMaxQLen || max_blocks_per_seq > (1 << 24) ||
       num_seqs * (max_tiles * kTileWeight + kSegWeight) > 0x7fffffffLL) {
     return fail(VMPS_ERR_UNSUPPORTED,
                 "%s: num_seqs=%d max_q_len=%d max_blocks=%d (num_seqs <= %d, max_q_len <= %d, "
-                "num_seqs * max_blocks < 2^31)",
+                "max_blocks <= 2^24, num_seqs * max_blocks < 2^31)",
                 what, num_seqs, max_q_len, max_blocks_per_seq, kTtMaxSeqs, kTtMaxQLen);
   }
   if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return VMPS_OK;

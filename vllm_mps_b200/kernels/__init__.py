@@ -784,7 +784,7 @@ def paged_tree_attention_workspace_bytes(num_seqs: int, max_q_len: int, n_q: int
     contexts that are worth it.
     """
     lib = _lib or load_library()
-    args = (num_seqs, max_q_len, n_q, n_kv, d, (1 << 26) if max_blocks is None else max_blocks,
+    args = (num_seqs, max_q_len, n_q, n_kv, d, (1 << 24) if max_blocks is None else max_blocks,
             dtype_code(dtype))
     if device is None or torch.cuda.current_device() == device:
         return lib.vmps_paged_tree_attention_workspace_bytes(*args)
