@@ -62,7 +62,6 @@ constexpr int kPage = 16;
 constexpr int kTtRows = 128;                  // MMA M
 constexpr int kTtKeys = 64;                   // keys per tile
 constexpr int kTtPages = kTtKeys / kPage;
-constexpr int kTtStages = 2;                  // K ring and V ring depth
 constexpr int kTtThreads = 224;
 constexpr int kTtKWarp = 4, kTtVWarp = 5, kTtMmaWarp = 6;
 constexpr int kTtQChunk = kTtRows * 128;      // 128 rows x 64 16-bit columns
@@ -72,7 +71,7 @@ constexpr int kTtMaxSeqs = 4096;
 constexpr int kTtMaxQLen = 1024;
 constexpr int kTtMaxRowTiles = 128;           // 1024 tokens x 16 heads / 128
 constexpr int kTileWeight = 4;
-constexpr int kSegWeight = 8;
+constexpr int kSegWeight = 16;
 constexpr int kMinTiles = 4;                  // a share holds at least this many tiles
 constexpr int kWholeTiles = 8;                // contexts up to this many tiles are not cut
 constexpr int kMergeThreads = 256;
@@ -80,11 +79,13 @@ constexpr int kMergeCols = 16;                // output columns per merge unit
 
 template <int D>
 struct TreeShape {
+  // K ring and V ring depth: what fits beside Q with two CTAs on an SM.
+  static constexpr int kStages = D == 64 ? 4 : 2;
   static constexpr int kChunks = D / 64;
   static constexpr int kQBytes = kChunks * kTtQChunk;
   static constexpr int kTileBytes = kChunks * kTtKChunk;  // K (or V) of one key tile
   static constexpr int kBarBytes = 512 + kTtMaxRowTiles * 4;
-  static constexpr int kFixedBytes = kQBytes + 2 * kTtStages * kTileBytes + kBarBytes;
+  static constexpr int kFixedBytes = kQBytes + 2 * kStages * kTileBytes + kBarBytes;
   static constexpr uint32_t kTmemCols = 256;  // S 2 x 64 columns, O up to 128
 };
 
@@ -318,8 +319,8 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
   }
   uint8_t* sQ = smem_raw;
   uint8_t* sK = sQ + Shape::kQBytes;
-  uint8_t* sV = sK + kTtStages * Shape::kTileBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kTtStages * Shape::kTileBytes);
+  uint8_t* sV = sK + Shape::kStages * Shape::kTileBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + Shape::kStages * Shape::kTileBytes);
   uint64_t* q_full = bars + 0;
   uint64_t* q_empty = bars + 1;  // the segment's last QK is done with Q
   // [2]: MMA -> softmax, PV of a tile complete, by tile parity.  S of tile i in
@@ -330,10 +331,10 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
   uint64_t* p_full = bars + 6;   // [2]: softmax -> MMA, P in that buffer and O rescaled
   uint64_t* mma_done = bars + 8; // everything issued has completed
   uint64_t* k_full = bars + 9;
-  uint64_t* k_empty = k_full + kTtStages;
-  uint64_t* v_full = k_empty + kTtStages;
-  uint64_t* v_empty = v_full + kTtStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + kTtStages);
+  uint64_t* k_empty = k_full + Shape::kStages;
+  uint64_t* v_full = k_empty + Shape::kStages;
+  uint64_t* v_empty = v_full + Shape::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + Shape::kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // Segment number (+1) whose V held a non-finite draft, by segment parity.
   volatile int* odd_seg = abort_flag + 1;  // [2]
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
       mbar_init(s_full + b, 1);
       mbar_init(p_full + b, 4);
     }
-    for (int st = 0; st < kTtStages; ++st) {
+    for (int st = 0; st < Shape::kStages; ++st) {
       mbar_init(k_full + st, 1);
       mbar_init(k_empty + st, 1);
       mbar_init(v_full + st, 1);
@@ -409,7 +410,9 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
     // used - 1 shares partly empty.
     const int div = p.n_cta - (used > 0 ? used - 1 : 0);
     long long chunk = tree_div(total + div - 1, div);
-    const long long least = kMinTiles * kTileWeight + kSegWeight;
+    // A piece has at least kMinTiles tiles; contexts that are not cut start a
+    // CTA each while there are CTAs left.
+    const long long least = p.whole ? 1 : kMinTiles * kTileWeight + kSegWeight;
     if (chunk < least) chunk = least;
     int first = 0, rt = 0;
     for (; rt < used; ++rt) {
@@ -456,6 +459,10 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const TreeShare sh = *share;
+  // Up to 64 rows need the softmax of two warps (or one).  The two CTAs of an SM
+  // then use different ones -- they hold different halves of its TMEM -- so
+  // that their exponentials do not queue for the same quarter of the SM.
+  const int row_shift = p.box_tokens * p.G <= kTtRows / 2 ? ((tmem_base >> 8) & 1) * (kTtRows / 2) : 0;
   const int tok0 = sh.rt * p.tokens_per_tile;
 
   if (warp == kTtKWarp || warp == kTtVWarp) {
@@ -498,7 +505,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
           mbar_arrive_expect_tx(q_full, Shape::kChunks * p.box_tokens * p.G * 128);
 #pragma unroll
           for (int c = 0; c < Shape::kChunks; ++c) {
-            tma_load_3d(sQ + c * kTtQChunk, &q_map, q_full, c * 64, kvh * p.G, q.row0 + tok0);
+            tma_load_3d(sQ + c * kTtQChunk + row_shift * 128, &q_map, q_full, c * 64, kvh * p.G, q.row0 + tok0);
           }
         }
       }
@@ -523,9 +530,9 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
           blk[pg] = __shfl_sync(0xffffffffu, ids, (page0 + pg) & 31);
         }
         if (lane == 0) {
-          const int st = it % kTtStages;
-          if (it >= kTtStages &&
-              (!mbar_wait(empty + st, ((it / kTtStages) - 1) & 1, p.err) || aborted(abort_flag))) {
+          const int st = it % Shape::kStages;
+          if (it >= Shape::kStages &&
+              (!mbar_wait(empty + st, ((it / Shape::kStages) - 1) & 1, p.err) || aborted(abort_flag))) {
             *abort_flag = 1;
             go = false;
           } else {
@@ -549,8 +556,8 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
     // is released.
     if (lane == 0) {
       if (!is_v && seg > 0) mbar_wait(q_full, (seg - 1) & 1, p.err);
-      for (int i = max(0, it - kTtStages); i < it; ++i) {
-        mbar_wait(full + (i % kTtStages), (i / kTtStages) & 1, p.err);
+      for (int i = max(0, it - Shape::kStages); i < it; ++i) {
+        mbar_wait(full + (i % Shape::kStages), (i / Shape::kStages) & 1, p.err);
       }
     }
   } else if (warp == kTtMmaWarp) {
@@ -569,9 +576,9 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
       bool ok = true;
       auto issue_qk = [&]() -> bool {  // one tile, if any is left
         if (!wq.valid) return true;
-        const int st = iq % kTtStages;
+        const int st = iq % Shape::kStages;
         if (jq == wq.at.j && !mbar_wait(q_full, seg_q & 1, p.err)) return false;
-        if (!mbar_wait(k_full + st, (iq / kTtStages) & 1, p.err) || aborted(abort_flag)) return false;
+        if (!mbar_wait(k_full + st, (iq / Shape::kStages) & 1, p.err) || aborted(abort_flag)) return false;
         tc_fence_after();
         const uint32_t k_addr = smem_u32(sK + st * Shape::kTileBytes);
         const uint32_t t_s = tmem_base + (iq & 1) * KEYS;
@@ -594,9 +601,9 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
       };
       ok = issue_qk() && issue_qk();
       while (ok && wp.valid) {
-        const int st = ip % kTtStages;
+        const int st = ip % Shape::kStages;
         if (!mbar_wait(p_full + (ip & 1), (ip >> 1) & 1, p.err) || aborted(abort_flag) ||
-            !mbar_wait(v_full + st, (ip / kTtStages) & 1, p.err) || aborted(abort_flag)) {
+            !mbar_wait(v_full + st, (ip / Shape::kStages) & 1, p.err) || aborted(abort_flag)) {
           ok = false;
           break;
         }
@@ -625,10 +632,10 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
     }
   } else {
     // ── softmax and epilogue: one row per thread ─────────────────────────────
-    const int m = threadIdx.x;  // row = TMEM lane
+    const int m = threadIdx.x - row_shift;  // row; TMEM lane threadIdx.x
     const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t t_o = tmem_base + lane_base + 2 * KEYS;
-    const int t_row = m / p.G;  // drafted token of the row tile
+    const int t_row = max(m, 0) / p.G;  // drafted token of the row tile
     const int head_in_group = m - t_row * p.G;
     const float scale = p.scale_log2;
     bool ok = true;
@@ -642,8 +649,8 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
       const int s = w.at.s, kvh = w.at.kvh, j0 = w.at.j, j1 = w.j1, tiles = w.tiles;
       const TreeSeq q = tree_seq(p, s, false);
       const int rows = min(p.tokens_per_tile, q.q_len - tok0) * p.G;
-      const bool active = warp * 32 < rows;  // warp-uniform
-      const bool valid = m < rows;
+      const bool active = warp * 32 >= row_shift && warp * 32 - row_shift < rows;  // warp-uniform
+      const bool valid = m >= 0 && m < rows;
       const int row = q.row0 + tok0 + (valid ? t_row : 0);
       const uint32_t* mrow = p.mask + static_cast<size_t>(row) * p.mask_words;
       float m_run = -INFINITY;
@@ -656,13 +663,13 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
         const bool tail = key0 + KEYS > q.ctx;  // reaches drafts or the end
         if (tail) {
           // Clean V: every warp takes its share of the tile's 128-byte lines.
-          const int st = it % kTtStages;
-          ok = mbar_wait(v_full + st, (it / kTtStages) & 1, p.err);
+          const int st = it % Shape::kStages;
+          ok = mbar_wait(v_full + st, (it / Shape::kStages) & 1, p.err);
           ok = __all_sync(0xffffffffu, ok) && !aborted(abort_flag);
           if (!ok) break;
-          if (m < Shape::kChunks * KEYS) {
-            const int t = key0 + (m & (KEYS - 1));
-            uint4* line = reinterpret_cast<uint4*>(sV + st * Shape::kTileBytes + m * 128);
+          if (threadIdx.x < Shape::kChunks * KEYS) {
+            const int t = key0 + (threadIdx.x & (KEYS - 1));
+            uint4* line = reinterpret_cast<uint4*>(sV + st * Shape::kTileBytes + threadIdx.x * 128);
             if (t >= q.n) {
 #pragma unroll
               for (int u = 0; u < 8; ++u) line[u ^ (lane & 7)] = make_uint4(0u, 0u, 0u, 0u);
@@ -872,7 +879,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
 // took 19 us for 74 pieces of 4 kv heads, eight always 30 us for 256 items of
 // two pieces.
 template <typename T, int D>
-__global__ void __launch_bounds__(kMergeThreads)
+__global__ void __launch_bounds__(kMergeThreads, 2)
     paged_tree_merge_kernel(const __grid_constant__ TreeParams p) {
   constexpr int kWarps = kMergeThreads / 32;
   constexpr int kQuads = kMergeCols / 4;
