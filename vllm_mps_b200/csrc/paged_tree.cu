@@ -47,8 +47,8 @@
 // the output once; scores, maxima, sums and accumulators are fp32.
 //
 // Safety.  Every mbarrier wait is bounded; a wait that gives up sets
-// kDevErrTimeout and a CTA-wide abort flag, all roles leave their loops, loads
-// and MMAs in flight are waited for (bounded) and the TMEM is always freed.
+// kDevErrTimeout and a CTA-wide abort flag, the loads and MMAs stop being
+// issued, those in flight are waited for (bounded) and the TMEM is always freed.
 #include <mutex>
 
 #include "vmps_abi_internal.h"
@@ -293,6 +293,23 @@ __device__ __noinline__ float tree_nonfinite(const TreeParams& p, const uint32_t
   return sum;
 }
 
+// Waits for a phase; false once a wait has given up (this one or another's:
+// the CTA's abort flag), which only the slow path looks at.
+__device__ __forceinline__ bool tt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                        int* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kWaitLimitCycles) {
+      set_error(err, kDevErrTimeout);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
 __device__ __forceinline__ void tt_pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void tt_pdl_trigger() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -458,7 +475,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const TreeShare sh = *share;
+  const TreeShare& sh = *share;
   // Up to 64 rows need the softmax of two warps (or one).  The two CTAs of an SM
   // then use different ones -- they hold different halves of its TMEM -- so
   // that their exponentials do not queue for the same quarter of the SM.
@@ -498,8 +515,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
       int ids = first_ids;
       int nxt = fetch(s, n_pages, page_begin + 32 + lane);
       if (!is_v && lane == 0) {
-        if (seg > 0 && (!mbar_wait(q_empty, (seg - 1) & 1, p.err) || aborted(abort_flag))) {
-          *abort_flag = 1;
+        if (seg > 0 && !tt_wait(q_empty, (seg - 1) & 1, abort_flag, p.err)) {
           go = false;
         } else {
           mbar_arrive_expect_tx(q_full, Shape::kChunks * p.box_tokens * p.G * 128);
@@ -532,8 +548,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
         if (lane == 0) {
           const int st = it % Shape::kStages;
           if (it >= Shape::kStages &&
-              (!mbar_wait(empty + st, ((it / Shape::kStages) - 1) & 1, p.err) || aborted(abort_flag))) {
-            *abort_flag = 1;
+              !tt_wait(empty + st, ((it / Shape::kStages) - 1) & 1, abort_flag, p.err)) {
             go = false;
           } else {
             mbar_arrive_expect_tx(full + st, Shape::kTileBytes);
@@ -568,64 +583,70 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
       const uint32_t t_o = tmem_base + 2 * KEYS;
       const uint32_t idesc_qk = f16_idesc<T>(KEYS, false);
       const uint32_t idesc_pv = f16_idesc<T>(D, true);
-      const uint32_t q_addr = smem_u32(sQ);
+      // One lane issues everything, so what it does per MMA counts: operand
+      // descriptors are a base (one per ring slot) plus a constant.
+      const uint64_t q_desc = sw128_desc(smem_u32(sQ), 16, 1024);
+      const uint64_t k_desc = sw128_desc(smem_u32(sK), 16, 1024);
+      const uint64_t v_desc = sw128_desc(smem_u32(sV), kTtKChunk, 1024);
+      constexpr uint64_t kTileStep = Shape::kTileBytes >> 4;
       TreeWalk wq, wp;  // the next QK's segment, the next PV's segment
       wq.start(wpref, num_seqs, sh);
       wp = wq;
-      int jq = wq.at.j, jp = wp.at.j, seg_q = 0, iq = 0, ip = 0;
-      bool ok = true;
+      int left_q = wq.valid ? wq.j1 - wq.at.j : 0, left_p = left_q;
+      int seg_q = 0, iq = 0, ip = 0;
+      bool new_q = true, first = true;
       auto issue_qk = [&]() -> bool {  // one tile, if any is left
         if (!wq.valid) return true;
         const int st = iq % Shape::kStages;
-        if (jq == wq.at.j && !mbar_wait(q_full, seg_q & 1, p.err)) return false;
-        if (!mbar_wait(k_full + st, (iq / Shape::kStages) & 1, p.err) || aborted(abort_flag)) return false;
+        if (new_q && !tt_wait(q_full, seg_q & 1, abort_flag, p.err)) return false;
+        if (!tt_wait(k_full + st, (iq / Shape::kStages) & 1, abort_flag, p.err)) return false;
         tc_fence_after();
-        const uint32_t k_addr = smem_u32(sK + st * Shape::kTileBytes);
+        const uint64_t kd = k_desc + st * kTileStep;
         const uint32_t t_s = tmem_base + (iq & 1) * KEYS;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint64_t a = sw128_desc(q_addr + (k >> 2) * kTtQChunk + (k & 3) * 32, 16, 1024);
-          const uint64_t b = sw128_desc(k_addr + (k >> 2) * kTtKChunk + (k & 3) * 32, 16, 1024);
-          tc_mma(t_s, a, b, idesc_qk, k > 0 ? 1u : 0u);
+          tc_mma(t_s, q_desc + (((k >> 2) * kTtQChunk + (k & 3) * 32) >> 4),
+                 kd + (((k >> 2) * kTtKChunk + (k & 3) * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u);
         }
         tc_commit(k_empty + st);
         tc_commit(s_full + (iq & 1));
         ++iq;
-        if (++jq == wq.j1) {
+        new_q = false;
+        if (--left_q == 0) {
           tc_commit(q_empty);
           wq.next(wpref, num_seqs, sh);
-          jq = wq.at.j;
+          left_q = wq.j1 - wq.at.j;
+          new_q = true;
           ++seg_q;
         }
         return true;
       };
-      ok = issue_qk() && issue_qk();
+      bool ok = issue_qk() && issue_qk();
       while (ok && wp.valid) {
         const int st = ip % Shape::kStages;
-        if (!mbar_wait(p_full + (ip & 1), (ip >> 1) & 1, p.err) || aborted(abort_flag) ||
-            !mbar_wait(v_full + st, (ip / Shape::kStages) & 1, p.err) || aborted(abort_flag)) {
-          ok = false;
+        if (!tt_wait(v_full + st, (ip / Shape::kStages) & 1, abort_flag, p.err) ||
+            !tt_wait(p_full + (ip & 1), (ip >> 1) & 1, abort_flag, p.err)) {
           break;
         }
         tc_fence_after();
-        const uint32_t v_addr = smem_u32(sV + st * Shape::kTileBytes);
+        const uint64_t vd = v_desc + st * kTileStep;
         const uint32_t t_p = tmem_base + (ip & 1) * KEYS;
-        const bool first = jp == wp.at.j;  // a segment's first PV overwrites O
 #pragma unroll
         for (int k = 0; k < KEYS / 16; ++k) {
-          const uint64_t b = sw128_desc(v_addr + k * 2048, kTtKChunk, 1024);
-          tc_mma_ts(t_o, t_p + k * 8, b, idesc_pv, (!first || k > 0) ? 1u : 0u);
+          // A segment's first PV overwrites O.
+          tc_mma_ts(t_o, t_p + k * 8, vd + ((k * 2048) >> 4), idesc_pv, (!first || k > 0) ? 1u : 0u);
         }
         tc_commit(v_empty + st);
         tc_commit(o_ready + (ip & 1));
         ++ip;
-        if (++jp == wp.j1) {
+        first = false;
+        if (--left_p == 0) {
           wp.next(wpref, num_seqs, sh);
-          jp = wp.at.j;
+          left_p = wp.j1 - wp.at.j;
+          first = true;
         }
         ok = issue_qk();
       }
-      if (!ok) *abort_flag = 1;
       // Every MMA this lane issued completes before the TMEM is freed.
       tc_commit(mma_done);
       mbar_wait(mma_done, 0, p.err);
@@ -638,14 +659,13 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
     const int t_row = max(m, 0) / p.G;  // drafted token of the row tile
     const int head_in_group = m - t_row * p.G;
     const float scale = p.scale_log2;
-    bool ok = true;
+    // (After a wait that gave up these warps go through the motions on whatever
+    // TMEM holds: nothing they touch is anyone else's.)
     int it = 0, seg = 0;
+    if (threadIdx.x == 0 && !p.whole) p.records[blockIdx.x] = -1;
     TreeWalk w;
     w.start(wpref, num_seqs, sh);
-    // A sequence that began in the CTA before this one and continues here:
-    // this CTA describes the join of its pieces (it is the second of them).
-    int rec[6] = {-1, 0, 0, 0, 0, 0};
-    while (w.valid && ok) {
+    while (w.valid) {
       const int s = w.at.s, kvh = w.at.kvh, j0 = w.at.j, j1 = w.j1, tiles = w.tiles;
       const TreeSeq q = tree_seq(p, s, false);
       const int rows = min(p.tokens_per_tile, q.q_len - tok0) * p.G;
@@ -656,17 +676,14 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
       float m_run = -INFINITY;
       float l_run = 0.f;
       for (int j = j0; j < j1; ++j, ++it) {
-        ok = mbar_wait(s_full + (it & 1), (it >> 1) & 1, p.err);
-        ok = __all_sync(0xffffffffu, ok) && !aborted(abort_flag);
-        if (!ok) break;
+        tt_wait(s_full + (it & 1), (it >> 1) & 1, abort_flag, p.err);
+        __syncwarp();
         const int key0 = j * KEYS;
         const bool tail = key0 + KEYS > q.ctx;  // reaches drafts or the end
         if (tail) {
           // Clean V: every warp takes its share of the tile's 128-byte lines.
           const int st = it % Shape::kStages;
-          ok = mbar_wait(v_full + st, (it / Shape::kStages) & 1, p.err);
-          ok = __all_sync(0xffffffffu, ok) && !aborted(abort_flag);
-          if (!ok) break;
+          tt_wait(v_full + st, (it / Shape::kStages) & 1, abort_flag, p.err);
           if (threadIdx.x < Shape::kChunks * KEYS) {
             const int t = key0 + (threadIdx.x & (KEYS - 1));
             uint4* line = reinterpret_cast<uint4*>(sV + st * Shape::kTileBytes + threadIdx.x * 128);
@@ -734,9 +751,8 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
           } else if (__any_sync(0xffffffffu, m_new > m_run + 8.f)) {
             // The running maximum only has to bound the scores to within 2^8:
             // O is rescaled (once the PV before has landed) when it grew by more.
-            ok = mbar_wait(o_ready + ((it - 1) & 1), ((it - 1) >> 1) & 1, p.err);
-            ok = __all_sync(0xffffffffu, ok) && !aborted(abort_flag);
-            if (!ok) break;
+            tt_wait(o_ready + ((it - 1) & 1), ((it - 1) >> 1) & 1, abort_flag, p.err);
+            __syncwarp();
             tc_fence_after();
             // -inf - -inf: a row that has seen nothing yet keeps its zeros.
             const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
@@ -785,26 +801,27 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + (it & 1));
       }
-      if (!ok) break;
       // ── the segment's result ──────────────────────────────────────────────
       const bool complete = j0 == 0 && j1 == tiles;
       int slot = 0;
       if (!complete) {
         const int c0 = tree_owner(wpref, num_seqs, sh, kvh, s, 0) + sh.first_cta;
         slot = c0 == static_cast<int>(blockIdx.x) ? 1 : 0;
-        if (c0 + 1 == static_cast<int>(blockIdx.x)) {
+        if (c0 + 1 == static_cast<int>(blockIdx.x) && threadIdx.x == 0) {
+          // The sequence began in the CTA before this one: this CTA describes
+          // the join of its pieces (it has the second of them).
+          int* rec = p.records + blockIdx.x;
           rec[0] = s;
-          rec[1] = kvh;
-          rec[2] = tok0;
-          rec[3] = c0;
-          rec[4] = tree_owner(wpref, num_seqs, sh, kvh, s, tiles - 1) + sh.first_cta;
-          rec[5] = rows;
+          rec[p.n_cta] = kvh;
+          rec[2 * p.n_cta] = tok0;
+          rec[3 * p.n_cta] = c0;
+          rec[4 * p.n_cta] = tree_owner(wpref, num_seqs, sh, kvh, s, tiles - 1) + sh.first_cta;
+          rec[5 * p.n_cta] = rows;
         }
       }
       if (active) {
-        ok = mbar_wait(o_ready + ((it - 1) & 1), ((it - 1) >> 1) & 1, p.err);
-        ok = __all_sync(0xffffffffu, ok) && !aborted(abort_flag);
-        if (!ok) break;
+        tt_wait(o_ready + ((it - 1) & 1), ((it - 1) >> 1) & 1, abort_flag, p.err);
+        __syncwarp();
         tc_fence_after();
         const bool odd = odd_seg[seg & 1] == seg + 1;
         // A row that saw nothing has l = 0 and O = 0.
@@ -852,11 +869,6 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
       }
       ++seg;
       w.next(wpref, num_seqs, sh);
-    }
-    if (!ok) *abort_flag = 1;
-    if (threadIdx.x == 0 && !p.whole) {
-#pragma unroll
-      for (int i = 0; i < 6; ++i) p.records[i * p.n_cta + blockIdx.x] = rec[i];
     }
   }
 
