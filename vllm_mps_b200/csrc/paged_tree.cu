@@ -487,7 +487,9 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
     const bool is_v = warp == kTtVWarp;
     const int oob = 2 * p.num_blocks;  // past the pool: the TMA fills zeros
     uint64_t* full = is_v ? v_full : k_full;
-    uint64_t* empty = is_v ? v_empty : k_empty;
+    // With two ring slots the slot and the tile parity are one, and the barrier
+    // that tells the softmax of a product tells the loader of its free slot.
+    uint64_t* empty = Shape::kStages == 2 ? (is_v ? o_ready : s_full) : (is_v ? v_empty : k_empty);
     uint8_t* ring = is_v ? sV : sK;
     auto fetch = [&](int s, int n_pages, int page) -> int {  // block id of `page`, or -1
       if (page >= n_pages) return -1;
@@ -608,7 +610,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
           tc_mma(t_s, q_desc + (((k >> 2) * kTtQChunk + (k & 3) * 32) >> 4),
                  kd + (((k >> 2) * kTtKChunk + (k & 3) * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u);
         }
-        tc_commit(k_empty + st);
+        if (Shape::kStages != 2) tc_commit(k_empty + st);
         tc_commit(s_full + (iq & 1));
         ++iq;
         new_q = false;
@@ -636,7 +638,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
           // A segment's first PV overwrites O.
           tc_mma_ts(t_o, t_p + k * 8, vd + ((k * 2048) >> 4), idesc_pv, (!first || k > 0) ? 1u : 0u);
         }
-        tc_commit(v_empty + st);
+        if (Shape::kStages != 2) tc_commit(v_empty + st);
         tc_commit(o_ready + (ip & 1));
         ++ip;
         first = false;
