@@ -38,10 +38,10 @@
 // do not fit the registers) over all of K belongs to one CTA;
 // contiguous equal shares of blocks go to one persistent CTA per SM.  The
 // warps form teams; a team takes every teams-th block, its warps the block's
-// chunks (4 KB of codes) in turn, and adds their partial sums of the block
+// chunks (2 or 4 KB of codes) in turn, and adds their partial sums of the block
 // through shared memory in a fixed order.  Every warp streams its own chunks
 // with 16-byte asynchronous copies into a private pair of slots, so nothing but
-// the block's sum is waited for by more than one warp; 64 KB are in flight.  (Bulk copies were tried:
+// the block's sum is waited for by more than one warp; 32 or 64 KB are in flight.  (Bulk copies were tried:
 // with one per row or one tensor box per block the copy engine's per-line cost
 // capped the stream at 60 % of the rate of these.)  Scales and zero points go
 // straight to the registers of the lane quad that uses them, as many chunks
@@ -66,15 +66,17 @@ namespace {
 constexpr int kW4MaxRows = 32;
 constexpr int kW4Warps = 16;
 constexpr int kW4Threads = 32 * kW4Warps;
-constexpr int kW4ChunkBytes = 4096;  // codes of a chunk: kRows rows x 8192 / kRows codes
+// Codes of a chunk (kRows rows x 2 * bytes / kRows codes): the larger amortises
+// more, but with more than one activation tile the activations need the room.
+__host__ __device__ constexpr int w4_chunk_bytes(int nt) { return nt == 1 ? 4096 : 2048; }
 constexpr int kW4Depth = 2;          // ring slots per warp: one chunk in flight, one in use
-constexpr int kW4SmemLimit = 227 * 1024;
+constexpr int kW4SmemLimit = 226 * 1024;  // beside the static 64 bytes
 constexpr int kW4XBatch = 8;         // activation loads in flight per thread
 
-// Buffers of partial sums: with two a team meets once per block instead of
-// twice; with more than one activation tile the second would cost the
-// activations their room.
-__host__ __device__ constexpr int w4_red_bufs(int nt) { return nt == 1 ? 2 : 1; }
+// Buffers of partial sums beside the rings: with two a team meets once per
+// block.  With more than one activation tile there is no room for them; a
+// warp's sums then go to its free ring slot, and the team meets twice.
+__host__ __device__ constexpr int w4_red_bufs(int nt) { return nt == 1 ? 2 : 0; }
 
 struct W4Params {
   void* out;
@@ -146,7 +148,8 @@ template <> struct ScaleZero<__nv_bfloat16> {
 template <typename T, int GROUP, int NT, int MT>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant__ W4Params p) {
   constexpr int kRows = 16 * MT;
-  constexpr int kCodes = kW4ChunkBytes * 2 / kRows;  // codes of a row in a chunk: 512 or 256
+  constexpr int kW4ChunkBytes = w4_chunk_bytes(NT);
+  constexpr int kCodes = kW4ChunkBytes * 2 / kRows;  // codes of a row in a chunk
   constexpr int kRowBytes = kCodes / 2;
   constexpr int kUnits = kRowBytes / 16;             // 32-code units of a row
   constexpr int GP = kCodes / GROUP;                 // groups per chunk
@@ -157,6 +160,8 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
   // Shared memory: rings | activations | group sums | partial sums | gate sums
   // (silu) | panel sums (several phases).
   extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint32_t s_free[kW4Warps];  // free ring slots that hold partial sums
+  static_assert(kFrag * 512 <= kW4ChunkBytes, "a block's sums fit a ring slot");
 
   const int tid = threadIdx.x;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // warp-uniform
@@ -199,7 +204,9 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
   // bank.  Copies of one row differ in the unit's bits 2 and up, untouched by
   // the lane's own, so their targets differ by an exclusive or.
   constexpr int kCols = kRowBytes / 64, kRowSets = kRows / 8;
-  auto swz = [](int row, int unit) -> int { return unit ^ (row & 7); };
+  auto swz = [](int row, int unit) -> int {  // two rows share 128 bytes where a row has 64
+    return unit ^ (kUnits == 4 ? (row >> 1) & 3 : row & 7);
+  };
   const int g = lane >> 2, c = lane & 3;
   const uint32_t l_dst = g * kRowBytes + swz(g, c) * 16;
   // (row, group) pairs e = 4 i + c of this lane's quad: group e % GP of the
@@ -523,9 +530,12 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
         for (; off < nch; off += T_) chunk(off);
         off -= nch;
         // The team's sum of the block, the warps in order.
-        const float* sums = red + (kRedBufs == 2 ? red_buf * kRedFloats : 0);
+        const float* sums = red + red_buf * kRedFloats;
+        if (kRedBufs == 0) sums = reinterpret_cast<const float*>(smem + (s_dst - smem_u32(smem)));
+        float4* mine = reinterpret_cast<float4*>(const_cast<float*>(sums) + (kRedBufs ? w * kFrag * 128 : 0));
         red_buf ^= 1;
-        float4* mine = reinterpret_cast<float4*>(const_cast<float*>(sums) + w * kFrag * 128);
+        if (kRedBufs == 0 && lane == 0) s_free[warp] = s_dst - smem_u32(smem);
+        __syncwarp();  // the slot's last chunk is read by all lanes
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -538,7 +548,10 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
         const bool up = p.silu && (v & 1);
         for (int x = w * 32 + lane; x < kFrag * 128; x += 32 * T_) {
           float y = ph > 0 ? acc[(v - pv) * kFrag * 128 + x] : 0.f;
-          for (int j = 0; j < T_; ++j) y += sums[j * kFrag * 128 + x];
+          for (int j = 0; j < T_; ++j) {
+            y += kRedBufs ? sums[j * kFrag * 128 + x]
+                          : reinterpret_cast<const float*>(smem + s_free[team * T_ + j])[x];
+          }
           if (ph + 1 < p.phases) {
             acc[(v - pv) * kFrag * 128 + x] = y;
           } else if (p.silu && !up) {
@@ -552,7 +565,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
             if (m < p.M && feat < p.N) out[m * p.out_stride + feat] = Elt<T>::from_f(y);
           }
         }
-        if (kRedBufs == 1) team_sync();  // the sums are taken before the next block's are written
+        if (kRedBufs == 0) team_sync();  // the sums are taken before the slots are filled again
       }
     }
   }
@@ -567,17 +580,19 @@ int w4_mt(int M) { return M > 8 && M <= 16 ? 2 : 1; }
 // panels) that leave room for everything else.
 bool w4_plan(W4Params* p, int group, int planes, int cta_blocks) {
   const int nt = w4_nt(p->M), mt = w4_mt(p->M);
-  const int codes = kW4ChunkBytes * 2 / (16 * mt);
+  const int codes = w4_chunk_bytes(nt) * 2 / (16 * mt);
   const int halves = p->silu ? 2 : 1;
-  // A warp should take about four chunks of a block (its share of the block's
-  // fixed costs), but all warps should have a block.
+  // A warp should take about 16 KB of a block (its share of the block's fixed
+  // costs: with teams of 4 instead of 8 the LM head at 16 rows took 80 us for
+  // 88), but all warps should have a block.
+  const int few = 16384 / w4_chunk_bytes(nt);
   p->team = 1;
   while (p->team < kW4Warps &&
-         (p->team * 4 < p->chunks || p->team * (cta_blocks / halves) < kW4Warps)) {
+         (p->team * few < p->chunks || p->team * (cta_blocks / halves) < kW4Warps)) {
     p->team *= 2;
   }
   const int block = mt * nt * 512;  // bytes of a block's sums
-  const int fixed = kW4Warps * kW4Depth * kW4ChunkBytes +
+  const int fixed = kW4Warps * kW4Depth * w4_chunk_bytes(nt) +
                     (w4_red_bufs(nt) * kW4Warps + (p->silu ? kW4Warps / p->team : 0)) * block;
   long long best = -1;
   for (int phases = 1; phases <= p->chunks; ++phases) {
@@ -612,7 +627,7 @@ bool w4_plan(W4Params* p, int group, int planes, int cta_blocks) {
 
 size_t w4_smem(const W4Params& p) {
   const int block = w4_mt(p.M) * w4_nt(p.M) * 512;
-  return kW4Warps * kW4Depth * kW4ChunkBytes + p.x_bytes + p.sx_bytes +
+  return kW4Warps * kW4Depth * w4_chunk_bytes(w4_nt(p.M)) + p.x_bytes + p.sx_bytes +
          static_cast<size_t>(w4_red_bufs(w4_nt(p.M)) * kW4Warps + (p.silu ? kW4Warps / p.team : 0) +
                              (p.phases > 1 ? p.panel : 0)) *
              block;
@@ -704,7 +719,7 @@ extern "C" int vmps_w4_gemm(void* out, int64_t out_row_stride, const void* x, in
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   const int rows = 16 * w4_mt(M);
-  const int codes_per_chunk = kW4ChunkBytes * 2 / rows;
+  const int codes_per_chunk = w4_chunk_bytes(w4_nt(M)) * 2 / rows;
   W4Params p;
   p.out = out;
   p.out_stride = out_row_stride;
