@@ -369,7 +369,7 @@ int vmps_commit_tree(int32_t* path, int32_t* count, int64_t* next_token, void* p
  *   out[m][n] = sum_g scales[n][g] * sum_{k in group g} x[m][k] * (code[n][k] - zeros[n][g])
  * codes:  uint8 [N][K / 2], row n's code k in byte k / 2, the even k in the
  *         low four bits.  scales: [N][K / group_size] in x's type.
- * zeros:  uint8 [N][K / group_size], below 128, or NULL for 8 everywhere.
+ * zeros:  uint8 [N][K / group_size], or NULL for 8 everywhere.
  * All contiguous and 16-byte aligned.  Sums and scaling in fp32, one rounding.
  * With silu_mul != 0 the weight is the fused [gate; up] of 2N rows and
  * out[m][n] = silu(gate) * up of the unrounded fp32 products.

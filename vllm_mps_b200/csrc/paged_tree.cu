@@ -1136,10 +1136,11 @@ extern "C" int vmps_paged_tree_attention(
   // The plan sums a row tile's tiles over all sequences in 31 bits.
   const long long max_tiles = (static_cast<long long>(max_blocks_per_seq) + kTtPages - 1) / kTtPages;
   if (num_seqs > kTtMaxSeqs || max_q_len > kTtMaxQLen || max_blocks_per_seq > (1 << 24) ||
+      num_blocks > (1 << 29) ||
       num_seqs * (max_tiles * kTileWeight + kSegWeight) > 0x7fffffffLL) {
     return fail(VMPS_ERR_UNSUPPORTED,
                 "%s: num_seqs=%d max_q_len=%d max_blocks=%d (num_seqs <= %d, max_q_len <= %d, "
-                "max_blocks <= 2^24, num_seqs * max_blocks < 2^31)",
+                "max_blocks <= 2^24, num_seqs * max_blocks < 2^31, num_blocks <= 2^29)",
                 what, num_seqs, max_q_len, max_blocks_per_seq, kTtMaxSeqs, kTtMaxQLen);
   }
   if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return VMPS_OK;

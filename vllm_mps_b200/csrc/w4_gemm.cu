@@ -52,8 +52,8 @@
 // its blocks through every phase and keeps the panel's sums in shared memory
 // between them.  No partial sums leave the CTA.
 //
-// Launched with programmatic dependent launch: codes, scales and zero points
-// do not depend on the kernel before, so the rings fill before the wait.
+// Launched with programmatic dependent launch (the prologue overlaps the end of
+// the kernel before; everything is read after its wait).
 #include <mutex>
 #include <type_traits>
 
@@ -120,7 +120,7 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t b
 }
 
 // A scale (low half) and a zero point packed for one shuffle, and back.  The
-// zero point travels as a number of the scale's type (exact below 128).
+// zero point travels as a number of the scale's type (exact for 8 bits).
 template <typename T> struct ScaleZero;
 template <> struct ScaleZero<__half> {
   static __device__ __forceinline__ uint32_t pack(uint32_t scale, uint32_t zero) {
@@ -309,9 +309,11 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
     if (s_dst == end_of_ring) s_dst = ring;
   };
   settle();
+  // Nothing is read before the kernels ahead are done: X is theirs, and the
+  // codes may be (a weight that was only just quantised).  The next launch's
+  // CTAs find no room beside this one's, so an early stream would gain nothing.
+  w4_pdl_wait();
   start_next();
-
-  w4_pdl_wait();  // X is the previous kernel's output, out may still be read by it
 
   // ── the products ───────────────────────────────────────────────────────────
   const int mi = lane >> 3, r8 = lane & 7;

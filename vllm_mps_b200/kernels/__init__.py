@@ -856,7 +856,7 @@ class W4Weight:
 
     ``codes``: uint8 (N, K/2), code k of a row in byte k // 2, even k in the
     low four bits; ``scales``: (N, K/group) in the activations' dtype;
-    ``zeros``: uint8 (N, K/group) below 128 or None (8 everywhere).  The weight it
+    ``zeros``: uint8 (N, K/group) or None (8 everywhere).  The weight it
     stands for is ``scales * (code - zeros)``.  All contiguous.
     """
 
