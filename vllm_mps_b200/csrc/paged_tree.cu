@@ -75,7 +75,9 @@ constexpr int kSegWeight = 16;
 constexpr int kMinTiles = 4;                  // a share holds at least this many tiles
 constexpr int kWholeTiles = 8;                // contexts up to this many tiles are not cut
 constexpr int kMergeThreads = 256;
+constexpr int kMergeBlocksPerSm = 2;
 constexpr int kMergeCols = 16;                // output columns per merge unit
+constexpr int kMaxCtas = 512;
 
 template <int D>
 struct TreeShape {
@@ -891,15 +893,16 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
 // and the warps' results are joined through shared memory, all in a fixed
 // order.  Bound: the partial results, read from L2; one warp per unit alone
 // took 19 us for 74 pieces of 4 kv heads, eight always 30 us for 256 items of
-// two pieces.
+// two pieces.  The records are brought into shared memory once: read per unit
+// they cost 1 us in 79.
 template <typename T, int D>
-__global__ void __launch_bounds__(kMergeThreads, 2)
+__global__ void __launch_bounds__(kMergeThreads, kMergeBlocksPerSm)
     paged_tree_merge_kernel(const __grid_constant__ TreeParams p) {
   constexpr int kWarps = kMergeThreads / 32;
   constexpr int kQuads = kMergeCols / 4;
   constexpr int kColUnits = D / kMergeCols;
   constexpr int kBatch = 4;     // pieces in flight per warp
-  __shared__ int s_item[1024];  // CTAs whose record is a join, in order
+  __shared__ int s_rec[kMaxCtas][6];  // the joins, in order
   __shared__ int s_base[kWarps + 1];
   __shared__ float s_ml[kWarps][32][2];
   __shared__ float4 s_o[kWarps][kQuads][32];
@@ -908,7 +911,13 @@ __global__ void __launch_bounds__(kMergeThreads, 2)
   int n_items = 0;
   for (int base = 0; base < p.n_cta; base += kMergeThreads) {
     const int b = base + threadIdx.x;
-    const bool on = b < p.n_cta && p.records[b] >= 0;
+    int rec[6];
+    rec[0] = -1;
+    if (b < p.n_cta) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) rec[i] = p.records[i * p.n_cta + b];
+    }
+    const bool on = rec[0] >= 0;
     const unsigned mask = __ballot_sync(0xffffffffu, on);
     if (lane == 0) s_base[warp + 1] = __popc(mask);
     __syncthreads();
@@ -917,7 +926,11 @@ __global__ void __launch_bounds__(kMergeThreads, 2)
       for (int i = 0; i < kWarps; ++i) s_base[i + 1] += s_base[i];
     }
     __syncthreads();
-    if (on) s_item[s_base[warp] + __popc(mask & ((1u << lane) - 1))] = b;
+    if (on) {
+      int* dst = s_rec[s_base[warp] + __popc(mask & ((1u << lane) - 1))];
+#pragma unroll
+      for (int i = 0; i < 6; ++i) dst[i] = rec[i];
+    }
     n_items = s_base[kWarps];
     __syncthreads();
   }
@@ -934,13 +947,13 @@ __global__ void __launch_bounds__(kMergeThreads, 2)
     const int ru = rest / kColUnits, cu = rest - ru * kColUnits;
     int s = 0, kvh = 0, tok0 = 0, c0 = 0, c1 = -1, rows = 0;
     if (unit < units) {
-      const int* rec = p.records + s_item[item];
+      const int* rec = s_rec[item];
       s = rec[0];
-      kvh = rec[p.n_cta];
-      tok0 = rec[2 * p.n_cta];
-      c0 = rec[3 * p.n_cta];
-      c1 = rec[4 * p.n_cta];
-      rows = rec[5 * p.n_cta];
+      kvh = rec[1];
+      tok0 = rec[2];
+      c0 = rec[3];
+      c1 = rec[4];
+      rows = rec[5];
     }
     const bool on = ru * 32 < rows;
     const int row = ru * 32 + lane;
@@ -1011,8 +1024,10 @@ __global__ void __launch_bounds__(kMergeThreads, 2)
         packed[2 * i + 1] = Elt<T>::pack(o[i].z * inv, o[i].w * inv);
       }
       uint4* d4 = reinterpret_cast<uint4*>(dst);
-      d4[0] = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-      d4[1] = make_uint4(packed[4], packed[5], packed[6], packed[7]);
+#pragma unroll
+      for (int i = 0; i < kQuads / 2; ++i) {
+        d4[i] = make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+      }
     }
     if (per_unit > 1) __syncthreads();
   }
@@ -1079,7 +1094,7 @@ int launch_tree(const CUtensorMap& kv_map, const CUtensorMap& q_map, const TreeP
   const size_t smem = Shape::kFixedBytes + static_cast<size_t>(p.num_seqs + 1) * sizeof(int);
   cudaError_t e = tree_launch(paged_tree_kernel<T, D>, p.n_cta, kTtThreads, smem, s, kv_map, q_map, p);
   if (e == cudaSuccess && !p.whole) {
-    e = tree_launch(paged_tree_merge_kernel<T, D>, 2 * sms, kMergeThreads, 0, s, p);
+    e = tree_launch(paged_tree_merge_kernel<T, D>, kMergeBlocksPerSm * sms, kMergeThreads, 0, s, p);
   }
   if (e != cudaSuccess) {
     return fail(VMPS_ERR_CUDA, "paged_tree_attention: launch failed: %s", cudaGetErrorString(e));
@@ -1164,7 +1179,7 @@ extern "C" int vmps_paged_tree_attention(
   if (int rc = device_sm_count(&sms)) return rc;
   TreeParams p;
   p.n_cta = sms * kTtCtasPerSm;
-  if (p.n_cta > 1024) return fail(VMPS_ERR_UNSUPPORTED, "%s: %d SMs", what, sms);
+  if (p.n_cta > kMaxCtas) return fail(VMPS_ERR_UNSUPPORTED, "%s: %d SMs", what, sms);
   const TreeLayout wl = tree_layout(max_q_len, n_q, n_kv, head_dim, p.n_cta);
   const bool whole = tree_whole(max_blocks_per_seq);
   // One that is given has to do for any context, one that is not needed may be missing.
