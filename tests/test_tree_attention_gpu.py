@@ -165,6 +165,18 @@ def test_many_short_sequences(cuda_device):
     _check(_call(K, c), _reference(c), torch.float16, 64)
 
 
+@pytest.mark.parametrize("ctx,n_kv,D", [(3000, 1, 128), (60000, 1, 64), (33000, 2, 128)])
+def test_sequences_in_many_pieces(cuda_device, ctx, n_kv, D):
+    """One sequence over the whole machine: its pieces are joined in groups, those again."""
+    from vllm_mps_b200 import kernels as K
+
+    c = _case(cuda_device, [(ctx, 5, 5)], 3 * n_kv, n_kv, D, torch.float16, seed=ctx)
+    got = _call(K, c)
+    _check(got, _reference(c), torch.float16, D)
+    for _ in range(5):
+        assert torch.equal(got, _call(K, c))  # whichever piece comes last
+
+
 def test_large_scores_and_scale(cuda_device):
     """Scores far apart (one key takes all) and a scale of the caller's."""
     from vllm_mps_b200 import kernels as K
