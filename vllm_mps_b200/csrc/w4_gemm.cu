@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
   };
 
   T* out = static_cast<T*>(p.out);
-  int red_buf = 0;
+  int red_buf = 0, turn = 0;
   for (int pv = v0; pv < v1; pv += p.panel) {
     const int pe = min(pv + p.panel, v1);
     for (int ph = 0; ph < p.phases; ++ph) {
@@ -548,25 +548,45 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
         }
         team_sync();
         const bool up = p.silu && (v & 1);
-        for (int x = w * 32 + lane; x < kFrag * 128; x += 32 * T_) {
-          float y = ph > 0 ? acc[(v - pv) * kFrag * 128 + x] : 0.f;
+        // A thread sums one lane's four values of a fragment; the warps that do
+        // (fragments may be fewer than warps) change from block to block.
+        for (int x = ((w + turn) & (T_ - 1)) * 32 + lane; x < kFrag * 32; x += 32 * T_) {
+          float4* kept = reinterpret_cast<float4*>(acc) + (v - pv) * kFrag * 32 + x;
+          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (ph > 0) y = *kept;
+#pragma unroll 4
           for (int j = 0; j < T_; ++j) {
-            y += kRedBufs ? sums[j * kFrag * 128 + x]
-                          : reinterpret_cast<const float*>(smem + s_free[team * T_ + j])[x];
+            const float4 z = kRedBufs ? reinterpret_cast<const float4*>(sums)[j * kFrag * 32 + x]
+                                      : reinterpret_cast<const float4*>(smem + s_free[team * T_ + j])[x];
+            y.x += z.x;
+            y.y += z.y;
+            y.z += z.z;
+            y.w += z.w;
           }
           if (ph + 1 < p.phases) {
-            acc[(v - pv) * kFrag * 128 + x] = y;
+            *kept = y;
           } else if (p.silu && !up) {
-            gate[x] = y;  // read back by this thread
+            reinterpret_cast<float4*>(gate)[x] = y;  // read back by this thread
           } else {
             // Fragment: (feature g, row 2c), (g, 2c + 1), (g + 8, 2c), (g + 8, 2c + 1).
-            const int f = x >> 7, l = (x & 127) >> 2, e = x & 3;
-            const int feat = (p.silu ? v >> 1 : v) * kRows + (f / NT) * 16 + (l >> 2) + (e >> 1) * 8;
-            const int m = (f % NT) * 8 + 2 * (l & 3) + (e & 1);
-            if (up) y = gate[x] / (1.f + expf(-gate[x])) * y;
-            if (m < p.M && feat < p.N) out[m * p.out_stride + feat] = Elt<T>::from_f(y);
+            const int f = x >> 5;
+            const int feat = (p.silu ? v >> 1 : v) * kRows + (f / NT) * 16 + g;
+            const int m = (f % NT) * 8 + 2 * c;
+            if (up) {
+              const float4 z = reinterpret_cast<const float4*>(gate)[x];
+              y.x *= z.x / (1.f + expf(-z.x));
+              y.y *= z.y / (1.f + expf(-z.y));
+              y.z *= z.z / (1.f + expf(-z.z));
+              y.w *= z.w / (1.f + expf(-z.w));
+            }
+            T* at = out + m * p.out_stride + feat;
+            if (m < p.M && feat < p.N) at[0] = Elt<T>::from_f(y.x);
+            if (m + 1 < p.M && feat < p.N) at[p.out_stride] = Elt<T>::from_f(y.y);
+            if (m < p.M && feat + 8 < p.N) at[8] = Elt<T>::from_f(y.z);
+            if (m + 1 < p.M && feat + 8 < p.N) at[p.out_stride + 8] = Elt<T>::from_f(y.w);
           }
         }
+        if (!p.silu || up) ++turn;
         if (kRedBufs == 0) team_sync();  // the sums are taken before the slots are filled again
       }
     }
