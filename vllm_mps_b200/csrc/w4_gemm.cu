@@ -78,6 +78,10 @@ constexpr int kW4XBatch = 8;         // activation loads in flight per thread
 // warp's sums then go to its free ring slot, and the team meets twice.
 __host__ __device__ constexpr int w4_red_bufs(int nt) { return nt == 1 ? 2 : 0; }
 
+// Per group and activation row: what its sum starts from, [sum x,] [what its
+// sum is multiplied by].
+__host__ __device__ constexpr int w4_planes(bool scaled, bool zp) { return 1 + (zp ? 1 : 0) + (scaled ? 1 : 0); }
+
 struct W4Params {
   void* out;
   int64_t out_stride;
@@ -145,7 +149,19 @@ template <> struct ScaleZero<__nv_bfloat16> {
   }
 };
 
-template <typename T, int GROUP, int NT, int MT>
+// The instruction of Mma<__half> with the sums' start in registers of its own.
+__device__ __forceinline__ void w4_mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                            float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+
+// ZP: with zero points.  Without, every row's sum of a group starts from the
+// same numbers: 128256 x 4096 at 16 rows takes 73.4 us so, 75.0 with the 8 as
+// a zero point of every group.
+template <typename T, int GROUP, int NT, int MT, bool ZP>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant__ W4Params p) {
   constexpr int kRows = 16 * MT;
   constexpr int kW4ChunkBytes = w4_chunk_bytes(NT);
@@ -156,7 +172,8 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
   constexpr int UPG = GROUP / 32;
   constexpr int NSZ = (2 * MT * GP + 3) / 4;         // (row, group) pairs a lane fetches per chunk
   constexpr int kFrag = MT * NT;
-  constexpr int kPlanes = std::is_same<T, __half>::value ? 2 : 3;
+  constexpr bool kScaled = !std::is_same<T, __half>::value;
+  constexpr int kPlanes = w4_planes(kScaled, ZP);
   // Shared memory: rings | activations | group sums | partial sums | gate sums
   // (silu) | panel sums (several phases).
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -170,8 +187,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
   const int w = warp & (T_ - 1);  // place in the team
   const int team = warp / T_;     // takes blocks pv + team, + teams, ...
   uint8_t* xs = smem + kW4Warps * kW4Depth * kW4ChunkBytes;
-  // Per group and activation row: -sum x OFF, sum x and, for bf16, what the
-  // group's sum is multiplied by, [group][plane][row].
+  // [group][plane][row]; see w4_planes.
   float* sx = reinterpret_cast<float*>(xs + p.x_bytes);
   float* red = sx + p.sx_bytes / 4 + team * T_ * kFrag * 128;  // the team's (first buffer)
   constexpr int kRedFloats = kW4Warps * kFrag * 128;           // of a buffer, all teams
@@ -266,8 +282,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
         for (int i = 0; i < NSZ; ++i) {
           const uint32_t j = s_at + (4 * i) % GP + 8 * (4 * i / GP) * p.ng;
           if (2 * MT * GP >= 4 || c < 2 * MT * GP) sc_next[i] = scales[j];
-          zp_next[i] = 8;
-          if (p.zeros && (2 * MT * GP >= 4 || c < 2 * MT * GP)) zp_next[i] = p.zeros[j];
+          if (ZP && (2 * MT * GP >= 4 || c < 2 * MT * GP)) zp_next[i] = p.zeros[j];
         }
       } else {
         // The weight's last rows or a row's last codes: only what exists, and
@@ -288,11 +303,11 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
         for (int i = 0; i < NSZ; ++i) {
           const int e = 4 * i + c;
           sc_next[i] = 0;
-          zp_next[i] = 8;
+          zp_next[i] = 8;  // any that is finite
           if (ch * GP + e % GP < p.ng && row0 + g + 8 * (e / GP) < wrows && e < 2 * MT * GP) {
             const uint32_t j = s_at + (4 * i) % GP + 8 * (4 * i / GP) * p.ng;
             sc_next[i] = scales[j];
-            if (p.zeros) zp_next[i] = p.zeros[j];
+            if (ZP) zp_next[i] = p.zeros[j];
           }
         }
       }
@@ -341,7 +356,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
     __syncwarp();  // every lane's copies have landed, and the last chunk is read
     uint32_t sz[NSZ];
 #pragma unroll
-    for (int i = 0; i < NSZ; ++i) sz[i] = ScaleZero<T>::pack(sc_next[i], zp_next[i]);
+    for (int i = 0; i < NSZ; ++i) sz[i] = ZP ? ScaleZero<T>::pack(sc_next[i], zp_next[i]) : sc_next[i];
     start_next();
     const uint32_t base = r_src + a_lane;
     r_src += kW4ChunkBytes;
@@ -351,7 +366,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
     uint32_t a[MT][4];  // a pair of units: [(row half) + 2 * (unit in pair)]
 #pragma unroll
     for (int gp = 0; gp < GP; ++gp) {
-      float part[MT][NT][4];
+      float part[MT][NT][4], start[MT][NT][4];
       float sc[MT][2];
       const float* sg = s_chunk + gp * (kPlanes * 8 * NT);
 #pragma unroll
@@ -365,9 +380,13 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const float2 off2 = *reinterpret_cast<const float2*>(sg + nt * 8);
-            const float2 sum2 = *reinterpret_cast<const float2*>(sg + 8 * NT + nt * 8);
-            part[mt][nt][2 * h] = fmaf(-zero, sum2.x, off2.x);
-            part[mt][nt][2 * h + 1] = fmaf(-zero, sum2.y, off2.y);
+            start[mt][nt][2 * h] = off2.x;
+            start[mt][nt][2 * h + 1] = off2.y;
+            if (ZP) {
+              const float2 sum2 = *reinterpret_cast<const float2*>(sg + 8 * NT + nt * 8);
+              start[mt][nt][2 * h] = fmaf(-zero, sum2.x, off2.x);
+              start[mt][nt][2 * h + 1] = fmaf(-zero, sum2.y, off2.y);
+            }
           }
         }
       }
@@ -397,7 +416,12 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
                                   and_or(lo8, mask_hi, bits_hi), and_or(hi8, mask_hi, bits_hi)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            Mma<__half>::run(part[mt][nt], f0, xv[nt].x, xv[nt].y);
+            if (u == 0) {
+              const float* from = start[mt][nt];
+              w4_mma_from(part[mt][nt], f0, xv[nt].x, xv[nt].y, from[0], from[1], from[2], from[3]);
+            } else {
+              Mma<__half>::run(part[mt][nt], f0, xv[nt].x, xv[nt].y);
+            }
             Mma<__half>::run(part[mt][nt], f1, xv[nt].z, xv[nt].w);
           }
         }
@@ -405,13 +429,12 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float2 down = make_float2(1.f, 1.f);
-        if (kPlanes == 3) down = *reinterpret_cast<const float2*>(sg + 16 * NT + nt * 8);
+        if (kScaled) down = *reinterpret_cast<const float2*>(sg + (kPlanes - 1) * 8 * NT + nt * 8);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float y = kPlanes == 3 ? part[mt][nt][e] * ((e & 1) ? down.y : down.x)
-                                         : part[mt][nt][e];
+            const float y = kScaled ? part[mt][nt][e] * ((e & 1) ? down.y : down.x) : part[mt][nt][e];
             total[mt][nt][e] = fmaf(sc[mt][e >> 1], y, total[mt][nt][e]);
           }
         }
@@ -490,7 +513,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
               uint32_t* hw = reinterpret_cast<uint32_t*>(&h);
 #pragma unroll
               for (int j = 0; j < 4; ++j) hw[j] = Elt<__half>::pack(f[2 * j] * up, f[2 * j + 1] * up);
-              if (lead) sx[(grp * kPlanes + 2) * (8 * NT) + um[i]] = 1.f / up;
+              if (lead) sx[(grp * kPlanes + kPlanes - 1) * (8 * NT) + um[i]] = 1.f / up;
             }
             uint4 o;
             o.x = __byte_perm(h.x, h.z, 0x5410);
@@ -510,8 +533,9 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
               odd += __shfl_xor_sync(0xffffffffu, odd, sh);
             }
             if (lead) {
-              sx[grp * kPlanes * (8 * NT) + um[i]] = -(1024.f * even + 64.f * odd);
-              sx[(grp * kPlanes + 1) * (8 * NT) + um[i]] = even + odd;
+              sx[grp * kPlanes * (8 * NT) + um[i]] =
+                  ZP ? -(1024.f * even + 64.f * odd) : -(1032.f * even + 72.f * odd);
+              if (ZP) sx[(grp * kPlanes + 1) * (8 * NT) + um[i]] = even + odd;
             }
           }
         }
@@ -655,14 +679,14 @@ size_t w4_smem(const W4Params& p) {
              block;
 }
 
-template <typename T, int GROUP, int NT, int MT>
+template <typename T, int GROUP, int NT, int MT, bool ZP>
 int w4_launch(const W4Params& p, int grid, cudaStream_t s) {
   static std::once_flag flags[64];
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return fail(VMPS_ERR_CUDA, "device index %d", dev);
   std::call_once(flags[dev], [] {
-    cudaFuncSetAttribute(w4_kernel<T, GROUP, NT, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaFuncSetAttribute(w4_kernel<T, GROUP, NT, MT, ZP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          kW4SmemLimit);
   });
   cudaLaunchConfig_t cfg = {};
@@ -675,29 +699,34 @@ int w4_launch(const W4Params& p, int grid, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_kernel<T, GROUP, NT, MT>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_kernel<T, GROUP, NT, MT, ZP>, p);
   if (e != cudaSuccess) {
     return fail(VMPS_ERR_CUDA, "w4_gemm: launch failed: %s", cudaGetErrorString(e));
   }
   return VMPS_OK;
 }
 
-template <typename T, int GROUP>
+template <typename T, int GROUP, bool ZP>
 int w4_by_rows(const W4Params& p, int grid, cudaStream_t s) {
   switch (w4_nt(p.M)) {
-    case 1: return w4_launch<T, GROUP, 1, 1>(p, grid, s);
-    case 2: return w4_launch<T, GROUP, 2, 2>(p, grid, s);
-    default: return w4_launch<T, GROUP, 4, 1>(p, grid, s);
+    case 1: return w4_launch<T, GROUP, 1, 1, ZP>(p, grid, s);
+    case 2: return w4_launch<T, GROUP, 2, 2, ZP>(p, grid, s);
+    default: return w4_launch<T, GROUP, 4, 1, ZP>(p, grid, s);
+  }
+}
+
+template <typename T, bool ZP>
+int w4_by_group(int group, const W4Params& p, int grid, cudaStream_t s) {
+  switch (group) {
+    case 32: return w4_by_rows<T, 32, ZP>(p, grid, s);
+    case 64: return w4_by_rows<T, 64, ZP>(p, grid, s);
+    default: return w4_by_rows<T, 128, ZP>(p, grid, s);
   }
 }
 
 template <typename T>
-int w4_by_group(int group, const W4Params& p, int grid, cudaStream_t s) {
-  switch (group) {
-    case 32: return w4_by_rows<T, 32>(p, grid, s);
-    case 64: return w4_by_rows<T, 64>(p, grid, s);
-    default: return w4_by_rows<T, 128>(p, grid, s);
-  }
+int w4_by_zeros(int group, const W4Params& p, int grid, cudaStream_t s) {
+  return p.zeros ? w4_by_group<T, true>(group, p, grid, s) : w4_by_group<T, false>(group, p, grid, s);
 }
 
 }  // namespace
@@ -758,11 +787,11 @@ extern "C" int vmps_w4_gemm(void* out, int64_t out_row_stride, const void* x, in
   p.chunks = (K + codes_per_chunk - 1) / codes_per_chunk;
   p.blocks = (N + rows - 1) / rows;
   const int grid = p.blocks < sms ? p.blocks : sms;
-  if (!w4_plan(&p, group_size, dtype == VMPS_DTYPE_F16 ? 2 : 3,
+  if (!w4_plan(&p, group_size, w4_planes(dtype != VMPS_DTYPE_F16, zeros != nullptr),
                (p.blocks + grid - 1) / grid * (p.silu ? 2 : 1))) {
     return fail(VMPS_ERR_UNSUPPORTED, "%s: no shared-memory plan for M=%d K=%d", what, M, K);
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == VMPS_DTYPE_F16 ? w4_by_group<__half>(group_size, p, grid, s)
-                                 : w4_by_group<__nv_bfloat16>(group_size, p, grid, s);
+  return dtype == VMPS_DTYPE_F16 ? w4_by_zeros<__half>(group_size, p, grid, s)
+                                 : w4_by_zeros<__nv_bfloat16>(group_size, p, grid, s);
 }
