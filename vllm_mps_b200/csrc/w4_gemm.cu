@@ -71,7 +71,6 @@ constexpr int kW4Threads = 32 * kW4Warps;
 __host__ __device__ constexpr int w4_chunk_bytes(int nt) { return nt == 1 ? 4096 : 2048; }
 constexpr int kW4Depth = 2;          // ring slots per warp: one chunk in flight, one in use
 constexpr int kW4SmemLimit = 226 * 1024;  // beside the static 64 bytes
-constexpr int kW4XBatch = 8;         // activation loads in flight per thread
 
 // Buffers of partial sums beside the rings: with two a team meets once per
 // block.  With more than one activation tile there is no room for them; a
@@ -457,86 +456,82 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
       const int nch = min(p.slice, p.chunks - ph * p.slice);
       if (p.phases > 1) __syncthreads();  // the last phase's X is done with
       {
-        // Stage the slice of X: 8 values a thread, in the order (0 4 1 5 2 6 3
-        // 7), and each group's sums.  A group is GROUP / 8 adjacent lanes.
-        // kW4XBatch loads are in flight per thread.
-        const int k0 = ph * p.slice * kCodes;
-        const int units = nch * (kCodes / 8);  // a multiple of 16
-        int m = 0, u = tid;
-        while (u >= units && m < p.M) {
-          u -= units;
-          ++m;
-        }
+        // Stage the slice of X, in the order (0 4 1 5 2 6 3 7), and each group's
+        // sums.  GROUP / 32 adjacent lanes take a row's group, 32 values each: one
+        // maximum and sum across lanes per 32 values (16 rows x 4096 took 5 us
+        // longer with one per 8).
+        constexpr int kLanes = GROUP / 32, kAtOnce = kW4Threads / kLanes;
+        const int groups = nch * GP, g0 = ph * p.slice * GP;
+        const int t = tid % kLanes;
+        int m = tid / kLanes / groups, gr = tid / kLanes - m * groups;
+        const int step_m = kAtOnce / groups, step_g = kAtOnce - step_m * groups;
         while (__any_sync(0xffffffffu, m < p.M)) {
-          uint4 v[kW4XBatch];
-          int um[kW4XBatch], uu[kW4XBatch];
+          const bool on = m < p.M;
+          uint4 v[4];
 #pragma unroll
-          for (int i = 0; i < kW4XBatch; ++i) {
-            um[i] = m;
-            uu[i] = u;
-            v[i] = make_uint4(0u, 0u, 0u, 0u);
-            const int k = k0 + u * 8;
-            if (m < p.M && k < p.K) {
-              v[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + m * p.x_stride + k);
+          for (int j = 0; j < 4; ++j) v[j] = make_uint4(0u, 0u, 0u, 0u);
+          if (on && g0 + gr < p.ng) {
+            const uint4* src = reinterpret_cast<const uint4*>(
+                static_cast<const T*>(p.x) + m * p.x_stride + (g0 + gr) * GROUP + t * 8);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = src[j * kLanes];
+          }
+          float up = 1.f;
+          if (kScaled) {
+            // Bit patterns of magnitudes order as integers, NaN above all.
+            uint32_t top2 = 0u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              top2 = __vmaxu2(__vmaxu2(top2, v[j].x & 0x7FFF7FFFu), v[j].y & 0x7FFF7FFFu);
+              top2 = __vmaxu2(__vmaxu2(top2, v[j].z & 0x7FFF7FFFu), v[j].w & 0x7FFF7FFFu);
             }
-            u += kW4Threads;
-            while (u >= units && m < p.M) {
-              u -= units;
-              ++m;
+            uint32_t top = max(top2 >> 16, top2 & 0xFFFFu);
+#pragma unroll
+            for (int sh = 1; sh < kLanes; sh <<= 1) {
+              top = max(top, __shfl_xor_sync(0xffffffffu, top, sh));
+            }
+            // 2^14 over the power of two at or below the largest, at most 2^127.
+            const int e = min(268 - static_cast<int>(top >> 7), 254);
+            up = __uint_as_float(static_cast<uint32_t>(e) << 23);
+          }
+          float even = 0.f, odd = 0.f;
+          uint8_t* dst = xs + m * p.x_pitch + (gr * (GROUP / 8) + t) * 16;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t h[4] = {v[j].x, v[j].y, v[j].z, v[j].w};  // eight fp16, in order
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (kScaled) {
+                h[k] = Elt<__half>::pack(__uint_as_float(h[k] << 16) * up,
+                                         __uint_as_float(h[k] & 0xFFFF0000u) * up);
+              }
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+              even += f.x;
+              odd += f.y;
+            }
+            if (on) {
+              *reinterpret_cast<uint4*>(dst + j * kLanes * 16) =
+                  make_uint4(__byte_perm(h[0], h[2], 0x5410), __byte_perm(h[0], h[2], 0x7632),
+                             __byte_perm(h[1], h[3], 0x5410), __byte_perm(h[1], h[3], 0x7632));
             }
           }
 #pragma unroll
-          for (int i = 0; i < kW4XBatch; ++i) {
-            if (!__any_sync(0xffffffffu, um[i] < p.M)) break;
-            const bool on = um[i] < p.M;
-            const int grp = uu[i] / (GROUP / 8);
-            const bool lead = on && uu[i] % (GROUP / 8) == 0;
-            uint4 h = v[i];  // eight fp16 activations, in order
-            if (!std::is_same<T, __half>::value) {
-              const uint32_t b4[4] = {h.x, h.y, h.z, h.w};
-              // Bit patterns of magnitudes order as integers, NaN above all.
-              uint32_t top = 0u;
-              float f[8];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                f[2 * j] = __uint_as_float(b4[j] << 16);
-                f[2 * j + 1] = __uint_as_float(b4[j] & 0xFFFF0000u);
-                top = max(top, max((b4[j] << 16) & 0x7FFFFFFFu, b4[j] & 0x7FFF0000u));
-              }
-#pragma unroll
-              for (int sh = 1; sh < GROUP / 8; sh <<= 1) {
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, sh));
-              }
-              // 2^14 over the power of two at or below the largest, at most 2^127.
-              const int e = min(268 - static_cast<int>(top >> 23), 254);
-              const float up = __uint_as_float(static_cast<uint32_t>(e) << 23);
-              uint32_t* hw = reinterpret_cast<uint32_t*>(&h);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) hw[j] = Elt<__half>::pack(f[2 * j] * up, f[2 * j + 1] * up);
-              if (lead) sx[(grp * kPlanes + kPlanes - 1) * (8 * NT) + um[i]] = 1.f / up;
-            }
-            uint4 o;
-            o.x = __byte_perm(h.x, h.z, 0x5410);
-            o.y = __byte_perm(h.x, h.z, 0x7632);
-            o.z = __byte_perm(h.y, h.w, 0x5410);
-            o.w = __byte_perm(h.y, h.w, 0x7632);
-            if (on) *reinterpret_cast<uint4*>(xs + um[i] * p.x_pitch + uu[i] * 16) = o;
+          for (int sh = 1; sh < kLanes; sh <<= 1) {
+            even += __shfl_xor_sync(0xffffffffu, even, sh);
+            odd += __shfl_xor_sync(0xffffffffu, odd, sh);
+          }
+          if (on && t == 0) {
+            float* at = sx + gr * kPlanes * (8 * NT) + m;
             // Offsets: 1024 for the pairs (0,4) and (2,6), 64 for the others.
-            const float2 x0 = __half22float2(*reinterpret_cast<const __half2*>(&o.x));
-            const float2 x1 = __half22float2(*reinterpret_cast<const __half2*>(&o.y));
-            const float2 x2 = __half22float2(*reinterpret_cast<const __half2*>(&o.z));
-            const float2 x3 = __half22float2(*reinterpret_cast<const __half2*>(&o.w));
-            float even = (x0.x + x0.y) + (x2.x + x2.y), odd = (x1.x + x1.y) + (x3.x + x3.y);
-#pragma unroll
-            for (int sh = 1; sh < GROUP / 8; sh <<= 1) {
-              even += __shfl_xor_sync(0xffffffffu, even, sh);
-              odd += __shfl_xor_sync(0xffffffffu, odd, sh);
-            }
-            if (lead) {
-              sx[grp * kPlanes * (8 * NT) + um[i]] =
-                  ZP ? -(1024.f * even + 64.f * odd) : -(1032.f * even + 72.f * odd);
-              if (ZP) sx[(grp * kPlanes + 1) * (8 * NT) + um[i]] = even + odd;
-            }
+            at[0] = ZP ? -(1024.f * even + 64.f * odd) : -(1032.f * even + 72.f * odd);
+            if (ZP) at[8 * NT] = even + odd;
+            if (kScaled) at[(kPlanes - 1) * 8 * NT] = 1.f / up;
+          }
+          m += step_m;
+          gr += step_g;
+          if (gr >= groups) {
+            gr -= groups;
+            ++m;
           }
         }
       }
