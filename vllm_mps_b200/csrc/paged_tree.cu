@@ -70,10 +70,19 @@ constexpr int kTtCtasPerSm = 2;
 constexpr int kTtMaxSeqs = 4096;
 constexpr int kTtMaxQLen = 1024;
 constexpr int kTtMaxRowTiles = 128;           // 1024 tokens x 16 heads / 128
+// A sequence's start costs a share about four tiles: with 2 in place of 4, 32
+// ragged sequences took 80.5 us for 77.9 and one of 8000 slots 21.5 for 19.8;
+// with 6, 77.3 and 20.3 (8 kv heads, head size 128).
 constexpr int kTileWeight = 4;
-constexpr int kSegWeight = 16;
-constexpr int kMinTiles = 4;                  // a share holds at least this many tiles
-constexpr int kWholeTiles = 8;                // contexts up to this many tiles are not cut
+constexpr int kSegWeight = 4 * kTileWeight;
+// Weight of a share, at least.  Short calls gain from small pieces until the
+// join costs as much: one sequence of 1000 slots takes 17.4 us with 8 tiles,
+// 13.7 with 3, 13.3 with 2; four of them (8 kv heads) 21.0, 17.4 and 17.6.
+constexpr int kMinShare = 3 * kTileWeight;
+// Contexts up to this many tiles are not cut, which saves the second launch:
+// one sequence of 500 slots takes 13.1 us whole and 14.0 cut, 32 of them 17.7
+// and 32.4; of 1000 slots one takes 19.1 whole and 13.7 cut.
+constexpr int kWholeTiles = 8;
 constexpr int kMergeThreads = 256;
 constexpr int kMergeBlocksPerSm = 2;
 constexpr int kMergeCols = 16;                // output columns per merge unit
@@ -429,9 +438,8 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
     // used - 1 shares partly empty.
     const int div = p.n_cta - (used > 0 ? used - 1 : 0);
     long long chunk = tree_div(total + div - 1, div);
-    // A piece has at least kMinTiles tiles; contexts that are not cut start a
-    // CTA each while there are CTAs left.
-    const long long least = p.whole ? 1 : kMinTiles * kTileWeight + kSegWeight;
+    // Contexts that are not cut start a CTA each while there are CTAs left.
+    const long long least = p.whole ? 1 : kMinShare;
     if (chunk < least) chunk = least;
     int first = 0, rt = 0;
     for (; rt < used; ++rt) {
