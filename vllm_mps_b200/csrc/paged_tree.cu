@@ -10,7 +10,14 @@
 // What bounds it.  Every K and V element is read once for all rows of its kv
 // head: 128 rows do 128 flops per byte, so up to about 200 rows per kv head
 // the cache stream from HBM is the bound, above that the arithmetic (first
-// the softmax, which the MMAs of the other CTA on the SM overlap).
+// the softmax, which the MMAs of the other CTA on the SM overlap).  Short calls
+// are bound by latency: 3.4 us of plan, 4.5 us to the first scores and, where
+// sequences are cut, about 10 us from the last CTA's end to the joined output.
+// Measured, 32 query and 8 kv heads of size 128 in bf16: 4 x 131072 slots, 16
+// drafts 333 us (6.45 TB/s, the copy rate); 32 ragged sequences of up to 4096
+// slots and 26 drafts 78 us (3.7 TB/s); with 64 query heads, 8 x 64 drafts over
+// up to 8192 slots 147 us (780 TFLOP/s, 0.48 of the bf16 peak).  One sequence
+// of 137 slots (heads 32/4 x 64) takes 9.6 us.
 //
 // Work split.  A row tile is 128 MMA rows: 128 / G drafted tokens x the G
 // query heads of a kv head, so K and V are read once per kv head and GQA is

@@ -5,7 +5,12 @@
 //
 // What bounds it.  Half a byte per weight and 2 M flops: the code stream from
 // HBM is the bound for every M here.  At 6.5 TB/s an SM has to take in ~46
-// codes a clock, so the work per code decides whether the stream is reached.
+// codes a clock, so the work per code decides whether the stream is reached:
+// it is not quite (about 290 instructions per 4096 codes, half the issue slots
+// used).  Measured, bf16, groups of 128: 128256 x 4096 at 16 rows 68 us (4.0
+// TB/s), [gate; up] 2 x 14336 x 4096 at one row 18.1 us (3.4 TB/s), of which 4 us
+// are the launch and the activations; 4096 x 14336 at 5 rows, groups of 64,
+// 20.5 us (1.6 TB/s: its activations are staged in two phases, 4 us each).
 //
 // Mathematics.  A code q becomes the fp16 number OFF + q by putting its four
 // bits into the mantissa of a constant (1024 where they land in bits 0-3 of a
@@ -41,9 +46,9 @@
 // chunks (2 or 4 KB of codes) in turn, and adds their partial sums of the block
 // through shared memory in a fixed order.  Every warp streams its own chunks
 // with 16-byte asynchronous copies into a private pair of slots, so nothing but
-// the block's sum is waited for by more than one warp; 32 or 64 KB are in flight.  (Bulk copies were tried:
-// with one per row or one tensor box per block the copy engine's per-line cost
-// capped the stream at 60 % of the rate of these.)  Scales and zero points go
+// the block's sum is waited for by more than one warp; 32 or 64 KB are in
+// flight.  (With one bulk copy per row or one tensor box per block the copy
+// engine's cost per line capped the stream at 60 % of this.)  Scales and zero points go
 // straight to the registers of the lane quad that uses them, as many chunks
 // ahead as the codes.
 //
