@@ -918,37 +918,47 @@ __global__ void __launch_bounds__(kMergeThreads, kMergeBlocksPerSm)
   constexpr int kColUnits = D / kMergeCols;
   constexpr int kBatch = 4;     // pieces in flight per warp
   __shared__ int s_rec[kMaxCtas][6];  // the joins, in order
-  __shared__ int s_base[kWarps + 1];
+  __shared__ int s_count[kWarps];
   __shared__ float s_ml[kWarps][32][2];
   __shared__ float4 s_o[kWarps][kQuads][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   tt_pdl_wait();
-  int n_items = 0;
-  for (int base = 0; base < p.n_cta; base += kMergeThreads) {
-    const int b = base + threadIdx.x;
-    int rec[6];
-    rec[0] = -1;
+  constexpr int kRecords = kMaxCtas / kMergeThreads;  // a thread's, loaded together
+  int rec[kRecords][6];
+  unsigned mask[kRecords];
+#pragma unroll
+  for (int r = 0; r < kRecords; ++r) {
+    const int b = r * kMergeThreads + threadIdx.x;
+    rec[r][0] = -1;
     if (b < p.n_cta) {
 #pragma unroll
-      for (int i = 0; i < 6; ++i) rec[i] = p.records[i * p.n_cta + b];
+      for (int i = 0; i < 6; ++i) rec[r][i] = p.records[i * p.n_cta + b];
     }
-    const bool on = rec[0] >= 0;
-    const unsigned mask = __ballot_sync(0xffffffffu, on);
-    if (lane == 0) s_base[warp + 1] = __popc(mask);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      s_base[0] = n_items;
-      for (int i = 0; i < kWarps; ++i) s_base[i + 1] += s_base[i];
-    }
-    __syncthreads();
-    if (on) {
-      int* dst = s_rec[s_base[warp] + __popc(mask & ((1u << lane) - 1))];
-#pragma unroll
-      for (int i = 0; i < 6; ++i) dst[i] = rec[i];
-    }
-    n_items = s_base[kWarps];
-    __syncthreads();
   }
+  int n_warp = 0;
+#pragma unroll
+  for (int r = 0; r < kRecords; ++r) {
+    mask[r] = __ballot_sync(0xffffffffu, rec[r][0] >= 0);
+    n_warp += __popc(mask[r]);
+  }
+  if (lane == 0) s_count[warp] = n_warp;
+  __syncthreads();
+  int at = 0, n_items = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) at += s_count[i];
+    n_items += s_count[i];
+  }
+#pragma unroll
+  for (int r = 0; r < kRecords; ++r) {
+    if (rec[r][0] >= 0) {
+      int* dst = s_rec[at + __popc(mask[r] & ((1u << lane) - 1))];
+#pragma unroll
+      for (int i = 0; i < 6; ++i) dst[i] = rec[r][i];
+    }
+    at += __popc(mask[r]);
+  }
+  __syncthreads();
   const int row_units = p.part_rows / 32;
   const int units = n_items * row_units * kColUnits;
   int per_unit = 1;  // warps
