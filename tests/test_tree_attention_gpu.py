@@ -384,3 +384,37 @@ def test_refusals(cuda_device):
         _call(K, _case(dev, [(20, 4, 4)], 8, 2, 96, torch.float16, seed=19))
     with pytest.raises(NotImplementedError):
         _call(K, _case(dev, [(20, 4, 4)], 17, 1, 64, torch.float16, seed=19))
+
+
+@pytest.mark.parametrize("n_q,nodes", [(8, 4), (16, 8), (32, 8)])
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (64, torch.bfloat16), (128, torch.float16)])
+def test_bad_drafts_in_many_short_sequences(cuda_device, n_q, nodes, D, dtype):
+    """Every CTA runs through several sequences of one or two key tiles, most of them with a
+    draft that holds an infinity: exactly the rows that see it carry it, every time.  The
+    shapes have rows for one, two and four of a CTA's four softmax warps."""
+    from vllm_mps_b200 import kernels as K
+
+    rng = np.random.default_rng(n_q + D)
+    seqs = []
+    for _ in range(700):
+        n = int(rng.integers(1, nodes + 1))
+        seqs.append((int(rng.choice([0, 3, 20, 60])), n, n))
+    seqs[0] = (60, nodes, nodes)
+    c = _case(cuda_device, seqs, n_q, 2, D, dtype, seed=n_q, spare=float("nan"))
+    want = _call(K, c)
+    assert torch.isfinite(want).all()
+    sees = torch.zeros(want.shape[0], dtype=torch.bool)
+    mask, bt, at = c["mask"].cpu(), c["bt"].cpu(), 0
+    blocks, slots = [], []
+    for i, (ctx, n, _) in enumerate(seqs):
+        if i % 5:  # the others stay as they are
+            node = int(rng.integers(0, n))
+            blocks.append(int(bt[i, (ctx + node) // 16]))
+            slots.append((ctx + node) % 16)
+            sees[at:at + n] = ((mask[at:at + n, 0] >> node) & 1).bool()
+        at += n
+    c["pool"][torch.tensor(blocks), 1, torch.tensor(slots), :, 5] = float("inf")
+    expected = want.clone()
+    expected[sees.to(cuda_device), :, 5] = float("inf")
+    for _ in range(20):
+        assert torch.equal(_call(K, c), expected)

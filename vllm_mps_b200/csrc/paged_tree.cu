@@ -371,8 +371,13 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
   uint64_t* v_empty = v_full + Shape::kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + Shape::kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  // Segment number (+1) whose V held a non-finite draft, by segment parity.
-  volatile int* odd_seg = abort_flag + 1;  // [2]
+  // Segment number (+1) whose V held a non-finite draft, by segment modulo 4.
+  // Two entries are not enough: a warp without rows of its own cleans V and
+  // skips the epilogues, and can be two segments ahead of one that has yet to
+  // read its entry (S(i + 2) follows PV(i), whatever the epilogue of the segment
+  // that ends with tile i does).  It is never three ahead: S(i + 3) follows
+  // PV(i + 1), for which every warp must have arrived in the segment after.
+  volatile int* odd_seg = abort_flag + 1;  // [4]
   TreeShare* share = reinterpret_cast<TreeShare*>(smem_raw + (reinterpret_cast<uint8_t*>(bars) - smem_raw) + 256);
   int* rt_weight = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 512);
   int* wpref = rt_weight + kTtMaxRowTiles;
@@ -397,7 +402,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
       mbar_init(v_empty + st, 1);
     }
     *abort_flag = 0;
-    odd_seg[0] = odd_seg[1] = 0;
+    for (int i = 0; i < 4; ++i) odd_seg[i] = 0;
     fence_mbar_init();
   }
   if (warp == kTtMmaWarp) {
@@ -726,7 +731,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
                   found = true;
                 }
               }
-              if (found) odd_seg[seg & 1] = seg + 1;
+              if (found) odd_seg[seg & 3] = seg + 1;
             }
           }
           tt_fence_async();
@@ -842,7 +847,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
         tt_wait(o_ready + ((it - 1) & 1), ((it - 1) >> 1) & 1, abort_flag, p.err);
         __syncwarp();
         tc_fence_after();
-        const bool odd = odd_seg[seg & 1] == seg + 1;
+        const bool odd = odd_seg[seg & 3] == seg + 1;
         // A row that saw nothing has l = 0 and O = 0.
         const float inv_l = l_run == 0.f ? 0.f : 1.f / l_run;
         const size_t piece = static_cast<size_t>(blockIdx.x) * 2 + slot;
