@@ -373,7 +373,8 @@ int vmps_commit_tree(int32_t* path, int32_t* count, int64_t* next_token, void* p
  * All contiguous and 16-byte aligned.  Sums and scaling in fp32, one rounding.
  * With silu_mul != 0 the weight is the fused [gate; up] of 2N rows and
  * out[m][n] = silu(gate) * up of the unrounded fp32 products.
- * Shapes: M <= 32, any N, group_size 32, 64 or 128, K a multiple of it; x
+ * Shapes: M <= 32, any N, group_size 32, 64 or 128, K a multiple of it below
+ * 2^31 - 1023, 2N * K / group_size below 2^31; x
  * 16-byte aligned with rows a multiple of 8 elements apart, out rows at least
  * N apart, 2-byte aligned.  vmps_w4_gemm_supported says whether a shape is
  * built (1) or not (0).

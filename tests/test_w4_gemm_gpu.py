@@ -204,3 +204,24 @@ def test_refusals(cuda_device):
         K_.w4_gemm(x, K_.W4Weight(w.codes, w.scales[:, :1].contiguous()))
     with pytest.raises(ValueError):
         K_.quantize_w4(torch.zeros((4, 100), device=dev).half())
+
+
+def test_rows_whose_bytes_pass_31_bits(cuda_device):
+    """32 rows of 2^26 columns (4 GB), zero but for a few columns all along them."""
+    from vllm_mps_b200 import kernels as K_
+
+    dev, K, M = cuda_device, 2 ** 26, 32
+    w = _weight(K_, dev, 2, K, 128, False, torch.float16, seed=4)
+    g = torch.Generator(device=dev).manual_seed(5)
+    at = torch.unique(torch.randint(0, K, (3000,), generator=g, device=dev))
+    at = torch.unique(torch.cat([at, torch.tensor([0, K - 1], device=dev)]))
+    x = torch.zeros((M, K), dtype=torch.float16, device=dev)
+    x[:, at] = torch.randn((M, len(at)), generator=g, device=dev).half() * 100
+    got = K_.w4_gemm(x, w).double()
+    assert K_.error_word(dev) == 0
+    code = w.codes[:, at // 2]
+    code = torch.where(at % 2 == 1, code >> 4, code & 15).double() - 8
+    s = w.scales[:, at // 128].double()
+    xd = x[:, at].double()
+    y, mag = xd @ (code * s).t(), xd.abs() @ s.t()
+    assert ((got - y).abs() <= EPS * mag + U[torch.float16] * y.abs() + 1e-7).all()

@@ -64,29 +64,12 @@
 
 #include "vmps_abi_internal.h"
 #include "vmps_common.cuh"
+#include "w4_plan.h"
 
 namespace vmps {
 namespace {
 
-constexpr int kW4MaxRows = 32;
-constexpr int kW4Warps = 16;
-constexpr int kW4Threads = 32 * kW4Warps;
-// Codes of a chunk (kRows rows x 2 * bytes / kRows codes): the larger amortises
-// more, but with more than one activation tile the activations need the room.
-__host__ __device__ constexpr int w4_chunk_bytes(int nt) { return nt == 1 ? 4096 : 2048; }
-constexpr int kW4Depth = 2;          // ring slots per warp: one chunk in flight, one in use
-constexpr int kW4SmemLimit = 226 * 1024;  // beside the static 64 bytes
-
-// Buffers of partial sums beside the rings: with two a team meets once per
-// block.  With more than one activation tile there is no room for them; a
-// warp's sums then go to its free ring slot, and the team meets twice.
-__host__ __device__ constexpr int w4_red_bufs(int nt) { return nt == 1 ? 2 : 0; }
-
-// Per group and activation row: what its sum starts from, [sum x,] [what its
-// sum is multiplied by].
-__host__ __device__ constexpr int w4_planes(bool scaled, bool zp) { return 1 + (zp ? 1 : 0) + (scaled ? 1 : 0); }
-
-struct W4Params {
+struct W4Params : W4Plan {
   void* out;
   int64_t out_stride;
   const void* x;
@@ -96,14 +79,7 @@ struct W4Params {
   const uint8_t* zeros;  // NULL: 8
   int M, N, K, ng;       // N: output features (half the weight's rows with silu)
   int silu;
-  int chunks;            // of K (the last may be partial)
-  int slice;             // chunks per phase
-  int phases;
-  int panel;             // blocks a CTA carries through the phases at once
-  int team;              // warps that share a block (a power of two)
   int blocks;            // of kRows features (per half with silu)
-  int x_pitch;           // bytes between activation rows in shared memory
-  int x_bytes, sx_bytes;
 };
 
 __device__ __forceinline__ void w4_pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -619,66 +595,6 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
 
 // ── host side ────────────────────────────────────────────────────────────────
 
-int w4_nt(int M) { return M <= 8 ? 1 : (M <= 16 ? 2 : 4); }
-int w4_mt(int M) { return M > 8 && M <= 16 ? 2 : 1; }
-
-// Shared-memory plan: the fewest bytes of X staged per CTA (phases times
-// panels) that leave room for everything else.
-bool w4_plan(W4Params* p, int group, int planes, int cta_blocks) {
-  const int nt = w4_nt(p->M), mt = w4_mt(p->M);
-  const int codes = w4_chunk_bytes(nt) * 2 / (16 * mt);
-  const int halves = p->silu ? 2 : 1;
-  // A warp should take about 16 KB of a block (its share of the block's fixed
-  // costs: with teams of 4 instead of 8 the LM head at 16 rows took 80 us for
-  // 88), but all warps should have a block.
-  const int few = 16384 / w4_chunk_bytes(nt);
-  p->team = 1;
-  while (p->team < kW4Warps &&
-         (p->team * few < p->chunks || p->team * (cta_blocks / halves) < kW4Warps)) {
-    p->team *= 2;
-  }
-  const int block = mt * nt * 512;  // bytes of a block's sums
-  const int fixed = kW4Warps * kW4Depth * w4_chunk_bytes(nt) +
-                    (w4_red_bufs(nt) * kW4Warps + (p->silu ? kW4Warps / p->team : 0)) * block;
-  long long best = -1;
-  for (int phases = 1; phases <= p->chunks; ++phases) {
-    const int slice = (p->chunks + phases - 1) / phases;
-    if ((p->chunks + slice - 1) / slice != phases) continue;
-    const int pitch = slice * codes * 2 + 64;  // 64 mod 128: rows g and g + 1 fill all banks
-    const int x_bytes = (p->M * pitch + 127) / 128 * 128;
-    const int sx_bytes = slice * (codes / group) * 8 * nt * 4 * planes;
-    const int left = kW4SmemLimit - fixed - x_bytes - sx_bytes;
-    int panel = cta_blocks;
-    if (left < 0) continue;
-    if (phases > 1) {
-      panel = left / block / halves * halves;
-      if (panel < halves) continue;
-      if (panel > cta_blocks) panel = cta_blocks;
-    }
-    const long long cost = phases == 1 ? 0 : static_cast<long long>((cta_blocks + panel - 1) / panel) *
-                                                  (p->chunks + 8 * phases);
-    if (best < 0 || cost < best) {
-      best = cost;
-      p->slice = slice;
-      p->phases = phases;
-      p->panel = panel;
-      p->x_pitch = pitch;
-      p->x_bytes = x_bytes;
-      p->sx_bytes = sx_bytes;
-    }
-    if (best == 0) break;
-  }
-  return best >= 0;
-}
-
-size_t w4_smem(const W4Params& p) {
-  const int block = w4_mt(p.M) * w4_nt(p.M) * 512;
-  return kW4Warps * kW4Depth * w4_chunk_bytes(w4_nt(p.M)) + p.x_bytes + p.sx_bytes +
-         static_cast<size_t>(w4_red_bufs(w4_nt(p.M)) * kW4Warps + (p.silu ? kW4Warps / p.team : 0) +
-                             (p.phases > 1 ? p.panel : 0)) *
-             block;
-}
-
 template <typename T, int GROUP, int NT, int MT, bool ZP>
 int w4_launch(const W4Params& p, int grid, cudaStream_t s) {
   static std::once_flag flags[64];
@@ -692,7 +608,7 @@ int w4_launch(const W4Params& p, int grid, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kW4Threads);
-  cfg.dynamicSmemBytes = w4_smem(p);
+  cfg.dynamicSmemBytes = p.smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -737,7 +653,7 @@ using namespace vmps;
 extern "C" int vmps_w4_gemm_supported(int M, int N, int K, int group_size) {
   if (M < 0 || M > kW4MaxRows || N <= 0 || K <= 0) return 0;
   if (group_size != 32 && group_size != 64 && group_size != 128) return 0;
-  if (K % group_size) return 0;
+  if (K % group_size || K > kW4MaxK) return 0;
   // Indices into the scales (of up to 2 N rows) are 31 bits.
   return 2 * static_cast<int64_t>(N) * (K / group_size) <= 0x7fffffff ? 1 : 0;
 }
@@ -770,7 +686,6 @@ extern "C" int vmps_w4_gemm(void* out, int64_t out_row_stride, const void* x, in
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   const int rows = 16 * w4_mt(M);
-  const int codes_per_chunk = w4_chunk_bytes(w4_nt(M)) * 2 / rows;
   W4Params p;
   p.out = out;
   p.out_stride = out_row_stride;
@@ -784,10 +699,9 @@ extern "C" int vmps_w4_gemm(void* out, int64_t out_row_stride, const void* x, in
   p.K = K;
   p.ng = K / group_size;
   p.silu = silu_mul ? 1 : 0;
-  p.chunks = (K + codes_per_chunk - 1) / codes_per_chunk;
   p.blocks = (N + rows - 1) / rows;
   const int grid = p.blocks < sms ? p.blocks : sms;
-  if (!w4_plan(&p, group_size, w4_planes(dtype != VMPS_DTYPE_F16, zeros != nullptr),
+  if (!w4_plan(&p, M, K, group_size, p.silu != 0, w4_planes(dtype != VMPS_DTYPE_F16, zeros != nullptr),
                (p.blocks + grid - 1) / grid * (p.silu ? 2 : 1))) {
     return fail(VMPS_ERR_UNSUPPORTED, "%s: no shared-memory plan for M=%d K=%d", what, M, K);
   }
