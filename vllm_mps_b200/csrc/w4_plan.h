@@ -3,11 +3,7 @@
 // a GPU.
 #pragma once
 
-#ifdef __CUDACC__
-#define VMPS_HD __host__ __device__
-#else
-#define VMPS_HD
-#endif
+#include "vmps_hd.h"
 
 namespace vmps {
 
