@@ -371,6 +371,8 @@ int vmps_commit_tree(int32_t* path, int32_t* count, int64_t* next_token, void* p
  *         low four bits.  scales: [N][K / group_size] in x's type.
  * zeros:  uint8 [N][K / group_size], or NULL for 8 everywhere.
  * All contiguous and 16-byte aligned.  Sums and scaling in fp32, one rounding.
+ * A row's infinities and NaN give what the formula gives and reach no other row
+ * (such a call takes longer).
  * With silu_mul != 0 the weight is the fused [gate; up] of 2N rows and
  * out[m][n] = silu(gate) * up of the unrounded fp32 products.
  * Shapes: M <= 32, any N, group_size 32, 64 or 128, K a multiple of it below

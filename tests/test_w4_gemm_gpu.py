@@ -225,3 +225,40 @@ def test_rows_whose_bytes_pass_31_bits(cuda_device):
     xd = x[:, at].double()
     y, mag = xd @ (code * s).t(), xd.abs() @ s.t()
     assert ((got - y).abs() <= EPS * mag + U[torch.float16] * y.abs() + 1e-7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("M,N,K,group", [(2, 100, 640, 64), (5, 130, 576, 64), (12, 70, 640, 128),
+                                         (20, 36, 96, 32), (32, 40, 8192, 128)])
+def test_non_finite_activations_follow_the_formula(cuda_device, M, N, K, group, silu, zeros, dtype):
+    """One infinity is an infinity of the code's sign (NaN where the code is the zero point),
+    two may cancel to NaN, and the rows without any are untouched."""
+    from vllm_mps_b200 import kernels as K_
+
+    dev = cuda_device
+    w = _weight(K_, dev, N, K, group, zeros, dtype, seed=M)
+    g = torch.Generator(device=dev).manual_seed(M + 1)
+    x = torch.randn((M, K), generator=g, device=dev).to(dtype)
+    clean = K_.w4_gemm(x, w, silu_mul=silu)
+    x[1, 41] = float("inf")
+    x[M - 1, 5] = float("-inf")
+    x[M - 1, K - 1] = float("inf")
+    if M > 2:
+        x[M // 2, K // 2] = float("nan")
+    y, _ = _parts(w, x)
+    if silu:
+        y = y[:, :N // 2] / (1.0 + torch.exp(-y[:, :N // 2])) * y[:, N // 2:]
+    got = K_.w4_gemm(x, w, silu_mul=silu)
+    touched = {1, M - 1} | ({M // 2} if M > 2 else set())
+    for r in range(M):
+        if r in touched:
+            want = y[r]
+            assert torch.equal(torch.isnan(got[r].cpu()), torch.isnan(want))
+            sure = ~torch.isnan(want)
+            assert torch.equal(got[r].cpu().double()[sure], want[sure])
+        else:
+            assert torch.equal(got[r], clean[r])
+    if M > 2:  # (of two rows the second has all three: NaN throughout)
+        assert torch.isinf(y[1]).any()

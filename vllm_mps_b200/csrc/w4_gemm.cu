@@ -30,6 +30,10 @@
 // than 2^-39 of it).  bf16's own mantissa holds the four bits in one place
 // only, which costs seven operations per word instead of five.
 //
+// A row with an infinity or NaN would come out as NaN throughout, the offsets'
+// share being taken off as inf - inf.  Such values decide the whole sum, so where
+// the staging meets one the epilogue sums them alone, from the definition.
+//
 // The eight codes of a 32-bit word are taken in the order (0,4) (1,5) (2,6)
 // (3,7): each pair is one mask of the word or of the word shifted by 8, and is
 // one operand register.  The activations are stored in the same order in
@@ -136,6 +140,50 @@ __device__ __forceinline__ void w4_mma_from(float (&d)[4], const uint32_t (&a)[4
       "{%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+
+// What row m's infinities and NaN make of weight row n's sum, or y if it has none.
+template <typename T, int GROUP>
+__device__ __forceinline__ float w4_nonfinite(const W4Params& p, int n, int m, float y) {
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  const uint4* row = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + m * p.x_stride);
+  const uint8_t* codes = p.codes + static_cast<int64_t>(n) * (p.K / 2);
+  bool found = false;
+  float sum = 0.f;
+#pragma unroll 1
+  for (int k8 = 0; k8 < p.K / 8; ++k8) {
+    const uint4 v = row[k8];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t bits = (w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu;
+      if ((bits & kExp) == kExp) {
+        const int k = k8 * 8 + i;
+        const int64_t at = static_cast<int64_t>(n) * p.ng + k / GROUP;
+        const int q = (codes[k >> 1] >> (4 * (k & 1))) & 15;
+        const int z = p.zeros ? p.zeros[at] : 8;
+        const unsigned short half = static_cast<unsigned short>(bits);
+        const float x = Elt<T>::to_f(*reinterpret_cast<const T*>(&half));
+        found = true;
+        sum += Elt<T>::to_f(static_cast<const T*>(p.scales)[at]) * (x * static_cast<float>(q - z));
+      }
+    }
+  }
+  return found ? sum : y;
+}
+
+// The same for a fragment's four values: (feature feat, row m), (feat, m + 1),
+// (feat + 8, m), (feat + 8, m + 1), of the weight's second half with `up`.  Only
+// ever runs after the staging met such a value.
+template <typename T, int GROUP>
+__device__ __noinline__ float4 w4_nonfinite4(const W4Params& p, int feat, int m, bool up, float4 y) {
+  float v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int n = feat + (e >> 1) * 8, r = m + (e & 1);
+    if (n < p.N && r < p.M) v[e] = w4_nonfinite<T, GROUP>(p, n + (up ? p.N : 0), r, v[e]);
+  }
+  return make_float4(v[0], v[1], v[2], v[3]);
 }
 
 // ZP: with zero points.  Without, every row's sum of a group starts from the
@@ -431,11 +479,13 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
 
   T* out = static_cast<T*>(p.out);
   int red_buf = 0, turn = 0;
+  int nonfinite = 0;  // an activation is (the same for all threads)
   for (int pv = v0; pv < v1; pv += p.panel) {
     const int pe = min(pv + p.panel, v1);
     for (int ph = 0; ph < p.phases; ++ph) {
       const int nch = min(p.slice, p.chunks - ph * p.slice);
       if (p.phases > 1) __syncthreads();  // the last phase's X is done with
+      int met = 0;
       {
         // Stage the slice of X, in the order (0 4 1 5 2 6 3 7), and each group's
         // sums.  GROUP / 32 adjacent lanes take a row's group, 32 values each: one
@@ -501,6 +551,8 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
             even += __shfl_xor_sync(0xffffffffu, even, sh);
             odd += __shfl_xor_sync(0xffffffffu, odd, sh);
           }
+          // (Finite ones cannot overflow: 128 fp16 numbers.)
+          met |= !(fabsf(even + odd) <= 3.4e38f);
           if (on && t == 0) {
             float* at = sx + gr * kPlanes * (8 * NT) + m;
             // Offsets: 1024 for the pairs (0,4) and (2,6), 64 for the others.
@@ -516,7 +568,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
           }
         }
       }
-      __syncthreads();
+      nonfinite |= __syncthreads_or(met);
       if (pv == v0 && ph == 0) w4_pdl_trigger();
 
       int off = w;  // this warp's next chunk, counted from the block's first
@@ -565,13 +617,16 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const __grid_constant
           }
           if (ph + 1 < p.phases) {
             *kept = y;
-          } else if (p.silu && !up) {
+            continue;
+          }
+          // Fragment: (feature g, row 2c), (g, 2c + 1), (g + 8, 2c), (g + 8, 2c + 1).
+          const int f = x >> 5;
+          const int feat = (p.silu ? v >> 1 : v) * kRows + (f / NT) * 16 + g;
+          const int m = (f % NT) * 8 + 2 * c;
+          if (nonfinite) y = w4_nonfinite4<T, GROUP>(p, feat, m, up, y);
+          if (p.silu && !up) {
             reinterpret_cast<float4*>(gate)[x] = y;  // read back by this thread
           } else {
-            // Fragment: (feature g, row 2c), (g, 2c + 1), (g + 8, 2c), (g + 8, 2c + 1).
-            const int f = x >> 5;
-            const int feat = (p.silu ? v >> 1 : v) * kRows + (f / NT) * 16 + g;
-            const int m = (f % NT) * 8 + 2 * c;
             if (up) {
               const float4 z = reinterpret_cast<const float4*>(gate)[x];
               y.x *= z.x / (1.f + expf(-z.x));
