@@ -418,3 +418,32 @@ def test_bad_drafts_in_many_short_sequences(cuda_device, n_q, nodes, D, dtype):
     expected[sees.to(cuda_device), :, 5] = float("inf")
     for _ in range(20):
         assert torch.equal(_call(K, c), expected)
+
+
+@pytest.mark.parametrize("bits", [16.3, 20.05, 25.5])
+@pytest.mark.parametrize("ctx", [200, 510, 8000])
+@pytest.mark.parametrize("dtype,D", [(torch.float16, 64), (torch.float16, 128), (torch.bfloat16, 64)])
+def test_many_small_weights_behind_a_large_one(cuda_device, ctx, bits, dtype, D):
+    """One key holds the row, all others weigh 2^-bits of it and alone have a value.
+
+    The bound of this file, and what a rounded weight may lose where the type runs out of
+    exponents: an fp16 weight is at least 2^7 times its share of the largest, so half of
+    its smallest step, 2^-25, is at most 2^-32 of the row's sum (bf16 has fp32's exponents).
+    """
+    from vllm_mps_b200 import kernels as K
+
+    c = _case(cuda_device, [(ctx, 1, 1)], 2, 1, D, dtype, seed=1)
+    t = torch.arange(ctx + 1, device=cuda_device)
+    blk = c["bt"][0, t // 16].long()
+    c["q"].zero_()
+    c["q"][..., 0] = 1.0
+    pool = c["pool"]
+    pool[blk, :, t % 16] = 0.0
+    pool[blk, 0, t % 16, :, 0] = -bits * math.log(2)
+    pool[blk, 1, t % 16] = 1.0
+    pool[blk[3], :, 3] = 0.0
+    got = _call(K, c, scale=1.0)
+    out, big, mag = _reference(c, scale=1.0)
+    lost = (ctx + 1) * 2.0 ** -32 if dtype == torch.float16 else 0.0
+    tol = (2 * U[dtype] + 4 * D * 2.0 ** -23 * mag) * big + lost + U[dtype] * out.abs() + 1e-6
+    assert ((got.double().cpu() - out).abs() <= tol).all()

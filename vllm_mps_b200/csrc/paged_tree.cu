@@ -51,7 +51,11 @@
 // them); a row that does see such a value adds it in its epilogue.
 //
 // Rounding: P is rounded to the 16-bit type as PV's operand (its sum is not),
-// the output once; scores, maxima, sums and accumulators are fp32.
+// the output once; scores, maxima, sums and accumulators are fp32.  fp16 has no
+// bits to spare below 2^-14, so its P is 2^kLift times as large: weights down to
+// 2^-21 of the row's largest keep all their bits, and what one loses below that is
+// at most 2^-32 of the largest (2^-25 without: many small weights behind a large
+// one then vanish from the product while the sum they are divided by has them).
 //
 // Safety.  Every mbarrier wait is bounded; a wait that gives up sets
 // kDevErrTimeout and a CTA-wide abort flag, the loads and MMAs stop being
@@ -77,6 +81,11 @@ constexpr int kTtCtasPerSm = 2;
 constexpr int kTtMaxSeqs = 4096;
 constexpr int kTtMaxQLen = 1024;
 constexpr int kTtMaxRowTiles = 128;           // 1024 tokens x 16 heads / 128
+// The running maximum bounds a score to within 2^kSlack; P <= 2^(kSlack + kLift),
+// which is below fp16's 65504.
+constexpr float kSlack = 8.f;
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
 constexpr int kMergeThreads = 256;
 constexpr int kMergeBlocksPerSm = 2;
 constexpr int kMergeCols = 16;                // output columns per merge unit
@@ -644,8 +653,8 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
           const float m_new = fmaxf(m_run, mx);
           if (j == j0) {
             m_run = m_new;
-          } else if (__any_sync(0xffffffffu, m_new > m_run + 8.f)) {
-            // The running maximum only has to bound the scores to within 2^8:
+          } else if (__any_sync(0xffffffffu, m_new > m_run + kSlack)) {
+            // The running maximum only has to bound the scores to within 2^kSlack:
             // O is rescaled (once the PV before has landed) when it grew by more.
             tt_wait(o_ready + ((it - 1) & 1), ((it - 1) >> 1) & 1, abort_flag, p.err);
             __syncwarp();
@@ -667,7 +676,7 @@ __global__ void __launch_bounds__(kTtThreads, kTtCtasPerSm)
           }
           uint32_t pk[KEYS / 32][16];
           uint64_t acc2[2] = {0ull, 0ull};
-          const float base = m_run == -INFINITY ? 0.f : m_run;
+          const float base = m_run == -INFINITY ? 0.f : m_run - kLift<T>;
           const uint64_t scale2 = f2_make(scale, scale);
           const uint64_t neg_m2 = f2_make(-base, -base);
 #pragma unroll
