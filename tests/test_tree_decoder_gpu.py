@@ -97,3 +97,38 @@ def test_refusals(engine):
     with pytest.raises(MemoryError):
         dec.generate([[1] * (16 * 200)], 4)
     assert eng.kv_cache_manager.get_num_free_gpu_blocks() == free
+
+
+@pytest.mark.parametrize("widths", [(3, 2, 2), (4, 4, 4)])
+def test_up_to_the_models_length(engine, widths):
+    """Prompt and tokens fill the model's length, the table holds less than a whole tree more."""
+    from vllm_mps_b200.engine.tree_decoder import TreeDecoder
+
+    eng, reference = engine
+    g = torch.Generator().manual_seed(8)
+    long = torch.randint(0, 1000, (990,), generator=g).tolist()
+    dec = TreeDecoder(eng, widths=widths)
+    outs = dec.generate([long, [3, 4]], 34)  # 1024 tokens
+    assert [len(o) for o in outs] == [34, 34]
+    _check_greedy(reference, [long, [3, 4]], outs)
+    # One sequence to the table's last slot: at the end the tree is the root alone.
+    slots = eng._graphs.max_blocks * 16
+    short = long[:slots - 40 - 24 + 1]
+    outs = dec.generate([short + [9] * 40], 24)
+    _check_greedy(reference, [short + [9] * 40], outs)
+    with pytest.raises(ValueError):
+        dec.generate([long], slots - 990 + 2)
+
+
+def test_a_pool_that_does_not_hold_all_sequences(engine):
+    from vllm_mps_b200.engine.tree_decoder import TreeDecoder
+
+    eng, reference = engine
+    free = eng.kv_cache_manager.get_num_free_gpu_blocks()
+    g = torch.Generator().manual_seed(9)
+    prompts = [torch.randint(0, 1000, (480 + i,), generator=g).tolist() for i in range(5)]
+    dec = TreeDecoder(eng)
+    outs = dec.generate(prompts, 60)  # 5 x 540 tokens in 2048 slots
+    assert [len(o) for o in outs] == [60] * 5
+    _check_greedy(reference, prompts, outs)
+    assert eng.kv_cache_manager.get_num_free_gpu_blocks() == free

@@ -218,8 +218,26 @@ class TreeDecoder:
             self._body(st)
         return g, st
 
-    def _round(self, sids: list[int], last: list[int], ctx: list[int]):
-        """One draft, check and commit of every sequence: (accepted tokens, next token) each."""
+    def _claim(self, sids: list[int], ctx: list[int]) -> list[int]:
+        """How many nodes of the tree each sequence has in this round, with their slots.
+
+        The first of them (a parent comes before its children): all, unless the
+        block table ends or the pool is full before.  The roots' slots are there."""
+        kv, n = self.engine.kv_cache_manager, len(self.tree)
+        limit = self.engine._graphs.max_blocks * BLOCK_SIZE
+        keep = []
+        for s, c in zip(sids, ctx):
+            want = min(n, limit - c)
+            room = kv.free_slots_in_last_block(s) + BLOCK_SIZE * kv.get_num_free_gpu_blocks()
+            kv.append_slots(s, min(c + want - kv.num_tokens(s), room))
+            keep.append(min(want, kv.num_tokens(s) - c))
+        return keep
+
+    def _round(self, sids: list[int], last: list[int], ctx: list[int], keep: list[int]):
+        """One draft, check and commit of every sequence: (accepted tokens, next token) each.
+
+        ``keep``: the nodes of each sequence's tree.  The rows of the others run along, own no
+        slot, and are past the sequence's length for the commit and every other row."""
         kv = self.engine.kv_cache_manager
         n, B = len(self.tree), len(sids)
         Bb = 1
@@ -231,18 +249,15 @@ class TreeDecoder:
         h = st.host.numpy()
         h[:] = 0
         bt = h[st.bt[0]:st.bt[1]].reshape(Bb, st.W)
-        for i, (s, c) in enumerate(zip(sids, ctx)):
-            short = c + n - kv.num_tokens(s)
-            if short > 0:
-                kv.append_slots(s, short)
+        for i, s in enumerate(sids):
             table = kv.get_block_ids(s)
-            if len(table) > st.W:
-                raise ValueError(f"a context of {c} tokens with {n} drafts needs more than the "
-                                 f"{st.W} blocks the model's length allows")
             bt[i, :len(table)] = table
-        host_ctx = np.asarray(ctx, dtype=np.int64)
-        at = host_ctx[:, None] + np.arange(n)
+        host_ctx, kept = np.asarray(ctx, dtype=np.int64), np.asarray(keep, dtype=np.int64)
+        nodes = np.arange(n)
+        own = nodes < kept[:, None]
+        at = np.where(own, host_ctx[:, None] + nodes, 0)
         slots = np.take_along_axis(bt[:B], at // BLOCK_SIZE, 1).astype(np.int64) * BLOCK_SIZE + at % BLOCK_SIZE
+        slots[~own] = -1
         h[st.ctx[0]:st.ctx[0] + B] = host_ctx
         h[st.root[0]:st.root[0] + B] = last
         for nodes, (v_slots, v_pos, v_lens) in zip(st.passes, st.views):
@@ -250,7 +265,7 @@ class TreeDecoder:
             rows = B * len(nodes)
             h[v_slots[0]:v_slots[0] + rows] = slots[:, nodes].reshape(-1)
             h[v_pos[0]:v_pos[0] + rows] = (host_ctx[:, None] + self.tree.depths[nodes]).reshape(-1)
-            h[v_lens[0]:v_lens[0] + B] = host_ctx + int(nodes[-1]) + 1
+            h[v_lens[0]:v_lens[0] + B] = host_ctx + np.minimum(kept, int(nodes[-1]) + 1)
         st.dev.copy_(st.host, non_blocking=True)
         g.replay()
         st.landed.copy_(st.result, non_blocking=True)
@@ -286,37 +301,74 @@ class TreeDecoder:
 
     @torch.no_grad()
     def generate(self, prompts: list[list[int]], max_tokens: int) -> list[list[int]]:
-        """``max_tokens`` greedy tokens for each prompt (lists of token ids, none empty)."""
+        """``max_tokens`` greedy tokens for each prompt (lists of token ids, none empty).
+
+        Near the end of the block table or with a full pool a round's trees get
+        smaller, down to the root alone (a plain step).  Where the pool does not
+        hold all sequences, the last ones wait, or give their blocks back and are
+        prefilled again later.  A prompt that could never be finished is refused
+        before anything runs: ``MemoryError`` if the free blocks do not hold it
+        and its tokens, ``ValueError`` if the block table does not.
+        """
         if any(len(p) == 0 for p in prompts):
             raise ValueError("every prompt needs at least one token")
         if max_tokens < 1:
             raise ValueError("max_tokens must be at least 1")
         kv = self.engine.kv_cache_manager
+        free, width = kv.get_num_free_gpu_blocks(), self.engine._graphs.max_blocks
+        for p in prompts:
+            slots = len(p) + max_tokens - 1  # the last token's K/V is never written
+            blocks = -(-slots // BLOCK_SIZE)
+            if blocks > free:
+                raise MemoryError(f"a prompt of {len(p)} tokens and {max_tokens} more need {blocks} "
+                                  f"blocks, {free} are free")
+            if blocks > width:
+                raise ValueError(f"a prompt of {len(p)} tokens and {max_tokens} more need {blocks} "
+                                 f"blocks, the model's length allows {width}")
         taken = set(kv.get_all_seq_ids())
         sids, sid = [], -1
         while len(sids) < len(prompts):
             if sid not in taken:
                 sids.append(sid)
             sid -= 1
-        allocated = []
+        out = [[] for _ in prompts]
+        live, waiting = [], list(range(len(prompts)))
         try:
-            for s, p in zip(sids, prompts):
-                kv.allocate(s)
-                allocated.append(s)
-                kv.append_slots(s, len(p))
-            self._prefill(sids, prompts)
-            out = [[] for _ in prompts]
-            live = list(range(len(prompts)))
-            while live:
+            while live or waiting:
+                fresh = []
+                # One that joins others leaves each of them a block to go on with.
+                while waiting and (kv.blocks_needed(sids[waiting[0]], len(prompts[waiting[0]] + out[waiting[0]]))
+                                   + len(live) <= kv.get_num_free_gpu_blocks() or not live):
+                    i = waiting.pop(0)
+                    live.append(i)
+                    fresh.append(i)
+                    kv.allocate(sids[i])
+                    kv.append_slots(sids[i], len(prompts[i]) + len(out[i]))
+                self._prefill([sids[i] for i in fresh], [prompts[i] + out[i] for i in fresh])
+                # A slot for every root; the last sequences make room for the first.
+                at = 0
+                while at < len(live):
+                    i = live[at]
+                    short = len(prompts[i]) + len(out[i]) - kv.num_tokens(sids[i])
+                    if short > 0 and not kv.can_allocate(sids[i], short):
+                        waiting.insert(0, live.pop())
+                        kv.free(sids[waiting[0]])
+                    else:
+                        kv.append_slots(sids[i], short)
+                        at += 1
+                ids = [sids[i] for i in live]
                 last = [(out[i] or prompts[i])[-1] for i in live]
                 ctx = [len(prompts[i]) + len(out[i]) - 1 for i in live]
-                for i, (path, nxt) in zip(live, self._round([sids[i] for i in live], last, ctx)):
+                for i, (path, nxt) in zip(live, self._round(ids, last, ctx, self._claim(ids, ctx))):
                     out[i] += path + [nxt]
+                    if len(out[i]) >= max_tokens:
+                        kv.free(sids[i])
                 live = [i for i in live if len(out[i]) < max_tokens]
             return [o[:max_tokens] for o in out]
         finally:
-            for s in allocated:
-                kv.free(s)
+            for s in sids:
+                if kv.has_sequence(s):
+                    kv.free(s)
 
 
 def _w4(x: torch.Tensor, w: K.W4Weight, silu_mul: bool = False) -> torch.Tensor:
