@@ -262,3 +262,17 @@ def test_non_finite_activations_follow_the_formula(cuda_device, M, N, K, group, 
             assert torch.equal(got[r], clean[r])
     if M > 2:  # (of two rows the second has all three: NaN throughout)
         assert torch.isinf(y[1]).any()
+
+
+@pytest.mark.parametrize("size", [1e-4, 1e-6])
+def test_subnormal_scales(cuda_device, size):
+    """Weights so small that their fp16 scales are subnormal: their codes are used in full."""
+    from vllm_mps_b200 import kernels as K_
+
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    full = (torch.randn((40, 512), generator=g, device=cuda_device) * size).half()
+    w = K_.quantize_w4(full, 64)
+    assert (w.scales < torch.finfo(torch.float16).smallest_normal).all() and (w.scales > 0).all()
+    assert len(torch.unique(w.codes & 15)) > 4
+    x = torch.randn((3, 512), generator=g, device=cuda_device).half() * 1000
+    _check(K_.w4_gemm(x, w), w, x)

@@ -888,7 +888,8 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, zero_points: bool = True
 
     With ``zero_points`` a group's codes span its range (extended to hold
     zero); without, they are symmetric around code 8.  The scale is rounded
-    to ``w``'s dtype first and the codes are the nearest to that scale.
+    to ``w``'s dtype first (up, where that is subnormal) and the codes are the
+    nearest to that scale.
     """
     if w.dim() != 2 or w.shape[1] % group_size or group_size not in (32, 64, 128):
         raise ValueError("w must be (N, K) with K a multiple of group_size (32, 64 or 128)")
@@ -899,9 +900,12 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, zero_points: bool = True
         scale = (hi - lo) / 15.0
     else:
         scale = g.abs().amax(2) / 7.0
-    scale = torch.where(scale > 0, scale, torch.ones_like(scale)).to(w.dtype)
-    # A scale that underflows the dtype would divide by zero: the smallest normal stands in.
-    scale = scale.clamp(min=torch.finfo(w.dtype).tiny)
+    scale = torch.where(scale > 0, scale, torch.ones_like(scale))
+    # A subnormal scale is rounded up: to nearest, it could be zero, or so far below that
+    # the codes no longer reach the group's ends.
+    info = torch.finfo(w.dtype)
+    least = info.smallest_normal * info.eps
+    scale = torch.where(scale < info.smallest_normal, torch.ceil(scale / least) * least, scale).to(w.dtype)
     s = scale.float()
     zeros = torch.round(-lo / s).clamp(0, 15) if zero_points else torch.full_like(s, 8.0)
     q = (torch.round(g / s.unsqueeze(2)) + zeros.unsqueeze(2)).clamp(0, 15).to(torch.uint8).view(N, K)
