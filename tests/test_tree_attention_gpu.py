@@ -447,3 +447,16 @@ def test_many_small_weights_behind_a_large_one(cuda_device, ctx, bits, dtype, D)
     lost = (ctx + 1) * 2.0 ** -32 if dtype == torch.float16 else 0.0
     tol = (2 * U[dtype] + 4 * D * 2.0 ** -23 * mag) * big + lost + U[dtype] * out.abs() + 1e-6
     assert ((got.double().cpu() - out).abs() <= tol).all()
+
+
+def test_queries_as_a_matrix(cuda_device):
+    """(total_q, n_q * D) queries, none of them included."""
+    from vllm_mps_b200 import kernels as K
+
+    c = _case(cuda_device, [(20, 4, 4)], 8, 2, 64, torch.float16, seed=20, q_pad=64)
+    flat = torch.as_strided(c["q"], (4, 8 * 64), (c["q"].stride(0), 1))
+    assert torch.equal(_call(K, dict(c, q=flat)), _call(K, c))
+    c = _case(cuda_device, [(20, 0, 0)], 8, 2, 64, torch.float16, seed=20)
+    assert _call(K, dict(c, q=c["q"].flatten(1))).shape == (0, 8, 64)
+    with pytest.raises(ValueError):
+        _call(K, dict(c, q=c["q"].flatten(1)[:, :500]))

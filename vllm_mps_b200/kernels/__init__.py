@@ -728,8 +728,8 @@ def paged_tree_attention(q: torch.Tensor, pool: torch.Tensor, block_tables: torc
     if len(shape) != 5 or shape[1] != 2 or not pool.is_contiguous():
         _check_pool(pool)
     num_blocks, _, block_size, n_kv, D = shape
-    if q.dim() == 2:
-        q = q.view(q.shape[0], -1, D)
+    if q.dim() == 2 and q.shape[1] % D == 0:
+        q = q.unflatten(1, (q.shape[1] // D, D))
     if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or q.stride(1) != D:
         raise ValueError(f"q must be (total_q, n_q, {D}) with packed heads; got {tuple(q.shape)}")
     total_q, n_q, _ = q.shape
