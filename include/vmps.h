@@ -370,7 +370,11 @@ int vmps_commit_tree(int32_t* path, int32_t* count, int64_t* next_token, void* p
  * codes:  uint8 [N][K / 2], row n's code k in byte k / 2, the even k in the
  *         low four bits.  scales: [N][K / group_size] in x's type.
  * zeros:  uint8 [N][K / group_size], or NULL for 8 everywhere.
- * All contiguous and 16-byte aligned.  Sums and scaling in fp32, one rounding.
+ * All contiguous and 16-byte aligned.  Sums and scaling in fp32, one rounding;
+ * codes are carried as 1024 + code, whose share of a group's fp32 sum is taken
+ * off again: before its rounding an output is within 2^-12 * sum_k |x| * scale
+ * of the formula (for zero points up to 15).  fp16 activations that share their
+ * sign come near that, random signs stay below a hundredth of it.
  * A row's infinities and NaN give what the formula gives and reach no other row
  * (such a call takes longer).
  * With silu_mul != 0 the weight is the fused [gate; up] of 2N rows and

@@ -276,3 +276,57 @@ def test_subnormal_scales(cuda_device, size):
     assert len(torch.unique(w.codes & 15)) > 4
     x = torch.randn((3, 512), generator=g, device=cuda_device).half() * 1000
     _check(K_.w4_gemm(x, w), w, x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M", [1, 10, 25])
+def test_zero_points_of_all_eight_bits(cuda_device, M, dtype):
+    """A zero point above 15 adds up to 255 to the magnitudes that the bound's 1032 stands for."""
+    from vllm_mps_b200 import kernels as K_
+
+    dev = cuda_device
+    w = _weight(K_, dev, 90, 1024, 64, True, dtype, seed=11)
+    w.zeros.copy_(torch.arange(90 * 16, device=dev).view(90, 16) % 256)
+    g = torch.Generator(device=dev).manual_seed(M)
+    x = torch.randn((M, 1024), generator=g, device=dev).to(dtype)
+    y, mag = _parts(w, x)
+    diff = (K_.w4_gemm(x, w).double().cpu() - y).abs()
+    assert (diff <= EPS * (1032 + 255) / 1032 * mag + U[dtype] * y.abs() + 1e-7).all()
+
+
+@pytest.mark.parametrize("M", [1, 7, 16, 32])
+def test_bf16_activations_of_any_size(cuda_device, M):
+    """bf16 groups enter the fp16 products scaled by a power of two of their own: a power of
+    two in x is the same one in y, bit for bit, and within a group small and large values,
+    zeros and the smallest numbers stand side by side."""
+    from vllm_mps_b200 import kernels as K_
+
+    dev = cuda_device
+    w = _weight(K_, dev, 100, 1024, 64, True, torch.bfloat16, seed=12)
+    g = torch.Generator(device=dev).manual_seed(M)
+    x = torch.randn((M, 1024), generator=g, device=dev).bfloat16()
+    want = K_.w4_gemm(x, w).double()
+    for power in (-100, -40, 40, 100):
+        got = K_.w4_gemm((x.double() * 2.0 ** power).bfloat16(), w).double()
+        assert torch.equal(got * 2.0 ** -power, want)
+    wide = (x.double() * torch.exp2(torch.randint(-40, 41, x.shape, generator=g, device=dev))).bfloat16()
+    wide[:, :64] = 0                      # a group of zeros
+    wide[:, 64:128] = 2.0 ** -133         # a group of bf16's smallest numbers
+    wide[:, 200] = 2.0 ** -133            # one beside ordinary ones
+    wide[0] = 0
+    _check(K_.w4_gemm(wide, w), w, wide)
+    assert (K_.w4_gemm(wide, w)[0] == 0).all()
+
+
+def test_fp16_outliers_and_large_means(cuda_device):
+    from vllm_mps_b200 import kernels as K_
+
+    dev = cuda_device
+    g = torch.Generator(device=dev).manual_seed(13)
+    w = _weight(K_, dev, 150, 2048, 128, False, torch.float16, seed=13)
+    for M in (2, 12, 30):
+        x = torch.randn((M, 2048), generator=g, device=dev)
+        x[:, 700] = 4000.0
+        _check(K_.w4_gemm(x.half(), w), w, x.half())
+        x = torch.randn((M, 2048), generator=g, device=dev) + 30
+        _check(K_.w4_gemm(x.half(), w), w, x.half())

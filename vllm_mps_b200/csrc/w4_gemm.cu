@@ -21,7 +21,12 @@
 // CTA) and are what the group's fp32 accumulator starts from.  The matrix
 // instruction (m16n8k16, codes as the 16-row side, activations as the 8-wide
 // side) sums a group in fp32; the scale multiplies that sum in fp32, so
-// neither scale nor zero point is ever rounded into a weight.
+// neither scale nor zero point is ever rounded into a weight.  What the offset
+// costs is fp32 bits of that sum: measured (fp16, K 4096) 0.012 x 2^-12 of
+// sum |x| scale at most for activations of random sign, 0.76 x 2^-12 where all
+// are near 30.  Rounding a weight to four bits costs such a sum thirty times as
+// much, and taking half of the offset off after the products instead (0.24 x
+// 2^-12) 2 to 5 % of the time.
 //
 // bf16 activations go through the same fp16 instruction: each group of a row
 // is multiplied by the power of two that brings its largest magnitude into
