@@ -2,8 +2,10 @@
 
 Builds a random-weight Llama of the given size (there is nothing to download),
 decodes a few prompts with the engine and with ``TreeDecoder`` and prints how
-many tokens a round decided.  Random weights have no structure a drafter could
-exploit beyond rounding, so real checkpoints accept more.
+many tokens a round decided, and how many it would have to for the same time.
+Random weights have no structure a drafter could exploit beyond rounding, so
+real checkpoints accept more; but a drafted level costs about as much as a plain
+step here, and at none of the sizes tried was the break-even reached.
 
     python examples/tree_speculation.py [--layers 8] [--hidden 2048] [--batch 4] [--tokens 64]
 """
@@ -63,8 +65,9 @@ def main() -> None:
     decoder = TreeDecoder(engine, widths=a.widths)
     got, t1 = timed(lambda: decoder.generate(prompts, a.tokens))
     same = sum(x == y for p, q in zip(want, got) for x, y in zip(p, q))
+    per_round = decoder.accepted / max(1, decoder.rounds)
     print(f"engine {t0 * 1e3:.1f} ms, tree of {len(decoder.tree)} nodes {t1 * 1e3:.1f} ms, "
-          f"{decoder.accepted / max(1, decoder.rounds):.2f} tokens a round, "
+          f"{per_round:.2f} tokens a round (as fast at {per_round * t1 / t0:.2f}), "
           f"{same} of {a.batch * a.tokens} tokens equal")
 
 

@@ -13,11 +13,13 @@
 // the softmax, which the MMAs of the other CTA on the SM overlap).  Short calls
 // are bound by latency: 3.4 us of plan, 4.5 us to the first scores and, where
 // sequences are cut, about 10 us from the last CTA's end to the joined output.
-// Measured, 32 query and 8 kv heads of size 128 in bf16: 4 x 131072 slots, 16
-// drafts 333 us (6.45 TB/s, the copy rate); 32 ragged sequences of up to 4096
-// slots and 26 drafts 78 us (3.7 TB/s); with 64 query heads, 8 x 64 drafts over
-// up to 8192 slots 147 us (780 TFLOP/s, 0.48 of the bf16 peak).  One sequence
-// of 137 slots (heads 32/4 x 64) takes 9.6 us.
+// Measured, 32 query and 8 kv heads of size 128 in bf16, calls in a row: 4 x
+// 131072 slots, 16 drafts 332 to 348 us (6.2 to 6.5 TB/s, the copy rate); 32 ragged
+// sequences of up to 4096 slots and 26 drafts 78 us (3.7 TB/s); with 64 query
+// heads, 8 x 64 drafts over up to 8192 slots 143 to 206 us by the box's power state
+// (0.34 to 0.49 of the bf16 peak; the softmax warps spill registers).  One sequence
+// of 137 slots (heads 32/4 x 64) takes 9.5 us, and 13.5 where the tables are wide
+// enough for contexts that would be cut.
 //
 // Work split.  A row tile is 128 MMA rows: 128 / G drafted tokens x the G
 // query heads of a kv head, so K and V are read once per kv head and GQA is

@@ -8,9 +8,11 @@
 // codes a clock, so the work per code decides whether the stream is reached:
 // it is not quite (about 290 instructions per 4096 codes, half the issue slots
 // used).  Measured, bf16, groups of 128: 128256 x 4096 at 16 rows 68 us (4.0
-// TB/s), [gate; up] 2 x 14336 x 4096 at one row 18.1 us (3.4 TB/s), of which 4 us
+// TB/s), [gate; up] 2 x 14336 x 4096 at one row 18.3 us (3.4 TB/s), of which 4 us
 // are the launch and the activations; 4096 x 14336 at 5 rows, groups of 64,
-// 20.5 us (1.6 TB/s: its activations are staged in two phases, 4 us each).
+// 20.5 us (1.6 TB/s: its activations are staged in two phases, 4 us each).  Above
+// 16 rows, with 2 to 5 phases and a fragment read per block, it is far from the
+// stream: 128256 x 4096 takes 135 us at 24 rows, 179 at 32.
 //
 // Mathematics.  A code q becomes the fp16 number OFF + q by putting its four
 // bits into the mantissa of a constant (1024 where they land in bits 0-3 of a
@@ -24,7 +26,7 @@
 // neither scale nor zero point is ever rounded into a weight.  What the offset
 // costs is fp32 bits of that sum: measured (fp16, K 4096) 0.012 x 2^-12 of
 // sum |x| scale at most for activations of random sign, 0.76 x 2^-12 where all
-// are near 30.  Rounding a weight to four bits costs such a sum thirty times as
+// are near 30.  Rounding a weight to four bits costs such a sum some 25 times as
 // much, and taking half of the offset off after the products instead (0.24 x
 // 2^-12) 2 to 5 % of the time.
 //
