@@ -300,6 +300,8 @@ int vmps_batch_gemm(void* out, int64_t out_row_stride, const void* x, int64_t x_
  * q_lens[i]; a row sees every slot t < ctx_lens[i] and the draft j whose bit
  * (j & 31) of tree_mask[row][j >> 5] is set:
  *   out[row][h] = softmax_t(scale * q[row][h] . K[t][h / G]) . V[t][h / G].
+ * Scores, maxima and sums are fp32; a softmax weight is rounded to the 16-bit
+ * type for its product with V, the output once.
  * A row that sees no slot is zero.  Slots no row sees and drafts outside a
  * row's mask take no part, whatever they hold (NaN and infinities included).
  * Mask bits of drafts past seq_lens[i] are ignored; drafts past

@@ -923,7 +923,8 @@ def w4_gemm(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None,
     """``x @ w.T`` with a 4-bit weight, for up to 32 rows (a drafter's projections).
 
     ``x``: (M, K) fp16 or bf16 with unit inner stride, rows a multiple of 8
-    elements apart.  Sums and scales in fp32, one rounding.  With
+    elements apart.  Sums and scales in fp32 (what the codes' offset costs them is
+    bounded in ``vmps.h``), one rounding.  With
     ``silu_mul`` the weight is the fused [gate; up] matrix of 2I rows and the
     result is ``silu(x @ Wg.T) * (x @ Wu.T)`` (M, I), rounded once at the end.
     Returns ``out`` (M, N).
