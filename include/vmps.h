@@ -45,6 +45,10 @@ extern "C" {
 #define VMPS_DTYPE_F16 0
 #define VMPS_DTYPE_BF16 1
 
+#define VMPS_CACHE_16BIT 0 /* the pool in the call's dtype */
+#define VMPS_CACHE_INT8 1  /* 8-bit cache of int8 codes */
+#define VMPS_CACHE_E4M3 2  /* 8-bit cache of e4m3 codes */
+
 /* Library version string, e.g. "vmps 0.1.0 sm_100a". */
 const char* vmps_version(void);
 
@@ -391,6 +395,97 @@ int vmps_w4_gemm_supported(int M, int N, int K, int group_size);
 int vmps_w4_gemm(void* out, int64_t out_row_stride, const void* x, int64_t x_row_stride,
                  const void* codes, const void* scales, const void* zeros, int M, int N, int K,
                  int group_size, int silu_mul, int dtype, void* stream);
+
+/*
+ * The 8-bit paged cache (VMPS_CACHE_INT8, VMPS_CACHE_E4M3), half the bytes of
+ * the 16-bit pool.  No counterpart in the reference.
+ *   codes  [num_blocks][2][16][n_kv][head_dim]  int8 or e4m3 (dim 1: 0 = K, 1 = V)
+ *   scales [num_blocks][n_kv][2][16]            fp32
+ * both contiguous and 16-byte aligned.  The value stored is code * scale of its
+ * token, head and kind.  Written by vmps_norm_rope_and_cache, the scale is the
+ * largest magnitude of the token's head_dim values over 127 (int8) or 448
+ * (e4m3) and the code the value over the scale, to nearest with ties to even
+ * (computed in fp32: a value within 2^-21 of a tie may go to either side).  Rows
+ * whose largest magnitude is below 2^-100 are stored as zeros with scale 0; a
+ * row that holds an infinity or a NaN has scale NaN and reads as NaN.
+ */
+
+/*
+ * Norms of queries and keys per head, rotation and cache write in one pass
+ * (kernel 9), for attention layers that normalise q and k, and for every layer
+ * over an 8-bit cache.  No counterpart in the reference, whose layers have
+ * neither; the write takes the place of vmps_rope_reshape_and_cache.
+ *   y = x * weight / sqrt(mean(x^2) + eps) over a head's head_dim values of q
+ *       and k (q_weight, k_weight: [head_dim] of `dtype`; NULL: y = x)
+ *   q_out = rope(y of q); K slot <- rope(y of k); V slot <- v
+ * rope() is the rotate-half form with the angle positions[i] * inv_freq[j],
+ * whose product is exact (vmps_rope_reshape_and_cache rounds it to fp32, as the
+ * reference does).  All of it is fp32 and rounded once, to `dtype` or to a code
+ * of `cache_format`.  inv_freq NULL: no rotation (positions may be NULL).
+ *
+ * q_out, q, k, v: num_rows rows of heads [heads][head_dim], row strides in
+ * elements (multiples of 8, at least a row); q_out may be q where the strides
+ * agree.  n_q 0: keys and values alone.  slot_mapping int32[num_rows]: block *
+ * 16 + slot, negative: nothing is cached for the row.  Two rows of a call must
+ * not share a slot.  A negative position sets error bit 16 and skips the row, a
+ * slot outside the cache sets bit 1 and is not written.  scales: NULL for
+ * VMPS_CACHE_16BIT.  Supported: head_dim 64 or 128, block_size 16; all pointers
+ * 16-byte aligned.
+ */
+int vmps_norm_rope_and_cache(void* q_out, int64_t q_out_row_stride, const void* q,
+                             int64_t q_row_stride, const void* k, int64_t k_row_stride,
+                             const void* v, int64_t v_row_stride, const void* q_weight,
+                             const void* k_weight, float eps, const int32_t* positions,
+                             const int32_t* slot_mapping, const float* inv_freq, void* cache,
+                             float* scales, int num_rows, int n_q, int n_kv, int head_dim,
+                             int block_size, int num_blocks, int cache_format, int dtype,
+                             void* stream);
+
+/*
+ * Pages of the 8-bit cache read back into 16-bit pages (kernel 10), e.g. for
+ * vmps_paged_prefill_attention or vmps_paged_tree_attention.  Page j of sequence
+ * i, block_tables[i][j], goes to block dst_tables[i][j] of `pool`
+ * ([pool_blocks][2][16][n_kv][head_dim] of `dtype`) for j < ceil(seq_lens[i] /
+ * 16); both tables have max_blocks_per_seq columns.  Slots at and past
+ * seq_lens[i] of the last page are set to zero, other blocks are left as they
+ * were.  code * scale is fp32, rounded once.  Two pages must not go to one
+ * block.  seq_lens[i] beyond the table sets error bit 4 (the table's pages are
+ * read); a block outside the cache or the pool sets bit 2 and is skipped.
+ * num_seqs <= 4096, n_kv <= 64, head_dim 64 or 128, block_size 16.
+ */
+int vmps_read_cache8(void* pool, int pool_blocks, const int32_t* dst_tables, const void* codes,
+                     const float* scales, const int32_t* block_tables, int max_blocks_per_seq,
+                     const int32_t* seq_lens, int num_seqs, int n_kv, int head_dim,
+                     int block_size, int num_blocks, int cache_format, int dtype, void* stream);
+
+/*
+ * Decode attention over the 8-bit cache (kernel 11): vmps_paged_decode_attention
+ * with K and V read from codes and scales.
+ *   out[i][h] = softmax_t(scale * q[i][h] . K[t][h / G]) . V[t][h / G], t < seq_lens[i]
+ * Scores, maxima and sums are fp32.  q is [num_seqs][n_q][head_dim] with a row
+ * stride (a multiple of 8 elements), out contiguous, both 16-byte aligned.  A
+ * sequence of length 0 gets a zero row; slots at and past seq_lens[i] take no
+ * part, whatever they hold.  seq_lens[i] beyond the table sets error bit 4 (the
+ * table's pages are read); a block outside the cache sets bit 2.
+ * Supported: head_dim 64 or 128, block_size 16, n_q / n_kv a whole number up to
+ * 16, n_kv <= 64, num_seqs <= 4096.
+ *
+ * The workspace (256-byte aligned) holds the partial results of sequences cut
+ * between CTAs and their arrival counters; its size does not depend on the
+ * lengths.  Its first 1 MiB (the counters) must be zero before the first call
+ * (vmps_paged_decode_workspace_init); every call leaves it zero, so one
+ * workspace serves calls of any shape, and vmps_paged_decode_attention's too.
+ * Calls that may overlap on the GPU need different workspaces.  0 bytes: the
+ * shape is not supported.
+ */
+size_t vmps_paged_decode_cache8_workspace_bytes(int num_seqs, int n_q, int n_kv, int head_dim);
+int vmps_paged_decode_attention_cache8(void* out, const void* q, int64_t q_row_stride,
+                                       const void* codes, const float* scales,
+                                       const int32_t* block_tables, int max_blocks_per_seq,
+                                       const int32_t* seq_lens, int num_seqs, int n_q, int n_kv,
+                                       int head_dim, int block_size, int num_blocks, float scale,
+                                       void* workspace, size_t workspace_bytes, int cache_format,
+                                       int dtype, void* stream);
 
 /*
  * Copies `bytes` from `src` to `dst` with the GPU's own loads and stores,

@@ -20,6 +20,10 @@ Public functions
   speculative decoding: attention of a tree of drafted tokens over the cache,
   the commit of the branch the model agrees with, and the 4-bit products of
   a drafter (:class:`W4Weight`, :func:`quantize_w4`).
+* :func:`norm_rope_and_cache`, :func:`read_cache8`,
+  :func:`paged_decode_attention_cache8` -- the 8-bit paged cache
+  (:class:`KVCache8`): norms, rotation and write in one pass (for the 16-bit
+  pool too), its read-back into 16-bit pages, decode attention over it.
 """
 
 from __future__ import annotations
@@ -36,6 +40,10 @@ LIB_PATH = os.path.join(_PKG_DIR, "libvmps_kernels.so")
 
 VMPS_DTYPE_F16 = 0
 VMPS_DTYPE_BF16 = 1
+
+VMPS_CACHE_16BIT = 0
+VMPS_CACHE_INT8 = 1
+VMPS_CACHE_E4M3 = 2
 
 _ERRORS = {
     -1: ValueError,        # VMPS_ERR_INVALID_ARG
@@ -68,6 +76,10 @@ EXPORTED_SYMBOLS = (
     "vmps_commit_tree",
     "vmps_w4_gemm_supported",
     "vmps_w4_gemm",
+    "vmps_norm_rope_and_cache",
+    "vmps_read_cache8",
+    "vmps_paged_decode_cache8_workspace_bytes",
+    "vmps_paged_decode_attention_cache8",
     "vmps_stage_copy",
     "vmps_debug_error_word",
 )
@@ -145,6 +157,19 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.vmps_w4_gemm_supported.argtypes = [i32, i32, i32, i32]
         lib.vmps_w4_gemm.restype = i32
         lib.vmps_w4_gemm.argtypes = [vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]
+        lib.vmps_norm_rope_and_cache.restype = i32
+        lib.vmps_norm_rope_and_cache.argtypes = [
+            vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, f32, vp, vp, vp, vp, vp,
+            i32, i32, i32, i32, i32, i32, i32, i32, vp]
+        lib.vmps_read_cache8.restype = i32
+        lib.vmps_read_cache8.argtypes = [vp, i32, vp, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32,
+                                         i32, i32, vp]
+        lib.vmps_paged_decode_cache8_workspace_bytes.restype = sz
+        lib.vmps_paged_decode_cache8_workspace_bytes.argtypes = [i32, i32, i32, i32]
+        lib.vmps_paged_decode_attention_cache8.restype = i32
+        lib.vmps_paged_decode_attention_cache8.argtypes = [
+            vp, vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, vp, sz, i32, i32,
+            vp]
         lib.vmps_stage_copy.restype = i32
         lib.vmps_stage_copy.argtypes = [vp, vp, sz, vp]
         lib.vmps_debug_error_word.restype = i32
@@ -297,6 +322,16 @@ class DecodeWorkspace:
             size = max(need, 0 if buf is None else 2 * buf.numel())
             buf = torch.zeros(size, dtype=torch.uint8, device=device)
             self._buf[device] = buf
+        return buf
+
+    def get_cache8(self, device: torch.device, num_seqs: int, n_q: int, n_kv: int,
+                   d: int) -> torch.Tensor:
+        """The same buffer, for :func:`paged_decode_attention_cache8`."""
+        need = _cache8_workspace_bytes(device.index, num_seqs, n_q, n_kv, d)
+        buf = self._buf.get(device)
+        if buf is None or buf.numel() < need:
+            size = max(need, 0 if buf is None else 2 * buf.numel())
+            buf = self._buf[device] = torch.zeros(size, dtype=torch.uint8, device=device)
         return buf
 
 
@@ -954,6 +989,276 @@ def w4_gemm(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None,
                  1 if silu_mul else 0, dtype_code(x.dtype))
     if rc:
         _check(rc, "w4_gemm")
+    return out
+
+
+# ── the 8-bit paged cache ────────────────────────────────────────────────────
+
+_CACHE_FORMATS = {torch.int8: VMPS_CACHE_INT8, torch.float8_e4m3fn: VMPS_CACHE_E4M3}
+_CACHE_TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+
+
+class KVCache8:
+    """A paged K/V cache of 8-bit codes with an fp32 scale per token, head and kind.
+
+    ``codes``: (num_blocks, 2, 16, n_kv, D) int8 or float8_e4m3fn, the pool's
+    layout; ``scales``: (num_blocks, n_kv, 2, 16) fp32.  Both contiguous.  A
+    stored value is ``code * scale``.
+    """
+
+    __slots__ = ("codes", "scales", "format")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
+        shape = codes.shape
+        if len(shape) != 5 or shape[1] != 2 or shape[2] != 16 or not codes.is_contiguous():
+            raise ValueError("codes must be contiguous (num_blocks, 2, 16, n_kv, head_dim); got "
+                             f"{tuple(shape)}")
+        fmt = _CACHE_FORMATS.get(codes.dtype)
+        if fmt is None:
+            raise TypeError(f"codes must be int8 or float8_e4m3fn (got {codes.dtype})")
+        if scales.dtype != torch.float32 or scales.shape != (shape[0], shape[3], 2, 16) \
+                or not scales.is_contiguous():
+            raise ValueError(f"scales must be contiguous float32 ({shape[0]}, {shape[3]}, 2, 16)")
+        self.codes, self.scales, self.format = codes, scales, fmt
+
+    @classmethod
+    def zeros(cls, num_blocks: int, n_kv: int, d: int, dtype: torch.dtype = torch.int8,
+              device: torch.device | str = "cuda") -> "KVCache8":
+        """An empty cache (every slot reads as zeros)."""
+        return cls(torch.zeros((num_blocks, 2, 16, n_kv, d), dtype=dtype, device=device),
+                   torch.zeros((num_blocks, n_kv, 2, 16), dtype=torch.float32, device=device))
+
+    def dequantize(self) -> torch.Tensor:
+        """The fp32 pool (num_blocks, 2, 16, n_kv, D) this cache stands for."""
+        return self.codes.float() * self.scales.permute(0, 2, 3, 1).unsqueeze(-1)
+
+
+def quantize_cache8(x: torch.Tensor, dtype: torch.dtype = torch.int8,
+                    ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and fp32 scales of rows ``x`` (..., D), as :func:`norm_rope_and_cache` stores them.
+
+    Plain torch, any device: for filling a :class:`KVCache8` on the host side
+    and for tests.
+    """
+    if dtype not in _CACHE_TOP:
+        raise TypeError(f"8-bit caches are int8 or float8_e4m3fn (got {dtype})")
+    top = _CACHE_TOP[dtype]
+    x = x.float()
+    amax = x.abs().amax(-1)
+    fine = torch.isfinite(x).all(-1)
+    some = fine & (amax >= 2.0 ** -100)
+    y = torch.where(some.unsqueeze(-1), x * (top / torch.where(some, amax, 1.0)).unsqueeze(-1), 0.0)
+    codes = (torch.round(y) if dtype == torch.int8 else y.clamp(-top, top)).to(dtype)
+    return codes, torch.where(some, amax / top, torch.where(fine, 0.0, float("nan")))
+
+
+def _head_rows(t: torch.Tensor, d: int, name: str) -> tuple[int, int]:
+    """(heads, row stride) of (B, heads, d) or (B, heads * d) rows with packed heads."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3 and shape[2] == d and stride[2] == 1 and (stride[1] == d or shape[1] <= 1):
+        heads = shape[1]
+    elif len(shape) == 2 and shape[1] % d == 0 and stride[1] == 1:
+        heads = shape[1] // d
+    else:
+        raise ValueError(f"{name} must be (rows, heads, {d}) or (rows, heads * {d}) with packed heads")
+    # torch gives a single row any stride; the kernel never steps by it.
+    return heads, stride[0] if shape[0] > 1 else heads * d
+
+
+def norm_rope_and_cache(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+                        positions: torch.Tensor | None, slot_mapping: torch.Tensor,
+                        inv_freq: torch.Tensor | None, cache: "KVCache8 | torch.Tensor",
+                        q_weight: torch.Tensor | None = None,
+                        k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                        q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Norm and rotate q and k per head, write k and v into ``cache``; one kernel.
+
+    ``x * weight / sqrt(mean(x^2) + eps)`` over each head of q and k (a weight
+    of None: no norm), then RoPE at ``positions`` (``inv_freq`` None: no
+    rotation), in fp32, rounded once.  ``cache``: a 16-bit pool (num_blocks, 2,
+    16, n_kv, D) of the rows' dtype, or a :class:`KVCache8`, into which k and v
+    are quantised.  ``q``: (rows, n_q, D) or (rows, n_q * D), ``k``/``v``
+    likewise (slices of a fused QKV output work), fp16 or bf16; ``q`` None:
+    keys and values alone.  ``positions``/``slot_mapping``: int32 (rows,), a
+    negative slot caches nothing.  Returns ``q_out`` (rows, n_q, D), a new
+    tensor unless given (``q`` itself works).
+    """
+    eight = type(cache) is KVCache8
+    pool = cache.codes if eight else cache
+    shape = pool.shape
+    if not eight and (len(shape) != 5 or shape[1] != 2 or not pool.is_contiguous()):
+        _check_pool(pool)
+    num_blocks, _, block_size, n_kv, D = shape
+    dtype = k.dtype
+    if v.dtype != dtype or (q is not None and q.dtype != dtype) or \
+            (not eight and pool.dtype != dtype):
+        raise TypeError("q, k, v and a 16-bit pool must have one dtype")
+    rows = k.shape[0]
+    heads, ks = _head_rows(k, D, "k")
+    v_heads, vs = _head_rows(v, D, "v")
+    if heads != n_kv or v_heads != n_kv or v.shape[0] != rows:
+        raise ValueError(f"k and v must have {n_kv} heads and the same rows")
+    n_q = qs = os_ = 0
+    q_ptr = o_ptr = None
+    if q is not None:
+        n_q, qs = _head_rows(q, D, "q")
+        if q.shape[0] != rows:
+            raise ValueError("q must have k's rows")
+        if q_out is None:
+            q_out = q.new_empty((rows, n_q, D))
+            os_ = n_q * D
+        else:
+            o_heads, os_ = _head_rows(q_out, D, "q_out")
+            if o_heads != n_q or q_out.shape[0] != rows or q_out.dtype != dtype:
+                raise ValueError("q_out must have q's shape and dtype")
+            if q_out.data_ptr() == q.data_ptr() and os_ != qs:
+                raise ValueError("q_out in q's place must have its row stride")
+        q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    _lengths(rows, slot_mapping=slot_mapping)
+    if inv_freq is not None:
+        if inv_freq.dtype != torch.float32 or inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
+            raise ValueError(f"inv_freq must be contiguous float32 of {D // 2} entries")
+        if positions is None:
+            raise ValueError("inv_freq needs positions")
+    if positions is not None:
+        _lengths(rows, positions=positions)
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.dtype != dtype or w.numel() != D or not w.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous ({D},) of the rows' dtype")
+    scales = cache.scales if eight else None
+    dev = _device_index(k, v, q, q_out, positions, slot_mapping, inv_freq, pool, scales, q_weight,
+                        k_weight)
+    lib = _lib or load_library()
+    rc = _launch(lib.vmps_norm_rope_and_cache, dev,
+                 o_ptr, os_, q_ptr, qs, k.data_ptr(), ks, v.data_ptr(), vs,
+                 None if q_weight is None else q_weight.data_ptr(),
+                 None if k_weight is None else k_weight.data_ptr(), eps,
+                 None if positions is None else positions.data_ptr(), slot_mapping.data_ptr(),
+                 None if inv_freq is None else inv_freq.data_ptr(), pool.data_ptr(),
+                 None if scales is None else scales.data_ptr(), rows, n_q, n_kv, D, block_size,
+                 num_blocks, cache.format if eight else VMPS_CACHE_16BIT, dtype_code(dtype))
+    if rc:
+        _check(rc, "norm_rope_and_cache")
+    return q_out
+
+
+def read_cache8(cache: KVCache8, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                pool: torch.Tensor, dst_tables: torch.Tensor) -> torch.Tensor:
+    """Read sequences' pages of an 8-bit cache back into 16-bit pages of ``pool``.
+
+    Page j of sequence i (``block_tables[i, j]``) goes to block
+    ``dst_tables[i, j]`` of ``pool`` (pool_blocks, 2, 16, n_kv, D), fp16 or
+    bf16, for ``j < ceil(seq_lens[i] / 16)``; the slots past the length in the
+    last page become zeros, other blocks stay as they were.  The 16-bit
+    attention calls then take ``pool`` and ``dst_tables`` in place of a pool
+    and its tables.  Both tables int32 (B, max_blocks), no block twice in
+    ``dst_tables``.  Returns ``pool``.
+    """
+    codes = cache.codes
+    num_blocks, _, block_size, n_kv, D = codes.shape
+    shape = pool.shape
+    if len(shape) != 5 or shape[1:] != codes.shape[1:] or not pool.is_contiguous():
+        raise ValueError(f"pool must be contiguous (blocks, 2, 16, {n_kv}, {D}); got {tuple(shape)}")
+    B = seq_lens.numel()
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or dst_tables.shape != block_tables.shape:
+        raise ValueError("block_tables and dst_tables must be (B, max_blocks)")
+    _lengths(B, seq_lens=seq_lens)
+    _int32(block_tables, "block_tables")
+    _int32(dst_tables, "dst_tables")
+    dev = _device_index(codes, cache.scales, block_tables, seq_lens, pool, dst_tables)
+    lib = _lib or load_library()
+    rc = _launch(lib.vmps_read_cache8, dev,
+                 pool.data_ptr(), shape[0], dst_tables.data_ptr(), codes.data_ptr(),
+                 cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.shape[1],
+                 seq_lens.data_ptr(), B, n_kv, D, block_size, num_blocks, cache.format,
+                 dtype_code(pool.dtype))
+    if rc:
+        _check(rc, "read_cache8")
+    return pool
+
+
+def _cache8_workspace_bytes(device: int, num_seqs: int, n_q: int, n_kv: int, d: int) -> int:
+    lib = _lib or load_library()
+    if torch.cuda.current_device() == device:
+        need = lib.vmps_paged_decode_cache8_workspace_bytes(num_seqs, n_q, n_kv, d)
+    else:
+        with torch.cuda.device(device):
+            need = lib.vmps_paged_decode_cache8_workspace_bytes(num_seqs, n_q, n_kv, d)
+    if need == 0:
+        raise NotImplementedError(
+            f"paged_decode_attention_cache8: num_seqs={num_seqs} n_q={n_q} n_kv={n_kv} "
+            f"head_dim={d} not supported")
+    return need
+
+
+#: Zeroed workspaces of eager calls that bring none, one per device and stream.
+_cache8_buffers: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def _cache8_workspace(ref: torch.Tensor, dev: int, B: int, n_q: int, n_kv: int, d: int) -> torch.Tensor:
+    need = _cache8_workspace_bytes(dev, B, n_q, n_kv, d)
+    if torch.cuda.is_current_stream_capturing():
+        # A graph's own: it may be replayed while other calls or graphs run.
+        buf = ref.new_empty(need, dtype=torch.uint8)
+        buf[:4 * n_kv * B].zero_()
+        return buf
+    key = (dev, torch._C._cuda_getCurrentRawStream(dev))
+    buf = _cache8_buffers.get(key)
+    if buf is None or buf.numel() < need:
+        buf = _cache8_buffers[key] = ref.new_zeros(need, dtype=torch.uint8)
+    return buf
+
+
+def paged_decode_attention_cache8(q: torch.Tensor, cache: KVCache8, block_tables: torch.Tensor,
+                                  seq_lens: torch.Tensor, scale: float | None = None,
+                                  out: torch.Tensor | None = None,
+                                  workspace: DecodeWorkspace | torch.Tensor | None = None,
+                                  ) -> torch.Tensor:
+    """Decode attention of one query token per sequence over an 8-bit cache.
+
+    ``q``: (B, n_q, D) or (B, n_q * D) fp16 or bf16, rotated, heads packed (rows
+    may be strided); ``block_tables``: int32 (B, max_blocks); ``seq_lens``:
+    int32 (B,) counting the new token.  ``n_q`` is up to 16 times ``n_kv``.
+    ``scale`` defaults to ``1/sqrt(D)``.  ``workspace``: a
+    :class:`DecodeWorkspace`, or a uint8 tensor whose first MiB is zero (the
+    call leaves it so), for calls that do not overlap; None: one that belongs
+    to the current stream, or to the graph being captured.  Returns ``out``
+    (B, n_q, D) of q's dtype.
+    """
+    codes = cache.codes
+    num_blocks, _, block_size, n_kv, D = codes.shape
+    n_q, qs = _head_rows(q, D, "q")
+    B = q.shape[0]
+    if block_tables.dim() != 2 or block_tables.shape[0] != B:
+        raise ValueError("block_tables must be (B, max_blocks)")
+    _lengths(B, seq_lens=seq_lens)
+    _int32(block_tables, "block_tables")
+    if out is None:
+        out = q.new_empty((B, n_q, D))
+    elif out.shape != (B, n_q, D) or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be a contiguous (B, n_q, D) tensor of q's dtype")
+    dev = _device_index(q, codes, cache.scales, block_tables, seq_lens, out)
+    code = dtype_code(q.dtype)
+    if B == 0:
+        return out
+    if workspace is None:
+        workspace = _cache8_workspace(codes, dev, B, n_q, n_kv, D)
+    elif isinstance(workspace, DecodeWorkspace):
+        workspace = workspace.get_cache8(q.device, B, n_q, n_kv, D)
+    elif workspace.get_device() != dev:
+        _require_cuda(q, workspace)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    lib = _lib or load_library()
+    rc = _launch(lib.vmps_paged_decode_attention_cache8, dev,
+                 out.data_ptr(), q.data_ptr(), qs, codes.data_ptr(), cache.scales.data_ptr(),
+                 block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(), B, n_q, n_kv,
+                 D, block_size, num_blocks, scale, workspace.data_ptr(),
+                 workspace.numel() * workspace.element_size(), cache.format, code)
+    if rc:
+        _check(rc, "paged_decode_attention_cache8")
     return out
 
 
