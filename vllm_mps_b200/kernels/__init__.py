@@ -1193,6 +1193,8 @@ def _cache8_workspace_bytes(device: int, num_seqs: int, n_q: int, n_kv: int, d: 
     return need
 
 
+#: Of a workspace's first MiB what the 8-bit decode counts in.
+_CACHE8_COUNTER_BYTES = 128 << 10
 #: Zeroed workspaces of eager calls that bring none, one per device and stream.
 _cache8_buffers: dict[tuple[int, int], torch.Tensor] = {}
 
@@ -1202,7 +1204,7 @@ def _cache8_workspace(ref: torch.Tensor, dev: int, B: int, n_q: int, n_kv: int, 
     if torch.cuda.is_current_stream_capturing():
         # A graph's own: it may be replayed while other calls or graphs run.
         buf = ref.new_empty(need, dtype=torch.uint8)
-        buf[:4 * n_kv * B].zero_()
+        buf[:_CACHE8_COUNTER_BYTES].zero_()
         return buf
     key = (dev, torch._C._cuda_getCurrentRawStream(dev))
     buf = _cache8_buffers.get(key)
