@@ -138,6 +138,12 @@ def _ragged(seed, n, most):
     (4096, 6, 4, 1, 64, torch.float16, INT8),
     (1500, 33, 8, 8, 128, torch.float16, E4M3),
     (300, 700, 16, 1, 128, torch.bfloat16, E4M3),
+    # Tables of one to three pages: several heads a CTA.
+    (4096, 16, 64, 4, 128, torch.bfloat16, INT8),
+    (700, 17, 128, 8, 128, torch.float16, E4M3),
+    (513, 32, 48, 16, 64, torch.bfloat16, INT8),
+    (100, 33, 24, 12, 64, torch.float16, INT8),
+    (100, 47, 21, 7, 64, torch.float16, E4M3),
 ])
 def test_ragged_batches(n, most, n_q, n_kv, D, dtype, fmt):
     c = _case(_ragged(n, n, most), n_q, n_kv, D, dtype, fmt, n)

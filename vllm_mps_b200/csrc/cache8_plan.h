@@ -16,7 +16,12 @@
 namespace vmps {
 
 constexpr int kC8TileWeight = 4;
-constexpr int kC8SegWeight = 8;
+// A sequence's start costs a share about two tiles: with 1 in place of 2, 64
+// ragged sequences took 20.0 us for 19.4 and 16 x 1..8192 43.6 for 42.2; with
+// 3, 256 x 511..1537 99.3 for 96.8.
+constexpr int kC8SegWeight = 2 * kC8TileWeight;
+// Weight of a share, at least: with twice as much, one sequence of 128 tokens
+// took 9.8 us for 6.5 and one of 1024 12.1 for 10.2 (8 kv heads).
 constexpr int kC8MinShare = 2 * kC8TileWeight;
 
 struct C8Shape {
@@ -46,25 +51,25 @@ struct C8Pos {  // a tile in the linear order
   int hg, s, j;
 };
 
-// The first tile at or after weighted position w; wpref: prefix sums of the
-// sequences' weights (num_seqs + 1 of them).
-VMPS_HD C8Pos c8_pos(const int* wpref, const C8Shape& sh, long long w) {
-  C8Pos r;
-  const int total = wpref[sh.num_seqs];
-  r.s = r.j = 0;
-  r.hg = sh.groups;
-  if (w >= static_cast<long long>(sh.groups) * total) return r;
+// Weighted position w as a head group and a position in its sequences (hg is the
+// number of groups behind the last).
+struct C8Cut {
+  int hg, at;
+};
+
+VMPS_HD C8Cut c8_cut(int total, int groups, long long w) {
+  C8Cut r;
+  r.hg = groups;
+  r.at = 0;
+  if (w >= static_cast<long long>(groups) * total) return r;
   r.hg = static_cast<int>(c8_div(w, total));
-  const int f = static_cast<int>(w - static_cast<long long>(r.hg) * total);
-  int lo = 0, hi = sh.num_seqs;  // the last sequence that starts at or before f
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (wpref[mid] <= f) lo = mid; else hi = mid;
-  }
-  r.s = lo;
-  const int off = f - wpref[lo];
-  r.j = off <= kC8SegWeight ? 0 : (off - kC8SegWeight + kC8TileWeight - 1) / kC8TileWeight;
+  r.at = static_cast<int>(w - static_cast<long long>(r.hg) * total);
   return r;
+}
+
+// The first tile at or after weighted position `off` of a sequence.
+VMPS_HD int c8_tile_at(int off) {
+  return off <= kC8SegWeight ? 0 : (off - kC8SegWeight + kC8TileWeight - 1) / kC8TileWeight;
 }
 
 // The CTA that has tile j of the sequence.
@@ -117,16 +122,9 @@ struct C8Walk {
 };
 
 // Pieces are joined by the CTA that finishes last.  Runs of many pieces are
-// joined in two rounds, groups of this many first, so that no one CTA reads them
-// all: the largest power of two whose square is at most the number of pieces.
-// Up to kC8OneRound pieces: one round.
-constexpr int kC8OneRound = 8;
+// joined in two rounds, groups of 16 first, so that no one CTA reads them all.
+constexpr int kC8OneRound = 24;
 
-VMPS_HD int c8_join_group(int pieces) {
-  if (pieces <= kC8OneRound) return pieces;
-  int g = 1;
-  while (4 * g * g <= pieces) g *= 2;
-  return g;
-}
+VMPS_HD int c8_join_group(int pieces) { return pieces <= kC8OneRound ? pieces : 16; }
 
 }  // namespace vmps

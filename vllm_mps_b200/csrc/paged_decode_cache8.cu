@@ -6,14 +6,16 @@
 // What bounds it: the codes' bytes from HBM (4 G operations per K and V code
 // byte pair, G query heads a kv head).
 //
-//  * Work: tiles of 16 TG tokens of HPC kv heads, HPC * TG <= 8 consumer warps
-//    (HPC: the largest divisor of n_kv up to 8; TG fills the CTA up to 8 warps
-//    where there are few kv heads).  The tiles of all sequences are cut into equal
-//    contiguous shares, one per CTA of a persistent grid (cache8_plan.h), so that
-//    ragged batches and single long sequences both keep every SM streaming.
-//  * A producer warp streams pages: a tiled TMA for the codes (K and V of HPC
-//    heads, swizzled) and a bulk copy for their scales, into a ring of stages.
-//  * A consumer warp takes 16 tokens of one kv head a stage.  The G query heads
+//  * Work: tiles of 2 TG pages of HPC kv heads for HPC * TG = 8 consumer warps (HPC
+//    2 where n_kv is even, else 1).  The tiles of all sequences are cut into equal
+//    contiguous shares, one per CTA of a persistent grid, one CTA per SM
+//    (cache8_plan.h), so that ragged batches and single long sequences both keep
+//    every SM streaming.  Few heads a CTA mean few pieces: with all 8 kv heads of a
+//    page in a CTA, 32 ragged sequences took 77 us where two take 40, and one 43.
+//  * Four producer warps stream pages: a tiled TMA for the codes (K and V of HPC
+//    heads, swizzled) and a bulk copy for their scales, into a ring of stages,
+//    and the query rows of the next sequences into a ring of their own.
+//  * A consumer warp takes two pages of one kv head a stage.  The G query heads
 //    are the N side of m16n8k16 in fp16 with fp32 sums:
 //        S^T[16 tok x 8 heads] = K . Q^T,   O^T[D x 8] += V^T . P^T
 //    Codes become fp16 in registers, exactly: a byte under 0x64 is 1024 + byte
@@ -32,11 +34,16 @@
 //  * bf16 queries are scaled by a power of two per head, so that their largest
 //    is in [2^13, 2^14), which fp16 holds as exactly as bf16 did but for values
 //    below 2^-28 of it.
+//  * At a sequence's end the warps of a kv head tell each other their bounds and sums,
+//    write their outputs over the codes that they have just read and add up a part each.
 //  * A cut sequence: every piece leaves its normalised output and the logarithm
 //    of its weights' sum in fp32 and arrives on a counter; the last to arrive
 //    joins, in two rounds where there are many pieces.  Sums are in a fixed order:
 //    results do not depend on who is last.
+#include <limits.h>
+
 #include <mutex>
+#include <type_traits>
 #include <utility>
 
 #include "cache8.cuh"
@@ -50,12 +57,19 @@ constexpr int kMaxSeqs8 = 4096;
 constexpr int kMaxKvHeads8 = 64;
 constexpr int kMaxGroup8 = 16;
 constexpr int kMaxStages8 = 8;
-constexpr int kMaxWarps8 = 8;
-constexpr int kThreads8 = 32 * (1 + kMaxWarps8);
+constexpr int kParts8 = 4;      // parts of a kv head's output, each joined by a warp of its own
+constexpr int kWarps8 = 8;      // consumer warps of a CTA, at most
+constexpr int kProducers8 = 4;  // producer warps: issuing a copy takes one about 100 clocks
+constexpr int kMaxHeads8 = 8;   // kv heads of a CTA
+// Pages that a warp takes of a tile.  Two share the waits and the checks of the scores and
+// their products overlap: 4 x 131072 tokens 173.5 us for 176.0, 256 x 511..1537 96.8 for
+// 102.8 (head size 128), 64 ragged sequences at head size 64 19.3 for 21.8.
+constexpr int kPages8 = 2;
 // The workspace's counters; the records start where the 16-bit decode kernel's
 // do, so that one workspace serves both.
 constexpr size_t kCounterBytes8 = size_t(128) << 10;
 constexpr size_t kRecordsAt8 = size_t(1) << 20;
+constexpr int kMostSmem8 = 220 << 10;  // dynamic shared memory of a CTA
 constexpr float kLowest8 = -1e30f;  // the score bound of a piece that has seen nothing
 
 struct Decode8Params {
@@ -69,17 +83,18 @@ struct Decode8Params {
   int hpc, tg;        // kv heads per CTA, pages per tile
   int stages;
   float scale_log2;   // scale * log2(e)
-  int* group_counters;  // [n_cta][2][hpc]
-  int* top_counters;    // [n_cta][hpc]
-  float* part_lse;      // [n_cta][2][hpc][NT][4][2]
-  float* part_o;        // [n_cta][2][hpc][NT * D / 16][32 lanes][4]
+  int* group_counters;  // [n_cta][2][hpc][kParts8]
+  int* top_counters;    // [n_cta][hpc][kParts8]
+  // Records of the pieces (first half) and of the groups they are joined in.
+  float* part_lse;      // [2][n_cta][2][hpc][NT][kParts8][4][2]
+  float* part_o;        // [2][n_cta][2][hpc][NT * D / 16][32 lanes][4]
   int* err;
 };
 
-// A published piece of a cut sequence: its run of CTAs, the sequence and its kv head, and
-// how many arrivals were missing before its own (0: it was the last; lane 0 writes it).
+// A warp's note of a published piece of a cut sequence: its run of CTAs, the sequence and
+// its kv head.
 struct Piece8 {
-  int c0, c1, s, kvh, missing;
+  int c0, c1, s, kvh;
 };
 
 __device__ __forceinline__ int arrive_piece8(int* counter) {
@@ -127,158 +142,186 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& first, uint32_t& sec
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
-// Joins `count` records (every `step`-th CTA's from `cta` on, slot 1 in CTA c0, 0 in the
-// others): the normalised output in o, the logarithm of the weights' sum in lse.
-template <int D, int NT>
-__device__ __forceinline__ void join_records(const Decode8Params& p, int cta, int step, int count,
-                                             int c0, int h, int lane, float (&lse)[NT][2],
-                                             float (&o)[NT][D / 16][4]) {
+// Joins part `part` (M m-tiles) of n-tile nt of `count` records (from `base` on, every
+// `step`-th CTA's from `cta` on, slot 1 in CTA c0, 0 in the others): the normalised output
+// in o, the logarithm of the weights' sum in lse.  The loads of a batch of records are in
+// flight at once.
+template <int D, int NT, int M>
+__device__ __forceinline__ void join_records(const Decode8Params& p, size_t base, int cta, int step,
+                                             int count, int c0, int h, int nt, int part, int lane,
+                                             float (&lse)[2], float (&o)[M][4]) {
   constexpr int KS = D / 16;
+  constexpr int kBatch = 8 / M;
   const int c = lane & 3;
-  const float2* ml = reinterpret_cast<const float2*>(p.part_lse) + c;
-  const float4* po = reinterpret_cast<const float4*>(p.part_o) + lane;
-  auto rec = [&](int k) {
-    const int b = cta + k * step;
-    return (static_cast<size_t>(b) * 2 + (b == c0 ? 1 : 0)) * p.hpc + h;
-  };
-  float top[NT][2], sum[NT][2];
+  // Lanes whose heads are padding (nothing was stored for them) read their neighbour's.
+  const int from = nt * 8 + 2 * c < p.G ? lane : lane & ~3;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_lse) + (nt * kParts8 + part) * 4 + c;
+  const float4* po = reinterpret_cast<const float4*>(p.part_o) + (nt * KS + part * M) * 32 + from;
+  float top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    top[nt][0] = top[nt][1] = -INFINITY;
-    sum[nt][0] = sum[nt][1] = 0.f;
+  for (int i = 0; i < M; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int k0 = 0; k0 < count; k0 += kBatch) {
+    float2 z[kBatch];
+    float4 x[kBatch][M];
 #pragma unroll
-    for (int mt = 0; mt < KS; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
-  }
-#pragma unroll 8
-  for (int k = 0; k < count; ++k) {
+    for (int k = 0; k < kBatch; ++k) {
+      const int b = cta + min(k0 + k, count - 1) * step;
+      const size_t rec = base + (static_cast<size_t>(b) * 2 + (b == c0 ? 1 : 0)) * p.hpc + h;
+      z[k] = __ldcg(ml + rec * NT * kParts8 * 4);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float2 v = __ldcg(ml + (rec(k) * NT + nt) * 4);
-      top[nt][0] = fmaxf(top[nt][0], v.x);
-      top[nt][1] = fmaxf(top[nt][1], v.y);
+      for (int i = 0; i < M; ++i) x[k][i] = __ldcg(po + (rec * NT * KS + i) * 32);
     }
-  }
-#pragma unroll 2
-  for (int k = 0; k < count; ++k) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float2 v = __ldcg(ml + (rec(k) * NT + nt) * 4);
-      const float w0 = fast_exp2(v.x - top[nt][0]), w1 = fast_exp2(v.y - top[nt][1]);
-      sum[nt][0] += w0;
-      sum[nt][1] += w1;
+    for (int k = 0; k < kBatch; ++k) {
+      if (k0 + k >= count) z[k] = make_float2(-INFINITY, -INFINITY);
+    }
+    float t0 = top0, t1 = top1;
 #pragma unroll
-      for (int mt = 0; mt < KS; ++mt) {
-        const float4 x = __ldcg(po + ((rec(k) * NT + nt) * KS + mt) * 32);
-        o[nt][mt][0] = fmaf(w0, x.x, o[nt][mt][0]);
-        o[nt][mt][1] = fmaf(w1, x.y, o[nt][mt][1]);
-        o[nt][mt][2] = fmaf(w0, x.z, o[nt][mt][2]);
-        o[nt][mt][3] = fmaf(w1, x.w, o[nt][mt][3]);
+    for (int k = 0; k < kBatch; ++k) {
+      t0 = fmaxf(t0, z[k].x);
+      t1 = fmaxf(t1, z[k].y);
+    }
+    // -inf alone: nothing so far, and no factor that would be NaN.
+    const float a0 = t0 == top0 ? 1.f : fast_exp2(top0 - t0);
+    const float a1 = t1 == top1 ? 1.f : fast_exp2(top1 - t1);
+    top0 = t0;
+    top1 = t1;
+    sum0 *= a0;
+    sum1 *= a1;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      o[i][0] *= a0;
+      o[i][1] *= a1;
+      o[i][2] *= a0;
+      o[i][3] *= a1;
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float w0 = z[k].x == -INFINITY ? 0.f : fast_exp2(z[k].x - top0);
+      const float w1 = z[k].y == -INFINITY ? 0.f : fast_exp2(z[k].y - top1);
+      sum0 += w0;
+      sum1 += w1;
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        o[i][0] = fmaf(w0, x[k][i].x, o[i][0]);
+        o[i][1] = fmaf(w1, x[k][i].y, o[i][1]);
+        o[i][2] = fmaf(w0, x[k][i].z, o[i][2]);
+        o[i][3] = fmaf(w1, x[k][i].w, o[i][3]);
       }
     }
   }
+  const float r0 = __fdividef(1.f, sum0), r1 = __fdividef(1.f, sum1);
+  lse[0] = top0 + __log2f(sum0);
+  lse[1] = top1 + __log2f(sum1);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const float r0 = 1.f / sum[nt][0], r1 = 1.f / sum[nt][1];
-    lse[nt][0] = top[nt][0] + log2f(sum[nt][0]);
-    lse[nt][1] = top[nt][1] + log2f(sum[nt][1]);
-#pragma unroll
-    for (int mt = 0; mt < KS; ++mt) {
-      o[nt][mt][0] *= r0;
-      o[nt][mt][1] *= r1;
-      o[nt][mt][2] *= r0;
-      o[nt][mt][3] *= r1;
-    }
+  for (int i = 0; i < M; ++i) {
+    o[i][0] *= r0;
+    o[i][1] *= r1;
+    o[i][2] *= r0;
+    o[i][3] *= r1;
   }
 }
 
-// Output rows of a kv head from O^T fragments (rows g, g + 8 of m-tile mt: elements
-// 16 mt + 2g and the next; columns 2c, 2c + 1: heads).
-template <typename T, int D, int NT>
-__device__ __forceinline__ void store_rows(T* rows, int G, int lane, const float (&f)[NT][2],
-                                           const float (&o)[NT][D / 16][4]) {
+// M m-tiles (from mt on) of n-tile nt of the output rows of a kv head, from O^T fragments
+// (rows g, g + 8 of an m-tile: elements 16 mt + 2g and the next; columns 2c, 2c + 1: heads).
+template <typename T, int D, int M>
+__device__ __forceinline__ void store_rows(T* rows, int G, int nt, int mt, int lane,
+                                           const float (&o)[M][4]) {
   const int g = lane >> 2, c = lane & 3;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+  for (int e = 0; e < 2; ++e) {
+    const int n = nt * 8 + 2 * c + e;
+    if (n >= G) continue;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(rows + n * D) + mt * 8 + g;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int n = nt * 8 + 2 * c + e;
-      if (n >= G) continue;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(rows + n * D) + g;
-#pragma unroll
-      for (int mt = 0; mt < D / 16; ++mt) {
-        dst[mt * 8] = Elt<T>::pack(o[nt][mt][e] * f[nt][e], o[nt][mt][2 + e] * f[nt][e]);
-      }
-    }
+    for (int i = 0; i < M; ++i) dst[i * 8] = Elt<T>::pack(o[i][e], o[i][2 + e]);
   }
 }
 
-template <int D, int NT>
-__device__ __forceinline__ void store_record(const Decode8Params& p, size_t rec, int lane,
-                                             const float (&lse)[NT][2], const float (&f)[NT][2],
-                                             const float (&o)[NT][D / 16][4]) {
-  constexpr int KS = D / 16;
-  float4* po = reinterpret_cast<float4*>(p.part_o) + rec * NT * KS * 32 + lane;
-  float2* ml = reinterpret_cast<float2*>(p.part_lse) + rec * NT * 4;
+// The same into part `part` of a record, which has its own copy of the lse.
+template <int D, int NT, int M>
+__device__ __forceinline__ void store_record(const Decode8Params& p, size_t rec, int nt, int part,
+                                             int lane, const float (&lse)[2], const float (&o)[M][4]) {
+  if (nt * 8 + 2 * (lane & 3) < p.G) {
+    float4* po =
+        reinterpret_cast<float4*>(p.part_o) + ((rec * NT + nt) * (D / 16) + part * M) * 32 + lane;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int mt = 0; mt < KS; ++mt) {
-      __stcg(po + (nt * KS + mt) * 32,
-             make_float4(o[nt][mt][0] * f[nt][0], o[nt][mt][1] * f[nt][1],
-                         o[nt][mt][2] * f[nt][0], o[nt][mt][3] * f[nt][1]));
+    for (int i = 0; i < M; ++i) {
+      __stcg(po + i * 32, make_float4(o[i][0], o[i][1], o[i][2], o[i][3]));
     }
-    if (lane < 4) __stcg(ml + nt * 4 + lane, make_float2(lse[nt][0], lse[nt][1]));
+  }
+  if (lane < 4) {
+    __stcg(reinterpret_cast<float2*>(p.part_lse) + ((rec * NT + nt) * kParts8 + part) * 4 + lane,
+           make_float2(lse[0], lse[1]));
   }
 }
-
-// NT = 2 at head size 128 keeps 150 registers alive: one CTA per SM.
-template <int D, int NT>
-constexpr int kResident8 = (D == 128 && NT == 2) ? 1 : 2;
 
 template <typename T, int D, int NT, bool kInt8>
-__global__ void __launch_bounds__(kThreads8, kResident8<D, NT>)
+__global__ void __launch_bounds__(32 * (kProducers8 + kWarps8), 1)
 decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) {
   constexpr int KS = D / 16;
   constexpr bool kF16 = std::is_same<T, __half>::value;
   __shared__ uint64_t full_bar[kMaxStages8];
   __shared__ uint64_t empty_bar[kMaxStages8];
+  __shared__ uint64_t q_full[kMaxStages8 + 1];
+  __shared__ uint64_t q_empty[kMaxStages8 + 1];
+  // What a warp tells the others of its kv head at a segment's end: bounds and sums of heads
+  // 2c, 2c + 1.  Two segments' worth: a warp can be writing the next one's
+  // while another still reads.
+  __shared__ float4 hand_ml_of[2][kWarps8][NT][4];
   __shared__ volatile int s_abort;
-  __shared__ int warp_sum[1 + kMaxWarps8];
-  __shared__ Piece8 pieces_of[kMaxWarps8][2];
+  __shared__ int warp_sum[kProducers8 + kWarps8];
+  __shared__ C8Pos share[2];
+  __shared__ Piece8 pieces_of[kWarps8][2];
   extern __shared__ uint8_t dyn_smem[];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n = p.num_seqs, hpc = p.hpc, TG = p.tg, stages = p.stages;
   const int page_bytes = 2 * hpc * kCachePage * D;
-  const int stage_bytes = TG * page_bytes;
+  constexpr int PP = kPages8;
+  const int TP = TG * PP;  // pages of a tile
+  const int stage_bytes = TP * page_bytes;
   const int scale_bytes = hpc * 2 * kCachePage * 4;  // of one page
-  constexpr int kStateFloats = NT * (KS * 4 + 5);    // per lane: o, m, l, vref
+  constexpr int kQRow = D * 2 + 16;                  // a query row, padded: other banks
+  const int q_bytes = hpc * p.G * kQRow;
+  const int q_slots = stages + 1;
 
-  // [ring][scales][states that warps of one kv head hand over][prefix sums][lengths]
+  // [ring][scales][query rows][prefix sums][lengths]
   const uint32_t base = smem_u32(dyn_smem);
   uint8_t* ring = dyn_smem + (((base + 1023u) & ~1023u) - base);
   float* ring_scales = reinterpret_cast<float*>(ring + stages * stage_bytes);
-  float* states = ring_scales + stages * TG * scale_bytes / 4;
-  int* wpref = reinterpret_cast<int*>(states + (TG / 2) * hpc * kStateFloats * 32);
+  uint8_t* q_ring = reinterpret_cast<uint8_t*>(ring_scales + stages * TP * scale_bytes / 4);
+  int* wpref = reinterpret_cast<int*>(q_ring + q_slots * q_bytes);
   int* lens = wpref + n + 1;
 
   if (tid == 0) {
     s_abort = 0;
     for (int i = 0; i < stages; ++i) {
-      mbar_init(&full_bar[i], 1);
+      mbar_init(&full_bar[i], kProducers8);
       mbar_init(&empty_bar[i], hpc * TG);
+    }
+    for (int i = 0; i < q_slots; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], hpc * TG);
     }
     fence_mbar_init();
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // ── lengths and the prefix sums of their weights ──────────────────────────
-  const int tile_tokens = TG * kCachePage;
+  // ── the plan: lengths, prefix sums of their weights, this CTA's share ───────
+  // Every thread owns `per` sequences; those in which the share begins and ends
+  // are found by their owners.
+  const int tile_tokens = TP * kCachePage;
+  C8Shape sh;
+  sh.num_seqs = n;
+  sh.groups = p.n_kv / hpc;
+  sh.n_cta = gridDim.x;
   {
-    const int threads = blockDim.x;
-    const int per = (n + threads - 1) / threads;
-    for (int s = tid; s < n; s += threads) {
+    const int per = (n + blockDim.x - 1) / blockDim.x;
+    const int lo = min(n, tid * per), hi = min(n, lo + per);
+    int sum = 0;
+    for (int s = lo; s < hi; ++s) {
       int len = p.seq_lens[s];
       if (len <= 0) len = 0;
       if ((len + kCachePage - 1LL) / kCachePage > p.max_blocks) {
@@ -286,51 +329,66 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
         len = p.max_blocks * kCachePage;
       }
       lens[s] = len;
+      sum += c8_weight(c8_tiles(len, tile_tokens));
     }
-    __syncthreads();
-    const int lo = min(n, tid * per), hi = min(n, lo + per);
-    int sum = 0;
-    for (int s = lo; s < hi; ++s) sum += c8_weight(c8_tiles(lens[s], tile_tokens));
     int incl = sum;
 #pragma unroll
-    for (int sh = 1; sh < 32; sh <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, incl, sh);
-      if (lane >= sh) incl += y;
+    for (int sft = 1; sft < 32; sft <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, sft);
+      if (lane >= sft) incl += y;
     }
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
-    int run = incl - sum;
-    for (int w = 0; w < warp; ++w) run += warp_sum[w];
-    if (tid == 0) wpref[0] = 0;
+    int run = incl - sum, total = 0;
+    for (int x = 0; x < static_cast<int>(blockDim.x >> 5); ++x) {
+      const int y = warp_sum[x];
+      if (x < warp) run += y;
+      total += y;
+    }
+    sh.chunk = c8_chunk(total, sh.groups, sh.n_cta);
+    const long long w0 = static_cast<long long>(blockIdx.x) * sh.chunk;
+    C8Cut cut[2] = {c8_cut(total, sh.groups, w0), c8_cut(total, sh.groups, w0 + sh.chunk)};
+    if (tid == 0) {
+      wpref[0] = 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (cut[e].hg == sh.groups) share[e] = C8Pos{sh.groups, 0, 0};
+      }
+    }
     for (int s = lo; s < hi; ++s) {
+      const int before = run;
       run += c8_weight(c8_tiles(lens[s], tile_tokens));
       wpref[s + 1] = run;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (cut[e].hg < sh.groups && before <= cut[e].at && cut[e].at < run) {
+          share[e] = C8Pos{cut[e].hg, s, c8_tile_at(cut[e].at - before)};
+        }
+      }
     }
     __syncthreads();
   }
-  C8Shape sh;
-  sh.num_seqs = n;
-  sh.groups = p.n_kv / hpc;
-  sh.n_cta = gridDim.x;
-  sh.chunk = c8_chunk(wpref[n], sh.groups, sh.n_cta);
-  const C8Pos begin = c8_pos(wpref, sh, static_cast<long long>(blockIdx.x) * sh.chunk);
-  const C8Pos end = c8_pos(wpref, sh, static_cast<long long>(blockIdx.x + 1) * sh.chunk);
+  const C8Pos begin = share[0], end = share[1];
   C8Walk w;
   w.start(wpref, sh, begin, end);
 
-  if (warp == 0) {
-    // ── producer ────────────────────────────────────────────────────────────
+  if (warp < kProducers8) {
+    // ── producers ────────────────────────────────────────────────────────────
     // Block-table entries are fetched 32 pages ahead of their use.
     if (lane == 0) prefetch_tmap(&tmap);
     int pg = 0, pg_end = 0;
+    bool fresh = false;  // the next batch is a segment's first
     auto enter = [&]() {
-      pg = w.j0 * TG;
-      pg_end = min(w.j1 * TG, (lens[w.s] - 1) / kCachePage + 1);
+      pg = w.j0 * TP;
+      pg_end = min(w.j1 * TP, (lens[w.s] - 1) / kCachePage + 1);
+      fresh = true;
     };
-    auto fetch = [&](int& hg, int& count, int& phys) {
+    auto fetch = [&](int& hg, int& count, int& phys, int& first_of) {
       count = 0;
       if (!w.valid) return;
       hg = w.hg;
+      first_of = fresh ? w.s : -1;
+      fresh = false;
       count = min(32, pg_end - pg);
       phys = 0;
       if (lane < count) phys = p.block_tables[static_cast<int64_t>(w.s) * p.max_blocks + pg + lane];
@@ -341,31 +399,59 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       }
     };
     if (w.valid) enter();
-    int hg, count, phys, hg2 = 0, count2, phys2 = 0;
-    fetch(hg, count, phys);
-    int stage = 0;
-    uint32_t parity = 1;
+    int hg = 0, count, phys = 0, seq = -1, hg2 = 0, count2, phys2 = 0, seq2 = -1;
+    fetch(hg, count, phys, seq);
+    int stage = 0, q_slot = 0;
+    uint32_t parity = 1, q_parity = 1;
     while (count > 0) {
-      fetch(hg2, count2, phys2);
+      if (seq >= 0 && warp == 0) {
+        // The segment's query rows.
+        const bool ok = !s_abort && mbar_wait(&q_empty[q_slot], q_parity, p.err);
+        if (!__all_sync(0xffffffffu, ok)) {
+          s_abort = 1;
+          return;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&q_full[q_slot], hpc * p.G * D * 2);
+        __syncwarp();
+        for (int row = lane; row < hpc * p.G; row += 32) {
+          bulk_load(q_ring + q_slot * q_bytes + row * kQRow,
+                    static_cast<const T*>(p.q) + seq * p.q_stride +
+                        (static_cast<int64_t>(hg) * hpc * p.G + row) * D,
+                    D * 2, &q_full[q_slot]);
+        }
+        if (++q_slot == q_slots) {
+          q_slot = 0;
+          q_parity ^= 1;
+        }
+      }
+      fetch(hg2, count2, phys2, seq2);
       const bool bad = phys < 0 || phys >= p.num_blocks;
       if (bad) set_error(p.err, kDevErrBlockRange);
       // Such a page's codes read as zeros (the tensor map's bounds), its scales as block 0's.
       const float* src = p.scales + (static_cast<size_t>(bad ? 0 : phys) * p.n_kv + hg * hpc) * 2 * kCachePage;
       if (bad) phys = p.num_blocks;
-      for (int k = 0; k < count; k += TG) {
-        const int np = min(TG, count - k);
+      for (int k = 0; k < count; k += TP) {
+        const int np = min(TP, count - k);
         const bool ok = !s_abort && mbar_wait(&empty_bar[stage], parity, p.err);
         if (!__all_sync(0xffffffffu, ok)) {
           s_abort = 1;
           return;
         }
-        if (lane == 0) mbar_arrive_expect_tx(&full_bar[stage], np * (page_bytes + scale_bytes));
+        // This warp's pages of the tile: every kProducers8-th.
+        const int mine = (np - warp + kProducers8 - 1) / kProducers8;
+        if (lane == 0) {
+          if (mine > 0) {
+            mbar_arrive_expect_tx(&full_bar[stage], mine * (page_bytes + scale_bytes));
+          } else {
+            mbar_arrive(&full_bar[stage]);
+          }
+        }
         __syncwarp();
-        if (lane >= k && lane < k + np) {
-          const int i = lane - k;
+        const int i = lane - k;
+        if (i >= 0 && i < np && i % kProducers8 == warp) {
           tma_load_4d(ring + stage * stage_bytes + i * page_bytes, &tmap, &full_bar[stage], 0, 0,
-                      hg * hpc, 2 * phys);
-          bulk_load(ring_scales + (stage * TG + i) * (scale_bytes / 4), src, scale_bytes,
+                      D == 64 && hpc % 2 == 0 ? hg * (hpc / 2) : hg * hpc, 2 * phys);
+          bulk_load(ring_scales + (stage * TP + i) * (scale_bytes / 4), src, scale_bytes,
                     &full_bar[stage]);
         }
         if (++stage == stages) {
@@ -376,12 +462,13 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       hg = hg2;
       count = count2;
       phys = phys2;
+      seq = seq2;
     }
     return;
   }
 
   // ── consumers ─────────────────────────────────────────────────────────────
-  const int cw = warp - 1;
+  const int cw = warp - kProducers8;
   const int h = cw % hpc, tg = cw / hpc;
   const int g = lane >> 2, c = lane & 3;
   T* out = static_cast<T*>(p.out);
@@ -389,27 +476,33 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
   for (int s = blockIdx.x; s < n; s += gridDim.x) {  // rows of empty sequences
     if (lens[s] > 0) continue;
     uint4* o4 = reinterpret_cast<uint4*>(out + static_cast<int64_t>(s) * n_q * D);
-    for (int e = tid - 32; e < n_q * D / 8; e += blockDim.x - 32) o4[e] = make_uint4(0u, 0u, 0u, 0u);
+    for (int e = tid - 32 * kProducers8; e < n_q * D / 8; e += blockDim.x - 32 * kProducers8) o4[e] = make_uint4(0u, 0u, 0u, 0u);
   }
 
-  // This lane's ldmatrix row: token r (+ 8 for matrices 1 and 3), 16-byte chunk 2 kk (+ 1 for
-  // matrices 2 and 3), at the place the tensor map's swizzle put it.
-  uint32_t off[D / 32];
-  {
-    const int tok = (lane & 7) + ((lane >> 3) & 1) * 8;
-#pragma unroll
-    for (int kk = 0; kk < D / 32; ++kk) {
-      const int chunk = 2 * kk + (lane >> 4);
-      const int at = D == 128 ? chunk ^ (tok & 7) : chunk ^ ((tok >> 1) & 3);
-      off[kk] = tok * D + at * 16;
+  // Where the tensor map's box and swizzle put 16-byte chunk `chunk` of this head's row of
+  // token `tok` in a page (K; V is v_add further): rows of 128 bytes, at head size 64 of two
+  // heads, or of 64 where n_kv is odd.
+  const bool two = D == 64 && hpc % 2 == 0;
+  auto place = [&](int tok, int chunk) -> uint32_t {
+    if (D == 128) return h * (kCachePage * D) + tok * 128 + ((chunk ^ (tok & 7)) << 4);
+    if (two) {
+      return (h >> 1) * (kCachePage * 128) + tok * 128 + ((((h & 1) * 4 + chunk) ^ (tok & 7)) << 4);
     }
+    return h * (kCachePage * D) + tok * 64 + ((chunk ^ ((tok >> 1) & 3)) << 4);
+  };
+  // This lane's ldmatrix row: token r (+ 8 for matrices 1 and 3), chunk 2 kk (+ 1 for matrices
+  // 2 and 3).
+  uint32_t off[D / 32];
+#pragma unroll
+  for (int kk = 0; kk < D / 32; ++kk) {
+    off[kk] = place((lane & 7) + ((lane >> 3) & 1) * 8, 2 * kk + (lane >> 4));
   }
-  const uint32_t k_base = smem_u32(ring) + tg * page_bytes + h * kCachePage * D;
+  const uint32_t k_base = smem_u32(ring) + tg * page_bytes;
   const uint32_t v_add = hpc * kCachePage * D;
   const float* my_scales = ring_scales + (tg * hpc + h) * 2 * kCachePage + g;
 
   Piece8* pend = pieces_of[cw];
-  int n_pend = 0, n_arrived = 0, arrive_at = -1;
+  int n_pend = 0;
   // The counter a piece arrives on, and how many do.
   auto counter_of = [&](int i, int& members) -> int* {
     const int pieces = pend[i].c1 - pend[i].c0 + 1;
@@ -417,13 +510,19 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
     const int first = (static_cast<int>(blockIdx.x) - pend[i].c0) / size * size;
     members = min(size, pieces - first);
     const int lead = pend[i].c0 + first;
-    return p.group_counters + (static_cast<size_t>(lead) * 2 + (first == 0 ? 1 : 0)) * hpc + h;
+    return p.group_counters +
+           ((static_cast<size_t>(lead) * 2 + (first == 0 ? 1 : 0)) * hpc + h) * kParts8 + tg;
   };
 
-  int stage = 0, it = 0;
-  uint32_t parity = 0;
-  for (; w.valid; w.next(wpref, sh, end)) {
+  // The warps of a kv head, at one point.
+  auto together = [&]() { named_barrier_sync(1 + h, TG * 32); };
+  constexpr int M = KS / kParts8;  // m-tiles that a warp takes of a kv head's output at a time
+
+  int stage = 0, q_slot = 0, turn = 0;
+  uint32_t parity = 0, q_parity = 0;
+  for (; w.valid; w.next(wpref, sh, end), turn ^= 1) {
     const int s = w.s, kvh = w.hg * hpc + h, len = lens[s];
+    if (!s_abort && !mbar_wait(&q_full[q_slot], q_parity, p.err)) s_abort = 1;
     // Q^T as the B operand: k indices 2c, 2c+1 and 2c+8, 2c+9 of step ks are elements
     // 16 ks + 4c .. + 3 of head g.
     uint32_t qf[NT][KS][2];
@@ -431,11 +530,11 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int head = nt * 8 + g;
-      const T* row = static_cast<const T*>(p.q) + s * p.q_stride +
-                     (static_cast<int64_t>(kvh) * p.G + (head < p.G ? head : 0)) * D + 4 * c;
+      const uint8_t* row =
+          q_ring + q_slot * q_bytes + (h * p.G + (head < p.G ? head : 0)) * kQRow + 8 * c;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const uint2 v = *reinterpret_cast<const uint2*>(row + 16 * ks);
+        const uint2 v = *reinterpret_cast<const uint2*>(row + 32 * ks);
         qf[nt][ks][0] = head < p.G ? v.x : 0u;
         qf[nt][ks][1] = head < p.G ? v.y : 0u;
       }
@@ -471,8 +570,15 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       fac[nt][1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
     }
 
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&q_empty[q_slot]);
+    if (++q_slot == q_slots) {
+      q_slot = 0;
+      q_parity ^= 1;
+    }
+
     float m[NT][2], l[NT][2], o[NT][KS][4];  // m: the score bound less 11
-    float vref = pow2(-126), vinv = pow2(126);
+    float vref = pow2(-126), vinv = pow2(126);  // V's scales so far are at most vref
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = kLowest8;
@@ -481,130 +587,148 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       for (int mt = 0; mt < KS; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
     }
 
-    for (int j = w.j0; j < w.j1; ++j, ++it) {
-      // After a wait that gave up, the rest runs through without waiting: the barriers
-      // between warps still meet.
-      if (!s_abort && !mbar_wait(&full_bar[stage], parity, p.err)) s_abort = 1;
-      const int live = len - (j * TG + tg) * kCachePage;  // tokens from this page on
-      if (live > 0) {
-        const bool tail = live < kCachePage;
-        const uint32_t kb = k_base + stage * stage_bytes;
-        const float* sc = my_scales + stage * TG * (scale_bytes / 4);
-        const float ks0 = sc[0], ks1 = sc[8];
-        float vs0 = sc[16], vs1 = sc[24];
-        // Two chains of products, so that they do not wait on each other.
-        float x[NT][4], y[NT][4];
+    // One page or PP of a tile: `live` tokens from the first on, the others TG pages further
+    // each (all but the last whole).
+    auto work = [&](auto pages_tag, int live) {
+      constexpr int P = decltype(pages_tag)::value;
+      const uint32_t kb = k_base + stage * stage_bytes;
+      const float* sc = my_scales + stage * TP * (scale_bytes / 4);
+      const int last_live = live - (P - 1) * TG * kCachePage;  // of the last page
+      const bool tail = last_live < kCachePage;
+      float x[P][NT][4], ks0[P], ks1[P], vs0[P], vs1[P];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
-          y[nt][0] = y[nt][1] = y[nt][2] = y[nt][3] = 0.f;
-        }
+      for (int i = 0; i < P; ++i) {
+        const float* si = sc + i * TG * (scale_bytes / 4);
+        ks0[i] = si[0];
+        ks1[i] = si[8];
+        vs0[i] = si[16];
+        vs1[i] = si[24];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) x[i][nt][0] = x[i][nt][1] = x[i][nt][2] = x[i][nt][3] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < D / 32; ++kk) {
-          uint32_t a[4];
-          ldmatrix_x4(a, kb + off[kk]);
-          uint32_t b[4], d[4];
+          uint32_t a[4], b[4], d[4];
+          ldmatrix_x4(a, kb + i * TG * page_bytes + off[kk]);
           widen<kInt8, true>(a[0], b[0], b[2]);
           widen<kInt8, true>(a[1], b[1], b[3]);
           widen<kInt8, true>(a[2], d[0], d[2]);
           widen<kInt8, true>(a[3], d[1], d[3]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            Mma<__half>::run(x[nt], b, qf[nt][2 * kk][0], qf[nt][2 * kk][1]);
-            Mma<__half>::run(y[nt], d, qf[nt][2 * kk + 1][0], qf[nt][2 * kk + 1][1]);
+            Mma<__half>::run(x[i][nt], b, qf[nt][2 * kk][0], qf[nt][2 * kk][1]);
+            Mma<__half>::run(x[i][nt], d, qf[nt][2 * kk + 1][0], qf[nt][2 * kk + 1][1]);
           }
         }
-        bool raise = false;
+      }
+      // Scores in log2 units less m; behind the length, whatever the slots hold, none.
+      float y[P][NT][4];
+      auto score = [&]() {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          x[nt][0] = (x[nt][0] + y[nt][0]) * fac[nt][0] * ks0;
-          x[nt][1] = (x[nt][1] + y[nt][1]) * fac[nt][1] * ks0;
-          x[nt][2] = (x[nt][2] + y[nt][2]) * fac[nt][0] * ks1;
-          x[nt][3] = (x[nt][3] + y[nt][3]) * fac[nt][1] * ks1;
-        }
-        if (tail) {
-          // Whatever the slots behind the length hold takes no part.
-          if (g >= live) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = -INFINITY;
-            vs0 = 0.f;
-          }
-          if (g + 8 >= live) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) x[nt][2] = x[nt][3] = -INFINITY;
-            vs1 = 0.f;
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          raise |= fmaxf(x[nt][0], x[nt][2]) > m[nt][0] + 15.f;
-          raise |= fmaxf(x[nt][1], x[nt][3]) > m[nt][1] + 15.f;
-        }
-        raise |= fmaxf(vs0, vs1) > vref;
-        if (__any_sync(0xffffffffu, raise)) {
-          float vm = fmaxf(vs0, vs1);
-#pragma unroll
-          for (int b = 4; b < 32; b <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, b));
-          float down = 1.f;
-          if (vm > vref && vm < INFINITY) {
-            const int e = min(127, static_cast<int>(__float_as_uint(vm) >> 23) - 126);
-            vref = pow2(e);
-            down = vinv;  // old reference over the new one, below
-            vinv = e < 127 ? pow2(-e) : __int_as_float(0x00400000);  // 2^-127
-            down = vinv / down;
-          }
+        for (int i = 0; i < P; ++i) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float m0 = fmaxf(x[nt][0], x[nt][2]), m1 = fmaxf(x[nt][1], x[nt][3]);
-#pragma unroll
-            for (int b = 4; b < 32; b <<= 1) {
-              m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, b));
-              m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, b));
-            }
-            m0 = fmaxf(m[nt][0], m0 - 11.f);
-            m1 = fmaxf(m[nt][1], m1 - 11.f);
-            const float a0 = fast_exp2(m[nt][0] - m0), a1 = fast_exp2(m[nt][1] - m1);
-            m[nt][0] = m0;
-            m[nt][1] = m1;
-            l[nt][0] *= a0;
-            l[nt][1] *= a1;
-#pragma unroll
-            for (int mt = 0; mt < KS; ++mt) {
-              o[nt][mt][0] *= a0 * down;
-              o[nt][mt][1] *= a1 * down;
-              o[nt][mt][2] *= a0 * down;
-              o[nt][mt][3] *= a1 * down;
-            }
+            y[i][nt][0] = fmaf(x[i][nt][0], fac[nt][0] * ks0[i], -m[nt][0]);
+            y[i][nt][1] = fmaf(x[i][nt][1], fac[nt][1] * ks0[i], -m[nt][1]);
+            y[i][nt][2] = fmaf(x[i][nt][2], fac[nt][0] * ks1[i], -m[nt][0]);
+            y[i][nt][3] = fmaf(x[i][nt][3], fac[nt][1] * ks1[i], -m[nt][1]);
           }
         }
-        vs0 *= vinv;
-        vs1 *= vinv;
-        uint32_t pb[NT][2];
+        if (tail) {
+          if (g >= last_live) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) y[P - 1][nt][0] = y[P - 1][nt][1] = -INFINITY;
+            vs0[P - 1] = 0.f;
+          }
+          if (g + 8 >= last_live) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) y[P - 1][nt][2] = y[P - 1][nt][3] = -INFINITY;
+            vs1[P - 1] = 0.f;
+          }
+        }
+      };
+      score();
+      float ym = -INFINITY, vm = 0.f;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        vm = fmaxf(vm, fmaxf(vs0[i], vs1[i]));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float p0 = fast_exp2(x[nt][0] - m[nt][0]), p1 = fast_exp2(x[nt][1] - m[nt][1]);
-          const float p2 = fast_exp2(x[nt][2] - m[nt][0]), p3 = fast_exp2(x[nt][3] - m[nt][1]);
+          ym = fmaxf(ym, fmaxf(fmaxf(y[i][nt][0], y[i][nt][1]), fmaxf(y[i][nt][2], y[i][nt][3])));
+        }
+      }
+      if (__any_sync(0xffffffffu, ym > 15.f || vm > vref)) {
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, b));
+        float down = 1.f;
+        if (vm > vref && vm < INFINITY) {
+          const int e = min(126, static_cast<int>(__float_as_uint(vm) >> 23) - 126);
+          down = vref;
+          vref = pow2(e);
+          vinv = pow2(-e);
+          down *= vinv;  // (sums below 2^-126 of it are gone)
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const bool in0 = i < P - 1 || g < last_live, in1 = i < P - 1 || g + 8 < last_live;
+            if (in0) m0 = fmaxf(m0, x[i][nt][0] * (fac[nt][0] * ks0[i]));
+            if (in0) m1 = fmaxf(m1, x[i][nt][1] * (fac[nt][1] * ks0[i]));
+            if (in1) m0 = fmaxf(m0, x[i][nt][2] * (fac[nt][0] * ks1[i]));
+            if (in1) m1 = fmaxf(m1, x[i][nt][3] * (fac[nt][1] * ks1[i]));
+          }
+#pragma unroll
+          for (int b = 4; b < 32; b <<= 1) {
+            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, b));
+            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, b));
+          }
+          m0 = fmaxf(m[nt][0], m0 - 11.f);
+          m1 = fmaxf(m[nt][1], m1 - 11.f);
+          const float a0 = fast_exp2(m[nt][0] - m0), a1 = fast_exp2(m[nt][1] - m1);
+          m[nt][0] = m0;
+          m[nt][1] = m1;
+          l[nt][0] *= a0;
+          l[nt][1] *= a1;
+#pragma unroll
+          for (int mt = 0; mt < KS; ++mt) {
+            o[nt][mt][0] *= a0 * down;
+            o[nt][mt][1] *= a1 * down;
+            o[nt][mt][2] *= a0 * down;
+            o[nt][mt][3] *= a1 * down;
+          }
+        }
+        score();
+      }
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        uint32_t pb[NT][2];
+        const float v0 = vs0[i] * vinv, v1 = vs1[i] * vinv;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float p0 = fast_exp2(y[i][nt][0]), p1 = fast_exp2(y[i][nt][1]);
+          const float p2 = fast_exp2(y[i][nt][2]), p3 = fast_exp2(y[i][nt][3]);
           l[nt][0] += p0 + p2;
           l[nt][1] += p1 + p3;
           // C fragment (row = token, col = head) -> B fragment (k = token, n = head).
-          pb[nt][0] = movmatrix_trans(Elt<__half>::pack(p0 * vs0, p1 * vs0));
-          pb[nt][1] = movmatrix_trans(Elt<__half>::pack(p2 * vs1, p3 * vs1));
+          pb[nt][0] = movmatrix_trans(Elt<__half>::pack(p0 * v0, p1 * v0));
+          pb[nt][1] = movmatrix_trans(Elt<__half>::pack(p2 * v1, p3 * v1));
         }
-        const uint32_t vb = kb + v_add;
 #pragma unroll
         for (int kk = 0; kk < D / 32; ++kk) {
-          uint32_t a[4];
-          ldmatrix_x4_trans(a, vb + off[kk]);
-          if (!kInt8 && tail) {
+          uint32_t a[4], b[4], d[4];
+          ldmatrix_x4_trans(a, kb + i * TG * page_bytes + v_add + off[kk]);
+          if (!kInt8 && i == P - 1 && tail) {
             // e4m3 has NaN codes, and 0 * NaN is one: tokens 2c, 2c+1 and 2c+8, 2c+9.
-            const uint32_t lo = (2 * c < live ? 0xffffu : 0u) | (2 * c + 1 < live ? 0xffff0000u : 0u);
-            const uint32_t hi = (2 * c + 8 < live ? 0xffffu : 0u) | (2 * c + 9 < live ? 0xffff0000u : 0u);
+            const uint32_t lo = (2 * c < last_live ? 0xffffu : 0u) |
+                                (2 * c + 1 < last_live ? 0xffff0000u : 0u);
+            const uint32_t hi = (2 * c + 8 < last_live ? 0xffffu : 0u) |
+                                (2 * c + 9 < last_live ? 0xffff0000u : 0u);
             a[0] &= lo;
             a[1] &= hi;
             a[2] &= lo;
             a[3] &= hi;
           }
-          uint32_t b[4], d[4];
           widen<kInt8, false>(a[0], b[0], b[1]);
           widen<kInt8, false>(a[1], b[2], b[3]);
           widen<kInt8, false>(a[2], d[0], d[1]);
@@ -616,23 +740,38 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty_bar[stage]);
-      if (++stage == stages) {
-        stage = 0;
-        parity ^= 1;
+    };
+
+    int live = len - (w.j0 * TP + tg) * kCachePage;  // tokens from this warp's first page on
+    for (int j = w.j0; j < w.j1; ++j, live -= tile_tokens) {
+      // After a wait that gave up, the rest runs through without waiting: the barriers
+      // between warps still meet.
+      if (!mbar_try_wait(&full_bar[stage], parity) && !s_abort &&
+          !mbar_wait(&full_bar[stage], parity, p.err)) {
+        s_abort = 1;
       }
-      if (n_arrived < n_pend && it >= arrive_at) {
-        // A piece published two tiles ago: its stores are done, so the release is cheap.
-        if (lane == 0) {
-          int members;
-          int* counter = counter_of(n_arrived, members);
-          pend[n_arrived].missing = members - 1 - arrive_piece8(counter);
+      if (PP > 1 && live > (PP - 1) * TG * kCachePage) {
+        work(std::integral_constant<int, PP>{}, live);
+      } else if (live > 0) {
+        work(std::integral_constant<int, 1>{}, live);
+      }
+      if (j + 1 < w.j1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty_bar[stage]);
+        if (++stage == stages) {
+          stage = 0;
+          parity ^= 1;
         }
-        ++n_arrived;
       }
     }
 
+    // ── the segment's end: the warps of a kv head put their sums together ─────
+    const int active = min(TG, (len - 1) / kCachePage + 1 - w.j0 * TP);  // warps that had a page
+    const bool whole = w.j0 == 0 && w.j1 == w.tiles;
+    const bool alone = whole && active == 1;
+    T* rows = out + (static_cast<int64_t>(s) * n_q + kvh * p.G) * D;
+    // Bounds and sums first.
+    float4(*hand_ml)[NT][4] = hand_ml_of[turn];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -640,134 +779,174 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
         l[nt][0] += __shfl_xor_sync(0xffffffffu, l[nt][0], b);
         l[nt][1] += __shfl_xor_sync(0xffffffffu, l[nt][1], b);
       }
+      if (g == 0) hand_ml[cw][nt][c] = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
     }
-    // The warps of a kv head hand their states over, half of them to the other half each time.
-    for (int half = TG / 2; half >= 1; half >>= 1) {
-      float* slot = states + static_cast<size_t>(((tg & (half - 1)) * hpc + h) * kStateFloats) * 32 + lane;
-      if (tg >= half && tg < 2 * half) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float* z = slot + nt * (KS * 4 + 5) * 32;
-#pragma unroll
-          for (int mt = 0; mt < KS; ++mt) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[(mt * 4 + e) * 32] = o[nt][mt][e];
-          }
-          z[KS * 4 * 32] = m[nt][0];
-          z[(KS * 4 + 1) * 32] = m[nt][1];
-          z[(KS * 4 + 2) * 32] = l[nt][0];
-          z[(KS * 4 + 3) * 32] = l[nt][1];
-          z[(KS * 4 + 4) * 32] = vref;
-        }
-      }
-      named_barrier_sync(1 + h, TG * 32);
-      if (tg < half) {
-        const float vr = slot[(KS * 4 + 4) * 32];
-        const float v = fmaxf(vref, vr);
-        const float va = vref / v, vb = vr / v;
-        vref = v;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float* z = slot + nt * (KS * 4 + 5) * 32;
-          const float n0 = z[KS * 4 * 32], n1 = z[(KS * 4 + 1) * 32];
-          const float m0 = fmaxf(m[nt][0], n0), m1 = fmaxf(m[nt][1], n1);
-          float a0 = fast_exp2(m[nt][0] - m0), a1 = fast_exp2(m[nt][1] - m1);
-          float b0 = fast_exp2(n0 - m0), b1 = fast_exp2(n1 - m1);
-          m[nt][0] = m0;
-          m[nt][1] = m1;
-          l[nt][0] = l[nt][0] * a0 + z[(KS * 4 + 2) * 32] * b0;
-          l[nt][1] = l[nt][1] * a1 + z[(KS * 4 + 3) * 32] * b1;
-          a0 *= va;
-          a1 *= va;
-          b0 *= vb;
-          b1 *= vb;
-#pragma unroll
-          for (int mt = 0; mt < KS; ++mt) {
-            o[nt][mt][0] = o[nt][mt][0] * a0 + z[(mt * 4) * 32] * b0;
-            o[nt][mt][1] = o[nt][mt][1] * a1 + z[(mt * 4 + 1) * 32] * b1;
-            o[nt][mt][2] = o[nt][mt][2] * a0 + z[(mt * 4 + 2) * 32] * b0;
-            o[nt][mt][3] = o[nt][mt][3] * a1 + z[(mt * 4 + 3) * 32] * b1;
-          }
-        }
-      }
-      named_barrier_sync(1 + h, TG * 32);
+    if (alone) {
+      __syncwarp();
+    } else {
+      together();
     }
-    if (tg != 0) continue;
-
-    float f[NT][2];
+    float lse[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      f[nt][0] = vref / l[nt][0];
-      f[nt][1] = vref / l[nt][1];
+      float4 ml[kWarps8];
+      float top0 = kLowest8, top1 = kLowest8, sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+      for (int t = 0; t < kWarps8; ++t) {
+        ml[t] = make_float4(kLowest8, kLowest8, 0.f, 0.f);
+        if (t < active) ml[t] = hand_ml[t * hpc + h][nt][c];
+        top0 = fmaxf(top0, ml[t].x);
+        top1 = fmaxf(top1, ml[t].y);
+      }
+#pragma unroll
+      for (int t = 0; t < kWarps8; ++t) {
+        if (t < active) {
+          sum0 += ml[t].z * fast_exp2(ml[t].x - top0);
+          sum1 += ml[t].w * fast_exp2(ml[t].y - top1);
+        }
+      }
+      lse[nt][0] = top0 + __log2f(sum0);
+      lse[nt][1] = top1 + __log2f(sum1);
+      // A cut piece whose weights are all zero (scores of -inf) adds nothing.
+      const float r0 = !whole && sum0 == 0.f ? 0.f : __fdividef(1.f, sum0);
+      const float r1 = !whole && sum1 == 0.f ? 0.f : __fdividef(1.f, sum1);
+      const float a0 = fast_exp2(m[nt][0] - top0) * r0 * vref;
+      const float a1 = fast_exp2(m[nt][1] - top1) * r1 * vref;
+#pragma unroll
+      for (int mt = 0; mt < KS; ++mt) {
+        o[nt][mt][0] *= a0;
+        o[nt][mt][1] *= a1;
+        o[nt][mt][2] *= a0;
+        o[nt][mt][3] *= a1;
+      }
     }
-    if (w.j0 == 0 && w.j1 == w.tiles) {
-      store_rows<T, D, NT>(out + (static_cast<int64_t>(s) * n_q + kvh * p.G) * D, p.G, lane, f, o);
-      continue;
+    if (alone) {
+      if (tg == 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) store_rows<T, D, KS>(rows, p.G, nt, 0, lane, o[nt]);
+      }
+    } else {
+      // Then the output: each warp writes its share over the codes that it has just read (the
+      // last tile's slot is given back after that), and adds up all warps' in M m-tiles.
+      uint8_t* slot = ring + stage * stage_bytes;
+      // A fragment of m-tile mt takes the head's chunks from 32 mt on, K's and then V's.
+      auto chunk_of = [&](int mt) -> uint32_t {
+        const int at = (mt % (KS / 2)) * 32 + lane;
+        return (mt >= KS / 2 ? v_add : 0u) + place(at / (D / 16), at % (D / 16));
+      };
+      // Record of this CTA's end (slot 0) or start (slot 1) of a cut sequence.
+      const size_t rec = (static_cast<size_t>(blockIdx.x) * 2 + (w.j0 == 0)) * hpc + h;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (nt > 0) together();  // the n-tile before has been read
+        if (tg < active) {
+#pragma unroll
+          for (int mt = 0; mt < KS; ++mt) {
+            *reinterpret_cast<float4*>(slot + tg * page_bytes + chunk_of(mt)) =
+                make_float4(o[nt][mt][0], o[nt][mt][1], o[nt][mt][2], o[nt][mt][3]);
+          }
+          // The next tile's copy into this slot comes after these writes.  (Here, where no
+          // global stores are under way that the fence would wait for.)
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        together();
+        for (int mt = tg * M; mt < KS; mt += TG * M) {
+          float x[M][4];
+          uint32_t at[M];
+#pragma unroll
+          for (int i = 0; i < M; ++i) {
+            at[i] = chunk_of(mt + i);
+            x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+          }
+#pragma unroll
+          for (int t = 0; t < kWarps8; ++t) {
+            if (t >= active) break;
+#pragma unroll
+            for (int i = 0; i < M; ++i) {
+              const float4 y = *reinterpret_cast<const float4*>(slot + t * page_bytes + at[i]);
+              x[i][0] += y.x;
+              x[i][1] += y.y;
+              x[i][2] += y.z;
+              x[i][3] += y.w;
+            }
+          }
+          if (whole) {
+            store_rows<T, D, M>(rows, p.G, nt, mt, lane, x);
+          } else {
+            store_record<D, NT, M>(p, rec, nt, mt / M, lane, lse[nt], x);
+          }
+        }
+      }
     }
+    // The slot goes back to the copies of the next tiles.
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty_bar[stage]);
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1;
+    }
+    if (whole) continue;
     if (n_pend == 2) {  // the plan leaves a CTA two pieces at most
       set_error(p.err, kDevErrSeqLen);
       continue;
     }
-    const int c0 = c8_owner(wpref, sh, w.hg, s, 0);
-    const int c1 = c8_owner(wpref, sh, w.hg, s, w.tiles - 1);
-    const size_t rec = (static_cast<size_t>(blockIdx.x) * 2 + (static_cast<int>(blockIdx.x) == c0)) * hpc + h;
-    float lse[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      lse[nt][0] = m[nt][0] + log2f(l[nt][0]);
-      lse[nt][1] = m[nt][1] + log2f(l[nt][1]);
-      // A piece whose weights are all zero (scores of -inf) adds nothing.
-      if (l[nt][0] == 0.f) f[nt][0] = 0.f;
-      if (l[nt][1] == 0.f) f[nt][1] = 0.f;
+    if (lane < 2) {
+      (lane == 0 ? pend[n_pend].c0 : pend[n_pend].c1) =
+          c8_owner(wpref, sh, w.hg, s, lane == 0 ? 0 : w.tiles - 1);
     }
-    store_record<D, NT>(p, rec, lane, lse, f, o);
-    if (lane == 0) pend[n_pend] = Piece8{c0, c1, s, kvh, -1};
+    pend[n_pend].s = s;
+    pend[n_pend].kvh = kvh;
     ++n_pend;
-    arrive_at = it + 2;
   }
+  if (n_pend == 0 || tg >= kParts8) return;
 
   // ── joining cut sequences ─────────────────────────────────────────────────
-  __syncwarp();  // every lane's stores before lane 0's releases
-  int last = 0;
-  if (lane == 0) {
-    for (int i = n_arrived; i < n_pend; ++i) {
-      int members;
-      int* counter = counter_of(i, members);
-      pend[i].missing = members - 1 - arrive_piece8(counter);
-    }
-    for (int i = 0; i < n_pend; ++i) last |= (pend[i].missing == 0) << i;
+  // The first kParts8 warps of a kv head join M m-tiles each, those that they stored of the
+  // pieces: a warp waits for nobody.
+  __syncwarp();  // every lane's stores before those lanes' releases
+  int missing = -1;
+  if (lane < n_pend) {
+    int members;
+    int* counter = counter_of(lane, members);
+    missing = members - 1 - arrive_piece8(counter);
   }
-  last = __shfl_sync(0xffffffffu, last, 0);
-  __syncwarp();  // every lane's loads after lane 0's acquire
   for (int i = 0; i < n_pend; ++i) {
-    if (!(last & (1 << i))) continue;
+    // (The shuffle also puts every lane's loads after the acquires.)
+    if (__shfl_sync(0xffffffffu, missing, i) != 0) continue;
     const int c0 = pend[i].c0, pieces = pend[i].c1 - c0 + 1;
     const int size = c8_join_group(pieces);
     const int first = (static_cast<int>(blockIdx.x) - c0) / size * size;
-    float lse[NT][2], o[NT][KS][4], one[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) one[nt][0] = one[nt][1] = 1.f;
+    T* rows = out + (static_cast<int64_t>(pend[i].s) * n_q + pend[i].kvh * p.G) * D;
     int members;
     int* counter = counter_of(i, members);
-    join_records<D, NT>(p, c0 + first, 1, members, c0, h, lane, lse, o);
     if (lane == 0) *counter = 0;
-    if (size < pieces) {
-      // Round two: this group's record takes the place of its first piece's.
-      const int lead = c0 + first;
-      store_record<D, NT>(p, (static_cast<size_t>(lead) * 2 + (first == 0)) * hpc + h, lane, lse,
-                          one, o);
-      __syncwarp();
-      const int groups = (pieces + size - 1) / size;
-      int* top = p.top_counters + static_cast<size_t>(c0) * hpc + h;
-      int final_one = 0;
-      if (lane == 0) final_one = arrive_piece8(top) == groups - 1;
-      if (!__shfl_sync(0xffffffffu, final_one, 0)) continue;
-      __syncwarp();
-      join_records<D, NT>(p, c0, size, groups, c0, h, lane, lse, o);
-      if (lane == 0) *top = 0;
+    const size_t round2 = static_cast<size_t>(gridDim.x) * 2 * hpc;  // records after the pieces'
+    float lse[2], x[M][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      join_records<D, NT, M>(p, 0, c0 + first, 1, members, c0, h, nt, tg, lane, lse, x);
+      if (size == pieces) {
+        store_rows<T, D, M>(rows, p.G, nt, tg * M, lane, x);
+      } else {
+        store_record<D, NT, M>(p, round2 + (static_cast<size_t>(c0 + first) * 2 + (first == 0)) * hpc + h,
+                               nt, tg, lane, lse, x);
+      }
     }
-    store_rows<T, D, NT>(out + (static_cast<int64_t>(pend[i].s) * n_q + pend[i].kvh * p.G) * D, p.G,
-                         lane, one, o);
+    if (size == pieces) continue;
+    const int groups = (pieces + size - 1) / size;
+    __syncwarp();
+    int before = 0;
+    if (lane == 0) {
+      int* top = p.top_counters + (static_cast<size_t>(c0) * hpc + h) * kParts8 + tg;
+      before = arrive_piece8(top);
+      if (before == groups - 1) *top = 0;
+    }
+    if (__shfl_sync(0xffffffffu, before, 0) != groups - 1) continue;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      join_records<D, NT, M>(p, round2, c0, size, groups, c0, h, nt, tg, lane, lse, x);
+      store_rows<T, D, M>(rows, p.G, nt, tg * M, lane, x);
+    }
   }
 }
 
@@ -786,26 +965,35 @@ bool shape_ok8(int num_seqs, int n_q, int n_kv, int D) {
 }
 
 // The launch for a shape (shape_ok8) on a device with `sms` SMs.
-Decode8Config configure8(int num_seqs, int n_q, int n_kv, int D, int sms) {
+Decode8Config configure8(int num_seqs, int n_q, int n_kv, int D, int max_blocks, int sms) {
   Decode8Config cfg;
-  cfg.hpc = kMaxWarps8;
+  // Two heads a CTA, so that a sequence is cut into few pieces and rows of a page are
+  // read 2 D bytes at a time; more where no sequence has the pages for the other warps.
+  cfg.tg = kWarps8 / 2;
+  while (cfg.tg > 1 && cfg.tg / 2 * kPages8 >= max_blocks) cfg.tg /= 2;
+  cfg.hpc = min(kMaxHeads8, kWarps8 / cfg.tg);
+  while (cfg.hpc > 2 && cfg.hpc * (n_q / n_kv) > 32) --cfg.hpc;  // query rows in shared memory
   while (n_kv % cfg.hpc) --cfg.hpc;
-  cfg.tg = 1;
-  while (cfg.hpc * cfg.tg * 2 <= kMaxWarps8) cfg.tg *= 2;
+  while (cfg.hpc * cfg.tg * 2 <= kWarps8 && cfg.tg * kPages8 < max_blocks) cfg.tg *= 2;
   cfg.nt = n_q / n_kv > 8 ? 2 : 1;
-  const int resident = (D == 128 && cfg.nt == 2) ? 1 : 2;
-  cfg.n_cta = sms * resident;
-  const size_t stage = static_cast<size_t>(cfg.tg) * cfg.hpc * (2 * kCachePage * D + 2 * kCachePage * 4);
-  const size_t rest = 1024 + static_cast<size_t>(cfg.tg / 2) * cfg.hpc * cfg.nt * (D / 4 + 5) * 32 * 4 +
-                      (2 * static_cast<size_t>(num_seqs) + 1) * 4;
-  // Shared memory of an SM: 228 KB, 1 KB of it taken per CTA.
-  const size_t room = resident == 1 ? 220u << 10 : 111u << 10;
+  cfg.n_cta = sms;
+  const size_t stage =
+      static_cast<size_t>(cfg.tg) * kPages8 * cfg.hpc * (2 * kCachePage * D + 2 * kCachePage * 4);
+  const size_t q_slot = static_cast<size_t>(cfg.hpc) * (n_q / n_kv) * (2 * D + 16);
+  const size_t rest = 1024 + q_slot + (2 * static_cast<size_t>(num_seqs) + 1) * 4;
+  // Bytes in flight: three stages at head size 128 (4 x 131072 tokens 173.5 us, 176.8 with
+  // two; 256 x 511..1537 96.8 and 104.3), four at 64 (16 x 1..8192 42.2 us, 44.5 with six and
+  // 45.9 with two: what is in flight beyond the need makes the waits of the joins longer).
+  const size_t most = D == 128 ? 208 << 10 : 160 << 10;
   cfg.stages = kMaxStages8;
-  while (cfg.stages > 2 && rest + cfg.stages * stage > room) --cfg.stages;
-  cfg.smem = rest + cfg.stages * stage;
-  const size_t recs = static_cast<size_t>(cfg.n_cta) * 2 * cfg.hpc;
+  while (cfg.stages > 2 && (cfg.stages * stage > most ||
+                            rest + cfg.stages * (stage + q_slot) > kMostSmem8)) {
+    --cfg.stages;
+  }
+  cfg.smem = rest + cfg.stages * (stage + q_slot);
+  const size_t recs = static_cast<size_t>(cfg.n_cta) * 2 * 2 * 2;
   cfg.lse_at = kRecordsAt8;
-  cfg.o_at = cfg.lse_at + align256_8(recs * cfg.nt * 8 * sizeof(float));
+  cfg.o_at = cfg.lse_at + align256_8(recs * cfg.nt * kParts8 * 8 * sizeof(float));
   cfg.workspace = cfg.o_at + recs * cfg.nt * (D / 16) * 128 * sizeof(float);
   return cfg;
 }
@@ -819,11 +1007,11 @@ int launch_decode8(const CUtensorMap& tmap, const Decode8Params& p, const Decode
   if (dev < 0 || dev >= 64) return fail(VMPS_ERR_CUDA, "device index %d", dev);
   std::call_once(flags[dev], [] {
     cudaFuncSetAttribute(decode8_kernel<T, D, NT, kInt8>,
-                         cudaFuncAttributeMaxDynamicSharedMemorySize, 226 << 10);
+                         cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem8);
   });
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(c.n_cta);
-  cfg.blockDim = dim3(32 * (1 + c.hpc * c.tg));
+  cfg.blockDim = dim3(32 * (kProducers8 + c.hpc * c.tg));
   cfg.dynamicSmemBytes = c.smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -857,7 +1045,7 @@ extern "C" size_t vmps_paged_decode_cache8_workspace_bytes(int num_seqs, int n_q
   using namespace vmps;
   int sms = 0;
   if (!shape_ok8(num_seqs, n_q, n_kv, head_dim) || device_sm_count(&sms)) return 0;
-  return configure8(num_seqs, n_q, n_kv, head_dim, sms).workspace;
+  return configure8(num_seqs, n_q, n_kv, head_dim, INT_MAX, sms).workspace;
 }
 
 extern "C" int vmps_paged_decode_attention_cache8(
@@ -913,8 +1101,8 @@ extern "C" int vmps_paged_decode_attention_cache8(
   }
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
-  const Decode8Config cfg = configure8(num_seqs, n_q, n_kv, head_dim, sms);
-  if (static_cast<size_t>(cfg.n_cta) * 3 * cfg.hpc * sizeof(int) > kCounterBytes8) {
+  const Decode8Config cfg = configure8(num_seqs, n_q, n_kv, head_dim, max_blocks_per_seq, sms);
+  if (static_cast<size_t>(cfg.n_cta) * 3 * 2 * kParts8 * sizeof(int) > kCounterBytes8) {
     return fail(VMPS_ERR_UNSUPPORTED, "%s: %d SMs", what, sms);
   }
   if (!workspace || workspace_bytes < cfg.workspace) {
@@ -926,17 +1114,20 @@ extern "C" int vmps_paged_decode_attention_cache8(
   }
   int* err = nullptr;
   if (int rc = device_error_word(&err)) return rc;
-  // The cache as {d, token, kv head, (block, K|V)}: the box [D][16][hpc][2] lands as
-  // [K|V][head][token] rows of D bytes, their 16-byte chunks swizzled.
+  // The cache as {row, token, heads, (block, K|V)}, a row being 128 bytes of one head or,
+  // at head size 64, of two (half as many lines for the copy engine; 64 bytes where n_kv is
+  // odd): the box lands as [K|V][heads][token] rows, their 16-byte chunks swizzled.
   CUtensorMap tmap;
-  const uint64_t dims[4] = {(uint64_t)head_dim, (uint64_t)kCachePage, (uint64_t)n_kv,
+  const int per_row = head_dim == 64 && cfg.hpc % 2 == 0 ? 2 : 1;
+  const uint64_t row = (uint64_t)per_row * head_dim;
+  const uint64_t dims[4] = {row, (uint64_t)kCachePage, (uint64_t)n_kv / per_row,
                             (uint64_t)2 * num_blocks};
-  const uint64_t strides[3] = {(uint64_t)n_kv * head_dim, (uint64_t)head_dim,
+  const uint64_t strides[3] = {(uint64_t)n_kv * head_dim, row,
                                (uint64_t)kCachePage * n_kv * head_dim};
-  const uint32_t box[4] = {(uint32_t)head_dim, (uint32_t)kCachePage, (uint32_t)cfg.hpc, 2};
+  const uint32_t box[4] = {(uint32_t)row, (uint32_t)kCachePage, (uint32_t)(cfg.hpc / per_row), 2};
   if (int rc = encode_tiled(&tmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(codes), dims,
                             strides, box,
-                            head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B)) {
+                            row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B)) {
     return rc;
   }
   Decode8Params p;
@@ -957,7 +1148,7 @@ extern "C" int vmps_paged_decode_attention_cache8(
   p.scale_log2 = scale * 1.4426950408889634f;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.group_counters = reinterpret_cast<int*>(ws);
-  p.top_counters = p.group_counters + static_cast<size_t>(cfg.n_cta) * 2 * cfg.hpc;
+  p.top_counters = p.group_counters + static_cast<size_t>(cfg.n_cta) * 2 * 2 * kParts8;
   p.part_lse = reinterpret_cast<float*>(ws + cfg.lse_at);
   p.part_o = reinterpret_cast<float*>(ws + cfg.o_at);
   p.err = err;
