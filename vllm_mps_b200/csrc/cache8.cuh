@@ -11,6 +11,8 @@
 
 #include <cuda_fp8.h>
 
+#include <utility>
+
 #include "vmps_common.cuh"
 
 namespace vmps {
@@ -23,13 +25,15 @@ constexpr float kCache8Tiny = 7.888609052210118e-31f;  // 2^-100
 
 struct Int8Code {
   static constexpr float kTop = 127.f;
-  // Nearest integer, ties to even; |y| <= 127 (1 + 2^-22).
-  static __device__ __forceinline__ uint32_t code(float y) {
-    return static_cast<uint32_t>(__float2int_rn(y)) & 0xffu;
-  }
-  // Four codes at once, the first in the lowest byte.
-  static __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-    return code(a) | (code(b) << 8) | (code(c) << 16) | (code(d) << 24);
+  // Codes of four values times inv, the first in the lowest byte: the nearest integer, ties to
+  // even, is the low byte of 1.5 * 2^23 plus the product (at most 127 (1 + 2^-22)).
+  static __device__ __forceinline__ uint32_t pack4(float2 x, float2 y, float inv) {
+    constexpr float kBase = 12582912.f;
+    const uint32_t ab = __byte_perm(__float_as_uint(fmaf(x.x, inv, kBase)),
+                                    __float_as_uint(fmaf(x.y, inv, kBase)), 0x0040);
+    const uint32_t cd = __byte_perm(__float_as_uint(fmaf(y.x, inv, kBase)),
+                                    __float_as_uint(fmaf(y.y, inv, kBase)), 0x0040);
+    return __byte_perm(ab, cd, 0x5410);
   }
   static __device__ __forceinline__ void unpack4(uint32_t w, float (&x)[4]) {
 #pragma unroll
@@ -41,9 +45,11 @@ struct Int8Code {
 
 struct E4m3Code {
   static constexpr float kTop = 448.f;
-  static __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  static __device__ __forceinline__ uint32_t pack4(float2 x, float2 y, float inv) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x.x * inv, x.y * inv), __NV_SATFINITE,
+                                                 __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y.x * inv, y.y * inv), __NV_SATFINITE,
+                                                 __NV_E4M3);
     return lo | (hi << 16);
   }
   static __device__ __forceinline__ void unpack4(uint32_t w, float (&x)[4]) {
@@ -57,5 +63,30 @@ struct E4m3Code {
     }
   }
 };
+
+// The 8-bit cache's kernels are links of a chain of kernels launched with programmatic
+// dependent launch: each waits for what is before it on the stream before it reads
+// anything, and only then lets the next one start.
+__device__ __forceinline__ void chain_link() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// `early`: whether the launch may start before what is ahead of it has ended.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_link(void (*kernel)(KArgs...), bool early, dim3 grid, dim3 block, size_t smem,
+                        cudaStream_t s, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
 
 }  // namespace vmps

@@ -306,8 +306,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
     }
     fence_mbar_init();
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  chain_link();
 
   // ── the plan: lengths, prefix sums of their weights, this CTA's share ───────
   // Every thread owns `per` sequences; those in which the share begins and ends
@@ -1009,17 +1008,9 @@ int launch_decode8(const CUtensorMap& tmap, const Decode8Params& p, const Decode
     cudaFuncSetAttribute(decode8_kernel<T, D, NT, kInt8>,
                          cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem8);
   });
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(c.n_cta);
-  cfg.blockDim = dim3(32 * (kProducers8 + c.hpc * c.tg));
-  cfg.dynamicSmemBytes = c.smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, decode8_kernel<T, D, NT, kInt8>, tmap, p);
+  const cudaError_t e =
+      launch_link(decode8_kernel<T, D, NT, kInt8>, true, dim3(c.n_cta),
+                  dim3(32 * (kProducers8 + c.hpc * c.tg)), c.smem, s, tmap, p);
   if (e != cudaSuccess) {
     return fail(VMPS_ERR_CUDA, "paged_decode_attention_cache8: launch failed: %s", cudaGetErrorString(e));
   }

@@ -2,6 +2,8 @@
 //
 //   pool[dst][kv][t][h][d] = round(code * scale)   for the sequence's tokens,
 //   0 for the rest of its last page (attention over those pages reads them).
+//
+// What bounds it: the bytes read and written.
 #include "cache8.cuh"
 #include "vmps_abi_internal.h"
 
@@ -16,61 +18,93 @@ struct ReadParams {
   const int32_t* dst_tables;
   const int32_t* seq_lens;
   int max_blocks, n_kv, num_blocks, pool_blocks;
+  int pages;  // of a sequence per CTA
   int* err;
 };
 
+constexpr int kReadThreads = 256;
+constexpr int kReadResident = 6;  // blocks of an SM
+
+// A thread keeps to one 16-byte column of the page's rows (32 of them: K and V of 16
+// tokens; n_kv * D codes each), so that nothing is divided per row.  What hides the
+// loads is the number of blocks: 131071 tokens (8 heads x 128) take 133 us (6.1 TB/s
+// read and written), with four rows' loads in flight per thread, and fewer blocks, 160.
 template <typename T, int D, typename Code>
-__global__ void __launch_bounds__(256) read_cache8_kernel(const ReadParams p) {
+__global__ void __launch_bounds__(kReadThreads, kReadResident) read_cache8_kernel(const ReadParams p) {
+  chain_link();
   const int s = blockIdx.y;
-  const int page = blockIdx.x;
   const int len = p.seq_lens[s];
-  if (len <= 0 || page > (len - 1) / kCachePage) return;
-  if ((len - 1) / kCachePage >= p.max_blocks && page == 0 && threadIdx.x == 0) {
+  const int page0 = blockIdx.x * p.pages;
+  if (len <= 0 || page0 > (len - 1) / kCachePage) return;
+  int page1 = min(page0 + p.pages, (len - 1) / kCachePage + 1);
+  if (page1 > p.max_blocks) page1 = p.max_blocks;
+  if ((len - 1) / kCachePage >= p.max_blocks && page0 == 0 && threadIdx.x == 0) {
     set_error(p.err, kDevErrSeqLen);
   }
-  const int64_t at = static_cast<int64_t>(s) * p.max_blocks + page;
-  const int src = p.block_tables[at], dst = p.dst_tables[at];
-  if (src < 0 || src >= p.num_blocks || dst < 0 || dst >= p.pool_blocks) {
-    if (threadIdx.x == 0) set_error(p.err, kDevErrBlockRange);
-    return;
-  }
-  const int per_kind = kCachePage * p.n_kv * D;
-  const int live = len - page * kCachePage;  // tokens of this page
-  const uint8_t* codes = p.codes + static_cast<int64_t>(src) * 2 * per_kind;
-  const float* scales = p.scales + static_cast<int64_t>(src) * 2 * p.n_kv * kCachePage;
-  T* out = static_cast<T*>(p.pool) + static_cast<int64_t>(dst) * 2 * per_kind;
-  for (int e = threadIdx.x * 8; e < 2 * per_kind; e += blockDim.x * 8) {
-    const int kind = e >= per_kind;
-    const int row = (e - kind * per_kind) / D;  // token * n_kv + head
-    const int t = row / p.n_kv, h = row % p.n_kv;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (t < live) {
-      const uint2 w = *reinterpret_cast<const uint2*>(codes + e);
-      const float sc = scales[(h * 2 + kind) * kCachePage + t];
-      float a[4], b[4];
-      Code::unpack4(w.x, a);
-      Code::unpack4(w.y, b);
+  const int row_codes = p.n_kv * D;
+  const int columns = row_codes / 16;
+  // Columns a pass, and rows of each at once.
+  const int width = min(columns, kReadThreads);
+  const int rows = kReadThreads / width;
+  const int c0 = threadIdx.x % width, r0 = threadIdx.x / width;
+  if (r0 >= rows) return;
+  for (int page = page0; page < page1; ++page) {
+    const int64_t at = static_cast<int64_t>(s) * p.max_blocks + page;
+    const int src = p.block_tables[at], dst = p.dst_tables[at];
+    if (src < 0 || src >= p.num_blocks || dst < 0 || dst >= p.pool_blocks) {
+      if (threadIdx.x == 0) set_error(p.err, kDevErrBlockRange);
+      continue;
+    }
+    const int live = len - page * kCachePage;  // tokens from this page on
+    for (int c = c0; c < columns; c += width) {
+      const int64_t block = static_cast<int64_t>(2 * kCachePage) * row_codes;
+      const uint8_t* codes = p.codes + src * block + c * 16;
+      const float* scales =
+          p.scales + (static_cast<int64_t>(src) * p.n_kv + c * 16 / D) * 2 * kCachePage;
+      T* out = static_cast<T*>(p.pool) + dst * block + c * 16;
+      for (int r = r0; r < 2 * kCachePage; r += rows) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);  // K's 16 tokens, then V's: the scales' order too
+        float sc = 0.f;
+        if (r % kCachePage < live) {
+          w = __ldcs(reinterpret_cast<const uint4*>(codes + static_cast<int64_t>(r) * row_codes));
+          sc = scales[r];
+        }
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+        uint32_t o[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = a[i] * sc;
-        x[4 + i] = b[i] * sc;
+        for (int i = 0; i < 4; ++i) {
+          float x[4];
+          Code::unpack4(v[i], x);
+          o[2 * i] = Elt<T>::pack(x[0] * sc, x[1] * sc);
+          o[2 * i + 1] = Elt<T>::pack(x[2] * sc, x[3] * sc);
+        }
+        uint4* dst4 = reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * row_codes);
+        dst4[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        dst4[1] = make_uint4(o[4], o[5], o[6], o[7]);
       }
     }
-    *reinterpret_cast<uint4*>(out + e) =
-        make_uint4(Elt<T>::pack(x[0], x[1]), Elt<T>::pack(x[2], x[3]), Elt<T>::pack(x[4], x[5]),
-                   Elt<T>::pack(x[6], x[7]));
   }
 }
 
 template <typename T, int D>
-int launch_read(const ReadParams& p, int num_seqs, int format, cudaStream_t s) {
-  const dim3 grid(p.max_blocks, num_seqs);
-  if (format == VMPS_CACHE_INT8) {
-    read_cache8_kernel<T, D, Int8Code><<<grid, 256, 0, s>>>(p);
-  } else {
-    read_cache8_kernel<T, D, E4m3Code><<<grid, 256, 0, s>>>(p);
+int launch_read(ReadParams p, int num_seqs, int format, cudaStream_t s) {
+  // One page a CTA, more where the tables are wide: a CTA without pages costs a launch slot.
+  const int64_t all = static_cast<int64_t>(p.max_blocks) * num_seqs;
+  p.pages = static_cast<int>((all + 16383) / 16384);
+  const dim3 grid((p.max_blocks + p.pages - 1) / p.pages, num_seqs);
+  int sms = 0;
+  if (int rc = device_sm_count(&sms)) return rc;
+  // An early start saves small calls half a microsecond (4 pages 3.9 -> 3.5 us), but costs
+  // grids of several waves (512 pages of 8 heads x 128, 2048 CTAs' worth of rows: 13 -> 17).
+  const bool early = static_cast<int64_t>(grid.x) * grid.y <= kReadResident * sms;
+  const cudaError_t e =
+      format == VMPS_CACHE_INT8
+          ? launch_link(read_cache8_kernel<T, D, Int8Code>, early, grid, dim3(kReadThreads), 0, s, p)
+          : launch_link(read_cache8_kernel<T, D, E4m3Code>, early, grid, dim3(kReadThreads), 0, s, p);
+  if (e != cudaSuccess) {
+    return fail(VMPS_ERR_CUDA, "read_cache8: launch failed: %s", cudaGetErrorString(e));
   }
-  return check_launch("read_cache8");
+  return VMPS_OK;
 }
 
 }  // namespace
@@ -115,7 +149,7 @@ extern "C" int vmps_read_cache8(void* pool, int pool_blocks, const int32_t* dst_
   if (int rc = device_error_word(&err)) return rc;
   ReadParams p{pool,     static_cast<const uint8_t*>(codes), scales, block_tables, dst_tables,
                seq_lens, max_blocks_per_seq,                 n_kv,   num_blocks,   pool_blocks,
-               err};
+               1,        err};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == VMPS_DTYPE_F16) {
     return head_dim == 64 ? launch_read<__half, 64>(p, num_seqs, cache_format, s)

@@ -1006,7 +1006,7 @@ class KVCache8:
     stored value is ``code * scale``.
     """
 
-    __slots__ = ("codes", "scales", "format")
+    __slots__ = ("codes", "scales", "format", "num_blocks", "n_kv", "head_dim")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
         shape = codes.shape
@@ -1020,6 +1020,7 @@ class KVCache8:
                 or not scales.is_contiguous():
             raise ValueError(f"scales must be contiguous float32 ({shape[0]}, {shape[3]}, 2, 16)")
         self.codes, self.scales, self.format = codes, scales, fmt
+        self.num_blocks, _, _, self.n_kv, self.head_dim = shape
 
     @classmethod
     def zeros(cls, num_blocks: int, n_kv: int, d: int, dtype: torch.dtype = torch.int8,
@@ -1052,17 +1053,20 @@ def quantize_cache8(x: torch.Tensor, dtype: torch.dtype = torch.int8,
     return codes, torch.where(some, amax / top, torch.where(fine, 0.0, float("nan")))
 
 
-def _head_rows(t: torch.Tensor, d: int, name: str) -> tuple[int, int]:
-    """(heads, row stride) of (B, heads, d) or (B, heads * d) rows with packed heads."""
+def _head_rows(t: torch.Tensor, d: int, name: str) -> tuple[int, int, int]:
+    """(rows, heads, row stride) of (rows, heads, d) or (rows, heads * d) with packed heads."""
     shape, stride = t.shape, t.stride()
-    if len(shape) == 3 and shape[2] == d and stride[2] == 1 and (stride[1] == d or shape[1] <= 1):
-        heads = shape[1]
-    elif len(shape) == 2 and shape[1] % d == 0 and stride[1] == 1:
-        heads = shape[1] // d
+    if len(shape) == 2 and shape[1] % d == 0 and stride[1] == 1:
+        rows, heads = shape[0], shape[1] // d
+    elif len(shape) == 3 and shape[2] == d and stride[2] == 1 and (stride[1] == d or shape[1] <= 1):
+        rows, heads, _ = shape
     else:
         raise ValueError(f"{name} must be (rows, heads, {d}) or (rows, heads * {d}) with packed heads")
     # torch gives a single row any stride; the kernel never steps by it.
-    return heads, stride[0] if shape[0] > 1 else heads * d
+    return rows, heads, stride[0] if rows > 1 else heads * d
+
+
+_INT32, _FLOAT32 = torch.int32, torch.float32
 
 
 def norm_rope_and_cache(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
@@ -1083,62 +1087,69 @@ def norm_rope_and_cache(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
     negative slot caches nothing.  Returns ``q_out`` (rows, n_q, D), a new
     tensor unless given (``q`` itself works).
     """
-    eight = type(cache) is KVCache8
-    pool = cache.codes if eight else cache
-    shape = pool.shape
-    if not eight and (len(shape) != 5 or shape[1] != 2 or not pool.is_contiguous()):
-        _check_pool(pool)
-    num_blocks, _, block_size, n_kv, D = shape
+    if type(cache) is KVCache8:
+        pool, scales, fmt = cache.codes, cache.scales, cache.format
+        num_blocks, n_kv, D = cache.num_blocks, cache.n_kv, cache.head_dim
+        block_size = 16
+    else:
+        pool, scales, fmt = cache, None, VMPS_CACHE_16BIT
+        num_blocks, block_size, n_kv, D = _check_pool(pool)
     dtype = k.dtype
     if v.dtype != dtype or (q is not None and q.dtype != dtype) or \
-            (not eight and pool.dtype != dtype):
+            (scales is None and pool.dtype != dtype):
         raise TypeError("q, k, v and a 16-bit pool must have one dtype")
-    rows = k.shape[0]
-    heads, ks = _head_rows(k, D, "k")
-    v_heads, vs = _head_rows(v, D, "v")
-    if heads != n_kv or v_heads != n_kv or v.shape[0] != rows:
+    rows, heads, ks = _head_rows(k, D, "k")
+    v_rows, v_heads, vs = _head_rows(v, D, "v")
+    if heads != n_kv or v_heads != n_kv or v_rows != rows:
         raise ValueError(f"k and v must have {n_kv} heads and the same rows")
     n_q = qs = os_ = 0
     q_ptr = o_ptr = None
     if q is not None:
-        n_q, qs = _head_rows(q, D, "q")
-        if q.shape[0] != rows:
+        q_rows, n_q, qs = _head_rows(q, D, "q")
+        if q_rows != rows:
             raise ValueError("q must have k's rows")
+        q_ptr = q.data_ptr()
         if q_out is None:
             q_out = q.new_empty((rows, n_q, D))
-            os_ = n_q * D
+            o_ptr, os_ = q_out.data_ptr(), n_q * D
         else:
-            o_heads, os_ = _head_rows(q_out, D, "q_out")
-            if o_heads != n_q or q_out.shape[0] != rows or q_out.dtype != dtype:
+            o_rows, o_heads, os_ = _head_rows(q_out, D, "q_out")
+            if o_heads != n_q or o_rows != rows or q_out.dtype != dtype:
                 raise ValueError("q_out must have q's shape and dtype")
-            if q_out.data_ptr() == q.data_ptr() and os_ != qs:
+            o_ptr = q_out.data_ptr()
+            if o_ptr == q_ptr and os_ != qs:
                 raise ValueError("q_out in q's place must have its row stride")
-        q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
-    _lengths(rows, slot_mapping=slot_mapping)
+    if slot_mapping.dtype != _INT32 or slot_mapping.numel() != rows or not slot_mapping.is_contiguous():
+        _lengths(rows, slot_mapping=slot_mapping)
+    pos_ptr = inv_ptr = qw_ptr = kw_ptr = None
     if inv_freq is not None:
-        if inv_freq.dtype != torch.float32 or inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
+        if inv_freq.dtype != _FLOAT32 or inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
             raise ValueError(f"inv_freq must be contiguous float32 of {D // 2} entries")
         if positions is None:
             raise ValueError("inv_freq needs positions")
+        inv_ptr = inv_freq.data_ptr()
     if positions is not None:
-        _lengths(rows, positions=positions)
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.dtype != dtype or w.numel() != D or not w.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous ({D},) of the rows' dtype")
-    scales = cache.scales if eight else None
+        if positions.dtype != _INT32 or positions.numel() != rows or not positions.is_contiguous():
+            _lengths(rows, positions=positions)
+        pos_ptr = positions.data_ptr()
+    if q_weight is not None:
+        if q_weight.dtype != dtype or q_weight.numel() != D or not q_weight.is_contiguous():
+            raise ValueError(f"q_weight must be contiguous ({D},) of the rows' dtype")
+        qw_ptr = q_weight.data_ptr()
+    if k_weight is not None:
+        if k_weight.dtype != dtype or k_weight.numel() != D or not k_weight.is_contiguous():
+            raise ValueError(f"k_weight must be contiguous ({D},) of the rows' dtype")
+        kw_ptr = k_weight.data_ptr()
     dev = _device_index(k, v, q, q_out, positions, slot_mapping, inv_freq, pool, scales, q_weight,
                         k_weight)
     lib = _lib or load_library()
     rc = _launch(lib.vmps_norm_rope_and_cache, dev,
-                 o_ptr, os_, q_ptr, qs, k.data_ptr(), ks, v.data_ptr(), vs,
-                 None if q_weight is None else q_weight.data_ptr(),
-                 None if k_weight is None else k_weight.data_ptr(), eps,
-                 None if positions is None else positions.data_ptr(), slot_mapping.data_ptr(),
-                 None if inv_freq is None else inv_freq.data_ptr(), pool.data_ptr(),
+                 o_ptr, os_, q_ptr, qs, k.data_ptr(), ks, v.data_ptr(), vs, qw_ptr, kw_ptr, eps,
+                 pos_ptr, slot_mapping.data_ptr(), inv_ptr, pool.data_ptr(),
                  None if scales is None else scales.data_ptr(), rows, n_q, n_kv, D, block_size,
-                 num_blocks, cache.format if eight else VMPS_CACHE_16BIT, dtype_code(dtype))
+                 num_blocks, fmt, dtype_code(dtype))
     if rc:
         _check(rc, "norm_rope_and_cache")
     return q_out
@@ -1156,24 +1167,23 @@ def read_cache8(cache: KVCache8, block_tables: torch.Tensor, seq_lens: torch.Ten
     and its tables.  Both tables int32 (B, max_blocks), no block twice in
     ``dst_tables``.  Returns ``pool``.
     """
-    codes = cache.codes
-    num_blocks, _, block_size, n_kv, D = codes.shape
+    codes, scales, n_kv, D = cache.codes, cache.scales, cache.n_kv, cache.head_dim
     shape = pool.shape
     if len(shape) != 5 or shape[1:] != codes.shape[1:] or not pool.is_contiguous():
         raise ValueError(f"pool must be contiguous (blocks, 2, 16, {n_kv}, {D}); got {tuple(shape)}")
     B = seq_lens.numel()
-    if block_tables.dim() != 2 or block_tables.shape[0] != B or dst_tables.shape != block_tables.shape:
+    tables = block_tables.shape
+    if len(tables) != 2 or tables[0] != B or dst_tables.shape != tables:
         raise ValueError("block_tables and dst_tables must be (B, max_blocks)")
     _lengths(B, seq_lens=seq_lens)
     _int32(block_tables, "block_tables")
     _int32(dst_tables, "dst_tables")
-    dev = _device_index(codes, cache.scales, block_tables, seq_lens, pool, dst_tables)
+    dev = _device_index(codes, scales, block_tables, seq_lens, pool, dst_tables)
     lib = _lib or load_library()
     rc = _launch(lib.vmps_read_cache8, dev,
                  pool.data_ptr(), shape[0], dst_tables.data_ptr(), codes.data_ptr(),
-                 cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.shape[1],
-                 seq_lens.data_ptr(), B, n_kv, D, block_size, num_blocks, cache.format,
-                 dtype_code(pool.dtype))
+                 scales.data_ptr(), block_tables.data_ptr(), tables[1], seq_lens.data_ptr(), B,
+                 n_kv, D, 16, cache.num_blocks, cache.format, dtype_code(pool.dtype))
     if rc:
         _check(rc, "read_cache8")
     return pool
@@ -1197,10 +1207,15 @@ def _cache8_workspace_bytes(device: int, num_seqs: int, n_q: int, n_kv: int, d: 
 _CACHE8_COUNTER_BYTES = 128 << 10
 #: Zeroed workspaces of eager calls that bring none, one per device and stream.
 _cache8_buffers: dict[tuple[int, int], torch.Tensor] = {}
+#: Their sizes: one for a device, head size and 8 or 16 query heads a kv head.
+_cache8_sizes: dict[tuple[int, int, bool], int] = {}
 
 
 def _cache8_workspace(ref: torch.Tensor, dev: int, B: int, n_q: int, n_kv: int, d: int) -> torch.Tensor:
-    need = _cache8_workspace_bytes(dev, B, n_q, n_kv, d)
+    size = (dev, d, n_q > 8 * n_kv)
+    need = _cache8_sizes.get(size)
+    if need is None:
+        need = _cache8_sizes[size] = _cache8_workspace_bytes(dev, B, n_q, n_kv, d)
     if torch.cuda.is_current_stream_capturing():
         # A graph's own: it may be replayed while other calls or graphs run.
         buf = ref.new_empty(need, dtype=torch.uint8)
@@ -1229,20 +1244,20 @@ def paged_decode_attention_cache8(q: torch.Tensor, cache: KVCache8, block_tables
     to the current stream, or to the graph being captured.  Returns ``out``
     (B, n_q, D) of q's dtype.
     """
-    codes = cache.codes
-    num_blocks, _, block_size, n_kv, D = codes.shape
-    n_q, qs = _head_rows(q, D, "q")
-    B = q.shape[0]
-    if block_tables.dim() != 2 or block_tables.shape[0] != B:
+    codes, scales, n_kv, D = cache.codes, cache.scales, cache.n_kv, cache.head_dim
+    B, n_q, qs = _head_rows(q, D, "q")
+    tables = block_tables.shape
+    if len(tables) != 2 or tables[0] != B:
         raise ValueError("block_tables must be (B, max_blocks)")
-    _lengths(B, seq_lens=seq_lens)
+    if seq_lens.dtype != _INT32 or seq_lens.numel() != B or not seq_lens.is_contiguous():
+        _lengths(B, seq_lens=seq_lens)
     _int32(block_tables, "block_tables")
+    dtype = q.dtype
     if out is None:
         out = q.new_empty((B, n_q, D))
-    elif out.shape != (B, n_q, D) or out.dtype != q.dtype or not out.is_contiguous():
+    elif out.shape != (B, n_q, D) or out.dtype != dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous (B, n_q, D) tensor of q's dtype")
-    dev = _device_index(q, codes, cache.scales, block_tables, seq_lens, out)
-    code = dtype_code(q.dtype)
+    dev = _device_index(q, codes, scales, block_tables, seq_lens, out)
     if B == 0:
         return out
     if workspace is None:
@@ -1251,14 +1266,13 @@ def paged_decode_attention_cache8(q: torch.Tensor, cache: KVCache8, block_tables
         workspace = workspace.get_cache8(q.device, B, n_q, n_kv, D)
     elif workspace.get_device() != dev:
         _require_cuda(q, workspace)
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
     lib = _lib or load_library()
     rc = _launch(lib.vmps_paged_decode_attention_cache8, dev,
-                 out.data_ptr(), q.data_ptr(), qs, codes.data_ptr(), cache.scales.data_ptr(),
-                 block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(), B, n_q, n_kv,
-                 D, block_size, num_blocks, scale, workspace.data_ptr(),
-                 workspace.numel() * workspace.element_size(), cache.format, code)
+                 out.data_ptr(), q.data_ptr(), qs, codes.data_ptr(), scales.data_ptr(),
+                 block_tables.data_ptr(), tables[1], seq_lens.data_ptr(), B, n_q, n_kv, D, 16,
+                 cache.num_blocks, 1.0 / math.sqrt(D) if scale is None else scale,
+                 workspace.data_ptr(), workspace.numel() * workspace.element_size(), cache.format,
+                 dtype_code(dtype))
     if rc:
         _check(rc, "paged_decode_attention_cache8")
     return out
