@@ -128,13 +128,16 @@ class DecodeGraphRunner:
 
         m = self.adapter.hf_model
         nl = len(m.model.layers)
+        # A layer's decode step: one kernel, or the write and the attention.
+        steps = sum(1 if getattr(layer.self_attn, "fused_step", True) else 2
+                    for layer in m.model.layers)
         if self._gate_up is None:
-            return nl  # the decode-step kernel; the rest is HF modules
+            return steps  # the decode-step kernel; the rest is HF modules
         Bb = self.bucket(batch) or batch
         d = self.adapter.model_config.d_model
         a0 = m.model.layers[0].self_attn
         # decode step; residual + RMSNorm twice a layer; embedding + the first RMSNorm
-        n = nl + 2 * nl + 1
+        n = steps + 2 * nl + 1
         n += nl * (K.decode_gemm_supported(Bb, a0._w_qkv.shape[0], d)
                    + K.decode_gemm_supported(Bb, d, a0.W_O.in_features))
         n += nl  # the [gate|up] decode GEMM with SiLU * up, or silu_mul after cuBLAS

@@ -17,6 +17,10 @@ Two modes:
   context.  ``swap=True`` also copies preempted blocks to pinned host memory
   and back (the reference's swap moves metadata only).
 
+``kv_cache="int8"`` or ``"fp8"`` (physical mode) keeps K and V as 8-bit codes
+with a scale per token and head: half the memory per block and half the
+bytes a decode step reads.
+
 Per step the decode batch runs every layer with one fused sm_100a attention
 kernel; on CUDA the step is a CUDA graph captured per batch bucket
 (``engine/decode_graph.py``, ``cuda_graphs=True``), else an eager HF forward.
@@ -49,7 +53,7 @@ from vllm_mps_b200.core.kv_cache_manager import KVCacheManager
 from vllm_mps_b200.core.model_config import ModelConfig
 from vllm_mps_b200.core.sequence import SamplingParams, Sequence, SequenceGroup, SequenceStatus
 from vllm_mps_b200.engine.scheduler import Scheduler
-from vllm_mps_b200.memory.cuda_memory_pool import CUDAMemoryPool, SwapSpace
+from vllm_mps_b200.memory.cuda_memory_pool import CUDACache8Pool, CUDAMemoryPool, SwapSpace
 from vllm_mps_b200.model.sampler import Sampler
 
 logger = logging.getLogger(__name__)
@@ -98,18 +102,28 @@ class LLMEngine:
                    dtype: torch.dtype | None = None,
                    device: torch.device | str | None = None,
                    max_prefill_rows: int = 8192, cuda_graphs: bool = True,
-                   pipeline: bool = False) -> "LLMEngine":
+                   pipeline: bool = False, kv_cache: str | None = None) -> "LLMEngine":
         from vllm_mps_b200.models.llama_adapter import LlamaAdapter
 
         if mode not in ("compat", "physical"):
             raise ValueError(f"mode must be 'compat' or 'physical', got {mode!r}")
+        if kv_cache not in (None, "int8", "fp8"):
+            raise ValueError(f"kv_cache must be None, 'int8' or 'fp8', got {kv_cache!r}")
+        if kv_cache is not None and mode != "physical":
+            raise ValueError("kv_cache='int8'/'fp8' needs mode='physical'")
         cfg = model_config or ModelConfig.from_hf_config(hf_model.config, model_name, dtype, device)
         if dtype is not None:
             cfg.dtype = dtype
         if device is not None:
             cfg.device = torch.device(device)
-        pool = CUDAMemoryPool(num_gpu_blocks, BLOCK_SIZE, cfg.n_kv_heads, cfg.d_k, cfg.dtype,
-                              cfg.device, num_layers=cfg.n_layers if mode == "physical" else None)
+        layers = cfg.n_layers if mode == "physical" else None
+        if kv_cache is None:
+            pool = CUDAMemoryPool(num_gpu_blocks, BLOCK_SIZE, cfg.n_kv_heads, cfg.d_k, cfg.dtype,
+                                  cfg.device, num_layers=layers)
+        else:
+            code = torch.int8 if kv_cache == "int8" else torch.float8_e4m3fn
+            pool = CUDACache8Pool(num_gpu_blocks, BLOCK_SIZE, cfg.n_kv_heads, cfg.d_k, cfg.dtype,
+                                  cfg.device, num_layers=layers, code_dtype=code)
         swap_space = SwapSpace(pool, num_cpu_blocks) if swap else None
         kv = KVCacheManager(num_gpu_blocks, num_cpu_blocks, swap_space=swap_space)
 

@@ -66,6 +66,8 @@ class TreeDecoder:
                 layer.mlp.down_proj.bias is not None or layer.self_attn.W_O.bias is not None
                 for layer in model.model.layers):
             raise ValueError("TreeDecoder needs projections without bias")
+        if model.model.layers[0].self_attn.eight_bit:
+            raise ValueError("TreeDecoder needs a 16-bit cache (an engine without kv_cache)")
         self.engine = engine
         self.tree = DraftTree.from_widths(tuple(widths))
         if len(self.tree) > 1024:
@@ -128,9 +130,8 @@ class TreeDecoder:
             a = layer.self_attn
             qkv = weights.project(i, "qkv", h)
             nq, nkv = a.n_heads * a.d_k, a.n_kv_heads * a.d_k
-            q = K.rope_reshape_and_cache(qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:],
-                                         meta["pos"], meta["slots"], a.rotary_emb.inv_freq,
-                                         pool.layer(i))
+            q = a.store(qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:], meta["pos"],
+                        meta["slots"])
             out = K.paged_tree_attention(q.unflatten(1, (a.n_heads, a.d_k)), pool.layer(i),
                                          meta["bt"], meta["ctx"], meta["lens"], meta["q_lens"],
                                          meta["cu"], meta["mask"], meta["max_q"],

@@ -12,6 +12,10 @@ reference runs as per-sequence Python loops (:275-359) or as a Metal shader
 -- is one call into the sm_100a kernel (``kernels.paged_decode_step``).  Q, K
 and V come from one fused projection GEMM and are passed as strided slices
 of its output, so nothing is copied or materialised.  There is no CPU path.
+
+Layers with norms of queries and keys per head (``q_norm``/``k_norm`` modules
+of head_dim weights) and pools of 8-bit codes take two kernels for the step:
+``kernels.norm_rope_and_cache``, then the attention over what it wrote.
 """
 
 from __future__ import annotations
@@ -35,7 +39,8 @@ class PagedAttentionLayer(nn.Module):
 
     def __init__(self, layer_idx: int, model_config: ModelConfig, kv_cache_manager: KVCacheManager,
                  memory_pool, W_Q: nn.Linear, W_K: nn.Linear, W_V: nn.Linear, W_O: nn.Linear,
-                 rotary_emb: RotaryEmbedding) -> None:
+                 rotary_emb: RotaryEmbedding, q_norm: torch.Tensor | None = None,
+                 k_norm: torch.Tensor | None = None, norm_eps: float = 1e-6) -> None:
         super().__init__()
         self.layer_idx = layer_idx
         self.model_config = model_config
@@ -55,6 +60,10 @@ class PagedAttentionLayer(nn.Module):
         # One GEMM for Q, K and V: rows [W_Q; W_K; W_V].
         self.register_buffer("_w_qkv", torch.cat([W_Q.weight, W_K.weight, W_V.weight], 0).detach(),
                              persistent=False)
+        # Norms of each head of q and k: weights (head_dim,), or None.
+        self.register_buffer("q_norm_weight", q_norm, persistent=False)
+        self.register_buffer("k_norm_weight", k_norm, persistent=False)
+        self.norm_eps = norm_eps
         self._workspace = None
 
     @classmethod
@@ -78,7 +87,26 @@ class PagedAttentionLayer(nn.Module):
         W_V = lin(srcs[2], n_kv * D, d)
         W_O = lin(srcs[3], d, n_q * D)
         rot = RotaryEmbedding(D, model_config.max_seq_len, model_config.rope_theta, dev)
-        return cls(layer_idx, model_config, kv_cache_manager, memory_pool, W_Q, W_K, W_V, W_O, rot)
+        q_norm, k_norm, eps = cls._head_norms(layer, D)
+        on = lambda w: None if w is None else w.detach().to(device=dev, dtype=dt).contiguous()  # noqa: E731
+        return cls(layer_idx, model_config, kv_cache_manager, memory_pool, W_Q, W_K, W_V, W_O, rot,
+                   on(q_norm), on(k_norm), eps)
+
+    @staticmethod
+    def _head_norms(layer, d: int):
+        """(q weight, k weight, eps) of an attention module's norms over each head, if it has them."""
+        if isinstance(layer, PagedAttentionLayer):
+            return layer.q_norm_weight, layer.k_norm_weight, layer.norm_eps
+        weights, eps = [], 1e-6
+        for name in ("q_norm", "k_norm"):
+            norm = getattr(layer, name, None)
+            w = getattr(norm, "weight", None)
+            if w is None or w.numel() != d:
+                weights.append(None)
+                continue
+            weights.append(w)
+            eps = float(getattr(norm, "variance_epsilon", getattr(norm, "eps", None) or eps))
+        return weights[0], weights[1], eps
 
     # ── forward ─────────────────────────────────────────────────────────────
 
@@ -90,8 +118,34 @@ class PagedAttentionLayer(nn.Module):
                                        _batch_context.positions, _batch_context.seq_lens)
         return self._forward_single(hidden_states)
 
-    def _pool(self) -> torch.Tensor:
+    def _pool(self):
+        """This layer's pool tensor, or its ``KVCache8``."""
         return self.memory_pool.layer(self.layer_idx)
+
+    @property
+    def eight_bit(self) -> bool:
+        """Whether the pool holds 8-bit codes."""
+        return hasattr(self.memory_pool, "code_dtype")
+
+    @property
+    def fused_step(self) -> bool:
+        """Whether a decode step's rotation, write and attention are one kernel."""
+        return not (self.eight_bit or self.q_norm_weight is not None
+                    or self.k_norm_weight is not None)
+
+    def store(self, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+              positions: torch.Tensor, slot_mapping: torch.Tensor,
+              in_place: bool = True) -> torch.Tensor | None:
+        """Norms and rotation of q and k; k and v into their slots.  Returns q, rotated in
+        its place or (layers without the fused step) in a tensor of its own."""
+        from vllm_mps_b200.kernels import norm_rope_and_cache, rope_reshape_and_cache
+
+        if self.fused_step:
+            return rope_reshape_and_cache(q, k, v, positions, slot_mapping,
+                                          self.rotary_emb.inv_freq, self._pool())
+        return norm_rope_and_cache(q, k, v, positions, slot_mapping, self.rotary_emb.inv_freq,
+                                   self._pool(), self.q_norm_weight, self.k_norm_weight,
+                                   self.norm_eps, q_out=q if in_place else None)
 
     def _workspace_buf(self):
         if self._workspace is None:
@@ -115,7 +169,8 @@ class PagedAttentionLayer(nn.Module):
 
     def _attend(self, hidden_states: torch.Tensor, meta) -> torch.Tensor:
         """Fused QKV GEMM -> one decode-step kernel -> W_O, for (B, 1, d_model)."""
-        from vllm_mps_b200.kernels import paged_decode_step
+        from vllm_mps_b200.kernels import (paged_decode_attention, paged_decode_attention_cache8,
+                                           paged_decode_step)
 
         B = hidden_states.shape[0]
         n_q, n_kv, D = self.n_heads, self.n_kv_heads, self.d_k
@@ -123,10 +178,19 @@ class PagedAttentionLayer(nn.Module):
         q = qkv[:, : n_q * D].view(B, n_q, D)
         k = qkv[:, n_q * D: (n_q + n_kv) * D]
         v = qkv[:, (n_q + n_kv) * D:]
-        out = paged_decode_step(q, k, v, meta.pos_tensor, meta.slot_mapping,
-                                self.rotary_emb.inv_freq, self._pool(), meta.bt_tensor,
-                                meta.sl_tensor, scale=1.0 / math.sqrt(D),
-                                workspace=self._workspace_buf())
+        if self.fused_step:
+            out = paged_decode_step(q, k, v, meta.pos_tensor, meta.slot_mapping,
+                                    self.rotary_emb.inv_freq, self._pool(), meta.bt_tensor,
+                                    meta.sl_tensor, scale=1.0 / math.sqrt(D),
+                                    workspace=self._workspace_buf())
+        else:
+            q = self.store(q, k, v, meta.pos_tensor, meta.slot_mapping, in_place=False)
+            if self.eight_bit:
+                out = paged_decode_attention_cache8(q, self._pool(), meta.bt_tensor, meta.sl_tensor,
+                                                    workspace=self._workspace_buf())
+            else:
+                out = paged_decode_attention(q, self._pool(), meta.bt_tensor, meta.sl_tensor,
+                                             workspace=self._workspace_buf())
         if self.W_O.bias is None:
             return self.project(out.view(B, n_q * D), self.W_O.weight).view(B, 1, -1)
         return self.W_O(out.view(B, 1, n_q * D))
@@ -138,14 +202,16 @@ class PagedAttentionLayer(nn.Module):
         rotated K and V of all rows into their slots; kernel 3 (tcgen05 causal
         prefill) then computes every row against its sequence's slots
         ``0..position`` -- the result of the reference's token-by-token
-        single-token path (:175-241) for the whole chunk at once.
+        single-token path (:175-241) for the whole chunk at once.  Over 8-bit
+        codes the chunk's sequences are read back into 16-bit pages first, so
+        a row attends to the values that later steps will read.
 
         ``hidden_states`` may carry padding rows after the chunk's
         ``meta.rows`` rows (a caller that rounds the GEMMs' row count): the
         projections run on every row, kernels 1 and 3 on the chunk's rows
         only, and the padding rows of the result are not meaningful.
         """
-        from vllm_mps_b200.kernels import paged_prefill_attention, rope_reshape_and_cache
+        from vllm_mps_b200.kernels import paged_prefill_attention
 
         B = hidden_states.shape[0]
         R = meta.rows
@@ -154,13 +220,16 @@ class PagedAttentionLayer(nn.Module):
         q = qkv[:R, : n_q * D]
         k = qkv[:R, n_q * D: (n_q + n_kv) * D]
         v = qkv[:R, (n_q + n_kv) * D:]
-        rope_reshape_and_cache(q, k, v, meta.pos_tensor, meta.slot_mapping,
-                               self.rotary_emb.inv_freq, self._pool())
+        self.store(q, k, v, meta.pos_tensor, meta.slot_mapping)
+        pool, tables = self._pool(), meta.bt_tensor
+        if self.eight_bit:
+            pool, tables = self.memory_pool.read_back(self.layer_idx, meta.bt_tensor, meta.kv_lens,
+                                                      meta.dst_tensor, meta.pages), meta.dst_tensor
         out = torch.empty((B, n_q * D), dtype=qkv.dtype, device=qkv.device)
         if B > R:
             out[R:].zero_()
-        paged_prefill_attention(q.view(R, n_q, D), self._pool(), meta.bt_tensor, meta.q_start,
-                                meta.q_lens, meta.cu_q, meta.max_q_len, scale=1.0 / math.sqrt(D),
+        paged_prefill_attention(q.view(R, n_q, D), pool, tables, meta.q_start, meta.q_lens,
+                                meta.cu_q, meta.max_q_len, scale=1.0 / math.sqrt(D),
                                 out=out[:R].view(R, n_q, D))
         return self.W_O(out.view(B, 1, n_q * D))
 
@@ -169,13 +238,11 @@ class PagedAttentionLayer(nn.Module):
         and kernel 1's write of every row's rotated K and V (no query, no
         attention).  The last layer of a prefill needs nothing more: no later
         layer reads its output."""
-        from vllm_mps_b200.kernels import rope_reshape_and_cache
-
         B, R = hidden_states.shape[0], meta.rows
         n_q, n_kv, D = self.n_heads, self.n_kv_heads, self.d_k
         kv = torch.matmul(hidden_states.reshape(B, self.d_model), self._w_qkv[n_q * D:].t())
-        rope_reshape_and_cache(None, kv[:R, : n_kv * D], kv[:R, n_kv * D:], meta.pos_tensor,
-                               meta.slot_mapping, self.rotary_emb.inv_freq, self._pool())
+        self.store(None, kv[:R, : n_kv * D], kv[:R, n_kv * D:], meta.pos_tensor,
+                   meta.slot_mapping)
 
     def _forward_batch(self, hidden_states: torch.Tensor, seq_ids: list[int],
                        positions: list[int], seq_lens: list[int]):

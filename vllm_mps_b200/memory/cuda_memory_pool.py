@@ -16,6 +16,9 @@ the layout the sm_100a kernels read with TMA.  The method set and the
 ``gather_*``/``read_*``/``write_kv`` are the reference's host-side helpers
 (torch indexing on the device); the decode hot path does not use them --
 the kernels read and write pages in place.
+
+:class:`CUDACache8Pool` keeps 8-bit codes with a scale per token, head and kind
+instead (``kernels.KVCache8``), half the memory for the same blocks.
 """
 
 from __future__ import annotations
@@ -130,8 +133,12 @@ class CUDAMemoryPool:
 
     # ── introspection ────────────────────────────────────────────────────────
 
+    def tensors(self) -> list[torch.Tensor]:
+        """Every tensor that holds blocks, blocks in dimension 0 (1 in per-layer mode)."""
+        return [self._all]
+
     def get_memory_mb(self) -> float:
-        return self._all.numel() * self._all.element_size() / (1024 * 1024)
+        return sum(t.numel() * t.element_size() for t in self.tensors()) / (1024 * 1024)
 
     def utilisation_snapshot(self) -> dict:
         return {"device": str(self.device), "shape": list(self._all.shape),
@@ -156,6 +163,121 @@ class CUDAMemoryPool:
                              f"(block_size={self.block_size}).")
 
 
+class CUDACache8Pool(CUDAMemoryPool):
+    """The pool as 8-bit codes and fp32 scales; no counterpart in the reference.
+
+    ``code_dtype``: int8 or float8_e4m3fn.  :meth:`layer` returns a
+    ``kernels.KVCache8``, which ``norm_rope_and_cache`` writes and
+    ``paged_decode_attention_cache8`` reads; :meth:`read_back` hands 16-bit
+    pages of some sequences to the attention calls that want them.  The
+    host-side helpers take and return values of ``dtype``.
+    """
+
+    def __init__(self, num_blocks: int, block_size: int, n_heads: int, d_k: int,
+                 dtype: torch.dtype = torch.float16, device: torch.device | str | None = None,
+                 num_layers: int | None = None, code_dtype: torch.dtype = torch.int8) -> None:
+        if device is None:
+            device = torch.device("cuda" if torch.cuda.is_available() else "cpu")
+        layers = () if num_layers is None else (num_layers,)
+        self._scales = torch.zeros((*layers, num_blocks, n_heads, 2, block_size),
+                                   dtype=torch.float32, device=device)
+        super().__init__(num_blocks, block_size, n_heads, d_k, code_dtype, device, num_layers)
+        self.code_dtype = code_dtype
+        self.dtype = dtype
+        self._scratch: torch.Tensor | None = None
+
+    @classmethod
+    def from_free_memory(cls, block_size: int, n_heads: int, d_k: int, dtype: torch.dtype,
+                         device: torch.device | str, num_layers: int | None = None,
+                         fraction: float = 0.85, max_blocks: int | None = None,
+                         code_dtype: torch.dtype = torch.int8) -> "CUDACache8Pool":
+        device = torch.device(device)
+        free, _ = torch.cuda.mem_get_info(device)
+        per_block = 2 * block_size * n_heads * (d_k + 4) * (num_layers or 1)
+        n = int(free * fraction) // per_block
+        if max_blocks is not None:
+            n = min(n, max_blocks)
+        if n <= 0:
+            raise MemoryError("CUDACache8Pool: no free device memory for a pool")
+        return cls(n, block_size, n_heads, d_k, dtype, device, num_layers, code_dtype)
+
+    def layer(self, i: int):
+        from vllm_mps_b200.kernels import KVCache8
+
+        if self.num_layers is None:
+            return KVCache8(self._all, self._scales)
+        return KVCache8(self._all[i], self._scales[i])
+
+    def tensors(self) -> list[torch.Tensor]:
+        return [self._all.view(torch.int8), self._scales]
+
+    def read_back(self, layer: int, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                  dst_tables: torch.Tensor, pages: int) -> torch.Tensor:
+        """16-bit pages of the sequences, at blocks ``dst_tables`` (below ``pages``) of a
+        pool that the next call overwrites (calls are ordered by the stream)."""
+        from vllm_mps_b200.kernels import read_cache8
+
+        if self._scratch is None or self._scratch.shape[0] < pages:
+            self._scratch = torch.empty((max(1, pages), 2, self.block_size, self.n_heads, self.d_k),
+                                        dtype=self.dtype, device=self.device)
+        return read_cache8(self.layer(layer), block_tables, seq_lens, self._scratch, dst_tables)
+
+    def write_kv(self, block_id: int, token_pos: int, k: torch.Tensor, v: torch.Tensor,
+                 layer: int = 0) -> None:
+        from vllm_mps_b200.kernels import quantize_cache8
+
+        self._validate_indices(block_id, token_pos)
+        cache = self.layer(layer)
+        for kind, x in enumerate((k, v)):
+            codes, scales = quantize_cache8(x, self.code_dtype)
+            cache.codes[block_id, kind, token_pos] = codes
+            cache.scales[block_id, :, kind, token_pos] = scales
+
+    def _values(self, ids, layer: int) -> torch.Tensor:
+        """(blocks, 2, block_size, n_heads, d_k) values of some blocks."""
+        cache = self.layer(layer)
+        codes = cache.codes.view(torch.int8)[ids].view(self.code_dtype).float()
+        return (codes * cache.scales[ids].permute(0, 2, 3, 1).unsqueeze(-1)).to(self.dtype)
+
+    def read_kv(self, block_id: int, token_pos: int, layer: int = 0):
+        self._validate_indices(block_id, token_pos)
+        x = self._values([block_id], layer)[0]
+        return x[0, token_pos], x[1, token_pos]
+
+    def read_block_kv(self, block_id: int, layer: int = 0):
+        self._check_block(block_id, "block_id")
+        x = self._values([block_id], layer)[0]
+        return x[0], x[1]
+
+    def gather_blocks_tensor(self, ids_tensor: torch.Tensor, layer: int = 0):
+        x = self._values(ids_tensor, layer)
+        return (x[:, 0].reshape(-1, self.n_heads, self.d_k),
+                x[:, 1].reshape(-1, self.n_heads, self.d_k))
+
+    def gather_blocks_batched(self, block_tables: list[list[int]], seq_lens: list[int],
+                              max_seq_len: int, layer: int = 0):
+        shape = (len(block_tables), max_seq_len, self.n_heads, self.d_k)
+        out = torch.zeros((2, *shape), dtype=self.dtype, device=self.device)
+        for i, (table, n) in enumerate(zip(block_tables, seq_lens)):
+            n = min(n, max_seq_len)
+            if n > 0:
+                ids = torch.as_tensor(table[:-(-n // self.block_size)], device=self.device)
+                out[0, i, :n], out[1, i, :n] = (t[:n] for t in self.gather_blocks_tensor(ids, layer))
+        return out[0], out[1]
+
+    def copy_block(self, src_block_id: int, dst_block_id: int) -> None:
+        self._check_block(src_block_id, "src_block_id")
+        self._check_block(dst_block_id, "dst_block_id")
+        for t in self.tensors():
+            if self.num_layers is None:
+                t[dst_block_id] = t[src_block_id]
+            else:
+                t[:, dst_block_id] = t[:, src_block_id]
+
+    def __repr__(self) -> str:
+        return super().__repr__().replace("CUDAMemoryPool", "CUDACache8Pool")
+
+
 class SwapSpace:
     """Pinned host copy of swapped-out blocks: the data half of preemption.
 
@@ -168,20 +290,23 @@ class SwapSpace:
 
     def __init__(self, gpu_pool: CUDAMemoryPool, num_cpu_blocks: int) -> None:
         self.gpu_pool = gpu_pool
-        shape = list(gpu_pool._all.shape)
-        blk_dim = 0 if gpu_pool.num_layers is None else 1
-        shape[blk_dim] = num_cpu_blocks
-        self._blk_dim = blk_dim
-        self.cpu = torch.zeros(shape, dtype=gpu_pool.dtype)
-        if torch.cuda.is_available():
-            self.cpu = self.cpu.pin_memory()
+        self._blk_dim = 0 if gpu_pool.num_layers is None else 1
+        self._cpu = []
+        for t in gpu_pool.tensors():
+            shape = list(t.shape)
+            shape[self._blk_dim] = num_cpu_blocks
+            host = torch.zeros(shape, dtype=t.dtype)
+            self._cpu.append(host.pin_memory() if torch.cuda.is_available() else host)
+        self.cpu = self._cpu[0]
 
     def copy_out(self, gpu_ids: list[int], cpu_ids: list[int]) -> None:
         g = torch.as_tensor(gpu_ids, dtype=torch.long, device=self.gpu_pool.device)
-        data = self.gpu_pool._all.index_select(self._blk_dim, g).to("cpu")
-        self.cpu.index_copy_(self._blk_dim, torch.as_tensor(cpu_ids, dtype=torch.long), data)
+        for t, host in zip(self.gpu_pool.tensors(), self._cpu):
+            data = t.index_select(self._blk_dim, g).to("cpu")
+            host.index_copy_(self._blk_dim, torch.as_tensor(cpu_ids, dtype=torch.long), data)
 
     def copy_in(self, cpu_ids: list[int], gpu_ids: list[int]) -> None:
-        data = self.cpu.index_select(self._blk_dim, torch.as_tensor(cpu_ids, dtype=torch.long))
         g = torch.as_tensor(gpu_ids, dtype=torch.long, device=self.gpu_pool.device)
-        self.gpu_pool._all.index_copy_(self._blk_dim, g, data.to(self.gpu_pool.device, non_blocking=True))
+        for t, host in zip(self.gpu_pool.tensors(), self._cpu):
+            data = host.index_select(self._blk_dim, torch.as_tensor(cpu_ids, dtype=torch.long))
+            t.index_copy_(self._blk_dim, g, data.to(self.gpu_pool.device, non_blocking=True))
