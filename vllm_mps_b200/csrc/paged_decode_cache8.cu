@@ -256,6 +256,9 @@ __device__ __forceinline__ void store_record(const Decode8Params& p, size_t rec,
   }
 }
 
+template <int D, int NT>
+constexpr bool kRegroup8 = D == 128 && NT == 2;
+
 template <typename T, int D, int NT, bool kInt8>
 __global__ void __launch_bounds__(32 * (kProducers8 + kWarps8), 1)
 decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) {
@@ -371,6 +374,16 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
   C8Walk w;
   w.start(wpref, sh, begin, end);
 
+  // At head size 128 the sums of 16 query heads take more registers than 12 warps have each:
+  // the producers' warpgroup hands some to the two of the consumers (128 * 56 + 256 * 224 =
+  // 384 * 168, what the block was launched with).
+  if constexpr (kRegroup8<D, NT>) {
+    if (warp < kProducers8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    }
+  }
   if (warp < kProducers8) {
     // ── producers ────────────────────────────────────────────────────────────
     // Block-table entries are fetched 32 pages ahead of their use.
@@ -477,6 +490,8 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
     uint4* o4 = reinterpret_cast<uint4*>(out + static_cast<int64_t>(s) * n_q * D);
     for (int e = tid - 32 * kProducers8; e < n_q * D / 8; e += blockDim.x - 32 * kProducers8) o4[e] = make_uint4(0u, 0u, 0u, 0u);
   }
+
+  if (cw >= hpc * TG) return;  // (whole warpgroups are launched where registers change hands)
 
   // Where the tensor map's box and swizzle put 16-byte chunk `chunk` of this head's row of
   // token `tok` in a page (K; V is v_add further): rows of 128 bytes, at head size 64 of two
@@ -968,13 +983,13 @@ Decode8Config configure8(int num_seqs, int n_q, int n_kv, int D, int max_blocks,
   Decode8Config cfg;
   // Two heads a CTA, so that a sequence is cut into few pieces and rows of a page are
   // read 2 D bytes at a time; more where no sequence has the pages for the other warps.
+  cfg.nt = n_q / n_kv > 8 ? 2 : 1;
   cfg.tg = kWarps8 / 2;
   while (cfg.tg > 1 && cfg.tg / 2 * kPages8 >= max_blocks) cfg.tg /= 2;
   cfg.hpc = min(kMaxHeads8, kWarps8 / cfg.tg);
   while (cfg.hpc > 2 && cfg.hpc * (n_q / n_kv) > 32) --cfg.hpc;  // query rows in shared memory
   while (n_kv % cfg.hpc) --cfg.hpc;
   while (cfg.hpc * cfg.tg * 2 <= kWarps8 && cfg.tg * kPages8 < max_blocks) cfg.tg *= 2;
-  cfg.nt = n_q / n_kv > 8 ? 2 : 1;
   cfg.n_cta = sms;
   const size_t stage =
       static_cast<size_t>(cfg.tg) * kPages8 * cfg.hpc * (2 * kCachePage * D + 2 * kCachePage * 4);
@@ -1010,7 +1025,8 @@ int launch_decode8(const CUtensorMap& tmap, const Decode8Params& p, const Decode
   });
   const cudaError_t e =
       launch_link(decode8_kernel<T, D, NT, kInt8>, true, dim3(c.n_cta),
-                  dim3(32 * (kProducers8 + c.hpc * c.tg)), c.smem, s, tmap, p);
+                  dim3(32 * (kProducers8 + (kRegroup8<D, NT> ? kWarps8 : c.hpc * c.tg))), c.smem, s,
+                  tmap, p);
   if (e != cudaSuccess) {
     return fail(VMPS_ERR_CUDA, "paged_decode_attention_cache8: launch failed: %s", cudaGetErrorString(e));
   }
