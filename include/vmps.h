@@ -421,7 +421,8 @@ int vmps_w4_gemm(void* out, int64_t out_row_stride, const void* x, int64_t x_row
  * rope() is the rotate-half form with the angle positions[i] * inv_freq[j],
  * whose product is exact (vmps_rope_reshape_and_cache rounds it to fp32, as the
  * reference does).  All of it is fp32 and rounded once, to `dtype` or to a code
- * of `cache_format`.  inv_freq NULL: no rotation (positions may be NULL).
+ * of `cache_format`; heads with values from about 1e18 on overflow the sum of
+ * squares.  inv_freq NULL: no rotation (positions may be NULL).
  *
  * q_out, q, k, v: num_rows rows of heads [heads][head_dim], row strides in
  * elements (multiples of 8, at least a row); q_out may be q where the strides
@@ -475,8 +476,9 @@ int vmps_read_cache8(void* pool, int pool_blocks, const int32_t* dst_tables, con
  * lengths.  Its first 1 MiB (the counters) must be zero before the first call
  * (vmps_paged_decode_workspace_init); every call leaves it zero, so one
  * workspace serves calls of any shape, and vmps_paged_decode_attention's too.
- * Calls that may overlap on the GPU need different workspaces.  0 bytes: the
- * shape is not supported.
+ * Calls that may overlap on the GPU need different workspaces; after error bit
+ * 8 it is to be zeroed again.  out must not be q's memory.  0 bytes: the shape
+ * is not supported.
  */
 size_t vmps_paged_decode_cache8_workspace_bytes(int num_seqs, int n_q, int n_kv, int head_dim);
 int vmps_paged_decode_attention_cache8(void* out, const void* q, int64_t q_row_stride,
@@ -486,6 +488,52 @@ int vmps_paged_decode_attention_cache8(void* out, const void* q, int64_t q_row_s
                                        int head_dim, int block_size, int num_blocks, float scale,
                                        void* workspace, size_t workspace_bytes, int cache_format,
                                        int dtype, void* stream);
+
+/*
+ * The three calls above with their arguments in a struct, field by field under the
+ * same names, for hosts whose foreign calls cost by the argument (0.2 us each from
+ * Python's ctypes, 4 us of 20 for the longest).  The struct is read before the
+ * call returns.
+ */
+typedef struct vmps_norm_rope_args {
+  void* q_out;
+  const void *q, *k, *v;
+  int64_t q_out_row_stride, q_row_stride, k_row_stride, v_row_stride;
+  const void *q_weight, *k_weight;
+  const int32_t *positions, *slot_mapping;
+  const float* inv_freq;
+  void* cache;
+  float* scales;
+  float eps;
+  int num_rows, n_q, n_kv, head_dim, block_size, num_blocks, cache_format, dtype;
+} vmps_norm_rope_args;
+int vmps_norm_rope_and_cache_args(const vmps_norm_rope_args* args, void* stream);
+
+typedef struct vmps_read_args {
+  void* pool;
+  const int32_t* dst_tables;
+  const void* codes;
+  const float* scales;
+  const int32_t *block_tables, *seq_lens;
+  int pool_blocks, max_blocks_per_seq, num_seqs, n_kv, head_dim, block_size, num_blocks,
+      cache_format, dtype;
+} vmps_read_args;
+int vmps_read_cache8_args(const vmps_read_args* args, void* stream);
+
+typedef struct vmps_decode_cache8_args {
+  void* out;
+  const void* q;
+  int64_t q_row_stride;
+  const void* codes;
+  const float* scales;
+  const int32_t *block_tables, *seq_lens;
+  void* workspace;
+  size_t workspace_bytes;
+  float scale;
+  int max_blocks_per_seq, num_seqs, n_q, n_kv, head_dim, block_size, num_blocks, cache_format,
+      dtype;
+} vmps_decode_cache8_args;
+int vmps_paged_decode_attention_cache8_args(const vmps_decode_cache8_args* args, void* stream);
 
 /*
  * Copies `bytes` from `src` to `dst` with the GPU's own loads and stores,

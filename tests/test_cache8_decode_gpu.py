@@ -250,6 +250,13 @@ def test_bad_tables_are_reported():
     assert _worst(got, _reference(c)) <= 1
 
 
+def test_shared_pages():
+    """Sequences with a common prefix read the same pages."""
+    c = _case([330, 100, 340], 8, 2, 64, torch.bfloat16, INT8, 13)
+    c["block_tables"][2, :20] = c["block_tables"][0, :20]
+    assert _worst(K.paged_decode_attention_cache8(**c), _reference(c)) <= 1
+
+
 def test_far_blocks():
     """Byte offsets past 2^31: blocks at both ends of a cache of more than 2 GiB."""
     n_kv, D = 16, 128

@@ -115,12 +115,16 @@ def test_store_refusals(change, error):
         K.norm_rope_and_cache(**{**_store_args(), **change})
 
 
+_Q = torch.zeros((3, 4, 64), dtype=torch.float16)
+
+
 @pytest.mark.parametrize("change, error", [
     (dict(q=torch.zeros((3, 4, 32), dtype=torch.float16)), ValueError),
     (dict(block_tables=torch.zeros((2, 5), dtype=torch.int32)), ValueError),
     (dict(block_tables=torch.zeros((3, 5), dtype=torch.int64)), TypeError),
     (dict(seq_lens=torch.zeros(2, dtype=torch.int32)), ValueError),
     (dict(out=torch.zeros((3, 4, 64), dtype=torch.bfloat16)), ValueError),
+    (dict(out=_Q, q=_Q), ValueError),
     (dict(), RuntimeError),
 ])
 def test_decode_refusals(change, error):
@@ -217,3 +221,43 @@ def test_c_signatures_take_every_argument():
                     ("vmps_paged_decode_attention_cache8", 20)):
         assert len(getattr(lib, name).argtypes) == n
         assert getattr(lib, name).restype is ctypes.c_int
+
+
+def test_argument_structs_match_the_header(tmp_path):
+    """Each field lies where the packed form puts it (compiled from include/vmps.h)."""
+    import re
+    import shutil
+    import struct
+    import subprocess
+
+    header = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "vmps.h")
+    text = open(header).read()
+    structs = {"vmps_norm_rope_args": K._STORE_ARGS, "vmps_read_args": K._READ_ARGS,
+               "vmps_decode_cache8_args": K._DECODE_ARGS}
+    lines, want = [], []
+    for name, packed in structs.items():
+        body = re.search(r"typedef struct %s \{(.*?)\}" % name, text, re.S).group(1)
+        fields = [f.replace("*", " ").split()[-1] for d in body.split(";") for f in d.split(",") if f.strip()]
+        codes = [c for n, c in re.findall(r"(\d*)([PqNfi])", packed.format) for _ in range(int(n or 1))]
+        assert len(fields) == len(codes)
+        at = 0
+        for f, c in zip(fields, codes):
+            size = struct.calcsize("@" + c)
+            at = -(-at // size) * size
+            want.append((name, f, at, size))
+            at += size
+            lines.append(f'printf("%zu %zu\\n", offsetof({name}, {f}), sizeof((({name}*)0)->{f}));')
+    src = tmp_path / "f.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "%s"\nint main(void) {%s return 0;}\n'
+                   % (header, "\n".join(lines)))
+    subprocess.run([shutil.which("gcc") or "cc", "-o", str(tmp_path / "f"), str(src)], check=True)
+    got = subprocess.run([str(tmp_path / "f")], check=True, capture_output=True, text=True).stdout.split("\n")
+    for (name, f, at, size), line in zip(want, got):
+        assert line == f"{at} {size}", (name, f)
+
+
+def test_null_argument_structs_are_refused():
+    lib = _lib()
+    for name in ("vmps_norm_rope_and_cache_args", "vmps_read_cache8_args",
+                 "vmps_paged_decode_attention_cache8_args"):
+        assert getattr(lib, name)(None, None) == -1

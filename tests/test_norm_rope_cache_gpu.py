@@ -284,6 +284,23 @@ def test_read_back(n_kv, D, lens, fmt, dtype):
     assert got is pool and torch.equal(pool.cpu(), want)
 
 
+def test_wide_tables():
+    """Tables far wider than the sequences, so many that a block takes several pages."""
+    lens = [0] * 400
+    lens[3], lens[200], lens[399] = 1000, 17, 16
+    cache = _cache(70, 2, 64, INT8, 3)
+    bt, dst = np.zeros((400, 130), np.int64), np.zeros((400, 130), np.int64)
+    at = 0
+    for i, n in enumerate(lens):
+        for j in range((n + 15) // 16):
+            bt[i, j], dst[i, j] = 69 - at, at
+            at += 1
+    pool = torch.full((70, 2, 16, 2, 64), 5.0, dtype=torch.float16, device="cuda")
+    i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+    want = _read_reference(cache, bt, lens, pool, dst)
+    assert torch.equal(K.read_cache8(cache, i32(bt), i32(lens), pool, i32(dst)).cpu(), want)
+
+
 def test_read_back_reports_bad_blocks():
     cache = _cache(3, 2, 64, INT8, 2)
     pool = torch.full((3, 2, 16, 2, 64), 5.0, dtype=torch.float16, device="cuda")

@@ -395,3 +395,12 @@ extern "C" int vmps_norm_rope_and_cache(
   return head_dim == 64 ? launch_store<__nv_bfloat16, 64>(p, cache_format, s)
                         : launch_store<__nv_bfloat16, 128>(p, cache_format, s);
 }
+
+extern "C" int vmps_norm_rope_and_cache_args(const vmps_norm_rope_args* a, void* stream) {
+  if (!a) return vmps::fail(VMPS_ERR_INVALID_ARG, "norm_rope_and_cache: NULL arguments");
+  return vmps_norm_rope_and_cache(a->q_out, a->q_out_row_stride, a->q, a->q_row_stride, a->k,
+                                  a->k_row_stride, a->v, a->v_row_stride, a->q_weight, a->k_weight,
+                                  a->eps, a->positions, a->slot_mapping, a->inv_freq, a->cache,
+                                  a->scales, a->num_rows, a->n_q, a->n_kv, a->head_dim,
+                                  a->block_size, a->num_blocks, a->cache_format, a->dtype, stream);
+}

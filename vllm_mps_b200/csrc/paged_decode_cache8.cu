@@ -1168,3 +1168,12 @@ extern "C" int vmps_paged_decode_attention_cache8(
   return int8 ? dispatch_decode8<__nv_bfloat16, true>(head_dim, tmap, p, cfg, s)
               : dispatch_decode8<__nv_bfloat16, false>(head_dim, tmap, p, cfg, s);
 }
+
+extern "C" int vmps_paged_decode_attention_cache8_args(const vmps_decode_cache8_args* a,
+                                                       void* stream) {
+  if (!a) return vmps::fail(VMPS_ERR_INVALID_ARG, "paged_decode_attention_cache8: NULL arguments");
+  return vmps_paged_decode_attention_cache8(
+      a->out, a->q, a->q_row_stride, a->codes, a->scales, a->block_tables, a->max_blocks_per_seq,
+      a->seq_lens, a->num_seqs, a->n_q, a->n_kv, a->head_dim, a->block_size, a->num_blocks,
+      a->scale, a->workspace, a->workspace_bytes, a->cache_format, a->dtype, stream);
+}

@@ -158,3 +158,11 @@ extern "C" int vmps_read_cache8(void* pool, int pool_blocks, const int32_t* dst_
   return head_dim == 64 ? launch_read<__nv_bfloat16, 64>(p, num_seqs, cache_format, s)
                         : launch_read<__nv_bfloat16, 128>(p, num_seqs, cache_format, s);
 }
+
+extern "C" int vmps_read_cache8_args(const vmps_read_args* a, void* stream) {
+  if (!a) return vmps::fail(VMPS_ERR_INVALID_ARG, "read_cache8: NULL arguments");
+  return vmps_read_cache8(a->pool, a->pool_blocks, a->dst_tables, a->codes, a->scales,
+                          a->block_tables, a->max_blocks_per_seq, a->seq_lens, a->num_seqs, a->n_kv,
+                          a->head_dim, a->block_size, a->num_blocks, a->cache_format, a->dtype,
+                          stream);
+}

@@ -31,6 +31,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 import threading
 
 import torch
@@ -80,6 +81,9 @@ EXPORTED_SYMBOLS = (
     "vmps_read_cache8",
     "vmps_paged_decode_cache8_workspace_bytes",
     "vmps_paged_decode_attention_cache8",
+    "vmps_norm_rope_and_cache_args",
+    "vmps_read_cache8_args",
+    "vmps_paged_decode_attention_cache8_args",
     "vmps_stage_copy",
     "vmps_debug_error_word",
 )
@@ -170,6 +174,10 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.vmps_paged_decode_attention_cache8.argtypes = [
             vp, vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, vp, sz, i32, i32,
             vp]
+        for name in ("vmps_norm_rope_and_cache_args", "vmps_read_cache8_args",
+                     "vmps_paged_decode_attention_cache8_args"):
+            getattr(lib, name).restype = i32
+            getattr(lib, name).argtypes = [ctypes.c_char_p, vp]
         lib.vmps_stage_copy.restype = i32
         lib.vmps_stage_copy.argtypes = [vp, vp, sz, vp]
         lib.vmps_debug_error_word.restype = i32
@@ -1067,6 +1075,10 @@ def _head_rows(t: torch.Tensor, d: int, name: str) -> tuple[int, int, int]:
 
 
 _INT32, _FLOAT32 = torch.int32, torch.float32
+# vmps_norm_rope_args, vmps_read_args and vmps_decode_cache8_args (0: NULL).
+_STORE_ARGS = struct.Struct("@4P4q7Pf8i")
+_READ_ARGS = struct.Struct("@6P9i")
+_DECODE_ARGS = struct.Struct("@2Pq5PNf9i")
 
 
 def norm_rope_and_cache(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
@@ -1103,7 +1115,7 @@ def norm_rope_and_cache(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
     if heads != n_kv or v_heads != n_kv or v_rows != rows:
         raise ValueError(f"k and v must have {n_kv} heads and the same rows")
     n_q = qs = os_ = 0
-    q_ptr = o_ptr = None
+    q_ptr = o_ptr = 0
     if q is not None:
         q_rows, n_q, qs = _head_rows(q, D, "q")
         if q_rows != rows:
@@ -1123,7 +1135,7 @@ def norm_rope_and_cache(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
         raise ValueError("q_out without q")
     if slot_mapping.dtype != _INT32 or slot_mapping.numel() != rows or not slot_mapping.is_contiguous():
         _lengths(rows, slot_mapping=slot_mapping)
-    pos_ptr = inv_ptr = qw_ptr = kw_ptr = None
+    pos_ptr = inv_ptr = qw_ptr = kw_ptr = 0
     if inv_freq is not None:
         if inv_freq.dtype != _FLOAT32 or inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
             raise ValueError(f"inv_freq must be contiguous float32 of {D // 2} entries")
@@ -1145,11 +1157,11 @@ def norm_rope_and_cache(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
     dev = _device_index(k, v, q, q_out, positions, slot_mapping, inv_freq, pool, scales, q_weight,
                         k_weight)
     lib = _lib or load_library()
-    rc = _launch(lib.vmps_norm_rope_and_cache, dev,
-                 o_ptr, os_, q_ptr, qs, k.data_ptr(), ks, v.data_ptr(), vs, qw_ptr, kw_ptr, eps,
-                 pos_ptr, slot_mapping.data_ptr(), inv_ptr, pool.data_ptr(),
-                 None if scales is None else scales.data_ptr(), rows, n_q, n_kv, D, block_size,
-                 num_blocks, fmt, dtype_code(dtype))
+    args = _STORE_ARGS.pack(o_ptr, q_ptr, k.data_ptr(), v.data_ptr(), os_, qs, ks, vs, qw_ptr,
+                            kw_ptr, pos_ptr, slot_mapping.data_ptr(), inv_ptr, pool.data_ptr(),
+                            0 if scales is None else scales.data_ptr(), eps, rows, n_q, n_kv, D,
+                            block_size, num_blocks, fmt, dtype_code(dtype))
+    rc = _launch(lib.vmps_norm_rope_and_cache_args, dev, args)
     if rc:
         _check(rc, "norm_rope_and_cache")
     return q_out
@@ -1180,10 +1192,11 @@ def read_cache8(cache: KVCache8, block_tables: torch.Tensor, seq_lens: torch.Ten
     _int32(dst_tables, "dst_tables")
     dev = _device_index(codes, scales, block_tables, seq_lens, pool, dst_tables)
     lib = _lib or load_library()
-    rc = _launch(lib.vmps_read_cache8, dev,
-                 pool.data_ptr(), shape[0], dst_tables.data_ptr(), codes.data_ptr(),
-                 scales.data_ptr(), block_tables.data_ptr(), tables[1], seq_lens.data_ptr(), B,
-                 n_kv, D, 16, cache.num_blocks, cache.format, dtype_code(pool.dtype))
+    args = _READ_ARGS.pack(pool.data_ptr(), dst_tables.data_ptr(), codes.data_ptr(),
+                           scales.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
+                           shape[0], tables[1], B, n_kv, D, 16, cache.num_blocks, cache.format,
+                           dtype_code(pool.dtype))
+    rc = _launch(lib.vmps_read_cache8_args, dev, args)
     if rc:
         _check(rc, "read_cache8")
     return pool
@@ -1255,8 +1268,9 @@ def paged_decode_attention_cache8(q: torch.Tensor, cache: KVCache8, block_tables
     dtype = q.dtype
     if out is None:
         out = q.new_empty((B, n_q, D))
-    elif out.shape != (B, n_q, D) or out.dtype != dtype or not out.is_contiguous():
-        raise ValueError("out must be a contiguous (B, n_q, D) tensor of q's dtype")
+    elif out.shape != (B, n_q, D) or out.dtype != dtype or not out.is_contiguous() \
+            or out.data_ptr() == q.data_ptr():
+        raise ValueError("out must be a contiguous (B, n_q, D) tensor of q's dtype, not q's memory")
     dev = _device_index(q, codes, scales, block_tables, seq_lens, out)
     if B == 0:
         return out
@@ -1267,12 +1281,12 @@ def paged_decode_attention_cache8(q: torch.Tensor, cache: KVCache8, block_tables
     elif workspace.get_device() != dev:
         _require_cuda(q, workspace)
     lib = _lib or load_library()
-    rc = _launch(lib.vmps_paged_decode_attention_cache8, dev,
-                 out.data_ptr(), q.data_ptr(), qs, codes.data_ptr(), scales.data_ptr(),
-                 block_tables.data_ptr(), tables[1], seq_lens.data_ptr(), B, n_q, n_kv, D, 16,
-                 cache.num_blocks, 1.0 / math.sqrt(D) if scale is None else scale,
-                 workspace.data_ptr(), workspace.numel() * workspace.element_size(), cache.format,
-                 dtype_code(dtype))
+    args = _DECODE_ARGS.pack(out.data_ptr(), q.data_ptr(), qs, codes.data_ptr(), scales.data_ptr(),
+                             block_tables.data_ptr(), seq_lens.data_ptr(), workspace.data_ptr(),
+                             workspace.numel() * workspace.element_size(),
+                             1.0 / math.sqrt(D) if scale is None else scale, tables[1], B, n_q,
+                             n_kv, D, 16, cache.num_blocks, cache.format, dtype_code(dtype))
+    rc = _launch(lib.vmps_paged_decode_attention_cache8_args, dev, args)
     if rc:
         _check(rc, "paged_decode_attention_cache8")
     return out
