@@ -534,7 +534,9 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
 
   int stage = 0, q_slot = 0, turn = 0;
   uint32_t parity = 0, q_parity = 0;
-  for (; w.valid; w.next(wpref, sh, end), turn ^= 1) {
+  for (C8Walk following; w.valid; w = following, turn ^= 1) {
+    following = w;  // worked out here, where the first tile is waited for anyway
+    following.next(wpref, sh, end);
     const int s = w.s, kvh = w.hg * hpc + h, len = lens[s];
     if (!s_abort && !mbar_wait(&q_full[q_slot], q_parity, p.err)) s_abort = 1;
     // Q^T as the B operand: k indices 2c, 2c+1 and 2c+8, 2c+9 of step ks are elements
@@ -554,15 +556,13 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       }
       float mine = p.scale_log2;
       if constexpr (!kF16) {
-        uint32_t top = 0;
+        uint32_t two = 0;  // the largest magnitudes of even and odd elements
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t x = qf[nt][ks][e];
-            top = max(top, max((x << 16) & 0x7fffffffu, x & 0x7fff0000u));
-          }
+          for (int e = 0; e < 2; ++e) two = __vmaxu2(two, qf[nt][ks][e] & 0x7fff7fffu);
         }
+        uint32_t top = max(two << 16, two & 0xffff0000u);
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         int e = 13 - (static_cast<int>(top >> 23) - 127);
@@ -803,21 +803,20 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
     float lse[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float4 ml[kWarps8];
-      float top0 = kLowest8, top1 = kLowest8, sum0 = 0.f, sum1 = 0.f;
+      // Lane (g, c) looks at warp g's; the butterflies leave every lane with the same sums.
+      float4 ml = make_float4(kLowest8, kLowest8, 0.f, 0.f);
+      if (g < active) ml = hand_ml[g * hpc + h][nt][c];
+      float top0 = ml.x, top1 = ml.y;
 #pragma unroll
-      for (int t = 0; t < kWarps8; ++t) {
-        ml[t] = make_float4(kLowest8, kLowest8, 0.f, 0.f);
-        if (t < active) ml[t] = hand_ml[t * hpc + h][nt][c];
-        top0 = fmaxf(top0, ml[t].x);
-        top1 = fmaxf(top1, ml[t].y);
+      for (int b = 4; b < 32; b <<= 1) {
+        top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, b));
+        top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, b));
       }
+      float sum0 = ml.z * fast_exp2(ml.x - top0), sum1 = ml.w * fast_exp2(ml.y - top1);
 #pragma unroll
-      for (int t = 0; t < kWarps8; ++t) {
-        if (t < active) {
-          sum0 += ml[t].z * fast_exp2(ml[t].x - top0);
-          sum1 += ml[t].w * fast_exp2(ml[t].y - top1);
-        }
+      for (int b = 4; b < 32; b <<= 1) {
+        sum0 += __shfl_xor_sync(0xffffffffu, sum0, b);
+        sum1 += __shfl_xor_sync(0xffffffffu, sum1, b);
       }
       lse[nt][0] = top0 + __log2f(sum0);
       lse[nt][1] = top1 + __log2f(sum1);
@@ -866,22 +865,25 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
         together();
         for (int mt = tg * M; mt < KS; mt += TG * M) {
           float x[M][4];
-          uint32_t at[M];
+          float4 y[kWarps8][M];
 #pragma unroll
           for (int i = 0; i < M; ++i) {
-            at[i] = chunk_of(mt + i);
-            x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+            const uint8_t* from = slot + chunk_of(mt + i);
+#pragma unroll
+            for (int t = 0; t < kWarps8; ++t) {
+              y[t][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (t < active) y[t][i] = *reinterpret_cast<const float4*>(from + t * page_bytes);
+            }
           }
 #pragma unroll
-          for (int t = 0; t < kWarps8; ++t) {
-            if (t >= active) break;
+          for (int i = 0; i < M; ++i) {
+            x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
 #pragma unroll
-            for (int i = 0; i < M; ++i) {
-              const float4 y = *reinterpret_cast<const float4*>(slot + t * page_bytes + at[i]);
-              x[i][0] += y.x;
-              x[i][1] += y.y;
-              x[i][2] += y.z;
-              x[i][3] += y.w;
+            for (int t = 0; t < kWarps8; ++t) {
+              x[i][0] += y[t][i].x;
+              x[i][1] += y[t][i].y;
+              x[i][2] += y[t][i].z;
+              x[i][3] += y[t][i].w;
             }
           }
           if (whole) {
