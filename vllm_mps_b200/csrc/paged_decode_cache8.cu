@@ -304,7 +304,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       mbar_init(&empty_bar[i], hpc * TG);
     }
     for (int i = 0; i < q_slots; ++i) {
-      mbar_init(&q_full[i], 1);
+      mbar_init(&q_full[i], kProducers8);
       mbar_init(&q_empty[i], hpc * TG);
     }
     fence_mbar_init();
@@ -416,16 +416,24 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
     int stage = 0, q_slot = 0;
     uint32_t parity = 1, q_parity = 1;
     while (count > 0) {
-      if (seq >= 0 && warp == 0) {
-        // The segment's query rows.
+      if (seq >= 0) {
+        // The segment's query rows, every kProducers8-th by this warp.
         const bool ok = !s_abort && mbar_wait(&q_empty[q_slot], q_parity, p.err);
         if (!__all_sync(0xffffffffu, ok)) {
           s_abort = 1;
           return;
         }
-        if (lane == 0) mbar_arrive_expect_tx(&q_full[q_slot], hpc * p.G * D * 2);
+        const int rows = hpc * p.G, mine = (rows - warp + kProducers8 - 1) / kProducers8;
+        if (lane == 0) {
+          if (mine > 0) {
+            mbar_arrive_expect_tx(&q_full[q_slot], mine * D * 2);
+          } else {
+            mbar_arrive(&q_full[q_slot]);
+          }
+        }
         __syncwarp();
-        for (int row = lane; row < hpc * p.G; row += 32) {
+        if (lane < mine) {
+          const int row = warp + lane * kProducers8;
           bulk_load(q_ring + q_slot * q_bytes + row * kQRow,
                     static_cast<const T*>(p.q) + seq * p.q_stride +
                         (static_cast<int64_t>(hg) * hpc * p.G + row) * D,
