@@ -10,8 +10,9 @@
 // the result is rounded once: to the 16-bit type, or to a code.
 //
 // What bounds it: the bytes of q, k and v in and out; 8192 rows of 32/8 heads x
-// 128 into the e4m3 cache take 39 us (4.7 TB/s; the instructions keep 60 % of the
-// issue slots), one row 2 us.
+// 128 into the e4m3 cache take 36 us (5.1 TB/s; the instructions keep two thirds of
+// the issue slots), one row 2.2 us.  What hides the loads is the number of warps: with
+// 64 registers and 32 warps an SM 36 us, with 80 and 24 39 us.
 #include "cache8.cuh"
 #include "vmps_abi_internal.h"
 
@@ -121,7 +122,7 @@ constexpr int kStoreWarps = 4;  // of a block
 // It works the row's angles out once, two a lane (one at head size 64), and hands
 // them round.
 template <typename T, int D, typename Code>
-__global__ void __launch_bounds__(32 * kStoreWarps, 6) norm_rope_cache_kernel(const StoreParams p) {
+__global__ void __launch_bounds__(32 * kStoreWarps, 8) norm_rope_cache_kernel(const StoreParams p) {
   constexpr int kHalf = D / 2;
   constexpr int kLanes = D / 16;
   constexpr int kHeads = 32 / kLanes;  // of a step
@@ -279,8 +280,8 @@ __global__ void __launch_bounds__(32 * kStoreWarps, 6) norm_rope_cache_kernel(co
   }
 }
 
-// Steps of a warp, at most: 8192 rows of 32/8 heads (head size 128, 12 steps) take 39.3 us
-// with 6, 40.4 with 12, 41.4 with 4 and 43.6 with 3.
+// Steps of a warp, at most (8192 rows of 32/8 heads, head size 128, 12 steps, with 24 warps
+// an SM: 39.3 us with 6, 40.4 with 12, 41.4 with 4 and 43.6 with 3).
 constexpr int kSteps = 6;
 
 template <typename T, int D, typename Code>
@@ -294,8 +295,11 @@ int launch_store(StoreParams p, cudaStream_t s) {
   const int64_t items = p.num_rows * p.parts;
   const int64_t grid = (items + kStoreWarps - 1) / kStoreWarps;
   if (grid > 0x7fffffff) return fail(VMPS_ERR_UNSUPPORTED, "norm_rope_and_cache: too many rows");
-  const cudaError_t e = launch_link(norm_rope_cache_kernel<T, D, Code>, true, dim3((unsigned)grid),
-                                    dim3(32 * kStoreWarps), 0, s, p);
+  // An early start saves small calls 0.4 us; the blocks of larger grids are then spread
+  // unevenly over the SMs that the launch before still holds (2000 rows of 40 heads x 64:
+  // 6.1 -> 7.7 us).
+  const cudaError_t e = launch_link(norm_rope_cache_kernel<T, D, Code>, grid <= sms,
+                                    dim3((unsigned)grid), dim3(32 * kStoreWarps), 0, s, p);
   if (e != cudaSuccess) {
     return fail(VMPS_ERR_CUDA, "norm_rope_and_cache: launch failed: %s", cudaGetErrorString(e));
   }

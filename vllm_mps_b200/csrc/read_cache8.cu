@@ -94,9 +94,10 @@ int launch_read(ReadParams p, int num_seqs, int format, cudaStream_t s) {
   const dim3 grid((p.max_blocks + p.pages - 1) / p.pages, num_seqs);
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
-  // An early start saves small calls half a microsecond (4 pages 3.9 -> 3.5 us), but costs
-  // grids of several waves (512 pages of 8 heads x 128, 2048 CTAs' worth of rows: 13 -> 17).
-  const bool early = static_cast<int64_t>(grid.x) * grid.y <= kReadResident * sms;
+  // An early start saves small calls half a microsecond (4 pages 3.9 -> 3.5 us), but the
+  // blocks of larger grids are then spread unevenly over the SMs that the launch before
+  // still holds (512 pages of 8 heads x 128: 13 -> 17 us).
+  const bool early = static_cast<int64_t>(grid.x) * grid.y <= sms;
   const cudaError_t e =
       format == VMPS_CACHE_INT8
           ? launch_link(read_cache8_kernel<T, D, Int8Code>, early, grid, dim3(kReadThreads), 0, s, p)
