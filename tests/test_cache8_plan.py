@@ -36,11 +36,11 @@ static C8Pos pos(const std::vector<int>& wpref, const C8Shape& sh, long long w) 
   r.j = c8_tile_at(cut.at - wpref[s]);
   return r;
 }
-extern "C" int check(int num_seqs, const int* lens, int tile_tokens, int groups, int n_cta) {
+extern "C" int check(int num_seqs, const int* lens, int shift, int groups, int n_cta) {
   std::vector<int> wpref(num_seqs + 1, 0);
   long long total = 0;
   for (int s = 0; s < num_seqs; ++s) {
-    total += c8_weight(c8_tiles(lens[s], tile_tokens));
+    total += c8_weight(c8_tiles(lens[s], shift));
     if (total > 0x7fffffffLL) return 1;  // the host refuses such calls
     wpref[s + 1] = (int)total;
   }
@@ -56,7 +56,7 @@ extern "C" int check(int num_seqs, const int* lens, int tile_tokens, int groups,
     C8Walk w;
     for (w.start(wpref.data(), sh, begin, end); w.valid; w.next(wpref.data(), sh, end)) {
       const size_t at = (size_t)w.hg * num_seqs + w.s;
-      if (w.tiles != c8_tiles(lens[w.s], tile_tokens)) return 2;
+      if (w.tiles != c8_tiles(lens[w.s], shift)) return 2;
       if (done[at] != w.j0 || w.j1 <= w.j0) return 3;
       done[at] = w.j1;
       if (w.j0 == 0 && w.j1 == w.tiles) continue;
@@ -73,7 +73,7 @@ extern "C" int check(int num_seqs, const int* lens, int tile_tokens, int groups,
   }
   for (int g = 0; g < groups; ++g)
     for (int s = 0; s < num_seqs; ++s)
-      if (done[(size_t)g * num_seqs + s] != c8_tiles(lens[s], tile_tokens)) return 8;
+      if (done[(size_t)g * num_seqs + s] != c8_tiles(lens[s], shift)) return 8;
   return 0;
 }
 extern "C" int join_group(int pieces) { return c8_join_group(pieces); }
@@ -93,7 +93,7 @@ def lib(tmp_path_factory):
 
 
 def _check(lib, lens, tile=16, groups=1, n_cta=296):
-    return lib.check(len(lens), (ctypes.c_int * len(lens))(*lens), tile, groups, n_cta)
+    return lib.check(len(lens), (ctypes.c_int * len(lens))(*lens), tile.bit_length() - 1, groups, n_cta)
 
 
 def test_shares_hold_every_tile_once(lib):

@@ -37,7 +37,8 @@ VMPS_HD long long c8_div(long long a, long long b) {
   return a / b;
 }
 
-VMPS_HD int c8_tiles(int len, int tile_tokens) { return len > 0 ? (len - 1) / tile_tokens + 1 : 0; }
+// Tiles of 2^shift tokens.
+VMPS_HD int c8_tiles(int len, int shift) { return len > 0 ? ((len - 1) >> shift) + 1 : 0; }
 
 VMPS_HD int c8_weight(int tiles) { return tiles > 0 ? tiles * kC8TileWeight + kC8SegWeight : 0; }
 
@@ -62,7 +63,7 @@ VMPS_HD C8Cut c8_cut(int total, int groups, long long w) {
   r.hg = groups;
   r.at = 0;
   if (w >= static_cast<long long>(groups) * total) return r;
-  r.hg = static_cast<int>(c8_div(w, total));
+  r.hg = groups == 1 ? 0 : static_cast<int>(c8_div(w, total));
   r.at = static_cast<int>(w - static_cast<long long>(r.hg) * total);
   return r;
 }

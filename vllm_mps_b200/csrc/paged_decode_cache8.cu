@@ -151,7 +151,7 @@ __device__ __forceinline__ void join_records(const Decode8Params& p, size_t base
                                              int count, int c0, int h, int nt, int part, int lane,
                                              float (&lse)[2], float (&o)[M][4]) {
   constexpr int KS = D / 16;
-  constexpr int kBatch = 8 / M;
+  constexpr int kBatch = 8;
   const int c = lane & 3;
   // Lanes whose heads are padding (nothing was stored for them) read their neighbour's.
   const int from = nt * 8 + 2 * c < p.G ? lane : lane & ~3;
@@ -314,13 +314,13 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
   // ── the plan: lengths, prefix sums of their weights, this CTA's share ───────
   // Every thread owns `per` sequences; those in which the share begins and ends
   // are found by their owners.
-  const int tile_tokens = TP * kCachePage;
+  const int tile_shift = 31 - __clz(TP * kCachePage), tile_tokens = 1 << tile_shift;
   C8Shape sh;
   sh.num_seqs = n;
   sh.groups = p.n_kv / hpc;
   sh.n_cta = gridDim.x;
   {
-    const int per = (n + blockDim.x - 1) / blockDim.x;
+    const int per = n <= blockDim.x ? 1 : (n + blockDim.x - 1) / blockDim.x;
     const int lo = min(n, tid * per), hi = min(n, lo + per);
     int sum = 0;
     for (int s = lo; s < hi; ++s) {
@@ -331,7 +331,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
         len = p.max_blocks * kCachePage;
       }
       lens[s] = len;
-      sum += c8_weight(c8_tiles(len, tile_tokens));
+      sum += c8_weight(c8_tiles(len, tile_shift));
     }
     int incl = sum;
 #pragma unroll
@@ -359,7 +359,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
     }
     for (int s = lo; s < hi; ++s) {
       const int before = run;
-      run += c8_weight(c8_tiles(lens[s], tile_tokens));
+      run += c8_weight(c8_tiles(lens[s], tile_shift));
       wpref[s + 1] = run;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -416,34 +416,6 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
     int stage = 0, q_slot = 0;
     uint32_t parity = 1, q_parity = 1;
     while (count > 0) {
-      if (seq >= 0) {
-        // The segment's query rows, every kProducers8-th by this warp.
-        const bool ok = !s_abort && mbar_wait(&q_empty[q_slot], q_parity, p.err);
-        if (!__all_sync(0xffffffffu, ok)) {
-          s_abort = 1;
-          return;
-        }
-        const int rows = hpc * p.G, mine = (rows - warp + kProducers8 - 1) / kProducers8;
-        if (lane == 0) {
-          if (mine > 0) {
-            mbar_arrive_expect_tx(&q_full[q_slot], mine * D * 2);
-          } else {
-            mbar_arrive(&q_full[q_slot]);
-          }
-        }
-        __syncwarp();
-        if (lane < mine) {
-          const int row = warp + lane * kProducers8;
-          bulk_load(q_ring + q_slot * q_bytes + row * kQRow,
-                    static_cast<const T*>(p.q) + seq * p.q_stride +
-                        (static_cast<int64_t>(hg) * hpc * p.G + row) * D,
-                    D * 2, &q_full[q_slot]);
-        }
-        if (++q_slot == q_slots) {
-          q_slot = 0;
-          q_parity ^= 1;
-        }
-      }
       fetch(hg2, count2, phys2, seq2);
       const bool bad = phys < 0 || phys >= p.num_blocks;
       if (bad) set_error(p.err, kDevErrBlockRange);
@@ -477,6 +449,34 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
         if (++stage == stages) {
           stage = 0;
           parity ^= 1;
+        }
+        if (k == 0 && seq >= 0) {
+          // The segment's query rows, every kProducers8-th by this warp, behind its first pages.
+          const bool ok = !s_abort && mbar_wait(&q_empty[q_slot], q_parity, p.err);
+          if (!__all_sync(0xffffffffu, ok)) {
+            s_abort = 1;
+            return;
+          }
+          const int rows = hpc * p.G, mine = (rows - warp + kProducers8 - 1) / kProducers8;
+          if (lane == 0) {
+            if (mine > 0) {
+              mbar_arrive_expect_tx(&q_full[q_slot], mine * D * 2);
+            } else {
+              mbar_arrive(&q_full[q_slot]);
+            }
+          }
+          __syncwarp();
+          if (lane < mine) {
+            const int row = warp + lane * kProducers8;
+            bulk_load(q_ring + q_slot * q_bytes + row * kQRow,
+                      static_cast<const T*>(p.q) + seq * p.q_stride +
+                          (static_cast<int64_t>(hg) * hpc * p.G + row) * D,
+                      D * 2, &q_full[q_slot]);
+          }
+          if (++q_slot == q_slots) {
+            q_slot = 0;
+            q_parity ^= 1;
+          }
         }
       }
       hg = hg2;
