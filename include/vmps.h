@@ -469,7 +469,7 @@ int vmps_read_cache8(void* pool, int pool_blocks, const int32_t* dst_tables, con
  * part, whatever they hold.  seq_lens[i] beyond the table sets error bit 4 (the
  * table's pages are read); a block outside the cache sets bit 2.
  * Supported: head_dim 64 or 128, block_size 16, n_q / n_kv a whole number up to
- * 16, n_kv <= 64, num_seqs <= 4096.
+ * 16, n_kv <= 64, num_seqs <= 4096, num_seqs * (max_blocks_per_seq + 2) below 2^29.
  *
  * The workspace (256-byte aligned) holds the partial results of sequences cut
  * between CTAs and their arrival counters; its size does not depend on the

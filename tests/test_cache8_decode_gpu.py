@@ -150,6 +150,15 @@ def test_ragged_batches(n, most, n_q, n_kv, D, dtype, fmt):
     assert _worst(K.paged_decode_attention_cache8(**c), _reference(c)) <= 1
 
 
+def test_sequences_without_tokens():
+    """No sequence has any: rows of zeros, whatever was there.  No sequences at all."""
+    c = _case([0, 0, 0], 8, 2, 64, torch.float16, INT8, 2)
+    out = torch.full((3, 8, 64), 9.0, dtype=torch.float16, device="cuda")
+    assert (K.paged_decode_attention_cache8(**c, out=out) == 0).all()
+    empty = dict(c, q=c["q"][:0], block_tables=c["block_tables"][:0], seq_lens=c["seq_lens"][:0])
+    assert K.paged_decode_attention_cache8(**empty).shape == (0, 8, 64)
+
+
 def test_strided_queries_given_scale_and_out():
     c = _case([90, 400, 0], 12, 4, 64, torch.bfloat16, INT8, 3, pad=72)
     assert not c["q"].is_contiguous()

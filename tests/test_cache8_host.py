@@ -192,7 +192,8 @@ def test_c_store_refusals(change, rc):
     (dict(codes=None), -1), (dict(scales=None), -1), (dict(bt=None), -1), (dict(lens=None), -1),
     (dict(q=A + 2), -3), (dict(out=A + 2), -3), (dict(codes=A + 8), -3), (dict(scales=A + 4), -3),
     (dict(qs=260), -3), (dict(qs=248), -1), (dict(scale=0.0), -1), (dict(scale=float("nan")), -1),
-    (dict(scale=float("inf")), -1),
+    (dict(scale=float("inf")), -1), (dict(B=4096, mb=1 << 17), -2), (dict(mb=1 << 27), -2),
+    (dict(nb=1 << 30), -2),
 ])
 def test_c_decode_refusals(change, rc):
     a = dict(out=A, q=A, qs=256, codes=A, scales=A, bt=A, mb=4, lens=A, B=3, n_q=4, n_kv=2, d=64,

@@ -1099,7 +1099,7 @@ def norm_rope_and_cache(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
     negative slot caches nothing.  Returns ``q_out`` (rows, n_q, D), a new
     tensor unless given (``q`` itself works).
     """
-    if type(cache) is KVCache8:
+    if isinstance(cache, KVCache8):
         pool, scales, fmt = cache.codes, cache.scales, cache.format
         num_blocks, n_kv, D = cache.num_blocks, cache.n_kv, cache.head_dim
         block_size = 16
