@@ -284,6 +284,15 @@ def test_read_back(n_kv, D, lens, fmt, dtype):
     assert got is pool and torch.equal(pool.cpu(), want)
 
 
+@pytest.mark.parametrize("n_kv, D, lens", [
+    (64, 128, [20]), (33, 128, [5, 47]), (32, 128, [700, 0, 900]), (8, 128, [4095, 3]),
+    (8, 128, [9000]), (5, 128, [1000]), (7, 64, [2000, 17]), (2, 128, [31, 1]),
+])
+def test_read_back_of_pages_shared_by_blocks(n_kv, D, lens):
+    """Few pages, whose rows one, two, four or eight blocks share."""
+    test_read_back(n_kv, D, lens, E4M3, torch.bfloat16)
+
+
 def test_wide_tables():
     """Tables far wider than the sequences, so many that a block takes several pages."""
     lens = [0] * 400

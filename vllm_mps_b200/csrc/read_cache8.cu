@@ -19,6 +19,7 @@ struct ReadParams {
   const int32_t* seq_lens;
   int max_blocks, n_kv, num_blocks, pool_blocks;
   int pages;  // of a sequence per CTA
+  int split;  // CTAs that share a page's rows
   int* err;
 };
 
@@ -38,7 +39,7 @@ __global__ void __launch_bounds__(kReadThreads, kReadResident) read_cache8_kerne
   if (len <= 0 || page0 > (len - 1) / kCachePage) return;
   int page1 = min(page0 + p.pages, (len - 1) / kCachePage + 1);
   if (page1 > p.max_blocks) page1 = p.max_blocks;
-  if ((len - 1) / kCachePage >= p.max_blocks && page0 == 0 && threadIdx.x == 0) {
+  if ((len - 1) / kCachePage >= p.max_blocks && blockIdx.x == 0 && threadIdx.x == 0) {
     set_error(p.err, kDevErrSeqLen);
   }
   const int row_codes = p.n_kv * D;
@@ -48,6 +49,8 @@ __global__ void __launch_bounds__(kReadThreads, kReadResident) read_cache8_kerne
   const int rows = kReadThreads / width;
   const int c0 = threadIdx.x % width, r0 = threadIdx.x / width;
   if (r0 >= rows) return;
+  const int span = 2 * kCachePage / p.split;  // rows of this CTA
+  const int ra = blockIdx.z * span + r0, rb = blockIdx.z * span + span;
   for (int page = page0; page < page1; ++page) {
     const int64_t at = static_cast<int64_t>(s) * p.max_blocks + page;
     const int src = p.block_tables[at], dst = p.dst_tables[at];
@@ -62,7 +65,7 @@ __global__ void __launch_bounds__(kReadThreads, kReadResident) read_cache8_kerne
       const float* scales =
           p.scales + (static_cast<int64_t>(src) * p.n_kv + c * 16 / D) * 2 * kCachePage;
       T* out = static_cast<T*>(p.pool) + dst * block + c * 16;
-      for (int r = r0; r < 2 * kCachePage; r += rows) {
+      for (int r = ra; r < rb; r += rows) {
         uint4 w = make_uint4(0u, 0u, 0u, 0u);  // K's 16 tokens, then V's: the scales' order too
         float sc = 0.f;
         if (r % kCachePage < live) {
@@ -91,13 +94,23 @@ int launch_read(ReadParams p, int num_seqs, int format, cudaStream_t s) {
   // One page a CTA, more where the tables are wide: a CTA without pages costs a launch slot.
   const int64_t all = static_cast<int64_t>(p.max_blocks) * num_seqs;
   p.pages = static_cast<int>((all + 16383) / 16384);
-  const dim3 grid((p.max_blocks + p.pages - 1) / p.pages, num_seqs);
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
-  // An early start saves small calls half a microsecond (4 pages 3.9 -> 3.5 us), but the
+  // Few pages are shared out by rows, as long as every thread keeps one (8 heads x 128, 4
+  // pages 4.6 -> 2.1 us, 64 pages 5.0 -> 3.4, 512 pages 12.8 -> 12.0; 32 heads, 128 pages
+  // 24.8 -> 13.0).  Eight ways only for one CTA an SM (64 pages 3.8 us), none for many pages
+  // (131071 tokens 133.5 -> 140).
+  const int rows = p.n_kv * D / 16 < kReadThreads ? kReadThreads / (p.n_kv * D / 16) : 1;
+  p.split = 1;
+  while (p.split < 8 && rows * p.split * 2 <= 2 * kCachePage &&
+         all * p.split * 2 <= (p.split < 4 ? 2048 : sms)) {
+    p.split *= 2;
+  }
+  const dim3 grid((p.max_blocks + p.pages - 1) / p.pages, num_seqs, p.split);
+  // An early start saves small calls half a microsecond, but the
   // blocks of larger grids are then spread unevenly over the SMs that the launch before
   // still holds (512 pages of 8 heads x 128: 13 -> 17 us).
-  const bool early = static_cast<int64_t>(grid.x) * grid.y <= sms;
+  const bool early = static_cast<int64_t>(grid.x) * grid.y * grid.z <= sms;
   const cudaError_t e =
       format == VMPS_CACHE_INT8
           ? launch_link(read_cache8_kernel<T, D, Int8Code>, early, grid, dim3(kReadThreads), 0, s, p)
@@ -150,7 +163,7 @@ extern "C" int vmps_read_cache8(void* pool, int pool_blocks, const int32_t* dst_
   if (int rc = device_error_word(&err)) return rc;
   ReadParams p{pool,     static_cast<const uint8_t*>(codes), scales, block_tables, dst_tables,
                seq_lens, max_blocks_per_seq,                 n_kv,   num_blocks,   pool_blocks,
-               1,        err};
+               1,        1,                                   err};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == VMPS_DTYPE_F16) {
     return head_dim == 64 ? launch_read<__half, 64>(p, num_seqs, cache_format, s)
