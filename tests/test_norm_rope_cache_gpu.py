@@ -293,6 +293,21 @@ def test_read_back_of_pages_shared_by_blocks(n_kv, D, lens):
     test_read_back(n_kv, D, lens, E4M3, torch.bfloat16)
 
 
+@pytest.mark.parametrize("n_kv, D", [(2, 64), (8, 128)])
+def test_read_back_into_a_pool_at_16_bytes(n_kv, D):
+    """The pool starts between two 32-byte boundaries."""
+    cache = _cache(4, n_kv, D, INT8, 4)
+    size = 4 * 2 * 16 * n_kv * D
+    memory = torch.full((size + 16,), 5.0, dtype=torch.float16, device="cuda")
+    pool = memory[8:8 + size].view(4, 2, 16, n_kv, D)
+    assert pool.data_ptr() % 32 == 16
+    bt, dst, lens = np.array([[3, 0], [2, 0]]), np.array([[1, 3], [0, 2]]), [30, 16]
+    i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+    want = _read_reference(cache, bt, lens, pool, dst)
+    assert torch.equal(K.read_cache8(cache, i32(bt), i32(lens), pool, i32(dst)).cpu(), want)
+    assert (memory[:8] == 5).all() and (memory[8 + size:] == 5).all()
+
+
 def test_wide_tables():
     """Tables far wider than the sequences, so many that a block takes several pages."""
     lens = [0] * 400

@@ -19,7 +19,9 @@ struct ReadParams {
   const int32_t* seq_lens;
   int max_blocks, n_kv, num_blocks, pool_blocks;
   int pages;  // of a sequence per CTA
-  int split;  // CTAs that share a page's rows
+  int width, rows;  // columns of a page that a CTA takes at a time, and rows of each
+  int span;         // rows of a page that are a CTA's
+  bool wide;        // 32-byte aligned pool
   int* err;
 };
 
@@ -27,9 +29,11 @@ constexpr int kReadThreads = 256;
 constexpr int kReadResident = 6;  // blocks of an SM
 
 // A thread keeps to one 16-byte column of the page's rows (32 of them: K and V of 16
-// tokens; n_kv * D codes each), so that nothing is divided per row.  What hides the
-// loads is the number of blocks: 131071 tokens (8 heads x 128) take 133 us (6.1 TB/s
-// read and written), with four rows' loads in flight per thread, and fewer blocks, 160.
+// tokens; n_kv * D codes each), so that nothing is divided per row, and stores a whole
+// 32-byte sector (with two 16-byte stores, half a sector of every lane each, 131071 tokens of
+// 8 heads x 128 took 150 us).  What hides the loads is the number of blocks: those tokens take
+// 131 us (6.2 TB/s read and written), with four rows' loads in flight per thread, and fewer
+// blocks, 160.
 template <typename T, int D, typename Code>
 __global__ void __launch_bounds__(kReadThreads, kReadResident) read_cache8_kernel(const ReadParams p) {
   chain_link();
@@ -44,13 +48,10 @@ __global__ void __launch_bounds__(kReadThreads, kReadResident) read_cache8_kerne
   }
   const int row_codes = p.n_kv * D;
   const int columns = row_codes / 16;
-  // Columns a pass, and rows of each at once.
-  const int width = min(columns, kReadThreads);
-  const int rows = kReadThreads / width;
+  const int width = p.width, rows = p.rows;
   const int c0 = threadIdx.x % width, r0 = threadIdx.x / width;
   if (r0 >= rows) return;
-  const int span = 2 * kCachePage / p.split;  // rows of this CTA
-  const int ra = blockIdx.z * span + r0, rb = blockIdx.z * span + span;
+  const int ra = blockIdx.z * p.span + r0, rb = blockIdx.z * p.span + p.span;
   for (int page = page0; page < page1; ++page) {
     const int64_t at = static_cast<int64_t>(s) * p.max_blocks + page;
     const int src = p.block_tables[at], dst = p.dst_tables[at];
@@ -65,6 +66,7 @@ __global__ void __launch_bounds__(kReadThreads, kReadResident) read_cache8_kerne
       const float* scales =
           p.scales + (static_cast<int64_t>(src) * p.n_kv + c * 16 / D) * 2 * kCachePage;
       T* out = static_cast<T*>(p.pool) + dst * block + c * 16;
+#pragma unroll 1
       for (int r = ra; r < rb; r += rows) {
         uint4 w = make_uint4(0u, 0u, 0u, 0u);  // K's 16 tokens, then V's: the scales' order too
         float sc = 0.f;
@@ -81,9 +83,16 @@ __global__ void __launch_bounds__(kReadThreads, kReadResident) read_cache8_kerne
           o[2 * i] = Elt<T>::pack(x[0] * sc, x[1] * sc);
           o[2 * i + 1] = Elt<T>::pack(x[2] * sc, x[3] * sc);
         }
-        uint4* dst4 = reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * row_codes);
-        dst4[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        dst4[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        T* row = out + static_cast<int64_t>(r) * row_codes;
+        if (p.wide) {
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row),
+                       "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]),
+                       "r"(o[7])
+                       : "memory");
+        } else {
+          *reinterpret_cast<uint4*>(row) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(row + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
       }
     }
   }
@@ -96,20 +105,19 @@ int launch_read(ReadParams p, int num_seqs, int format, cudaStream_t s) {
   p.pages = static_cast<int>((all + 16383) / 16384);
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
-  // Few pages are shared out by rows, as long as every thread keeps one (8 heads x 128, 4
-  // pages 4.6 -> 2.1 us, 64 pages 5.0 -> 3.4, 512 pages 12.8 -> 12.0; 32 heads, 128 pages
-  // 24.8 -> 13.0).  Eight ways only for one CTA an SM (64 pages 3.8 us), none for many pages
-  // (131071 tokens 133.5 -> 140).
-  const int rows = p.n_kv * D / 16 < kReadThreads ? kReadThreads / (p.n_kv * D / 16) : 1;
-  p.split = 1;
-  while (p.split < 8 && rows * p.split * 2 <= 2 * kCachePage &&
-         all * p.split * 2 <= (p.split < 4 ? 2048 : sms)) {
-    p.split *= 2;
-  }
-  const dim3 grid((p.max_blocks + p.pages - 1) / p.pages, num_seqs, p.split);
-  // An early start saves small calls half a microsecond, but the
-  // blocks of larger grids are then spread unevenly over the SMs that the launch before
-  // still holds (512 pages of 8 heads x 128: 13 -> 17 us).
+  // Equal passes over the columns (40 heads x 128, 16384 tokens 102 -> 91 us).
+  const int columns = p.n_kv * D / 16, passes = (columns + kReadThreads - 1) / kReadThreads;
+  p.width = (columns + passes - 1) / passes;
+  p.rows = kReadThreads / p.width;
+  // Few pages are shared out by rows while every thread keeps one, to 2048 CTAs: 8 heads x
+  // 128, 4 pages 4.1 -> 1.8 us, 64 pages 4.8 -> 3.1, 512 pages 12.5 -> 11.4 (12.1 with 4096
+  // CTAs); 64 heads, 13 pages 22.2 -> 3.4; 131071 tokens, however, 131 -> 137.
+  p.span = 2 * kCachePage;
+  for (int split = 2; p.rows <= p.span / 2 && all * split <= 2048; split *= 2) p.span /= 2;
+  const dim3 grid((p.max_blocks + p.pages - 1) / p.pages, num_seqs, 2 * kCachePage / p.span);
+  // An early start saves small calls half a microsecond, but the blocks of larger grids
+  // are then spread unevenly over the SMs that the launch before still holds (512 pages of
+  // 8 heads x 128, undivided: 13 -> 17 us).
   const bool early = static_cast<int64_t>(grid.x) * grid.y * grid.z <= sms;
   const cudaError_t e =
       format == VMPS_CACHE_INT8
@@ -161,9 +169,19 @@ extern "C" int vmps_read_cache8(void* pool, int pool_blocks, const int32_t* dst_
   }
   int* err = nullptr;
   if (int rc = device_error_word(&err)) return rc;
-  ReadParams p{pool,     static_cast<const uint8_t*>(codes), scales, block_tables, dst_tables,
-               seq_lens, max_blocks_per_seq,                 n_kv,   num_blocks,   pool_blocks,
-               1,        1,                                   err};
+  ReadParams p = {};
+  p.pool = pool;
+  p.codes = static_cast<const uint8_t*>(codes);
+  p.scales = scales;
+  p.block_tables = block_tables;
+  p.dst_tables = dst_tables;
+  p.seq_lens = seq_lens;
+  p.max_blocks = max_blocks_per_seq;
+  p.n_kv = n_kv;
+  p.num_blocks = num_blocks;
+  p.pool_blocks = pool_blocks;
+  p.wide = (reinterpret_cast<uintptr_t>(pool) & 31) == 0;
+  p.err = err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == VMPS_DTYPE_F16) {
     return head_dim == 64 ? launch_read<__half, 64>(p, num_seqs, cache_format, s)
