@@ -281,17 +281,28 @@ __global__ void __launch_bounds__(32 * kStoreWarps, 8) norm_rope_cache_kernel(co
 }
 
 // Steps of a warp, at most (8192 rows of 32/8 heads, head size 128, 12 steps, with 24 warps
-// an SM: 39.3 us with 6, 40.4 with 12, 41.4 with 4 and 43.6 with 3).
-constexpr int kSteps = 6;
+// an SM: 39.3 us with 6, 40.4 with 12, 41.4 with 4 and 43.6 with 3; 1000 rows of 40/40 heads,
+// 30 steps, 13.3 with 8 in one wave and 14.7 with 6 in two).
+constexpr int kSteps = 8;
 
 template <typename T, int D, typename Code>
 int launch_store(StoreParams p, cudaStream_t s) {
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
-  // Steps of a row; a warp takes several where there are rows enough without.
+  // Steps of a row, and the warps that share them: the fewest steps one after the other over
+  // all waves of warps, of which each costs two steps more (400 rows of 32/8 heads x 128 with
+  // 3 steps a warp 4.1 us, 5.4 with 6; 2500 rows 13.6 and 15.1).
   const int all = ((p.n_q + 2 * p.n_kv) * (D / 16) + 31) / 32;
-  p.parts = p.num_rows * all > 32 * sms ? (all + kSteps - 1) / kSteps : all;
-  p.steps = (all + p.parts - 1) / p.parts;
+  int64_t best = INT64_MAX;
+  for (int most = 1; most <= kSteps; ++most) {
+    const int parts = (all + most - 1) / most, steps = (all + parts - 1) / parts;
+    const int64_t waves = (p.num_rows * parts + 32 * sms - 1) / (32 * sms);
+    if (waves * (steps + 2) <= best) {
+      best = waves * (steps + 2);
+      p.parts = parts;
+      p.steps = steps;
+    }
+  }
   const int64_t items = p.num_rows * p.parts;
   const int64_t grid = (items + kStoreWarps - 1) / kStoreWarps;
   if (grid > 0x7fffffff) return fail(VMPS_ERR_UNSUPPORTED, "norm_rope_and_cache: too many rows");
