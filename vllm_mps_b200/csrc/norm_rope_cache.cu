@@ -10,9 +10,10 @@
 // the result is rounded once: to the 16-bit type, or to a code.
 //
 // What bounds it: the bytes of q, k and v in and out; 8192 rows of 32/8 heads x
-// 128 into the e4m3 cache take 36 us (5.1 TB/s; the instructions keep two thirds of
-// the issue slots), one row 2.2 us.  What hides the loads is the number of warps: with
-// 64 registers and 32 warps an SM 36 us, with 80 and 24 39 us.
+// 128 into the int8 cache take 35.4 us (5.2 TB/s; the instructions keep 70 % of the
+// issue slots), one row 2.1 us.  What hides the loads is the number of warps: with
+// 72 registers and 28 warps an SM 35.4 us, with 80 and 24 39.8, with 64 and 32, where a
+// few values are spilled, 36.9.
 #include "cache8.cuh"
 #include "vmps_abi_internal.h"
 
@@ -89,6 +90,13 @@ __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
   return r;
 }
 
+// NaN if one of them is (0x7fffffff, above every number's bits).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ void unpack8(const uint4& w, f2 (&x)[4]) {
   const uint32_t v[4] = {w.x, w.y, w.z, w.w};
@@ -114,7 +122,8 @@ __device__ __forceinline__ void store8(T* p, const f2 (&x)[4]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-constexpr int kStoreWarps = 4;  // of a block
+constexpr int kStoreWarps = 4;     // of a block
+constexpr int kStoreResident = 7;  // blocks of an SM
 
 // D / 16 lanes share a head: lane c holds elements 8c.. of each half, so that a
 // rotated pair is in one lane; a warp takes 512 / D heads a step.  A warp works
@@ -122,7 +131,8 @@ constexpr int kStoreWarps = 4;  // of a block
 // It works the row's angles out once, two a lane (one at head size 64), and hands
 // them round.
 template <typename T, int D, typename Code>
-__global__ void __launch_bounds__(32 * kStoreWarps, 8) norm_rope_cache_kernel(const StoreParams p) {
+__global__ void __launch_bounds__(32 * kStoreWarps, kStoreResident)
+norm_rope_cache_kernel(const StoreParams p) {
   constexpr int kHalf = D / 2;
   constexpr int kLanes = D / 16;
   constexpr int kHeads = 32 / kLanes;  // of a step
@@ -239,13 +249,14 @@ __global__ void __launch_bounds__(32 * kStoreWarps, 8) norm_rope_cache_kernel(co
     const bool mine = live && !is_q && write;
     if constexpr (!std::is_void<Code>::value) {
       // The largest magnitude, as bits: infinities and NaN are above every number.
-      uint32_t top = 0;
+      float most = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 a = split(lo[e]), b = split(hi[e]);
-        top = max(top, max(__float_as_uint(a.x) & 0x7fffffffu, __float_as_uint(a.y) & 0x7fffffffu));
-        top = max(top, max(__float_as_uint(b.x) & 0x7fffffffu, __float_as_uint(b.y) & 0x7fffffffu));
+        most = max3(most, fabsf(a.x), fabsf(a.y));
+        most = max3(most, fabsf(b.x), fabsf(b.y));
       }
+      uint32_t top = __float_as_uint(most);
 #pragma unroll
       for (int sh = 1; sh < kLanes; sh <<= 1) {
         top = max(top, __shfl_xor_sync(0xffffffffu, top, sh));
@@ -280,10 +291,9 @@ __global__ void __launch_bounds__(32 * kStoreWarps, 8) norm_rope_cache_kernel(co
   }
 }
 
-// Steps of a warp, at most (8192 rows of 32/8 heads, head size 128, 12 steps, with 24 warps
-// an SM: 39.3 us with 6, 40.4 with 12, 41.4 with 4 and 43.6 with 3; 1000 rows of 40/40 heads,
-// 30 steps, 13.3 with 8 in one wave and 14.7 with 6 in two).
-constexpr int kSteps = 8;
+// Steps of a warp, at most (8192 rows of 32/8 heads, head size 128, 12 steps: 35.4 us with
+// 12, 36.9 with 6; rows of 18 and 30 steps gain nothing from more).
+constexpr int kSteps = 12;
 
 template <typename T, int D, typename Code>
 int launch_store(StoreParams p, cudaStream_t s) {
@@ -291,12 +301,13 @@ int launch_store(StoreParams p, cudaStream_t s) {
   if (int rc = device_sm_count(&sms)) return rc;
   // Steps of a row, and the warps that share them: the fewest steps one after the other over
   // all waves of warps, of which each costs two steps more (400 rows of 32/8 heads x 128 with
-  // 3 steps a warp 4.1 us, 5.4 with 6; 2500 rows 13.6 and 15.1).
+  // 3 steps a warp 3.8 us, 5.4 with 6 (64 registers); 1000 rows of 40/40 heads 13.0 and 15.9).
   const int all = ((p.n_q + 2 * p.n_kv) * (D / 16) + 31) / 32;
   int64_t best = INT64_MAX;
   for (int most = 1; most <= kSteps; ++most) {
     const int parts = (all + most - 1) / most, steps = (all + parts - 1) / parts;
-    const int64_t waves = (p.num_rows * parts + 32 * sms - 1) / (32 * sms);
+    const int64_t warps = static_cast<int64_t>(kStoreResident) * kStoreWarps * sms;
+    const int64_t waves = (p.num_rows * parts + warps - 1) / warps;
     if (waves * (steps + 2) <= best) {
       best = waves * (steps + 2);
       p.parts = parts;
