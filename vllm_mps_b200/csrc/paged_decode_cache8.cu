@@ -934,8 +934,10 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
     int* counter = counter_of(lane, members);
     missing = members - 1 - arrive_piece8(counter);
   }
+  // Every lane's loads of other CTAs' records come after those lanes' acquires, and lane 0's
+  // reset of a counter after the lane's arrival on it.
+  __syncwarp();
   for (int i = 0; i < n_pend; ++i) {
-    // (The shuffle also puts every lane's loads after the acquires.)
     if (__shfl_sync(0xffffffffu, missing, i) != 0) continue;
     const int c0 = pend[i].c0, pieces = pend[i].c1 - c0 + 1;
     const int size = c8_join_group(pieces);
@@ -965,6 +967,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       before = arrive_piece8(top);
       if (before == groups - 1) *top = 0;
     }
+    __syncwarp();  // every lane's loads come after lane 0's acquire
     if (__shfl_sync(0xffffffffu, before, 0) != groups - 1) continue;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
