@@ -26,8 +26,8 @@
 //    V rows, whose even and odd columns become rows g and g + 8 of the A operand:
 //    the permutation that widens the codes also transposes them.
 //  * K's scale multiplies the score.  V's multiplies the weight before its
-//    rounding to fp16, relative to vref, a power of two that bounds V's scales so
-//    far.  Weights are relative to 2^-11 of a running bound of the scores that is
+//    rounding to fp16, relative to vref, a power of two that bounds the magnitudes
+//    of V's scales so far (a caller's own may be negative).  Weights are relative to 2^-11 of a running bound of the scores that is
 //    raised when a score passes it by 2^4: they stay below 2^15, and what fp16
 //    cannot hold of small ones is 2^-36 of the largest.  Sums of weights are
 //    fp32 and unrounded.
@@ -672,7 +672,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       float ym = -INFINITY, vm = 0.f;
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        vm = fmaxf(vm, fmaxf(vs0[i], vs1[i]));
+        vm = fmaxf(vm, fmaxf(fabsf(vs0[i]), fabsf(vs1[i])));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           ym = fmaxf(ym, fmaxf(fmaxf(y[i][nt][0], y[i][nt][1]), fmaxf(y[i][nt][2], y[i][nt][3])));
