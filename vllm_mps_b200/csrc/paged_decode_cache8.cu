@@ -26,15 +26,18 @@
 //    V rows, whose even and odd columns become rows g and g + 8 of the A operand:
 //    the permutation that widens the codes also transposes them.
 //  * K's scale multiplies the score.  V's multiplies the weight before its
-//    rounding to fp16, relative to vref, a power of two that bounds the magnitudes
-//    of V's scales so far (a caller's own may be negative).  Weights are relative to 2^-11 of a running bound of the scores that is
-//    raised when a score passes it by 2^4: they stay below 2^15, and what fp16
-//    cannot hold of small ones is 2^-36 of the largest.  Sums of weights are
-//    fp32 and unrounded.
+//    rounding to fp16.  Weights are relative to a power of two 2^r per head and
+//    warp that follows this product (its magnitude: a caller's scales may be
+//    negative), so that the largest so far is 2^10 to 2^15 and what fp16 cannot
+//    hold of small ones is 2^-35 of it, however large V is where the weights are
+//    small.  Weights themselves, whose sums are fp32 and unrounded, are then
+//    2^-111 (a product with V's largest possible scale) to 2^104; where V is so
+//    small that its products want larger ones they stay at that, and rows of
+//    V of 2^-100, the smallest that are stored, keep 17 bits.
 //  * bf16 queries are scaled by a power of two per head, so that their largest
 //    is in [2^13, 2^14), which fp16 holds as exactly as bf16 did but for values
 //    below 2^-28 of it.
-//  * At a sequence's end the warps of a kv head tell each other their bounds and sums,
+//  * At a sequence's end the warps of a kv head tell each other their references and sums,
 //    write their outputs over the codes that they have just read and add up a part each.
 //  * A cut sequence: every piece leaves its normalised output and the logarithm
 //    of its weights' sum in fp32 and arrives on a counter; the last to arrive
@@ -70,7 +73,11 @@ constexpr int kPages8 = 2;
 constexpr size_t kCounterBytes8 = size_t(128) << 10;
 constexpr size_t kRecordsAt8 = size_t(1) << 20;
 constexpr int kMostSmem8 = 220 << 10;  // dynamic shared memory of a CTA
-constexpr float kLowest8 = -1e30f;  // the score bound of a piece that has seen nothing
+constexpr float kLowest8 = -1e30f;  // the reference of weights where there were none
+// Logarithm of the largest weight times V's scale after the reference has been raised (which
+// it is when that has grown by 4), V's scales counted from 2^kLeastScale on: weights are at
+// most 2^104 then, and the sum of 2^23 of them is finite.
+constexpr float kMostProduct = 11.f, kLeastScale = -89.f;
 
 struct Decode8Params {
   void* out;
@@ -141,6 +148,17 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& first, uint32_t& sec
 }
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Exponent of x >= 0 (the whole number in the low bits of 2^23).
+__device__ __forceinline__ float exponent(float x) {
+  return __uint_as_float((__float_as_uint(x) >> 23) | 0x4b000000u) - (8388608.f + 127.f);
+}
 
 // Joins part `part` (M m-tiles) of n-tile nt of `count` records (from `base` on, every
 // `step`-th CTA's from `cta` on, slot 1 in CTA c0, 0 in the others): the normalised output
@@ -268,7 +286,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
   __shared__ uint64_t empty_bar[kMaxStages8];
   __shared__ uint64_t q_full[kMaxStages8 + 1];
   __shared__ uint64_t q_empty[kMaxStages8 + 1];
-  // What a warp tells the others of its kv head at a segment's end: bounds and sums of heads
+  // What a warp tells the others of its kv head at a segment's end: references and sums of heads
   // 2c, 2c + 1.  Two segments' worth: a warp can be writing the next one's
   // while another still reads.
   __shared__ float4 hand_ml_of[2][kWarps8][NT][4];
@@ -599,11 +617,10 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       q_parity ^= 1;
     }
 
-    float m[NT][2], l[NT][2], o[NT][KS][4];  // m: the score bound less 11
-    float vref = pow2(-126), vinv = pow2(126);  // V's scales so far are at most vref
+    float r[NT][2], l[NT][2], o[NT][KS][4];  // r: the weights' reference, a whole number
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = kLowest8;
+      r[nt][0] = r[nt][1] = kLowest8;
       l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
       for (int mt = 0; mt < KS; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
@@ -617,7 +634,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       const float* sc = my_scales + stage * TP * (scale_bytes / 4);
       const int last_live = live - (P - 1) * TG * kCachePage;  // of the last page
       const bool tail = last_live < kCachePage;
-      float x[P][NT][4], ks0[P], ks1[P], vs0[P], vs1[P];
+      float x[P][NT][4], ks0[P], ks1[P], vs0[P], vs1[P], lv0[P], lv1[P];
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         const float* si = sc + i * TG * (scale_bytes / 4);
@@ -625,6 +642,8 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
         ks1[i] = si[8];
         vs0[i] = si[16];
         vs1[i] = si[24];
+        lv0[i] = fmaxf(fast_log2(fabsf(vs0[i])), kLeastScale);
+        lv1[i] = fmaxf(fast_log2(fabsf(vs1[i])), kLeastScale);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) x[i][nt][0] = x[i][nt][1] = x[i][nt][2] = x[i][nt][3] = 0.f;
 #pragma unroll
@@ -642,17 +661,17 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
           }
         }
       }
-      // Scores in log2 units less m; behind the length, whatever the slots hold, none.
+      // Scores in log2 units less r; behind the length, whatever the slots hold, none.
       float y[P][NT][4];
       auto score = [&]() {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            y[i][nt][0] = fmaf(x[i][nt][0], fac[nt][0] * ks0[i], -m[nt][0]);
-            y[i][nt][1] = fmaf(x[i][nt][1], fac[nt][1] * ks0[i], -m[nt][1]);
-            y[i][nt][2] = fmaf(x[i][nt][2], fac[nt][0] * ks1[i], -m[nt][0]);
-            y[i][nt][3] = fmaf(x[i][nt][3], fac[nt][1] * ks1[i], -m[nt][1]);
+            y[i][nt][0] = fmaf(x[i][nt][0], fac[nt][0] * ks0[i], -r[nt][0]);
+            y[i][nt][1] = fmaf(x[i][nt][1], fac[nt][1] * ks0[i], -r[nt][1]);
+            y[i][nt][2] = fmaf(x[i][nt][2], fac[nt][0] * ks1[i], -r[nt][0]);
+            y[i][nt][3] = fmaf(x[i][nt][3], fac[nt][1] * ks1[i], -r[nt][1]);
           }
         }
         if (tail) {
@@ -669,55 +688,42 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
         }
       };
       score();
-      float ym = -INFINITY, vm = 0.f;
+      float most = -INFINITY;  // logarithm of the largest product
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        vm = fmaxf(vm, fmaxf(fabsf(vs0[i]), fabsf(vs1[i])));
+        float y0 = fmaxf(y[i][0][0], y[i][0][1]), y1 = fmaxf(y[i][0][2], y[i][0][3]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          ym = fmaxf(ym, fmaxf(fmaxf(y[i][nt][0], y[i][nt][1]), fmaxf(y[i][nt][2], y[i][nt][3])));
+        for (int nt = 1; nt < NT; ++nt) {
+          y0 = fmaxf(y0, fmaxf(y[i][nt][0], y[i][nt][1]));
+          y1 = fmaxf(y1, fmaxf(y[i][nt][2], y[i][nt][3]));
         }
+        most = fmaxf(most, fmaxf(y0 + lv0[i], y1 + lv1[i]));
       }
-      if (__any_sync(0xffffffffu, ym > 15.f || vm > vref)) {
-#pragma unroll
-        for (int b = 4; b < 32; b <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, b));
-        float down = 1.f;
-        if (vm > vref && vm < INFINITY) {
-          const int e = min(126, static_cast<int>(__float_as_uint(vm) >> 23) - 126);
-          down = vref;
-          vref = pow2(e);
-          vinv = pow2(-e);
-          down *= vinv;  // (sums below 2^-126 of it are gone)
-        }
+      if (__any_sync(0xffffffffu, most > kMostProduct + 4.f)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < P; ++i) {
-            const bool in0 = i < P - 1 || g < last_live, in1 = i < P - 1 || g + 8 < last_live;
-            if (in0) m0 = fmaxf(m0, x[i][nt][0] * (fac[nt][0] * ks0[i]));
-            if (in0) m1 = fmaxf(m1, x[i][nt][1] * (fac[nt][1] * ks0[i]));
-            if (in1) m0 = fmaxf(m0, x[i][nt][2] * (fac[nt][0] * ks1[i]));
-            if (in1) m1 = fmaxf(m1, x[i][nt][3] * (fac[nt][1] * ks1[i]));
-          }
+          for (int e = 0; e < 2; ++e) {
+            float to = -INFINITY;
 #pragma unroll
-          for (int b = 4; b < 32; b <<= 1) {
-            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, b));
-            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, b));
-          }
-          m0 = fmaxf(m[nt][0], m0 - 11.f);
-          m1 = fmaxf(m[nt][1], m1 - 11.f);
-          const float a0 = fast_exp2(m[nt][0] - m0), a1 = fast_exp2(m[nt][1] - m1);
-          m[nt][0] = m0;
-          m[nt][1] = m1;
-          l[nt][0] *= a0;
-          l[nt][1] *= a1;
+            for (int i = 0; i < P; ++i) {
+              const float s0 = x[i][nt][e] * (fac[nt][e] * ks0[i]);
+              const float s1 = x[i][nt][2 + e] * (fac[nt][e] * ks1[i]);
+              // (Scales are finite up to 2^128; infinite ones make infinite products.)
+              if (i < P - 1 || g < last_live) to = fmaxf(to, s0 + fminf(lv0[i], 128.f));
+              if (i < P - 1 || g + 8 < last_live) to = fmaxf(to, s1 + fminf(lv1[i], 128.f));
+            }
 #pragma unroll
-          for (int mt = 0; mt < KS; ++mt) {
-            o[nt][mt][0] *= a0 * down;
-            o[nt][mt][1] *= a1 * down;
-            o[nt][mt][2] *= a0 * down;
-            o[nt][mt][3] *= a1 * down;
+            for (int b = 4; b < 32; b <<= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, b));
+            to = fmaxf(r[nt][e], ceilf(to - kMostProduct));
+            const float down = fast_exp2(r[nt][e] - to);
+            r[nt][e] = to;
+            l[nt][e] *= down;
+#pragma unroll
+            for (int mt = 0; mt < KS; ++mt) {
+              o[nt][mt][e] *= down;
+              o[nt][mt][2 + e] *= down;
+            }
           }
         }
         score();
@@ -725,7 +731,6 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         uint32_t pb[NT][2];
-        const float v0 = vs0[i] * vinv, v1 = vs1[i] * vinv;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float p0 = fast_exp2(y[i][nt][0]), p1 = fast_exp2(y[i][nt][1]);
@@ -733,8 +738,8 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
           l[nt][0] += p0 + p2;
           l[nt][1] += p1 + p3;
           // C fragment (row = token, col = head) -> B fragment (k = token, n = head).
-          pb[nt][0] = movmatrix_trans(Elt<__half>::pack(p0 * v0, p1 * v0));
-          pb[nt][1] = movmatrix_trans(Elt<__half>::pack(p2 * v1, p3 * v1));
+          pb[nt][0] = movmatrix_trans(Elt<__half>::pack(p0 * vs0[i], p1 * vs0[i]));
+          pb[nt][1] = movmatrix_trans(Elt<__half>::pack(p2 * vs1[i], p3 * vs1[i]));
         }
 #pragma unroll
         for (int kk = 0; kk < D / 32; ++kk) {
@@ -801,7 +806,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
         l[nt][0] += __shfl_xor_sync(0xffffffffu, l[nt][0], b);
         l[nt][1] += __shfl_xor_sync(0xffffffffu, l[nt][1], b);
       }
-      if (g == 0) hand_ml[cw][nt][c] = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
+      if (g == 0) hand_ml[cw][nt][c] = make_float4(r[nt][0], r[nt][1], l[nt][0], l[nt][1]);
     }
     if (alone) {
       __syncwarp();
@@ -814,7 +819,9 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       // Lane (g, c) looks at warp g's; the butterflies leave every lane with the same sums.
       float4 ml = make_float4(kLowest8, kLowest8, 0.f, 0.f);
       if (g < active) ml = hand_ml[g * hpc + h][nt][c];
-      float top0 = ml.x, top1 = ml.y;
+      // A warp's sum may be far from 1: its exponent counts with the reference.  (What is lost
+      // of the others' is below 2^-22 of the whole.)
+      float top0 = ml.x + exponent(ml.z), top1 = ml.y + exponent(ml.w);
 #pragma unroll
       for (int b = 4; b < 32; b <<= 1) {
         top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, b));
@@ -831,8 +838,8 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       // A cut piece whose weights are all zero (scores of -inf) adds nothing.
       const float r0 = !whole && sum0 == 0.f ? 0.f : __fdividef(1.f, sum0);
       const float r1 = !whole && sum1 == 0.f ? 0.f : __fdividef(1.f, sum1);
-      const float a0 = fast_exp2(m[nt][0] - top0) * r0 * vref;
-      const float a1 = fast_exp2(m[nt][1] - top1) * r1 * vref;
+      const float a0 = fast_exp2(r[nt][0] - top0) * r0;
+      const float a1 = fast_exp2(r[nt][1] - top1) * r1;
 #pragma unroll
       for (int mt = 0; mt < KS; ++mt) {
         o[nt][mt][0] *= a0;
