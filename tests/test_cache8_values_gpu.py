@@ -11,7 +11,13 @@ fp16: 2^-11 of itself, or, where that is more, half of fp16's smallest step, 2^-
 with the largest product of the warp's tokens at 2^10 or above: 2^-35 of the
 largest, W = max_t p_t amax_t, for each of the n tokens (a code's 127 or 448 is
 amax over its scale).  With A = sum_t p_t |V_t| and one rounding of the result (u):
-    2 (sum_t p_t e_t |V_t| + |out| sum_t p_t e_t) + 2 * 2^-11 A + n 2^-35 W + u |out|
+    2 (sum_t p_t e_t |V_t| + |out| sum_t p_t e_t) + 2 * 2^-11 A + n 2^-35 W + u |out| + 2^-25
+(2^-25: half of fp16's smallest step, for results near zero).
+
+For fp16 outputs what the rounding to fp16 left is kept too (2^-22).  A weight's
+logarithm is then the largest term: fp32 below 2^5 (2^-20, and 2^-22 of the exponential),
+in cut sequences once more below 2^7 (2^-18), in the products and in the sum:
+2^-16 A in place of 2 * 2^-11 A.
 """
 
 from __future__ import annotations
@@ -65,7 +71,7 @@ def _built(scores, sizes, G, D, dtype, fmt, seed):
                 block_tables=i32(order[None, :pages]), seq_lens=i32([n]))
 
 
-def _off(c, got):
+def _off(c, got, weights=2 * 2.0 ** -11):
     """The largest error as a share of its bound."""
     q, cache, n = c["q"][0].double(), c["cache"], int(c["seq_lens"][0])
     G, D = q.shape
@@ -77,8 +83,8 @@ def _off(c, got):
     e = (D + 8) * 2.0 ** -23 * (q.abs() @ k.abs().T) / math.sqrt(D)
     out, a = p @ v, p @ v.abs()
     w = (p * v.abs().amax(1)).amax(1, keepdim=True)
-    tol = 2 * ((p * e) @ v.abs() + out.abs() * (p * e).sum(1, keepdim=True)) + 2 * 2.0 ** -11 * a \
-        + n * 2.0 ** -35 * w + U[got.dtype] * out.abs()
+    tol = 2 * ((p * e) @ v.abs() + out.abs() * (p * e).sum(1, keepdim=True)) + weights * a \
+        + n * 2.0 ** -35 * w + U[got.dtype] * out.abs() + 2.0 ** -25
     assert torch.isfinite(got).all()
     return float(((got[0].double() - out).abs() / tol).max())
 
@@ -105,3 +111,11 @@ def test_weights_and_values_that_drift_apart(G, D, dtype, fmt, rise, fall, n):
     step = np.arange(n) * 16 // n
     c = _built(math.log(2.0) * rise * step, np.exp2(-1.0 * fall * step), G, D, dtype, fmt, n)
     assert _off(c, K.paged_decode_attention_cache8(**c)) <= 1
+
+
+@pytest.mark.parametrize("n", [5, 137, 2000, 30000])
+@pytest.mark.parametrize("fmt", [INT8, E4M3])
+@pytest.mark.parametrize("G, D", [(1, 64), (8, 64), (4, 128), (16, 64), (11, 128)])
+def test_fp16_outputs_are_rounded_once(G, D, fmt, n):
+    c = _case([n], G, 1, D, torch.float16, fmt, n + G, spare=False)
+    assert _off(c, K.paged_decode_attention_cache8(**c), 2.0 ** -16) <= 1
