@@ -404,8 +404,9 @@ int vmps_w4_gemm(void* out, int64_t out_row_stride, const void* x, int64_t x_row
  * both contiguous and 16-byte aligned.  The value stored is code * scale of its
  * token, head and kind.  Written by vmps_norm_rope_and_cache, the scale is the
  * largest magnitude of the token's head_dim values over 127 (int8) or 448
- * (e4m3) and the code the value over the scale, to nearest with ties to even
- * (computed in fp32: a value within 2^-21 of a tie may go to either side).  Rows
+ * (e4m3) and the code the value times that over the largest magnitude, to nearest
+ * with ties to even (rotated and normalised values are fp32, and within 2^-21 of a tie
+ * may go to either side; the others go where the exact quotient does).  Rows
  * whose largest magnitude is below 2^-100 are stored as zeros with scale 0; a
  * row that holds an infinity or a NaN has scale NaN and reads as NaN.
  */

@@ -66,30 +66,6 @@ __device__ __forceinline__ void rotation(int pos, float inv_freq, float* cs, flo
   *sn = (quarter & 2) ? -y : y;
 }
 
-// Two fp32 values in one 64-bit register: Blackwell multiplies and adds both at once.
-using f2 = unsigned long long;
-
-__device__ __forceinline__ f2 pair(float a, float b) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 split(f2 x) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-  return r;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // NaN if one of them is (0x7fffffff, above every number's bits).
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -267,11 +243,9 @@ norm_rope_cache_kernel(const StoreParams p) {
         const bool some = finite && a >= kCache8Tiny;
         uint2 wl = make_uint2(0u, 0u), wh = make_uint2(0u, 0u);
         if (some) {
-          const float inv = Code::kTop / a;
-          wl = make_uint2(Code::pack4(split(lo[0]), split(lo[1]), inv),
-                          Code::pack4(split(lo[2]), split(lo[3]), inv));
-          wh = make_uint2(Code::pack4(split(hi[0]), split(hi[1]), inv),
-                          Code::pack4(split(hi[2]), split(hi[3]), inv));
+          const Quotient over(a, Code::kTop);
+          wl = make_uint2(Code::pack4(over(lo[0]), over(lo[1])), Code::pack4(over(lo[2]), over(lo[3])));
+          wh = make_uint2(Code::pack4(over(hi[0]), over(hi[1])), Code::pack4(over(hi[2]), over(hi[3])));
         }
         uint8_t* dst = static_cast<uint8_t*>(p.cache) +
                        (((blk * 2 + (is_v ? 1 : 0)) * kCachePage + off) * p.n_kv + hk) * D + c * 8;

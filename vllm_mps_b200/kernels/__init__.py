@@ -1056,7 +1056,8 @@ def quantize_cache8(x: torch.Tensor, dtype: torch.dtype = torch.int8,
     amax = x.abs().amax(-1)
     fine = torch.isfinite(x).all(-1)
     some = fine & (amax >= 2.0 ** -100)
-    y = torch.where(some.unsqueeze(-1), x * (top / torch.where(some, amax, 1.0)).unsqueeze(-1), 0.0)
+    y = x.double() * top / torch.where(some, amax, 1.0).double().unsqueeze(-1)  # ties stay ties
+    y = torch.where(some.unsqueeze(-1), y, 0.0).float()
     codes = (torch.round(y) if dtype == torch.int8 else y.clamp(-top, top)).to(dtype)
     return codes, torch.where(some, amax / top, torch.where(fine, 0.0, float("nan")))
 
