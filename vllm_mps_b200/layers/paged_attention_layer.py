@@ -92,21 +92,53 @@ class PagedAttentionLayer(nn.Module):
         return cls(layer_idx, model_config, kv_cache_manager, memory_pool, W_Q, W_K, W_V, W_O, rot,
                    on(q_norm), on(k_norm), eps)
 
-    @staticmethod
-    def _head_norms(layer, d: int):
-        """(q weight, k weight, eps) of an attention module's norms over each head, if it has them."""
+    @classmethod
+    def _head_norms(cls, layer, d: int):
+        """(q weight, k weight, eps) of an attention module's norms over each head, if it has them.
+
+        Only norms that the kernels compute are taken; a layer with others is refused.
+        """
         if isinstance(layer, PagedAttentionLayer):
             return layer.q_norm_weight, layer.k_norm_weight, layer.norm_eps
-        weights, eps = [], 1e-6
-        for name in ("q_norm", "k_norm"):
-            norm = getattr(layer, name, None)
-            w = getattr(norm, "weight", None)
-            if w is None or w.numel() != d:
-                weights.append(None)
-                continue
-            weights.append(w)
-            eps = float(getattr(norm, "variance_epsilon", getattr(norm, "eps", None) or eps))
-        return weights[0], weights[1], eps
+        for name, module in layer.named_children():
+            if "norm" in name and name not in ("q_norm", "k_norm") and not isinstance(module, nn.Identity):
+                raise NotImplementedError(f"attention with {name} ({type(module).__name__}): norms of "
+                                          "queries and keys are q_norm and k_norm")
+        q, k = (cls._rms_norm(getattr(layer, name, None), name, d) for name in ("q_norm", "k_norm"))
+        if q and k and q[1] != k[1]:
+            raise NotImplementedError(f"q_norm and k_norm with different eps ({q[1]:g}, {k[1]:g})")
+        return q and q[0], k and k[0], (q or k or (None, 1e-6))[1]
+
+    @staticmethod
+    def _rms_norm(module, name: str, d: int):
+        """(weight, eps) of an RMS norm over ``d`` values, by what the module computes: some
+        modules under these names take off a mean, multiply by 1 + weight or span all heads."""
+        if module is None or isinstance(module, nn.Identity):
+            return None
+        weight = getattr(module, "weight", None)
+        eps = getattr(module, "variance_epsilon", getattr(module, "eps", None))
+        eps = torch.finfo(torch.float32).eps if eps is None else float(eps)
+        plain = weight is not None and weight.numel() == d
+        if plain:
+            # Rows with a mean, of sizes 1, 30 and that at which eps is half of the sum.
+            with torch.no_grad():
+                x = 0.5 + torch.randn((3, d), generator=torch.Generator().manual_seed(0))
+                x *= torch.tensor([[1.0], [30.0], [max(eps, 1e-8) ** 0.5]])
+                x = x.to(weight)
+                want = x.float() * torch.rsqrt(x.float().square().mean(-1, keepdim=True) + eps)
+                want *= weight.float().flatten()
+                try:
+                    got = module(x.view(1, 3, 1, d)).view(3, d).float()
+                except Exception:  # made for another shape
+                    plain = False
+                else:
+                    # (The module's own roundings, one or two.)
+                    off = 2 * torch.finfo(weight.dtype).eps
+                    plain = bool(((got - want).abs() <= off * want.abs() + 1e-6).all())
+        if not plain:
+            raise NotImplementedError(f"attention whose {name} ({type(module).__name__}) is not "
+                                      f"x * weight / sqrt(mean(x^2) + eps) over a head's {d} values")
+        return weight, eps
 
     # ── forward ─────────────────────────────────────────────────────────────
 
