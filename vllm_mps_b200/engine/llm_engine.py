@@ -377,7 +377,7 @@ class LLMEngine:
         dev = self.model_config.device
         meta = la.build_prefill_metadata(self.kv_cache_manager,
                                          [(s.seq_id, qs, ql) for s, qs, ql in pieces],
-                                         BLOCK_SIZE, dev)
+                                         BLOCK_SIZE, dev, isinstance(self.memory_pool, CUDACache8Pool))
         toks = [t for s, qs, ql in pieces for t in s.token_ids[qs:qs + ql]]
         if self._graphs is not None and self._graphs.fused:
             toks += [0] * (self._graphs.padded_rows(len(toks)) - len(toks))

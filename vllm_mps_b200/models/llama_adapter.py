@@ -75,16 +75,16 @@ def build_step_metadata(kv_cache_manager, seq_ids, positions, seq_lens, block_si
     return meta
 
 
-def build_prefill_metadata(kv_cache_manager, pieces, block_size: int,
-                           device: torch.device) -> SimpleNamespace:
+def build_prefill_metadata(kv_cache_manager, pieces, block_size: int, device: torch.device,
+                           read_back: bool = False) -> SimpleNamespace:
     """Device metadata of one prefill chunk (one pinned host buffer, one copy).
 
     ``pieces``: ``(seq_id, q_start, q_len)`` per sequence; the chunk's rows
     are the ``q_len`` tokens at positions ``q_start ..`` of each sequence in
     order.  Per row: position and slot (kernel 1 writes each row's K/V); per
     sequence: block table, ``q_start``, ``q_len`` and first row ``cu_q``
-    (kernel 3 attends each row to its sequence's slots ``0..position``).  For
-    pools whose pages are read back first: ``kv_lens``, the slots each
+    (kernel 3 attends each row to its sequence's slots ``0..position``).
+    ``read_back``, for pools whose pages are read back first: ``kv_lens``, the slots each
     sequence holds with the chunk, and ``dst_tensor``, tables that number
     their ``pages`` pages through.
     """
@@ -102,27 +102,28 @@ def build_prefill_metadata(kv_cache_manager, pieces, block_size: int,
     seq_of_row = np.repeat(np.arange(S), q_lens)
     pos = (np.arange(rows) - cu[seq_of_row] + q_start[seq_of_row]).astype(np.int64)
     slots = bt[seq_of_row, pos // block_size].astype(np.int64) * block_size + pos % block_size
-    kv_lens = q_start + q_lens
-    kv_pages = -(-kv_lens // block_size)
-    dst = np.zeros((S, max_blocks), dtype=np.int32)
-    at = 0
-    for i, n in enumerate(kv_pages.tolist()):
-        dst[i, :n] = np.arange(at, at + n)
-        at += n
-    flat = np.concatenate([bt.reshape(-1), q_start, q_lens, cu, pos, slots, kv_lens,
-                           dst.reshape(-1)]).astype(np.int32)
+    parts = [bt.reshape(-1), q_start, q_lens, cu, pos, slots]
+    if read_back:
+        kv_lens = q_start + q_lens
+        ends = np.cumsum(-(-kv_lens // block_size))  # of the sequences' pages, numbered through
+        page = (ends + kv_lens // -block_size)[:, None] + np.arange(max_blocks)
+        parts += [kv_lens, np.where(page < ends[:, None], page, 0).reshape(-1)]
+    flat = np.concatenate(parts).astype(np.int32)
     pinned = torch.from_numpy(flat)
     if device.type == "cuda":
         pinned = pinned.pin_memory()
     dev = pinned.to(device, non_blocking=True)
     o = S * max_blocks
     tail = o + 3 * S + 2 * rows
-    return SimpleNamespace(
+    meta = SimpleNamespace(
         bt_tensor=dev[:o].view(S, max_blocks), q_start=dev[o:o + S], q_lens=dev[o + S:o + 2 * S],
         cu_q=dev[o + 2 * S:o + 3 * S], pos_tensor=dev[o + 3 * S:o + 3 * S + rows],
-        slot_mapping=dev[o + 3 * S + rows:tail], kv_lens=dev[tail:tail + S],
-        dst_tensor=dev[tail + S:].view(S, max_blocks), pages=at,
-        max_q_len=int(q_lens.max()) if S else 0, rows=rows)
+        slot_mapping=dev[o + 3 * S + rows:tail], max_q_len=int(q_lens.max()) if S else 0, rows=rows)
+    if read_back:
+        meta.kv_lens = dev[tail:tail + S]
+        meta.dst_tensor = dev[tail + S:].view(S, max_blocks)
+        meta.pages = int(ends[-1]) if S else 0
+    return meta
 
 
 class LlamaAdapter(BaseModelAdapter):
