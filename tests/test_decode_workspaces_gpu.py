@@ -1,0 +1,56 @@
+"""Workspaces of the decode kernels: grown, captured, abandoned, of many streams."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_cache8_decode_gpu import INT8, _case
+from vllm_mps_b200 import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+
+def _small(seed=1):
+    return _case([3000, 17], 8, 2, 64, torch.float16, INT8, seed)
+
+
+def _large(seed=2):
+    return _case([2000, 900], 32, 2, 128, torch.bfloat16, INT8, seed)
+
+
+def _capture(c, ws):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = K.paged_decode_attention_cache8(**c, workspace=ws)
+    return graph, out
+
+
+def test_outgrown_buffers_stay_for_the_graphs_that_use_them():
+    small, large, ws = _small(), _large(), K.DecodeWorkspace()
+    want = K.paged_decode_attention_cache8(**small, workspace=ws)
+    first = next(iter(ws._buf.values()))
+    graph, out = _capture(small, ws)
+    K.paged_decode_attention_cache8(**large, workspace=ws)
+    assert next(iter(ws._buf.values())).numel() > first.numel() and ws._outgrown[0] is first
+    # What would be handed out in its place is not written to.
+    others = [torch.full((n,), 7, dtype=torch.uint8, device="cuda") for n in [first.numel()] * 4]
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+    assert all((t == 7).all() for t in others)
+
+
+def test_a_capture_before_any_call():
+    """The graph has a buffer of its own; the workspace is as it was."""
+    small, ws = _small(), K.DecodeWorkspace()
+    want = K.paged_decode_attention_cache8(**small)
+    torch.cuda.synchronize()
+    graph, out = _capture(small, ws)
+    assert not ws._buf
+    assert torch.equal(K.paged_decode_attention_cache8(**small, workspace=ws), want)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)

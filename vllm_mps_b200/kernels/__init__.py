@@ -304,17 +304,40 @@ def rope_reshape_and_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 # ── kernel 2 ─────────────────────────────────────────────────────────────────
 
 
+#: A decode workspace's first bytes, which hold counters that are zero between calls.
+_WORKSPACE_COUNTER_BYTES = 1 << 20
+
+
 class DecodeWorkspace:
     """Zero-initialised scratch for the decode kernels, grown on demand.
 
     Holds the split-K partial results and per-sequence arrival counters of
     one call; the kernel leaves the counters at zero, so one buffer is reused
     across calls on the same stream.  Calls on different streams that may
-    overlap need different workspaces.
+    overlap need different workspaces.  A graph may be captured with it; a
+    capture that finds it too small gets a buffer of the graph's own.
     """
 
     def __init__(self) -> None:
         self._buf: dict[torch.device, torch.Tensor] = {}
+        #: Outgrown buffers: graphs captured with them go on using them.
+        self._outgrown: list[torch.Tensor] = []
+
+    def _at_least(self, device: torch.device, need: int) -> torch.Tensor:
+        buf = self._buf.get(device)
+        if buf is not None and buf.numel() >= need:
+            return buf
+        if torch.cuda.is_current_stream_capturing():
+            # Zeroed by every replay; other calls must not meet it before the first.
+            own = torch.empty(need, dtype=torch.uint8, device=device)
+            own[:_WORKSPACE_COUNTER_BYTES].zero_()
+            return own
+        # Grow geometrically; torch allocations are 512-byte aligned.
+        if buf is not None:
+            self._outgrown.append(buf)
+            need = max(need, 2 * buf.numel())
+        buf = self._buf[device] = torch.zeros(need, dtype=torch.uint8, device=device)
+        return buf
 
     def get(self, device: torch.device, num_seqs: int, n_q: int, n_kv: int, d: int,
             dtype: torch.dtype) -> torch.Tensor:
@@ -324,23 +347,12 @@ class DecodeWorkspace:
         if need == 0:
             raise NotImplementedError(
                 f"paged_decode_attention: n_q={n_q} n_kv={n_kv} head_dim={d} not supported")
-        buf = self._buf.get(device)
-        if buf is None or buf.numel() < need:
-            # Grow geometrically; torch allocations are 512-byte aligned.
-            size = max(need, 0 if buf is None else 2 * buf.numel())
-            buf = torch.zeros(size, dtype=torch.uint8, device=device)
-            self._buf[device] = buf
-        return buf
+        return self._at_least(device, need)
 
     def get_cache8(self, device: torch.device, num_seqs: int, n_q: int, n_kv: int,
                    d: int) -> torch.Tensor:
         """The same buffer, for :func:`paged_decode_attention_cache8`."""
-        need = _cache8_workspace_bytes(device.index, num_seqs, n_q, n_kv, d)
-        buf = self._buf.get(device)
-        if buf is None or buf.numel() < need:
-            size = max(need, 0 if buf is None else 2 * buf.numel())
-            buf = self._buf[device] = torch.zeros(size, dtype=torch.uint8, device=device)
-        return buf
+        return self._at_least(device, _cache8_workspace_bytes(device.index, num_seqs, n_q, n_kv, d))
 
 
 _default_workspace = DecodeWorkspace()
