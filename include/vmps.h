@@ -480,7 +480,7 @@ int vmps_read_cache8(void* pool, int pool_blocks, const int32_t* dst_tables, con
  * (vmps_paged_decode_workspace_init); every call leaves it zero, so one
  * workspace serves calls of any shape, and vmps_paged_decode_attention's too.
  * Calls that may overlap on the GPU need different workspaces; after error bit
- * 8 it is to be zeroed again.  out must not be q's memory.  0 bytes: the shape
+ * 8, when the calls that used it have ended, it is to be zeroed again.  out must not be q's memory.  0 bytes: the shape
  * is not supported.
  */
 size_t vmps_paged_decode_cache8_workspace_bytes(int num_seqs, int n_q, int n_kv, int head_dim);

@@ -54,3 +54,22 @@ def test_a_capture_before_any_call():
         out.zero_()
         graph.replay()
         assert torch.equal(out, want)
+
+
+def test_counters_are_zeroed_after_a_wait_that_gave_up(monkeypatch):
+    """A call that gave up leaves counters above zero (put there here by hand)."""
+    class GaveUp:
+        def vmps_debug_error_word(self, stream, word):
+            word._obj.value = 8
+            return 0
+
+    c, ws = _small(), K.DecodeWorkspace()
+    want = K.paged_decode_attention_cache8(**c, workspace=ws)
+    K.paged_decode_attention_cache8(**c)
+    for buf in (*ws._buf.values(), *K._cache8_buffers.values()):
+        buf[:K._CACHE8_COUNTER_BYTES] = 1
+    with monkeypatch.context() as m:
+        m.setattr(K, "load_library", GaveUp)
+        assert K.error_word() == 8
+    assert torch.equal(K.paged_decode_attention_cache8(**c, workspace=ws), want)
+    assert torch.equal(K.paged_decode_attention_cache8(**c), want)

@@ -33,6 +33,7 @@ import math
 import os
 import struct
 import threading
+import weakref
 
 import torch
 
@@ -306,6 +307,7 @@ def rope_reshape_and_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 #: A decode workspace's first bytes, which hold counters that are zero between calls.
 _WORKSPACE_COUNTER_BYTES = 1 << 20
+_workspaces: "weakref.WeakSet[DecodeWorkspace]" = weakref.WeakSet()
 
 
 class DecodeWorkspace:
@@ -322,6 +324,7 @@ class DecodeWorkspace:
         self._buf: dict[torch.device, torch.Tensor] = {}
         #: Outgrown buffers: graphs captured with them go on using them.
         self._outgrown: list[torch.Tensor] = []
+        _workspaces.add(self)
 
     def _at_least(self, device: torch.device, need: int) -> torch.Tensor:
         buf = self._buf.get(device)
@@ -338,6 +341,13 @@ class DecodeWorkspace:
             need = max(need, 2 * buf.numel())
         buf = self._buf[device] = torch.zeros(need, dtype=torch.uint8, device=device)
         return buf
+
+    def reset(self, device: torch.device | None = None) -> None:
+        """Zero the counters again, on one device or all: after error bit 8, once the calls
+        that used them have ended.  ``error_word`` does it for every workspace."""
+        for buf in (*self._buf.values(), *self._outgrown):
+            if device is None or buf.device == device:
+                buf[:_WORKSPACE_COUNTER_BYTES].zero_()
 
     def get(self, device: torch.device, num_seqs: int, n_q: int, n_kv: int, d: int,
             dtype: torch.dtype) -> torch.Tensor:
@@ -1335,12 +1345,24 @@ def stage_copy(dst: torch.Tensor, src: torch.Tensor) -> torch.Tensor:
 
 
 def error_word(device: torch.device | int | None = None) -> int:
-    """Read and clear the device error word (bit meanings in include/vmps.h)."""
+    """Read and clear the device error word (bit meanings in include/vmps.h).
+
+    After bit 8 (a wait that gave up) the device is waited for and the counters of its
+    decode workspaces are zeroed, all but those that a caller passes as tensors.
+    """
     dev = torch.device("cuda", device) if isinstance(device, int) else (device or torch.device("cuda"))
     word = ctypes.c_int(0)
     lib = load_library()
     with torch.cuda.device(dev):
         _check(lib.vmps_debug_error_word(_stream(dev), ctypes.byref(word)), "debug_error_word")
+        if word.value & 8:
+            torch.cuda.synchronize()
+            index = torch.cuda.current_device()
+            for key in [k for k in _cache8_buffers if k[0] == index]:
+                del _cache8_buffers[key]
+            for workspace in _workspaces:
+                workspace.reset(torch.device("cuda", index))
+            torch.cuda.synchronize()
     return word.value
 
 
