@@ -73,3 +73,19 @@ def test_counters_are_zeroed_after_a_wait_that_gave_up(monkeypatch):
         assert K.error_word() == 8
     assert torch.equal(K.paged_decode_attention_cache8(**c, workspace=ws), want)
     assert torch.equal(K.paged_decode_attention_cache8(**c), want)
+
+
+def test_many_streams(monkeypatch):
+    monkeypatch.setattr(K, "_CACHE8_STREAMS", 3)
+    cases = [_small(seed) for seed in range(6)]
+    want = [K.paged_decode_attention_cache8(**c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[] for _ in cases]
+    for _ in range(5):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(K.paged_decode_attention_cache8(**c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
+    assert len(K._cache8_buffers) <= 3

@@ -1241,8 +1241,11 @@ def _cache8_workspace_bytes(device: int, num_seqs: int, n_q: int, n_kv: int, d: 
 
 #: Of a workspace's first MiB what the 8-bit decode counts in.
 _CACHE8_COUNTER_BYTES = 128 << 10
-#: Zeroed workspaces of eager calls that bring none, one per device and stream.
+#: Zeroed workspaces of eager calls that bring none, one per device and stream, for the last
+#: streams that had none yet.  (One that goes is memory of its stream's: what is under way on
+#: the stream ends before the allocator hands it out again.)
 _cache8_buffers: dict[tuple[int, int], torch.Tensor] = {}
+_CACHE8_STREAMS = 32
 #: Their sizes: one for a device, head size and 8 or 16 query heads a kv head.
 _cache8_sizes: dict[tuple[int, int, bool], int] = {}
 
@@ -1261,6 +1264,8 @@ def _cache8_workspace(ref: torch.Tensor, dev: int, B: int, n_q: int, n_kv: int, 
     buf = _cache8_buffers.get(key)
     if buf is None or buf.numel() < need:
         buf = _cache8_buffers[key] = ref.new_zeros(need, dtype=torch.uint8)
+        while len(_cache8_buffers) > _CACHE8_STREAMS:
+            del _cache8_buffers[next(iter(_cache8_buffers))]
     return buf
 
 
