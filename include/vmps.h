@@ -427,7 +427,7 @@ int vmps_w4_gemm(void* out, int64_t out_row_stride, const void* x, int64_t x_row
  *
  * q_out, q, k, v: num_rows rows of heads [heads][head_dim], row strides in
  * elements (multiples of 8, at least a row); q_out may be q where the strides
- * agree.  n_q 0: keys and values alone.  slot_mapping int32[num_rows]: block *
+ * agree, and overlaps neither q otherwise, nor k or v.  n_q 0: keys and values alone.  slot_mapping int32[num_rows]: block *
  * 16 + slot, negative: nothing is cached for the row.  Two rows of a call must
  * not share a slot.  A negative position sets error bit 16 and skips the row, a
  * slot outside the cache sets bit 1 and is not written.  scales: NULL for
@@ -480,7 +480,7 @@ int vmps_read_cache8(void* pool, int pool_blocks, const int32_t* dst_tables, con
  * (vmps_paged_decode_workspace_init); every call leaves it zero, so one
  * workspace serves calls of any shape, and vmps_paged_decode_attention's too.
  * Calls that may overlap on the GPU need different workspaces; after error bit
- * 8, when the calls that used it have ended, it is to be zeroed again.  out must not be q's memory.  0 bytes: the shape
+ * 8, when the calls that used it have ended, it is to be zeroed again.  out must not overlap q.  0 bytes: the shape
  * is not supported.
  */
 size_t vmps_paged_decode_cache8_workspace_bytes(int num_seqs, int n_q, int n_kv, int head_dim);

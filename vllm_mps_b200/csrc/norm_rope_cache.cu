@@ -15,6 +15,7 @@
 // 72 registers and 28 warps an SM 35.4 us, with 80 and 24 39.8, with 64 and 32, where a
 // few values are spilled, 36.9.
 #include "cache8.cuh"
+#include "rows_overlap.h"
 #include "vmps_abi_internal.h"
 
 namespace vmps {
@@ -361,6 +362,14 @@ extern "C" int vmps_norm_rope_and_cache(
   if (num_rows > 1 && (q_row_stride < q_row || q_out_row_stride < q_row || k_row_stride < kv_row ||
                        v_row_stride < kv_row)) {
     return fail(VMPS_ERR_INVALID_ARG, "%s: row stride smaller than a row", what);
+  }
+  // Rows are read and written by several warps in no order.
+  const bool in_place = q_out == q && (num_rows == 1 || q_out_row_stride == q_row_stride);
+  if ((!in_place && rows_overlap(q_out, q_out_row_stride * 2, q_row * 2, q, q_row_stride * 2,
+                                 q_row * 2, num_rows)) ||
+      rows_overlap(q_out, q_out_row_stride * 2, q_row * 2, k, k_row_stride * 2, kv_row * 2, num_rows) ||
+      rows_overlap(q_out, q_out_row_stride * 2, q_row * 2, v, v_row_stride * 2, kv_row * 2, num_rows)) {
+    return fail(VMPS_ERR_INVALID_ARG, "%s: q_out overlaps q (but is not q), k or v", what);
   }
   if (!(eps >= 0.f)) return fail(VMPS_ERR_INVALID_ARG, "%s: eps %g", what, (double)eps);
   int* err = nullptr;

@@ -57,6 +57,7 @@
 
 #include "cache8.cuh"
 #include "cache8_plan.h"
+#include "rows_overlap.h"
 #include "vmps_abi_internal.h"
 
 namespace vmps {
@@ -1144,6 +1145,10 @@ extern "C" int vmps_paged_decode_attention_cache8(
   }
   if (num_seqs > 1 && q_row_stride < static_cast<int64_t>(n_q) * head_dim) {
     return fail(VMPS_ERR_INVALID_ARG, "%s: row stride smaller than a row", what);
+  }
+  const int64_t q_row = static_cast<int64_t>(n_q) * head_dim;
+  if (rows_overlap(out, q_row * 2, q_row * 2, q, q_row_stride * 2, q_row * 2, num_seqs)) {
+    return fail(VMPS_ERR_INVALID_ARG, "%s: out overlaps q", what);
   }
   if (!(scale > 0.f) || !(scale < 1e30f)) {
     return fail(VMPS_ERR_INVALID_ARG, "%s: scale %g", what, (double)scale);
