@@ -191,9 +191,11 @@ class CUDACache8Pool(CUDAMemoryPool):
                          device: torch.device | str, num_layers: int | None = None,
                          fraction: float = 0.85, max_blocks: int | None = None,
                          code_dtype: torch.dtype = torch.int8) -> "CUDACache8Pool":
+        """Size the pool, and the 16-bit pages of one layer that :meth:`read_back` may come to
+        hold for its blocks, to ``fraction`` of the device's free memory."""
         device = torch.device(device)
         free, _ = torch.cuda.mem_get_info(device)
-        per_block = 2 * block_size * n_heads * (d_k + 4) * (num_layers or 1)
+        per_block = 2 * block_size * n_heads * ((d_k + 4) * (num_layers or 1) + 2 * d_k)
         n = int(free * fraction) // per_block
         if max_blocks is not None:
             n = min(n, max_blocks)
@@ -214,11 +216,16 @@ class CUDACache8Pool(CUDAMemoryPool):
     def read_back(self, layer: int, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                   dst_tables: torch.Tensor, pages: int) -> torch.Tensor:
         """16-bit pages of the sequences, at blocks ``dst_tables`` (below ``pages``) of a
-        pool that the next call overwrites (calls are ordered by the stream)."""
+        pool that the next call overwrites (calls are ordered by the stream).  It is kept, as
+        large as the most pages so far; a pool whose sequences share no blocks has at most
+        ``num_blocks``."""
         from vllm_mps_b200.kernels import read_cache8
 
-        if self._scratch is None or self._scratch.shape[0] < pages:
-            self._scratch = torch.empty((max(1, pages), 2, self.block_size, self.n_heads, self.d_k),
+        held = 0 if self._scratch is None else self._scratch.shape[0]
+        if held == 0 or held < pages:
+            self._scratch = None  # its memory may serve the larger one
+            pages = max(1, pages, min(2 * held, self.num_blocks))
+            self._scratch = torch.empty((pages, 2, self.block_size, self.n_heads, self.d_k),
                                         dtype=self.dtype, device=self.device)
         return read_cache8(self.layer(layer), block_tables, seq_lens, self._scratch, dst_tables)
 
