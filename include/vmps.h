@@ -465,9 +465,8 @@ int vmps_read_cache8(void* pool, int pool_blocks, const int32_t* dst_tables, con
  * with K and V read from codes and scales.
  *   out[i][h] = softmax_t(scale * q[i][h] . K[t][h / G]) . V[t][h / G], t < seq_lens[i]
  * Scores, maxima and sums are fp32; for its products with V's codes a softmax weight
- * times V's scale is kept to 2^-22 of itself (2^-11 for bf16 outputs of more than 8
- * query heads a kv head), or 2^-35 of the head's largest such product where that is
- * more.  q is [num_seqs][n_q][head_dim] with a row
+ * times V's scale is kept to 2^-22 of itself for fp16 outputs, and rounded to fp16 (2^-11)
+ * for bf16 ones, or by 2^-35 of the head's largest such product where that is more.  q is [num_seqs][n_q][head_dim] with a row
  * stride (a multiple of 8 elements), out contiguous, both 16-byte aligned.  A
  * sequence of length 0 gets a zero row; slots at and past seq_lens[i] take no
  * part, whatever they hold.  seq_lens[i] beyond the table sets error bit 4 (the

@@ -34,11 +34,12 @@
 //    2^-111 (a product with V's largest possible scale) to 2^104; where V is so
 //    small that its products want larger ones they stay at that, and rows of
 //    V of 2^-100, the smallest that are stored, keep 17 bits.
-//  * A second product takes what that rounding left, so that outputs are as far from
-//    the exact result as their own rounding puts them: of the mean square, fp16 2.08e-4
-//    with it and 2.96e-4 without, bf16 1.66e-3 and 1.67e-3.  It costs fp16 2.5 % at 8
-//    heads and 4.5 % at 16, bf16 0.2 % at 4 heads and 1.5 % at 8; at 16 it would cost
-//    bf16 10 % (4 x 131072 tokens 72 us for 65.5), more than that 1 % is worth.
+//  * fp16 outputs get a second product with what that rounding left, without
+//    which they were half as far again from the exact result as their own rounding
+//    puts them (2.96e-4 in place of 2.08e-4 of the mean square).  bf16 outputs,
+//    whose own rounding is eight times the weights', gain 1 % from it and do
+//    without (16 heads, 4 x 131072 tokens 71 us with it, 65 without; fp16 pays 2.5 %
+//    at most at 8 heads, 4.5 % at 16).
 //  * bf16 queries are scaled by a power of two per head, so that their largest
 //    is in [2^13, 2^14), which fp16 holds as exactly as bf16 did but for values
 //    below 2^-28 of it.
@@ -288,10 +289,6 @@ __device__ __forceinline__ void store_record(const Decode8Params& p, size_t rec,
 
 template <int D, int NT>
 constexpr bool kRegroup8 = D == 128 && NT == 2;
-
-// Whether weights keep what their rounding to fp16 leaves.
-template <typename T, int NT>
-constexpr bool kRemainder8 = std::is_same<T, __half>::value || NT == 1;
 
 template <typename T, int D, int NT, bool kInt8>
 __global__ void __launch_bounds__(32 * (kProducers8 + kWarps8), 1)
@@ -746,7 +743,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       }
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        uint32_t pb[NT][2], pl[NT][2];  // rounded weights, and what that left
+        uint32_t pb[NT][2], pl[NT][2];  // rounded weights, and for fp16 what that left
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float p0 = fast_exp2(y[i][nt][0]), p1 = fast_exp2(y[i][nt][1]);
@@ -758,7 +755,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
           const uint32_t lo = Elt<__half>::pack(w0, w1), hi = Elt<__half>::pack(w2, w3);
           pb[nt][0] = movmatrix_trans(lo);
           pb[nt][1] = movmatrix_trans(hi);
-          if constexpr (kRemainder8<T, NT>) {
+          if constexpr (kF16) {
             pl[nt][0] = movmatrix_trans(remainder(w0, w1, lo));
             pl[nt][1] = movmatrix_trans(remainder(w2, w3, hi));
           }
@@ -786,7 +783,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
           for (int nt = 0; nt < NT; ++nt) {
             Mma<__half>::run(o[nt][2 * kk], b, pb[nt][0], pb[nt][1]);
             Mma<__half>::run(o[nt][2 * kk + 1], d, pb[nt][0], pb[nt][1]);
-            if constexpr (kRemainder8<T, NT>) {
+            if constexpr (kF16) {
               Mma<__half>::run(o[nt][2 * kk], b, pl[nt][0], pl[nt][1]);
               Mma<__half>::run(o[nt][2 * kk + 1], d, pl[nt][0], pl[nt][1]);
             }
