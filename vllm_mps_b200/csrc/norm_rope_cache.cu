@@ -10,10 +10,10 @@
 // the result is rounded once: to the 16-bit type, or to a code.
 //
 // What bounds it: the bytes of q, k and v in and out; 8192 rows of 32/8 heads x
-// 128 into the int8 cache take 35.4 us (5.2 TB/s; the instructions keep 70 % of the
+// 128 into the int8 cache take 35.4 us (5.2 TB/s; the instructions keep 67 % of the
 // issue slots), one row 2.1 us.  What hides the loads is the number of warps: with
-// 72 registers and 28 warps an SM 35.4 us, with 80 and 24 39.8, with 64 and 32, where a
-// few values are spilled, 36.9.
+// 72 registers and 28 warps an SM 34.7 us (before the codes' quotients were
+// corrected), with 80 and 24 39, with 64 and 32, where a few values are spilled, 36.9.
 #include "cache8.cuh"
 #include "rows_overlap.h"
 #include "vmps_abi_internal.h"
@@ -266,8 +266,8 @@ norm_rope_cache_kernel(const StoreParams p) {
   }
 }
 
-// Steps of a warp, at most (8192 rows of 32/8 heads, head size 128, 12 steps: 35.4 us with
-// 12, 36.9 with 6; rows of 18 and 30 steps gain nothing from more).
+// Steps of a warp, at most (8192 rows of 32/8 heads, head size 128, 12 steps: 34.7 us with
+// 12, 36.5 with 6; rows of 18 and 30 steps gain nothing from more).
 constexpr int kSteps = 12;
 
 template <typename T, int D, typename Code>

@@ -10,8 +10,9 @@
 //    2 where n_kv is even, else 1).  The tiles of all sequences are cut into equal
 //    contiguous shares, one per CTA of a persistent grid, one CTA per SM
 //    (cache8_plan.h), so that ragged batches and single long sequences both keep
-//    every SM streaming.  Few heads a CTA mean few pieces: with all 8 kv heads of a
-//    page in a CTA, 32 ragged sequences took 77 us where two take 40, and one 43.
+//    every SM streaming.  Few heads a CTA mean few pieces: the first
+//    kernel took 61.5 us for 32 ragged sequences with all 8 kv heads of a page in a
+//    CTA and 40.4 with two.
 //  * Four producer warps stream pages: a tiled TMA for the codes (K and V of HPC
 //    heads, swizzled) and a bulk copy for their scales, into a ring of stages,
 //    and the query rows of the next sequences into a ring of their own.
@@ -36,10 +37,10 @@
 //    V of 2^-100, the smallest that are stored, keep 17 bits.
 //  * fp16 outputs get a second product with what that rounding left, without
 //    which they were half as far again from the exact result as their own rounding
-//    puts them (2.96e-4 in place of 2.08e-4 of the mean square).  bf16 outputs,
-//    whose own rounding is eight times the weights', gain 1 % from it and do
-//    without (16 heads, 4 x 131072 tokens 71 us with it, 65 without; fp16 pays 2.5 %
-//    at most at 8 heads, 4.5 % at 16).
+//    puts them (2.96e-4 in place of 2.08e-4 of the mean square).  It costs fp16 2.5 %
+//    at 8 heads and 4.5 % at 16, in long runs, which the card's power holds back, 5 to
+//    9 %.  bf16 outputs, whose own rounding is eight times the weights', would gain 1 %
+//    of their error for as much, and do without.
 //  * bf16 queries are scaled by a power of two per head, so that their largest
 //    is in [2^13, 2^14), which fp16 holds as exactly as bf16 did but for values
 //    below 2^-28 of it.
