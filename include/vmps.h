@@ -402,7 +402,8 @@ int vmps_w4_gemm(void* out, int64_t out_row_stride, const void* x, int64_t x_row
  *   codes  [num_blocks][2][16][n_kv][head_dim]  int8 or e4m3 (dim 1: 0 = K, 1 = V)
  *   scales [num_blocks][n_kv][2][16]            fp32
  * both contiguous and 16-byte aligned.  The value stored is code * scale of its
- * token, head and kind.  Written by vmps_norm_rope_and_cache, the scale is the
+ * token, head and kind (scales of a caller's own may be negative).  Written by
+ * vmps_norm_rope_and_cache, the scale is the
  * largest magnitude of the token's head_dim values over 127 (int8) or 448
  * (e4m3) and the code the value times that over the largest magnitude, to nearest
  * with ties to even (rotated and normalised values are fp32, and within 2^-21 of a tie
@@ -466,7 +467,9 @@ int vmps_read_cache8(void* pool, int pool_blocks, const int32_t* dst_tables, con
  *   out[i][h] = softmax_t(scale * q[i][h] . K[t][h / G]) . V[t][h / G], t < seq_lens[i]
  * Scores, maxima and sums are fp32; for its products with V's codes a softmax weight
  * times V's scale is kept to 2^-22 of itself for fp16 outputs, and rounded to fp16 (2^-11)
- * for bf16 ones, or by 2^-35 of the head's largest such product where that is more.  q is [num_seqs][n_q][head_dim] with a row
+ * for bf16 ones, or by 2^-35 of the head's largest such product where that is more (by 2^-17
+ * where all of V is about 2^-100).  Weights are counted down to 2^-44 of the largest where V
+ * is below 2^100, to 2^-16 at fp32's largest.  q is [num_seqs][n_q][head_dim] with a row
  * stride (a multiple of 8 elements), out contiguous, both 16-byte aligned.  A
  * sequence of length 0 gets a zero row; slots at and past seq_lens[i] take no
  * part, whatever they hold.  seq_lens[i] beyond the table sets error bit 4 (the

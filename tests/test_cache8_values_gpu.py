@@ -11,8 +11,8 @@ fp16: 2^-11 of itself, or, where that is more, half of fp16's smallest step, 2^-
 with the largest product of the warp's tokens at 2^10 or above: 2^-35 of the
 largest, W = max_t p_t amax_t, for each of the n tokens (a code's 127 or 448 is
 amax over its scale).  With A = sum_t p_t |V_t| and one rounding of the result (u):
-    2 (sum_t p_t e_t |V_t| + |out| sum_t p_t e_t) + 2 * 2^-11 A + n 2^-35 W + u |out| + 2^-25
-(2^-25: half of fp16's smallest step, for results near zero).
+    2 (sum_t p_t e_t |V_t| + |out| sum_t p_t e_t) + 2 * 2^-11 A + n 2^-35 W + u |out| + half of
+the type's smallest step (fp16 2^-25, bf16 2^-134).
 
 For fp16 outputs what the rounding to fp16 left is kept too (2^-22).  A weight's
 logarithm is then the largest term: fp32 below 2^5 (2^-20, and 2^-22 of the exponential),
@@ -71,7 +71,7 @@ def _built(scores, sizes, G, D, dtype, fmt, seed):
                 block_tables=i32(order[None, :pages]), seq_lens=i32([n]))
 
 
-def _off(c, got, weights=2 * 2.0 ** -11):
+def _off(c, got, weights=2 * 2.0 ** -11, least=2.0 ** -35):
     """The largest error as a share of its bound."""
     q, cache, n = c["q"][0].double(), c["cache"], int(c["seq_lens"][0])
     G, D = q.shape
@@ -84,7 +84,8 @@ def _off(c, got, weights=2 * 2.0 ** -11):
     out, a = p @ v, p @ v.abs()
     w = (p * v.abs().amax(1)).amax(1, keepdim=True)
     tol = 2 * ((p * e) @ v.abs() + out.abs() * (p * e).sum(1, keepdim=True)) + weights * a \
-        + n * 2.0 ** -35 * w + U[got.dtype] * out.abs() + 2.0 ** -25
+        + n * least * w + U[got.dtype] * out.abs() \
+        + (2.0 ** -25 if got.dtype == torch.float16 else 2.0 ** -134)
     assert torch.isfinite(got).all()
     return float(((got[0].double() - out).abs() / tol).max())
 
@@ -119,3 +120,25 @@ def test_weights_and_values_that_drift_apart(G, D, dtype, fmt, rise, fall, n):
 def test_fp16_outputs_are_rounded_once(G, D, fmt, n):
     c = _case([n], G, 1, D, torch.float16, fmt, n + G, spare=False)
     assert _off(c, K.paged_decode_attention_cache8(**c), 2.0 ** -16) <= 1
+
+
+@pytest.mark.parametrize("G, D, fmt", [(4, 128, INT8), (9, 64, E4M3)])
+@pytest.mark.parametrize("size", [-99, -60, 60, 99])
+def test_values_near_the_ends_of_fp32(size, G, D, fmt):
+    """All of V tiny (products with weights of at most 2^104 leave fp16 2^-17 of the largest) or
+    huge; most weights 2^-30 of the others."""
+    rng = np.random.default_rng(3)
+    n = 3000
+    scores = np.where(rng.random(n) < 0.05, rng.normal(size=n), -30 * math.log(2.0))
+    c = _built(scores, np.exp2(size + rng.uniform(0, 1, n)), G, D, torch.bfloat16, fmt, 4)
+    got = K.paged_decode_attention_cache8(**c)
+    assert _off(c, got, least=2.0 ** -17 if size == -99 else 2.0 ** -35) <= 1
+
+
+def test_small_weights_beside_one_huge_value():
+    """One token with half of the weight and V of 2^99; 20000 share the other half."""
+    n = 20001
+    scores, sizes = np.zeros(n), np.ones(n)
+    scores[777], sizes[777] = math.log(n - 1.0), 2.0 ** 99
+    c = _built(scores, sizes, 8, 64, torch.bfloat16, INT8, 5)
+    assert _off(c, K.paged_decode_attention_cache8(**c)) <= 1
