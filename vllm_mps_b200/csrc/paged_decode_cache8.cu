@@ -744,7 +744,8 @@ decode8_kernel(const __grid_constant__ CUtensorMap tmap, const Decode8Params p) 
       }
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        uint32_t pb[NT][2], pl[NT][2];  // rounded weights, and for fp16 what that left
+        uint32_t pb[NT][2];  // rounded weights
+        [[maybe_unused]] uint32_t pl[NT][2];  // for fp16, what that left
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float p0 = fast_exp2(y[i][nt][0]), p1 = fast_exp2(y[i][nt][1]);
